@@ -7,8 +7,9 @@ is one pass (own: through ameva_compute_amd.ops, else in elementary torch operat
 without, exact() its outputs in 64 bits. Pools are made here, in plain torch, in the layout include/ameva_hip.h describes:
 
   F16         k, v f16 [page][KV head][key][d]
-  Q8_0, Q4_0  k, v bytes [page][KV head][integers of all keys | scales of all keys]: integers [key][d] (Q8_0: int8; Q4_0: two
-              elements a byte, the even one in the low bits, value + 8), scales f16 [key][d / 32]
+  Q8_0, Q4_0  k, v bytes [page][KV head][integers of all keys | scales of all keys]: integers [key][place] (Q8_0: int8; Q4_0:
+              two places a byte, the even one in the low bits, value + 8), scales f16 [key][d / 32]; a key's places hold its
+              elements in the order [8-element piece of a block][block][8], a value's in [pair of a block][block][2]
   bounds      f16 [page][KV head][min, max][d] over the keys in the page
 """
 import math
@@ -146,8 +147,13 @@ def _randn(gen, *shape):
     return torch.randn(shape, generator=gen, device=DEV)
 
 
-def _pack(c, x):
-    """x f32 [page][KV head][key][d] as the pool of the case's type."""
+def _places(x, of):
+    """Integers [..., block, 32] of keys (of "k") or values as places [..., d]."""
+    return x.unflatten(-1, (4, 8) if of == "k" else (16, 2)).transpose(-3, -2).flatten(-3)
+
+
+def _pack(c, x, of):
+    """x f32 [page][KV head][key][d], keys (of "k") or values, as the pool of the case's type."""
     if c["type"] == "f16":
         return x.half()
     p, g, s, d = x.shape
@@ -155,18 +161,19 @@ def _pack(c, x):
     if c["type"] == "q8_0":
         big = b.abs().amax(-1)
         scale, inv = big / 127, torch.where(big == 0, big, 127 / big)
-        q = (b * inv[..., None]).round().clamp(-127, 127).to(torch.int8).view(torch.uint8).view(p, g, s * d)
+        q = (b * inv[..., None]).round().clamp(-127, 127).to(torch.int8).view(torch.uint8)
+        q = _places(q, of).reshape(p, g, s * d)
     else:
         big = b.gather(-1, b.abs().argmax(-1, keepdim=True))[..., 0]
         scale = big / -8
         inv = torch.where(scale == 0, scale, 1 / scale)
-        u = (b * inv[..., None] + 8.5).to(torch.int32).clamp(0, 15).to(torch.uint8).view(p, g, s, d // 2, 2)
-        q = (u[..., 0] | u[..., 1] << 4).view(p, g, s * d // 2)
+        u = _places((b * inv[..., None] + 8.5).to(torch.int32).clamp(0, 15).to(torch.uint8), of)
+        q = (u[..., 0::2] | u[..., 1::2] << 4).reshape(p, g, s * d // 2)
     return torch.cat([q, scale.half().view(p, g, -1).contiguous().view(torch.uint8)], -1).contiguous()
 
 
-def _unpack(c, pool, dtype=torch.float32):
-    """Pages of a pool [..., KV head, chunk] as values [..., KV head, key, d]."""
+def _unpack(c, pool, of, dtype=torch.float32):
+    """Pages of a pool [..., KV head, chunk], of keys ("k") or values, as numbers [..., KV head, key, d]."""
     if c["type"] == "f16":
         return pool.to(dtype)
     d, s = c["d"], c["page"]
@@ -174,10 +181,11 @@ def _unpack(c, pool, dtype=torch.float32):
     lead = pool.shape[:-1]
     scale = pool[..., n:].contiguous().view(torch.float16).view(*lead, s, d // 32, 1).to(dtype)
     if c["type"] == "q8_0":
-        q = pool[..., :n].contiguous().view(torch.int8).view(*lead, s, d // 32, 32).to(dtype)
+        q = pool[..., :n].contiguous().view(torch.int8).to(dtype)
     else:
-        b = pool[..., :n].contiguous().view(*lead, s, d // 32, 16, 1)
-        q = torch.cat([b & 15, b >> 4], -1).view(*lead, s, d // 32, 32).to(dtype) - 8
+        b = pool[..., :n].unsqueeze(-1)
+        q = torch.cat([b & 15, b >> 4], -1).to(dtype) - 8
+    q = q.view(*lead, s, *((4, d // 32, 8) if of == "k" else (16, d // 32, 2))).transpose(-3, -2).flatten(-2)
     return (q * scale).view(*lead, s, d)
 
 
@@ -207,11 +215,11 @@ def prepare(c, seed):
     x += 0.5 * _randn(gen, 1, g, 1, d)
     if c["kind"] == "sparse":
         x += 0.7 * _randn(gen, n_pages, g, 1, d)
-    s["k"] = _pack(c, x)
+    s["k"] = _pack(c, x, "k")
     if c["kind"] in ("append", "sparse"):
         x16 = x.half()
         s["bounds"] = torch.stack([x16.amin(2), x16.amax(2)], 2).contiguous()
-    s["v"] = _pack(c, _randn(gen, n_pages, g, page, d))
+    s["v"] = _pack(c, _randn(gen, n_pages, g, page, d), "v")
     if c["kind"] in ("append", "step"):
         s["qkv"] = _randn(gen, n_tok, h + 2 * g, d)
     else:
@@ -282,8 +290,8 @@ def _append(s, c):
         s["k"][at, :, slot] = k.half()
         s["v"][at, :, slot] = v.half()
     else:
-        for pool, new in ((s["k"], k), (s["v"], v)):
-            one = _pack(c, new[:, :, None].contiguous())  # [token][KV head][integers | scales]
+        for of, new in (("k", k), ("v", v)):
+            pool, one = s[of], _pack(c, new[:, :, None].contiguous(), of)  # [token][KV head][integers | scales]
             ni = d if c["type"] == "q8_0" else d // 2
             n = pool.shape[-1] // (ni + d // 16) * ni
             col = slot[:, None, None]
@@ -315,7 +323,7 @@ def _attend(s, c, q):
     t = torch.arange(mq, device=DEV)
     tok, has = cu[:-1, None] + t, t < nq[:, None]
     rows = (q[tok.clamp(max=s["n_tok"] - 1)] * s["scale"]).view(n, mq, g, h // g, d).permute(0, 2, 1, 3, 4).reshape(n, g, -1, d)
-    k, v = (_unpack(c, p[s["table"].clamp(min=0).long()]).transpose(1, 2).reshape(n, g, -1, d) for p in (s["k"], s["v"]))
+    k, v = (_unpack(c, s[p][s["table"].clamp(min=0).long()], p).transpose(1, 2).reshape(n, g, -1, d) for p in "kv")
     key = torch.arange(k.shape[2], device=DEV)
     there = key < n_kv[:, None]
     k, v = (x.masked_fill(~there[:, None, :, None], 0.0) for x in (k, v))
@@ -324,7 +332,7 @@ def _attend(s, c, q):
     see = see.repeat_interleave(h // g, 1)[:, None]
     m, l, o = _softmax_parts(rows @ k.transpose(-1, -2).contiguous(), see, v)
     if c["prefix"]:
-        pk, pv = (_unpack(c, p[s["prefix_table"].long()]).transpose(0, 1).reshape(g, -1, d)[:, :c["prefix"]] for p in (s["k"], s["v"]))
+        pk, pv = (_unpack(c, s[p][s["prefix_table"].long()], p).transpose(0, 1).reshape(g, -1, d)[:, :c["prefix"]] for p in "kv")
         all_rows = rows.transpose(0, 1).reshape(g, -1, d)
         pm, pl, po = _softmax_parts(all_rows @ pk.transpose(-1, -2).contiguous(), torch.ones((), dtype=torch.bool, device=DEV), pv)
         pm, pl, po = (x.view(g, n, -1, x.shape[-1]).transpose(0, 1) for x in (pm, pl, po))
@@ -360,7 +368,7 @@ def _attend_selected(s, c, sel):
     t = s["n_tok"]
     at = s["table"][seq[:, None, None], sel.clamp(min=0).long()].clamp(min=0).long()  # [token][KV head][selected]
     head = torch.arange(g, device=DEV)[None, :, None]
-    k, v = (_unpack(c, p[at, head]).view(t, g, -1, d) for p in (s["k"], s["v"]))
+    k, v = (_unpack(c, s[p][at, head], p).view(t, g, -1, d) for p in "kv")
     key = (sel[..., None] * page + torch.arange(page, device=DEV)).view(t, g, -1)
     see = ((key <= place[:, None, None]) & (key >= 0))[:, :, None]
     k, v = (x.masked_fill(~see.transpose(-1, -2), 0.0) for x in (k, v))
@@ -373,13 +381,13 @@ def exact(c, seed):
     s = prepare(c, seed)
     h, g, d, page = c["heads"], c["kv_heads"], c["d"], c["page"]
     kv, nq = _lengths(c)
-    kval, vval = (_unpack(c, s[p], torch.float64) if c["kind"] == "step" else None for p in "kv")
+    kval, vval = (_unpack(c, s[p], p, torch.float64) if c["kind"] == "step" else None for p in "kv")
     table = s["table"].long()
 
     def rows(p, pages, head, n):  # the first n keys or values of a list of pages, one KV head
         if kval is not None:
             return (kval if p == "k" else vval)[pages, head].reshape(-1, d)[:n]
-        return _unpack(c, s[p][pages, head], torch.float64).reshape(-1, d)[:n]
+        return _unpack(c, s[p][pages, head], p, torch.float64).reshape(-1, d)[:n]
 
     out, first = [], 0
     q_all = []
@@ -410,8 +418,8 @@ def exact(c, seed):
                         bounds[at, :, 0] = torch.minimum(bounds[at, :, 0], low) if old else low
                         bounds[at, :, 1] = torch.maximum(bounds[at, :, 1], high) if old else high
                 else:
-                    kval[pg, :, sl], vval[pg, :, sl] = (_unpack({**c, "page": 1}, _pack(c, y[:, :, None].contiguous()), torch.float64)[:, :, 0]
-                                                        for y in new)
+                    kval[pg, :, sl], vval[pg, :, sl] = (_unpack({**c, "page": 1}, _pack(c, y[:, :, None].contiguous(), p), p, torch.float64)[:, :, 0]
+                                                        for y, p in zip(new, "kv"))
             first += nq[i]
         q = torch.cat(q_all)
         if c["kind"] == "append":
