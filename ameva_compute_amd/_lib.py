@@ -12,6 +12,18 @@ LIB_PATH = os.path.join(HERE, "libameva_hip.so")
 
 P, I32, I64, F32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 
+
+
+class PagedKVStruct(ctypes.Structure):  # amv_paged_kv
+    _fields_ = [(n, ctypes.c_int32) for n in ("type", "n_head_kv", "D", "page_size")] + \
+               [(n, ctypes.c_int64) for n in ("n_pages", "page_stride")] + [(n, P) for n in ("k", "v", "bounds")]
+
+
+class PagedBatchStruct(ctypes.Structure):  # amv_paged_batch
+    _fields_ = [(n, ctypes.c_int64) for n in ("n_seq", "n_tok", "max_q", "max_kv", "table_stride")] + \
+               [(n, P) for n in ("cu_q", "n_kv", "table")]
+
+
 # name -> (restype, argtypes); every symbol include/ameva_hip.h declares
 SIGNATURES = {
     "amv_last_error": (ctypes.c_char_p, []),
@@ -66,6 +78,14 @@ SIGNATURES = {
     "amv_flash_attn_decode": (I32, [P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, F32, P, I64, P, I32, P]),
     "amv_flash_attn_prefill": (I32, [P, I64, I64, P, P, P, I64, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, F32,
                                      I64, P]),
+    "amv_paged_chunk_bytes": (I64, [I32, I64, I64]),
+    "amv_paged_rope_append": (I32, [P, P, P, I64, I64, P, I32, I32, F32, F32, F32, I32, P, I64, P, P]),
+    "amv_paged_attn_workspace_bytes": (I64, [P, P, I64, I64, I64]),
+    "amv_paged_attn": (I32, [P, P, P, I64, P, I64, F32, P, I64, P]),
+    "amv_paged_attn_shared": (I32, [P, P, P, I64, P, I64, P, I64, F32, P, I64, P]),
+    "amv_paged_select_workspace_bytes": (I64, [P, P]),
+    "amv_paged_select": (I32, [P, P, P, I64, I64, I64, I64, I64, P, P, I64, P]),
+    "amv_paged_attn_sparse": (I32, [P, P, P, I64, P, I64, P, I64, F32, P, I64, P]),
     "amv_binary": (I32, [I32, P, P, P, I64, I64, I64, P]),
     "amv_set_rows_f16": (I32, [P, I64, P, I64, I64, I64, P, I32, I64, P, P]),
     "amv_i2s_gemv_acc": (I32, [P, I64, I64, P, F32, P, P]),

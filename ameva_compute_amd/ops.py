@@ -8,12 +8,14 @@ there is no CPU path.
 """
 from __future__ import annotations
 
+import contextlib
+import ctypes
 import functools
 import os
 
 import torch
 
-from ._lib import check, lib
+from ._lib import PagedBatchStruct, PagedKVStruct, check, lib
 
 # ggml_type values (reference include/ggml/ggml.h:394-437)
 F32, F16, Q4_0, Q8_0, Q4_K, Q6_K, Q8_K, I2_S = 0, 1, 2, 8, 12, 14, 15, 36
@@ -569,6 +571,216 @@ def flash_attn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale:
                                        0 if mask is None else mask.stride(0), out.data_ptr(), n_tok, n_head,
                                        n_head_kv, n_kv, D, k.stride(1), k.stride(0), v.stride(1), v.stride(0), scale,
                                        causal_pos0, _stream()), "amv_flash_attn_prefill")
+    return out
+
+
+# ---------------------------------------------------------------------------------------------- paged KV cache
+class PagedKV:
+    """A pool of pages for the keys and values of many sequences (include/ameva_hip.h amv_paged_kv). F16: k, v f16 [n_pages,
+    n_head_kv, page_size, D]; Q8_0, Q4_0: k, v uint8 [n_pages, n_head_kv, chunk bytes]. A page's KV heads are contiguous, pages may
+    be any multiple of 16 bytes apart (a layer's part of a common allocation). bounds: f16 [n_pages, n_head_kv, 2, D] or None."""
+
+    def __init__(self, kv_type: int, k: torch.Tensor, v: torch.Tensor, page_size: int, n_head_kv: int, head_dim: int,
+                 bounds: torch.Tensor | None = None):
+        chunk = lib().amv_paged_chunk_bytes(kv_type, head_dim, page_size)
+        if chunk < 0:
+            raise ValueError(f"PagedKV: type {kv_type} with heads of {head_dim} and pages of {page_size} is not supported")
+        for t, what in ((k, "PagedKV k"), (v, "PagedKV v")):
+            _need_gpu(t, what, contiguous=False)
+            shape = (n_head_kv, page_size, head_dim) if kv_type == F16 else (n_head_kv, chunk)
+            if t.dtype != (torch.float16 if kv_type == F16 else torch.uint8) or tuple(t.shape[1:]) != shape:
+                raise ValueError(f"{what}: {tuple(t.shape)} {t.dtype} is not pages of {shape}")
+            if t.shape[0] == 0 or not t[0].is_contiguous():
+                raise ValueError(f"{what}: a page must be contiguous")
+        if k.shape[0] != v.shape[0] or k.stride(0) != v.stride(0) or k.device != v.device:
+            raise ValueError("PagedKV: k and v must have the same pages")
+        if bounds is not None:
+            _need_gpu(bounds, "PagedKV bounds")
+            if bounds.dtype != torch.float16 or bounds.shape != (k.shape[0], n_head_kv, 2, head_dim) or bounds.device != k.device:
+                raise ValueError("PagedKV bounds: f16 [n_pages, n_head_kv, 2, D] expected")
+        self.type, self.page_size, self.n_head_kv, self.D = kv_type, page_size, n_head_kv, head_dim
+        self.k, self.v, self.bounds, self.n_pages, self.device = k, v, bounds, k.shape[0], k.device
+        stride = k.stride(0) * k.element_size() if self.n_pages > 1 else n_head_kv * chunk
+        self._c = PagedKVStruct(kv_type, n_head_kv, head_dim, page_size, self.n_pages, stride, k.data_ptr(), v.data_ptr(),
+                                _ptr(bounds))
+        self._p = ctypes.addressof(self._c)
+
+    @classmethod
+    def alloc(cls, kv_type: int, n_pages: int, page_size: int, n_head_kv: int, head_dim: int, device,
+              bounds: bool = False) -> "PagedKV":
+        """A pool of n_pages empty pages (their contents do not matter), with bounds where pages are to be selected."""
+        chunk = lib().amv_paged_chunk_bytes(kv_type, head_dim, page_size)
+        if chunk < 0:
+            raise ValueError(f"PagedKV: type {kv_type} with heads of {head_dim} and pages of {page_size} is not supported")
+        if kv_type == F16:
+            k, v = (torch.empty((n_pages, n_head_kv, page_size, head_dim), dtype=torch.float16, device=device) for _ in "kv")
+        else:
+            k, v = (torch.empty((n_pages, n_head_kv, chunk), dtype=torch.uint8, device=device) for _ in "kv")
+        b = torch.empty((n_pages, n_head_kv, 2, head_dim), dtype=torch.float16, device=device) if bounds else None
+        return cls(kv_type, k, v, page_size, n_head_kv, head_dim, b)
+
+
+class PagedBatch:
+    """The sequences of a call (include/ameva_hip.h amv_paged_batch), all on the GPU: n_kv int32 [n_seq] keys of each, this call's
+    own included; table int32 [n_seq, pages]; cu_q int32 [n_seq + 1], where each one's tokens begin among the n_tok rows (None:
+    one token each). max_q and max_kv: the most tokens and keys of a sequence that the launches are sized for. The tensors are
+    used as they are at each call (a program advances n_kv and the table in place), so they must stay alive and contiguous."""
+
+    def __init__(self, n_kv: torch.Tensor, table: torch.Tensor, max_kv: int, n_tok: int | None = None,
+                 cu_q: torch.Tensor | None = None, max_q: int = 1):
+        for t, what in ((n_kv, "PagedBatch n_kv"), (table, "PagedBatch table"), (cu_q, "PagedBatch cu_q")):
+            if t is None:
+                continue
+            _need_gpu(t, what)
+            if t.dtype != torch.int32 or t.device != n_kv.device:
+                raise ValueError(f"{what}: int32 on {n_kv.device} expected")
+        self.n_seq = n_kv.numel()
+        if table.dim() != 2 or table.shape[0] != self.n_seq or (cu_q is not None and cu_q.numel() != self.n_seq + 1):
+            raise ValueError("PagedBatch: table must be [n_seq, pages], cu_q [n_seq + 1]")
+        self.n_tok = self.n_seq if n_tok is None else n_tok
+        self.n_kv, self.table, self.cu_q, self.max_q, self.max_kv, self.device = n_kv, table, cu_q, max_q, max_kv, n_kv.device
+        self._c = PagedBatchStruct(self.n_seq, self.n_tok, max_q, max_kv, table.shape[1], _ptr(cu_q), n_kv.data_ptr(),
+                                   table.data_ptr())
+        self._p = ctypes.addressof(self._c)
+        self._bytes = {}
+
+    def _workspace(self, kv: PagedKV, n_head: int, n_prefix: int, n_sel: int) -> int:
+        """Bytes of amv_paged_attn's workspace (n_sel < 0: of amv_paged_select's) for this batch over kv."""
+        key = (kv.type, kv.page_size, kv.n_head_kv, kv.D, n_head, n_prefix, n_sel)
+        n = self._bytes.get(key)
+        if n is None:
+            L = lib()
+            n = (L.amv_paged_select_workspace_bytes(kv._p, self._p) if n_sel < 0 else
+                 L.amv_paged_attn_workspace_bytes(kv._p, self._p, n_head, n_prefix, n_sel))
+            check(min(n, 0), "paged workspace")
+            if len(self._bytes) > 64:  # (a program whose prefix grows key by key)
+                self._bytes.clear()
+            self._bytes[key] = n
+        return n
+
+
+def _paged_rows(kv: PagedKV, b: PagedBatch, x: torch.Tensor, heads: int | None, what: str) -> int:
+    """Checks x f32 [n_tok, heads, D] (contiguous heads, any row stride); the heads it has."""
+    if x.dim() != 3 or x.shape[0] != b.n_tok or x.shape[2] != kv.D or (heads is not None and x.shape[1] != heads):
+        raise ValueError(f"{what}: [{b.n_tok}, {'heads' if heads is None else heads}, {kv.D}] expected, got {tuple(x.shape)}")
+    if x.dtype != torch.float32 or x.device != kv.device or b.device != kv.device:
+        raise ValueError(f"{what}: f32 on {kv.device} expected (pool, batch and rows on one GPU)")
+    if b.n_tok and (x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != kv.D)):
+        raise ValueError(f"{what}: a row's heads must be contiguous")
+    return x.shape[1]
+
+
+def _paged_out(out: torch.Tensor | None, shape, like: torch.Tensor, what: str, dtype=torch.float32) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != like.device or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be contiguous {dtype} {tuple(shape)} on {like.device}")
+    return out
+
+
+def _paged_ws(ws: torch.Tensor | None, need: int, like: torch.Tensor, what: str):
+    """A workspace of at least `need` bytes: the caller's, which then has to do (captured graphs hold its address), or a new one."""
+    if ws is None:
+        return torch.empty(need, dtype=torch.uint8, device=like.device) if need else None
+    if ws.device != like.device or not ws.is_contiguous() or ws.numel() * ws.element_size() < need:
+        raise ValueError(f"{what}: workspace must be {need} contiguous bytes on {like.device}")
+    return ws
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
+
+
+def _on(device: torch.device):
+    """The device of the operands as the current one, where it is not."""
+    return contextlib.nullcontext() if device.index == _device() else torch.cuda.device(device)
+
+
+def paged_workspace_bytes(kv: PagedKV, batch: PagedBatch, n_head: int, n_prefix: int = 0, n_sel: int = 0) -> int:
+    """Bytes of workspace of paged_attn, paged_attn_shared (n_prefix) or paged_attn_sparse (n_sel) for this batch."""
+    return batch._workspace(kv, n_head, n_prefix, n_sel)
+
+
+def paged_rope_append(kv: PagedKV, batch: PagedBatch, qkv: torch.Tensor, n_head: int, pos: torch.Tensor | None = None,
+                      n_dims: int | None = None, mode: int = 0, freq_base: float = 10000.0, freq_scale: float = 1.0,
+                      attn_factor: float = 1.0, rule: int = Q8_X86, bad: torch.Tensor | None = None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """ROPE of the q and k heads of qkv f32 [n_tok, n_head + 2 n_head_kv, D]; the rotated k and the v go to the pages at their
+    tokens' places (and into the pool's bounds), the rotated q is returned, f32 [n_tok, n_head, D]. pos int32 [n_tok]: the
+    rotation's positions (None: the places in the cache). bad int32 [1]: counts tokens and KV heads that were not stored."""
+    _paged_rows(kv, batch, qkv, n_head + 2 * kv.n_head_kv, "paged_rope_append")
+    for t, dt, n, name in ((pos, torch.int32, batch.n_tok, "pos"), (bad, torch.int32, 1, "bad")):
+        if t is not None and (t.dtype != dt or t.device != kv.device or not t.is_contiguous() or t.numel() < n):
+            raise ValueError(f"paged_rope_append: {name} must be int32 [{n}] on {kv.device}")
+    with _on(kv.device):
+        out = _paged_out(out, (batch.n_tok, n_head, kv.D), qkv, "paged_rope_append")
+        check(lib().amv_paged_rope_append(kv._p, batch._p, qkv.data_ptr(), _row_stride(qkv), n_head, _ptr(pos),
+                                          kv.D if n_dims is None else n_dims, mode, freq_base, freq_scale, attn_factor, rule,
+                                          out.data_ptr(), n_head * kv.D, _ptr(bad), _stream()), "amv_paged_rope_append")
+    return out
+
+
+def paged_attn(kv: PagedKV, batch: PagedBatch, q: torch.Tensor, scale: float, out: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of the batch's tokens q f32 [n_tok, n_head, D] over their sequences' pages: decode steps, prompt chunks and
+    both together. Returns f32 [n_tok, n_head, D]; tokens that see no key give zeros."""
+    n_head = _paged_rows(kv, batch, q, None, "paged_attn")
+    with _on(kv.device):
+        out = _paged_out(out, q.shape, q, "paged_attn")
+        need = batch._workspace(kv, n_head, 0, 0)
+        ws = _paged_ws(workspace, need, q, "paged_attn")
+        check(lib().amv_paged_attn(kv._p, batch._p, q.data_ptr(), _row_stride(q), out.data_ptr(), n_head, scale, _ptr(ws), need,
+                                   _stream()), "amv_paged_attn")
+    return out
+
+
+def paged_attn_shared(kv: PagedKV, batch: PagedBatch, q: torch.Tensor, scale: float, prefix_table: torch.Tensor,
+                      n_prefix: int, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_attn of sequences that all begin with the n_prefix keys of the pages prefix_table (int32): these are read once for all
+    of them. batch has the keys behind the prefix only (rotate theirs and q with pos = n_prefix + place)."""
+    n_head = _paged_rows(kv, batch, q, None, "paged_attn_shared")
+    if prefix_table.dtype != torch.int32 or prefix_table.device != kv.device or not prefix_table.is_contiguous():
+        raise ValueError(f"paged_attn_shared: prefix_table must be contiguous int32 on {kv.device}")
+    if n_prefix < 0 or prefix_table.numel() * kv.page_size < n_prefix:
+        raise ValueError(f"paged_attn_shared: {prefix_table.numel()} pages for a prefix of {n_prefix} keys")
+    with _on(kv.device):
+        out = _paged_out(out, q.shape, q, "paged_attn_shared")
+        need = batch._workspace(kv, n_head, n_prefix, 0)
+        ws = _paged_ws(workspace, need, q, "paged_attn_shared")
+        check(lib().amv_paged_attn_shared(kv._p, batch._p, prefix_table.data_ptr(), n_prefix, q.data_ptr(), _row_stride(q),
+                                          out.data_ptr(), n_head, scale, _ptr(ws), need, _stream()), "amv_paged_attn_shared")
+    return out
+
+
+def paged_select(kv: PagedKV, batch: PagedBatch, q: torch.Tensor, n_sel: int, n_first: int = 1, n_last: int = 1,
+                 sel: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """For each token and KV head the n_sel pages of its sequence whose bounds allow the largest sum of q . k over the group's
+    heads, the first n_first and the last n_last always among them: int32 [n_tok, n_head_kv, n_sel], rising, -1 behind the last."""
+    n_head = _paged_rows(kv, batch, q, None, "paged_select")
+    if kv.bounds is None:
+        raise ValueError("paged_select: the pool has no bounds")
+    with _on(kv.device):
+        sel = _paged_out(sel, (batch.n_tok, kv.n_head_kv, n_sel), q, "paged_select", torch.int32)
+        need = batch._workspace(kv, n_head, 0, -1)
+        ws = _paged_ws(workspace, need, q, "paged_select")
+        check(lib().amv_paged_select(kv._p, batch._p, q.data_ptr(), _row_stride(q), n_head, n_sel, n_first, n_last,
+                                     sel.data_ptr(), _ptr(ws), need, _stream()), "amv_paged_select")
+    return sel
+
+
+def paged_attn_sparse(kv: PagedKV, batch: PagedBatch, q: torch.Tensor, sel: torch.Tensor, scale: float,
+                      out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_attn over the pages sel (paged_select's, or any choice with each page once) of each token and KV head."""
+    n_head = _paged_rows(kv, batch, q, None, "paged_attn_sparse")
+    if sel.dim() != 3 or sel.shape[:2] != (batch.n_tok, kv.n_head_kv) or sel.dtype != torch.int32 or not sel.is_contiguous() or \
+            sel.device != kv.device:
+        raise ValueError("paged_attn_sparse: sel must be contiguous int32 [n_tok, n_head_kv, pages] on the pool's GPU")
+    with _on(kv.device):
+        out = _paged_out(out, q.shape, q, "paged_attn_sparse")
+        need = batch._workspace(kv, n_head, 0, sel.shape[2])
+        ws = _paged_ws(workspace, need, q, "paged_attn_sparse")
+        check(lib().amv_paged_attn_sparse(kv._p, batch._p, sel.data_ptr(), sel.shape[2], q.data_ptr(), _row_stride(q),
+                                          out.data_ptr(), n_head, scale, _ptr(ws), need, _stream()), "amv_paged_attn_sparse")
     return out
 
 

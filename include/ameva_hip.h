@@ -444,6 +444,86 @@ int amv_flash_attn_prefill(const float* q, int64_t q_tok_stride, int64_t q_head_
                            int64_t v_head, float scale, int64_t causal_pos0, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------
+ * Paged KV cache (no counterpart in the reference, whose caches hold one sequence in one tensor): the keys and values of
+ * many sequences in pages of a common pool, and the attention of a batch over them.
+ *
+ * amv_paged_kv, the pool. type: 1 F16, 8 Q8_0, 2 Q4_0 (K and V both); D 64 or 128; page_size keys per page, a power of two from
+ * 16 to 1024. Page p starts at k (v) + p * page_stride bytes and holds a chunk per KV head, amv_paged_chunk_bytes each, one
+ * after the other; page_stride is a multiple of 16 and at least n_head_kv chunks, k and v are 16-byte aligned. A chunk:
+ *   F16:  f16 [page_size][D]
+ *   Q8_0: int8 [page_size][D] | scales f16 [page_size][D / 32]; value = integer * scale (ggml's block_q8_0 in pieces)
+ *   Q4_0: 4-bit integers [page_size][D], two a byte, the even place in the low bits, value + 8 | scales f16 [page_size][D / 32]
+ * The integers of a key lie in an order that the matrix cores take without exchanges: element d of a K row at place
+ * (d / 8 % 4) * (D / 4) + d / 32 * 8 + d % 8, of a V row at place (d % 32 / 2) * (D / 16) + d / 32 * 2 + d % 2.
+ * bounds (may be NULL): f16 [n_pages][n_head_kv][2][D], the smallest and largest element d of the keys in a page, taken from
+ * the rotated keys rounded to f16.
+ *
+ * amv_paged_batch, the sequences of a call, all in device memory but for the sizes. Sequence s has n_kv[s] keys, this call's
+ * own included; key j is row j % page_size of page table[s * table_stride + j / page_size]. Its tokens of this call are
+ * tokens cu_q[s] .. cu_q[s + 1] - 1 of the n_tok rows (cu_q int32 [n_seq + 1] from 0, not falling; NULL: token s, n_tok ==
+ * n_seq): the last of its keys, so token i of n_q stands at place n_kv - n_q + i and sees the keys 0 .. place. max_q >= every
+ * n_q and max_kv >= every n_kv size the launches, so a captured graph replays at growing lengths; keys from place max_kv on are
+ * neither stored nor seen.
+ * Rows from cu_q[n_seq] on are left as they were. A table entry outside [0, n_pages) is a page without keys; entries that no
+ * key needs are not looked at. What lies in a page behind a sequence's last key does not matter.
+ * ---------------------------------------------------------------------------------------------------------- */
+typedef struct amv_paged_kv {
+    int32_t type, n_head_kv, D, page_size;
+    int64_t n_pages, page_stride;
+    void *k, *v, *bounds;
+} amv_paged_kv;
+typedef struct amv_paged_batch {
+    int64_t n_seq, n_tok, max_q, max_kv, table_stride;
+    const int32_t *cu_q, *n_kv, *table;
+} amv_paged_batch;
+
+/* Bytes of one KV head's chunk of a page; -1 for a type, D or page size that is not supported. */
+int64_t amv_paged_chunk_bytes(int type, int64_t D, int64_t page_size);
+/* ROPE of the q and k heads of qkv f32 [n_tok][n_head + 2 n_head_kv][D] (rows qkv_stride floats apart), the rotated q to q_out
+ * f32 [n_tok][n_head][D] (both 16-byte aligned, strides multiples of 4), the rotated k and the v to the pages at their tokens' places, as F16, or as ggml's Q8_0 (`rule`) or
+ * Q4_0 of the f32 values. pos int32 [n_tok]: the rotation's positions (NULL: the places). mode 0 NORMAL or 2 NEOX, n_dims even,
+ * the rest of a head as it is. The angles pos * freq_scale * freq_base^(-2 i / n_dims), their sines and the rotation are
+ * computed in 64 bits and rounded once (amv_rope's are ggml's in 32, which have lost the angle of a far position). q_out rows are
+ * out_stride floats apart; q_out == qkv with out_stride == qkv_stride rotates q in place (k and v stay as they are in qkv). With
+ * bounds, those of the pages written to are brought up to date; a page's begin with its key 0. A token whose place is negative or
+ * from max_kv on, or whose page is outside the pool, is not stored, and adds 1 per KV head to *bad (device, may be NULL). Pages that a call writes
+ * belong to one of its sequences each. */
+int amv_paged_rope_append(const amv_paged_kv* kv, const amv_paged_batch* batch, const float* qkv, int64_t qkv_stride,
+                          int64_t n_head, const int32_t* pos, int n_dims, int mode, float freq_base, float freq_scale,
+                          float attn_factor, int rule, float* q_out, int64_t out_stride, unsigned int* bad, void* stream);
+/* Attention of the batch's tokens over their sequences' keys: out[t][h] = sum_j w_j v_j, w = softmax_j(scale * q[t][h] . k_j) over
+ * the keys the token sees, head h with KV head h / (n_head / n_head_kv). q f32 [n_tok][n_head][D] (rows q_stride floats apart,
+ * 16-byte aligned), out f32 [n_tok][n_head][D]; a token that sees no key gets zeros. q, the weights and the values meet in 32-bit
+ * arithmetic: q and the weights are given to the f16 matrix cores as two f16 each. workspace: amv_paged_attn_workspace_bytes
+ * (n_prefix and n_sel 0) bytes, 16-byte aligned. */
+int64_t amv_paged_attn_workspace_bytes(const amv_paged_kv* kv, const amv_paged_batch* batch, int64_t n_head,
+                                       int64_t n_prefix, int64_t n_sel);
+int amv_paged_attn(const amv_paged_kv* kv, const amv_paged_batch* batch, const float* q, int64_t q_stride, float* out,
+                   int64_t n_head, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+/* amv_paged_attn of sequences that all begin with the same n_prefix keys, those of the pages prefix_table (int32, device): every
+ * token sees them all, then its sequence's own keys as in amv_paged_attn (n_kv, the table and max_kv are the own keys'). The
+ * prefix is read once for all tokens rather than once for each sequence. */
+int amv_paged_attn_shared(const amv_paged_kv* kv, const amv_paged_batch* batch, const int32_t* prefix_table,
+                          int64_t n_prefix, const float* q, int64_t q_stride, float* out, int64_t n_head, float scale,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+/* The n_sel pages of its sequence that each token's attention is to read, for every KV head: sel int32 [n_tok][n_head_kv][n_sel],
+ * indices into the sequence's table in rising order, -1 behind the last where the token sees fewer pages. The first n_first and
+ * the last n_last pages that the token sees are taken (n_first + n_last <= n_sel), then those with the largest score, equal
+ * ones by the lower index: the sum over the KV head's query heads of the largest q . k that the page's bounds allow,
+ * sum_d (sum_h max(q_hd, 0)) high_d + (sum_h min(q_hd, 0)) low_d, computed in 64 bits. A score that is no number, and a page outside the pool, come last. The pool needs bounds; at most 16384 pages in
+ * max_kv. workspace: amv_paged_select_workspace_bytes bytes, 16-byte aligned. */
+int64_t amv_paged_select_workspace_bytes(const amv_paged_kv* kv, const amv_paged_batch* batch);
+int amv_paged_select(const amv_paged_kv* kv, const amv_paged_batch* batch, const float* q, int64_t q_stride,
+                     int64_t n_head, int64_t n_sel, int64_t n_first, int64_t n_last, int32_t* sel, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+/* amv_paged_attn over the selected pages only: sel as amv_paged_select writes it (or any choice of a sequence's pages, each once;
+ * entries outside the pages of max_kv are passed over). Keys a token does not see stay unseen. workspace:
+ * amv_paged_attn_workspace_bytes with n_sel. */
+int amv_paged_attn_sparse(const amv_paged_kv* kv, const amv_paged_batch* batch, const int32_t* sel, int64_t n_sel,
+                          const float* q, int64_t q_stride, float* out, int64_t n_head, float scale, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------
  * Glue ops of the decoder graph (ameva_binary.comp, ameva_cpy.comp, ameva_set_rows.comp, ameva_get_rows(_q).comp).
  * ---------------------------------------------------------------------------------------------------------- */
 /* ADD (op 0) / MUL (op 1), f32: dst[r][i] = a[r][i] op b[r % b_rows][i] for n_rows rows of n elements. */
