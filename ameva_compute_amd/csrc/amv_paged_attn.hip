@@ -26,6 +26,7 @@
 #include "amv_paged.h"
 
 #include <algorithm>
+#include <type_traits>
 
 typedef _Float16 pg_h8 __attribute__((ext_vector_type(8)));
 typedef float pg_f4 __attribute__((ext_vector_type(4)));
@@ -73,56 +74,88 @@ __device__ __forceinline__ void pg_load(uint32_t* to, const uint8_t* from) {  //
     }
 }
 
-// 32 keys of a wave, as they come from memory
-template <int TYPE, int D>
+// N bytes that no other instruction reads a part of the lines of: past the caches (64 sequences of 4096 f16 keys: 180 us, with the
+// values read so 162)
+template <int N>
+__device__ __forceinline__ void pg_load_once(uint32_t* to, const uint8_t* from) {
+    if constexpr (N == 16) {
+        const amv_v4u x = __builtin_nontemporal_load(reinterpret_cast<const amv_v4u*>(from));
+        to[0] = x.x;
+        to[1] = x.y;
+        to[2] = x.z;
+        to[3] = x.w;
+    } else {
+        typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+        const v2u x = __builtin_nontemporal_load(reinterpret_cast<const v2u*>(from));
+        to[0] = x.x;
+        to[1] = x.y;
+    }
+}
+
+// 32 keys of a wave, as they come from memory. KPL: scores a lane holds, of its keys 8 g + 4 u .. (u 0 where KPL is 8)
+template <int TYPE, int D, int KPL>
 struct PgK {
     static constexpr int NB = D / 32, W = TYPE == AMV_T_F16 ? 4 * NB : TYPE == AMV_T_Q8_0 ? 2 * NB : NB;
-    uint32_t k[2][W];                              // product u's key, the lane's elements
-    uint32_t s[TYPE == AMV_T_F16 ? 1 : 4 * NB];    // scales f16 [key 8 g + j][NB]
+    uint32_t k[2][W];                                  // product u's key, the lane's elements
+    uint32_t s[TYPE == AMV_T_F16 ? 1 : KPL * NB / 2];  // scales f16 [key][NB] of the lane's scores
 };
-template <int TYPE, int D>
+template <int TYPE, int D, int KPL>
 struct PgV {
     static constexpr int NB = D / 32, BYTES = TYPE == AMV_T_F16 ? D / 8 : TYPE == AMV_T_Q8_0 ? D / 16 : D / 32;
     static constexpr int W = BYTES < 4 ? 1 : BYTES / 4;
-    uint32_t v[8][W];                              // key 8 g + j, the lane's D / 16 elements
-    uint32_t s[TYPE == AMV_T_F16 ? 1 : 4 * NB];
+    uint32_t v[8][W];                                  // key 8 g + j, the lane's D / 16 elements
+    uint32_t s[TYPE == AMV_T_F16 ? 1 : KPL * NB / 2];
 };
-// where a wave's 32 keys are: the two halves' pages (the same one where a page holds 32 keys) and places
+// where a wave's 32 keys are, the same in every lane: their halves' places, bytes of their rows in the pool; e: the physical pages, -1
+// for no keys
 struct PgAt {
-    int e0, e1;      // physical pages; -1: no keys
-    int p0, p1;      // places of the halves' first keys
+    int e0, e1, p0, p1;
+};
+// a lane's parts of the addresses
+struct PgLane {
+    int k, v, s;   // of its K row and elements, its first V row and elements, its first scales
+    bool k1, v1;   // whether they are in the second half
 };
 
 template <int TYPE, int D>
-__device__ __forceinline__ void pg_load_k(PgK<TYPE, D>& t, const PgAttn& a, const uint8_t* kc, const PgAt& at, int c, int g) {
+__device__ __forceinline__ int64_t pg_off(const PgAttn& a, int e, int p, bool scales) {  // uniform
     using R = PgRow<TYPE, D>;
-    const int ps = 1 << a.b.pshift;
-    const int e = c >= 8 ? at.e1 : at.e0, row = ((c >= 8 ? at.p1 : at.p0) & (ps - 1)) + 8 * ((c >> 2) & 1) + (c & 3);
-    const uint8_t* p = kc + (int64_t)max(e, 0) * a.page_stride + (size_t)row * R::ROW;
+    const int row = p & ((1 << a.b.pshift) - 1);
+    return (int64_t)max(e, 0) * a.page_stride + (scales ? (int64_t)(R::ROW << a.b.pshift) + row * R::SC : (int64_t)row * R::ROW);
+}
+template <int TYPE, int D, int KPL>
+__device__ __forceinline__ void pg_load_k(PgK<TYPE, D, KPL>& t, const PgAttn& a, const uint8_t* kc, const PgAt& at, const PgLane& ln) {
+    using R = PgRow<TYPE, D>;
+    const int64_t o0 = pg_off<TYPE, D>(a, at.e0, at.p0, false), o1 = pg_off<TYPE, D>(a, at.e1, at.p1, false);
+    const uint8_t* p = kc + (ln.k1 ? o1 : o0) + ln.k;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         if constexpr (TYPE == AMV_T_F16) {
 #pragma unroll
-            for (int s = 0; s < R::NB; ++s) pg_load<16>(&t.k[u][4 * s], p + 4 * u * R::ROW + 64 * s + 16 * g);
+            for (int s = 0; s < R::NB; ++s) pg_load<16>(&t.k[u][4 * s], p + 4 * u * R::ROW + 64 * s);
         } else {
-            pg_load<R::ROW / 4>(t.k[u], p + 4 * u * R::ROW + g * (R::ROW / 4));
+            pg_load<R::ROW / 4>(t.k[u], p + 4 * u * R::ROW);
         }
     }
     if constexpr (TYPE != AMV_T_F16) {
-        const int eg = g >= 2 ? at.e1 : at.e0, rg = ((g >= 2 ? at.p1 : at.p0) & (ps - 1)) + 8 * (g & 1);
-        pg_load<8 * R::SC>(t.s, kc + (int64_t)max(eg, 0) * a.page_stride + (size_t)ps * R::ROW + (size_t)rg * R::SC);
+        const int64_t s0 = pg_off<TYPE, D>(a, at.e0, at.p0, true), s1 = pg_off<TYPE, D>(a, at.e1, at.p1, true);
+        pg_load<KPL * R::SC>(t.s, kc + (ln.v1 ? s1 : s0) + ln.s);
     }
 }
-template <int TYPE, int D>
-__device__ __forceinline__ void pg_load_v(PgV<TYPE, D>& t, const PgAttn& a, const uint8_t* vc, const PgAt& at, int c, int g) {
+template <int TYPE, int D, int KPL>
+__device__ __forceinline__ void pg_load_v(PgV<TYPE, D, KPL>& t, const PgAttn& a, const uint8_t* vc, const PgAt& at, const PgLane& ln) {
     using R = PgRow<TYPE, D>;
-    constexpr int B = PgV<TYPE, D>::BYTES;
-    const int ps = 1 << a.b.pshift;
-    const int e = g >= 2 ? at.e1 : at.e0, row = ((g >= 2 ? at.p1 : at.p0) & (ps - 1)) + 8 * (g & 1);
-    const uint8_t* base = vc + (int64_t)max(e, 0) * a.page_stride;
+    const int64_t o0 = pg_off<TYPE, D>(a, at.e0, at.p0, false), o1 = pg_off<TYPE, D>(a, at.e1, at.p1, false);
+    const uint8_t* p = vc + (ln.v1 ? o1 : o0) + ln.v;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) pg_load<B>(t.v[j], base + (size_t)(row + j) * R::ROW + B * c);
-    if constexpr (TYPE != AMV_T_F16) pg_load<8 * R::SC>(t.s, base + (size_t)ps * R::ROW + (size_t)row * R::SC);
+    for (int j = 0; j < 8; ++j) {
+        if constexpr (R::ROW >= 128) pg_load_once<PgV<TYPE, D, KPL>::BYTES>(t.v[j], p + j * R::ROW);
+        else pg_load<PgV<TYPE, D, KPL>::BYTES>(t.v[j], p + j * R::ROW);
+    }
+    if constexpr (TYPE != AMV_T_F16) {
+        const int64_t s0 = pg_off<TYPE, D>(a, at.e0, at.p0, true), s1 = pg_off<TYPE, D>(a, at.e1, at.p1, true);
+        pg_load<KPL * R::SC>(t.s, vc + (ln.v1 ? s1 : s0) + ln.s);
+    }
 }
 
 // integers u (value + 8 or + 128) in the low bits of a word's two halves, as f16 values times 2^-10: such a half is the f16 u 2^-24,
@@ -156,8 +189,8 @@ __device__ __forceinline__ pg_h8 pg_k_operand(const uint32_t* k, int s) {
     return __builtin_bit_cast(pg_h8, x);
 }
 // the operand of product t of V: element t of keys 0 .. 7
-template <int TYPE, int D>
-__device__ __forceinline__ pg_h8 pg_v_operand(const PgV<TYPE, D>& v, int t) {
+template <int TYPE, int D, int KPL>
+__device__ __forceinline__ pg_h8 pg_v_operand(const PgV<TYPE, D, KPL>& v, int t) {
     amv_v4u x;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
@@ -185,20 +218,33 @@ __device__ __forceinline__ void pg_split(const float (&x)[8], pg_h8& hi, pg_h8& 
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         hi[j] = (_Float16)x[j];
-        lo[j] = (_Float16)(x[j] - (float)hi[j]);
+        lo[j] = (_Float16)fmaf((float)hi[j], -1.0f, x[j]);
     }
 }
+// the f16 of a value (part 0) or the rest (part 1)
+__device__ __forceinline__ _Float16 pg_part(float x, float part) { return (_Float16)fmaf((float)(_Float16)x, -part, x); }
+template <int C>
+__device__ __forceinline__ float pg_dpp(float x) { return __int_as_float(amv_dpp_i<C>(__float_as_int(x))); }
+#define PG_ROR8 0x128        // lane c of a row of 16 and c ^ 8
+#define PG_HALF_MIRROR 0x141 // c and 7 - c (of its 8)
+#define PG_MIRROR 0x140      // c and 15 - c
 __device__ __forceinline__ pg_f4 pg_mfma(pg_h8 a, pg_h8 b, pg_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ float pg_half(const uint32_t* s, int i) { return amv_h2f(s[i >> 1] >> (16 * (i & 1))); }
 
-template <int TYPE, int D, int RT>
+template <int TYPE, int D, int RT, int P>
 __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
     using R = PgRow<TYPE, D>;
-    constexpr int NB = D / 32, T = D / 16;
+    constexpr int NB = D / 32, T = D / 16, ROWS = 16 / P, KPL = P == 4 ? 4 : 8;
     constexpr bool QUANT = TYPE != AMV_T_F16;
+    static_assert(P == 1 || RT == 1, "rows that share a product's columns are one tile");
     __shared__ float so[4][4][T][64];  // a row tile's O^T of the four waves, [wave][register][product][lane]
     __shared__ float sm[4][16 * RT], sl[4][16 * RT];
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    // what column c of the products is: row `col` of its tile, rounded (part 0) or the rest (part 1); u: whose keys it keeps
+    const int u = P == 4 ? c >> 3 : 0;
+    const bool rest = P == 4 ? (c & 4) != 0 : P == 2 && c >= 8;
+    const int col = P == 4 ? (rest ? 3 - (c & 3) : c & 3) : P == 2 ? (rest ? 15 - c : c) : c;
+    const float part = rest ? 1.0f : 0.0f;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hk = (int)blockIdx.x % a.n_head_kv, tile = (int)blockIdx.x / a.n_head_kv, z = blockIdx.y;
     const int psh = a.b.pshift, ps = 1 << psh;
@@ -211,7 +257,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
     int64_t part0 = -1;  // PG_ONE: where the rows of the sequence are in ml
     if (a.kind == PG_PREFIX) {
         tok0 = 0;
-        r0 = tile * 16 * RT;
+        r0 = tile * ROWS * RT;
         n_rows = a.b.n_tok * a.G;
         keys = a.n_list;
         place0 = keys;  // (every row sees them all)
@@ -228,7 +274,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
         } else {
             pg_find(a.b.n_seq, tile, [&](int q) {
                 const int r = (a.b.last(q) - a.b.first(q)) * a.G;
-                return r > a.rows_most ? (r + 16 * RT - 1) / (16 * RT) : 0;
+                return r > a.rows_most ? (r + ROWS * RT - 1) / (ROWS * RT) : 0;
             }, s, in);
         }
         if (s >= a.b.n_seq) return;
@@ -245,12 +291,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
             n_rows = n_q * a.G;
             if (a.kind == PG_ONE && n_rows > a.rows_most) return;
             if (a.kind == PG_ONE) part0 = ((int64_t)s * a.n_head_kv + hk) * a.rows_most;
-            if (a.kind == PG_FIND) in = (n_rows + 16 * RT - 1) / (16 * RT) - 1 - in;  // the rows with the most keys first
+            if (a.kind == PG_FIND) in = (n_rows + ROWS * RT - 1) / (ROWS * RT) - 1 - in;  // the rows with the most keys first
         }
-        r0 = in * 16 * RT;
+        r0 = in * ROWS * RT;
         if (r0 >= n_rows) return;
     }
-    const int r_last = min(r0 + 16 * RT, n_rows) - 1;
+    const int r_last = min(r0 + ROWS * RT, n_rows) - 1;
     // keys that every row of the tile sees, and the last that any does
     int see_all = keys, see_any = keys;
     if (a.kind != PG_PREFIX) {
@@ -292,34 +338,38 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
 
     const size_t chunk = (size_t)ps * (R::ROW + R::SC);
     const uint8_t *kc = a.k + hk * chunk, *vc = a.v + hk * chunk;
-    PgK<TYPE, D> tk;
-    PgV<TYPE, D> tv;
+    PgK<TYPE, D, KPL> tk;
+    PgV<TYPE, D, KPL> tv;
+    const PgLane ln = {(8 * ((c >> 2) & 1) + (c & 3)) * R::ROW + (QUANT ? g * (R::ROW / 4) : 16 * g),
+                       8 * (g & 1) * R::ROW + PgV<TYPE, D, KPL>::BYTES * c, (8 * (g & 1) + 4 * u) * R::SC, c >= 8, g >= 2};
     PgAt at = {-1, -1, 0, 0};
-    const int i_last = end - 1 - ((end - 1 - i) & 3);  // the wave's last tile
     if (i < end) {
         at = where(i);
-        pg_load_k(tk, a, kc, at, c, g);
-        pg_load_v(tv, a, vc, at, c, g);
+        pg_load_k(tk, a, kc, at, ln);
+        pg_load_v(tv, a, vc, at, ln);
     }
 
-    // Q^T operands; row c of tile rt: values times scale log2(e) 2^-e below 2, in two f16. f: 2^e (for quantized keys times the
-    // 2^10 that their operands lack); lim: keys the row sees
-    pg_h8 qh[RT][NB], ql[RT][NB];
+    // Q^T operands: values times scale log2(e) 2^-e below 2, P = 1: as f16 and the rest in two operands, P = 2: in the two halves of
+    // the columns of one, P = 4 and quantized keys: of two, one for each product u, that is 0 where the columns keep the other's keys,
+    // so that the products add up to what each column keeps (f16 keys may be infinite or no number where nobody sees them: 0 times
+    // them would not be 0, so there each column picks its product). f: 2^e (for quantized keys times the 2^10 that their operands
+    // lack); lim: keys the row sees
+    pg_h8 qa[RT][P == 2 || (P == 4 && !QUANT) ? 1 : 2][NB];
     float f[RT];
     int lim[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int r = min(r0 + 16 * rt + c, r_last), t = r / a.G;
+        const int r = min(r0 + 16 * rt + col, r_last), t = r / a.G;
         lim[rt] = a.kind == PG_PREFIX ? keys : min(keys, place0 + t + 1);
         const float* src = a.q + (tok0 + t) * a.q_stride + (int64_t)(hk * a.G + r - t * a.G) * D + 8 * g;
         float x[NB][8], am = 0.0f;
 #pragma unroll
         for (int s = 0; s < NB; ++s) {
-            const float4 u = *reinterpret_cast<const float4*>(src + 32 * s), v = *reinterpret_cast<const float4*>(src + 32 * s + 4);
-            const float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+            const float4 y = *reinterpret_cast<const float4*>(src + 32 * s), z = *reinterpret_cast<const float4*>(src + 32 * s + 4);
+            const float yz[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[s][j] = y[j] * a.scale2;
+                x[s][j] = yz[j] * a.scale2;
                 am = fmaxf(am, fabsf(x[s][j]));
             }
         }
@@ -331,7 +381,21 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
         for (int s = 0; s < NB; ++s) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[s][j] *= down;
-            pg_split(x[s], qh[rt][s], ql[rt][s]);
+            if constexpr (P == 1) {
+                pg_split(x[s], qa[rt][0][s], qa[rt][1][s]);
+            } else {
+                pg_h8 h;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[j] = pg_part(x[s][j], part);
+                if constexpr (P == 2 || !QUANT) {
+                    qa[rt][0][s] = h;
+                } else {
+                    const amv_v4u hw = __builtin_bit_cast(amv_v4u, h);
+                    const uint32_t k0 = u ? 0u : 0xFFFFFFFFu;
+                    qa[rt][0][s] = __builtin_bit_cast(pg_h8, hw & k0);
+                    qa[rt][1][s] = __builtin_bit_cast(pg_h8, hw & ~k0);
+                }
+            }
         }
         if constexpr (QUANT) f[rt] *= 1024.0f;
     }
@@ -347,52 +411,58 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
     }
     float vref = 0.0f, vdown = 0.0f;  // the power of two that values' scales are held below, its inverse
 
-    for (; i < end; i += 4) {
+    // one tile, with the wave's next one on its way into the registers as they fall free (`more`: there is one. The last tile has
+    // its own copy of this code: to load it again instead cost a tenth of the time of a wave of 8 tiles)
+    const auto step = [&](auto more) {
         const PgAt now = at;
-        at = where(min(i + 4, i_last));
-        // scores of the lane's keys 8 g + j, j = 4 u + register
-        float s[RT][8];
-        if constexpr (!QUANT) {
-            pg_f4 x[RT][2];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) x[rt][0] = x[rt][1] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const pg_h8 kf = pg_k_operand<TYPE, D>(tk.k[u], b);
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        x[rt][u] = pg_mfma(kf, ql[rt][b], x[rt][u]);
-                        x[rt][u] = pg_mfma(kf, qh[rt][b], x[rt][u]);
-                    }
-                }
+        if constexpr (more()) at = where(i + 4);
+        // scores of the lane's keys 8 g + 4 u + j
+        float s[RT][KPL];
+        if constexpr (QUANT) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) s[rt][j] = x[rt][j >> 2][j & 3];
-        } else {
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) s[rt][j] = 0.0f;
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const pg_h8 kf = pg_k_operand<TYPE, D>(tk.k[u], b);
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        pg_f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-                        x = pg_mfma(kf, ql[rt][b], x);
-                        x = pg_mfma(kf, qh[rt][b], x);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            s[rt][4 * u + r] = fmaf(x[r], pg_half(tk.s, (4 * u + r) * NB + b), s[rt][4 * u + r]);
-                    }
-                }
+                for (int j = 0; j < KPL; ++j) s[rt][j] = 0.0f;
         }
-        pg_load_k(tk, a, kc, at, c, g);
+        constexpr int X = P == 4 && QUANT ? 1 : 2;
+        pg_f4 x[RT][X];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (QUANT || b == 0) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int h = 0; h < X; ++h) x[rt][h] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const pg_h8 kf = pg_k_operand<TYPE, D>(tk.k[h], b);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    if constexpr (P == 4 && QUANT) {
+                        x[rt][0] = pg_mfma(kf, qa[rt][h][b], x[rt][0]);
+                    } else {
+                        if constexpr (P == 1) x[rt][h] = pg_mfma(kf, qa[rt][1][b], x[rt][h]);
+                        x[rt][h] = pg_mfma(kf, qa[rt][0][b], x[rt][h]);
+                    }
+                }
+            }
+            if constexpr (QUANT) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int j = 0; j < KPL; ++j) s[rt][j] = fmaf(x[rt][j >> 2][j & 3], pg_half(tk.s, j * NB + b), s[rt][j]);
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int j = 0; j < KPL; ++j) {
+                if constexpr (!QUANT) s[rt][j] = P == 4 ? (u ? x[rt][1][j & 3] : x[rt][0][j & 3]) : x[rt][j >> 2][j & 3];
+                if constexpr (P == 2) s[rt][j] += pg_dpp<PG_MIRROR>(s[rt][j]);  // the rounded q's and the rest's
+                if constexpr (P == 4) s[rt][j] += pg_dpp<PG_HALF_MIRROR>(s[rt][j]);
+            }
+        if constexpr (more()) pg_load_k(tk, a, kc, at, ln);
         // keys that are not there, or not seen by every row
         const int p = (g >= 2 ? now.p1 : now.p0) + 8 * (g & 1);
         const bool there = (g >= 2 ? now.e1 : now.e0) >= 0;
@@ -401,13 +471,17 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) s[rt][j] = there && p + j < lim[rt] ? s[rt][j] : -INFINITY;
+                for (int j = 0; j < KPL; ++j) s[rt][j] = there && p + 4 * u + j < lim[rt] ? s[rt][j] : -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {  // what lies there must not matter, 0 times infinity is no number
                 const uint32_t keep = there && p + j < keys ? 0xFFFFFFFFu : 0u;
 #pragma unroll
-                for (int x = 0; x < PgV<TYPE, D>::W; ++x) tv.v[j][x] &= keep;
-                if constexpr (QUANT) {
+                for (int x = 0; x < PgV<TYPE, D, KPL>::W; ++x) tv.v[j][x] &= keep;
+            }
+            if constexpr (QUANT) {
+#pragma unroll
+                for (int j = 0; j < KPL; ++j) {
+                    const uint32_t keep = there && p + 4 * u + j < keys ? 0xFFFFFFFFu : 0u;
 #pragma unroll
                     for (int b = 0; b < NB; b += 2) tv.s[(j * NB + b) >> 1] &= keep;
                 }
@@ -416,9 +490,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
         if constexpr (QUANT) {  // the values' largest scale
             amv_h2 big = {(_Float16)0.0f, (_Float16)0.0f};
 #pragma unroll
-            for (int x = 0; x < 4 * NB; ++x)
+            for (int x = 0; x < KPL * NB / 2; ++x)
                 big = __builtin_elementwise_max(big, __builtin_bit_cast(amv_h2, tv.s[x] & 0x7FFF7FFFu));
-            const float top = amv_max_x32(amv_max_x16(fmaxf((float)big.x, (float)big.y)));
+            float top = amv_max_x32(amv_max_x16(fmaxf((float)big.x, (float)big.y)));
+            if constexpr (P == 4) top = fmaxf(top, pg_dpp<PG_ROR8>(top));
             if (__builtin_amdgcn_readfirstlane(top > vref)) {
                 const uint32_t e = min(253u, (__float_as_uint(top) >> 23) + 1u);
                 const float up = __uint_as_float(e << 23), by = vref * __uint_as_float((254u - e) << 23);
@@ -430,13 +505,31 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
                     for (int t = 0; t < T; ++t) o[rt][t] *= by;
             }
         }
-        pg_h8 ph[RT], pl[RT];
-        float pw[RT][8];
+        pg_h8 ph[RT], pl[RT];  // P^T operands: the weights and their rest, or (P > 1) both in one
+        float pw[RT][KPL];
+        const auto operand = [&](int rt, const float (&y)[KPL]) {
+            if constexpr (P == 1) {
+                pg_split(y, ph[rt], pl[rt]);
+            } else if constexpr (P == 2) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ph[rt][j] = pg_part(y[j], part);
+            } else {  // columns c and c ^ 8 have the same row's keys of product 0 and of 1: each takes the other's
+                amv_v4u o4;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int mine = (int)pg_bits(amv_h2{pg_part(y[2 * h], part), pg_part(y[2 * h + 1], part)});
+                    o4[h] = (uint32_t)__builtin_amdgcn_update_dpp(mine, mine, PG_ROR8, 0xF, 0xC, false);
+                    o4[2 + h] = (uint32_t)__builtin_amdgcn_update_dpp(mine, mine, PG_ROR8, 0xF, 0x3, false);
+                }
+                ph[rt] = __builtin_bit_cast(pg_h8, o4);
+            }
+        };
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             float mx = s[rt][0];
 #pragma unroll
-            for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[rt][j]);
+            for (int j = 1; j < KPL; ++j) mx = fmaxf(mx, s[rt][j]);
+            if constexpr (P == 4) mx = fmaxf(mx, pg_dpp<PG_ROR8>(mx));
             mx = amv_max_x32(amv_max_x16(mx)) * f[rt];  // (f a power of two: exact)
             // the reference moves when a weight would pass 2^15 (or there is none yet), to 2^-12 of the maximum; where no difference
             // of 12 is exact, to the maximum
@@ -452,12 +545,17 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
             const float ref = m[rt] == -INFINITY ? 0.0f : m[rt];
             float sum = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < KPL; ++j) {
                 pw[rt][j] = __builtin_amdgcn_exp2f(fmaf(s[rt][j], f[rt], -ref));
                 sum += pw[rt][j];
             }
             l[rt] += sum;
-            if constexpr (!QUANT) pg_split(pw[rt], ph[rt], pl[rt]);
+            if constexpr (QUANT) {
+#pragma unroll
+                for (int j = 0; j < KPL; ++j) pw[rt][j] *= vdown;
+            } else {
+                operand(rt, pw[rt]);
+            }
         }
 #pragma unroll
         for (int t = 0; t < T; ++t) {
@@ -466,31 +564,34 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
                 if ((t & 1) == 0) {  // products 2 b and 2 b + 1 are block b
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) {
-                        float y[8];
+                        float y[KPL];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            y[j] = pw[rt][j] * (pg_half(tv.s, j * NB + (t >> 1)) * vdown);
+                        for (int j = 0; j < KPL; ++j) {
+                            y[j] = pw[rt][j] * pg_half(tv.s, j * NB + (t >> 1));
                             // The compiler would round the unrounded product to f16 (v_fma_mixlo_f16) but take the rest from the
                             // f16 of the rounded one; where the two differ, next to a tie, the parts do not sum to y.
                             asm("" : "+v"(y[j]));
                         }
-                        pg_split(y, ph[rt], pl[rt]);
+                        operand(rt, y);
                     }
                 }
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                o[rt][t] = pg_mfma(vf, pl[rt], o[rt][t]);
+                if constexpr (P == 1) o[rt][t] = pg_mfma(vf, pl[rt], o[rt][t]);
                 o[rt][t] = pg_mfma(vf, ph[rt], o[rt][t]);
             }
         }
-        pg_load_v(tv, a, vc, at, c, g);
-    }
+        if constexpr (more()) pg_load_v(tv, a, vc, at, ln);
+    };
+    for (; i + 4 < end; i += 4) step(std::true_type{});
+    if (i < end) step(std::false_type{});
 
     // the waves' parts together. Lane (c, g) of wave w takes register w of every product: elements of row c that lie side by side
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float lt = amv_sum_x32(amv_sum_x16(l[rt]));
+        float lt = amv_sum_x32(amv_sum_x16(l[rt]));
+        if constexpr (P == 4) lt += pg_dpp<PG_ROR8>(lt);
         if (g == 0) {
             sm[w][16 * rt + c] = m[rt];
             sl[w][16 * rt + c] = lt;
@@ -503,7 +604,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int t = 0; t < T; ++t) so[w][r][t][lane] = o[rt][t][r] * back;
+            for (int t = 0; t < T; ++t) {
+                float y = o[rt][t][r];
+                if constexpr (P == 2) y += pg_dpp<PG_MIRROR>(y);  // (lanes of part 0 end with their row's)
+                if constexpr (P == 4) y += pg_dpp<PG_HALF_MIRROR>(y);
+                so[w][r][t][lane] = y * back;
+            }
         __syncthreads();
         const int r = r0 + 16 * rt + c;
         float M = -INFINITY, L = 0.0f, x[T];
@@ -518,7 +624,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
 #pragma unroll
             for (int t = 0; t < T; ++t) x[t] = fmaf(so[j][w][t][lane], by, x[t]);
         }
-        if (r < n_rows) {
+        if (r < n_rows && c < ROWS) {
             const int tr = r / a.G;
             const int64_t row = (int64_t)(tok0 + tr) * a.n_head + hk * a.G + (r - tr * a.G);
             float* to = a.out + row * D;
@@ -610,20 +716,31 @@ __global__ __launch_bounds__(256) void k_paged_merge(PgMerge a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
+// Row tiles of a launch: rt times 16 rows, or 16 / pack of them where rows are few: the products' 16 columns then hold the two f16 of
+// every row side by side, and with pack 4 the two products' keys too, so that each lane's scores are of use to half the lanes
+// rather than an eighth.
+struct PgTiles {
+    int rt, pack;
+    int rows() const { return 16 * rt / pack; }
+    int of(int64_t n) const { return (int)((n + rows() - 1) / rows()); }
+};
+static PgTiles pg_tiles(int64_t rows) { return {rows > 16 ? 2 : 1, rows <= 4 ? 4 : rows <= 8 ? 2 : 1}; }
 // How a call is launched: up to two launches over the sequences' own keys and one over the prefix, and the workspace of the parts.
 struct PgPlan {
-    int rt_one, ta, n_one, len_one;         // sequences (or listed tokens) of few rows: row tiles of 16 rt_one, ta each; parts
+    PgTiles one, pre;                       // sequences (or listed tokens) of few rows, ta tiles each; the prefix's
+    int ta, n_one, len_one;                 // their parts
     int find, rows_most, n_find, len_find;  // sequences of more rows than rows_most, tiles of 32
     int64_t find_tiles;
     int n_pre, len_pre;                     // parts of the prefix
-    int64_t one, many, pre;                 // parts in the workspace
-    int64_t bytes(int64_t D) const { return (one + many + pre) * (8 + 4 * D); }
+    int64_t w_one, w_many, w_pre;           // parts in the workspace
+    int64_t bytes(int64_t D) const { return (w_one + w_many + w_pre) * (8 + 4 * D); }
 };
-// parts of `keys` keys for `units` workgroups' worth of rows: enough workgroups for two a CU twice over (1024: a range's last waves
-// then wait for few others), none of less than 256 keys (two tiles for each of its waves)
+// parts of `keys` keys for `units` workgroups' worth of rows: two workgroups a CU, none of less than 128 keys (a tile for each of its
+// waves). More and shorter parts cost their prologues and the merge (us at 512 / 1024 / 2048 workgroups: 64 sequences of up to 4096
+// f16 keys 136 / 147 / 144, 3 of 65536 Q8_0 keys 78 / 78 / 82, one of 777 with parts of 256 keys 9.6, of 128 9.3)
 static int pg_parts(int64_t units, int64_t keys, int* len) {
     units = std::max<int64_t>(1, units);
-    const int64_t n = std::max<int64_t>(1, std::min<int64_t>((1024 + units - 1) / units, (keys + 255) / 256));
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>(512 / units, (keys + 127) / 128));
     int64_t l = ((keys + n - 1) / n + 127) / 128 * 128;
     l = std::max<int64_t>(128, l);
     *len = (int)l;
@@ -633,26 +750,27 @@ static PgPlan pg_plan(const amv_paged_kv* kv, const amv_paged_batch* b, int64_t 
     PgPlan p = {};
     const int64_t G = n_head / kv->n_head_kv;
     if (n_sel > 0) {
-        p.rt_one = G > 16 ? 2 : 1;
-        p.ta = (int)((G + 16 * p.rt_one - 1) / (16 * p.rt_one));
+        p.one = pg_tiles(G);
+        p.ta = p.one.of(G);
         p.n_one = pg_parts(b->n_tok * kv->n_head_kv * p.ta, n_sel * kv->page_size, &p.len_one);
-        if (p.n_one > 1) p.many = b->n_tok * n_head * p.n_one;
+        if (p.n_one > 1) p.w_many = b->n_tok * n_head * p.n_one;
         return p;
     }
     const int64_t rows = std::min(b->max_q, b->n_tok) * G;
-    p.rt_one = rows > 16 && (rows <= 32 || G > 16) ? 2 : 1;
-    p.rows_most = (int)std::max<int64_t>(16 * p.rt_one, G);
-    p.ta = (int)((p.rows_most + 16 * p.rt_one - 1) / (16 * p.rt_one));
+    p.one = pg_tiles(rows <= 32 ? rows : G);
+    p.rows_most = (int)std::max<int64_t>(p.one.rows(), G);
+    p.ta = p.one.of(p.rows_most);
     p.n_one = pg_parts(b->n_seq * kv->n_head_kv * p.ta, b->max_kv, &p.len_one);
     p.find = rows > p.rows_most;
     if (p.find) {
         p.find_tiles = b->n_tok * G / 32 + b->n_seq;
         p.n_find = pg_parts(b->n_tok * G / 32 * kv->n_head_kv + 1, b->max_kv, &p.len_find);
     }
-    if (n_prefix > 0) p.n_pre = pg_parts((b->n_tok * G + 31) / 32 * kv->n_head_kv, n_prefix, &p.len_pre);
-    if (p.n_one > 1 || p.n_pre) p.one = b->n_seq * kv->n_head_kv * p.rows_most * p.n_one;
-    if (p.find && (p.n_find > 1 || p.n_pre)) p.many = b->n_tok * n_head * p.n_find;
-    p.pre = b->n_tok * n_head * p.n_pre;
+    p.pre = pg_tiles(b->n_tok * G);
+    if (n_prefix > 0) p.n_pre = pg_parts(p.pre.of(b->n_tok * G) * kv->n_head_kv, n_prefix, &p.len_pre);
+    if (p.n_one > 1 || p.n_pre) p.w_one = b->n_seq * kv->n_head_kv * p.rows_most * p.n_one;
+    if (p.find && (p.n_find > 1 || p.n_pre)) p.w_many = b->n_tok * n_head * p.n_find;
+    p.w_pre = b->n_tok * n_head * p.n_pre;
     return p;
 }
 
@@ -663,20 +781,22 @@ extern "C" int64_t amv_paged_attn_workspace_bytes(const amv_paged_kv* kv, const 
 }
 
 template <int TYPE, int D>
-static void pg_launch(const PgAttn& a, int rt, int64_t tiles, int parts, hipStream_t st) {
+static void pg_launch(const PgAttn& a, PgTiles t, int64_t tiles, int parts, hipStream_t st) {
     const dim3 grid((unsigned)(tiles * a.n_head_kv), (unsigned)parts);
-    if (rt == 1) hipLaunchKernelGGL((k_paged_attn<TYPE, D, 1>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_paged_attn<TYPE, D, 2>), grid, dim3(256), 0, st, a);
+    if (t.pack == 4) hipLaunchKernelGGL((k_paged_attn<TYPE, D, 1, 4>), grid, dim3(256), 0, st, a);
+    else if (t.pack == 2) hipLaunchKernelGGL((k_paged_attn<TYPE, D, 1, 2>), grid, dim3(256), 0, st, a);
+    else if (t.rt == 1) hipLaunchKernelGGL((k_paged_attn<TYPE, D, 1, 1>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_paged_attn<TYPE, D, 2, 1>), grid, dim3(256), 0, st, a);
 }
-static void pg_launch(int type, int D, const PgAttn& a, int rt, int64_t tiles, int parts, hipStream_t st) {
+static void pg_launch(int type, int D, const PgAttn& a, PgTiles t, int64_t tiles, int parts, hipStream_t st) {
     if (D == 128) {
-        if (type == AMV_T_F16) pg_launch<AMV_T_F16, 128>(a, rt, tiles, parts, st);
-        else if (type == AMV_T_Q8_0) pg_launch<AMV_T_Q8_0, 128>(a, rt, tiles, parts, st);
-        else pg_launch<AMV_T_Q4_0, 128>(a, rt, tiles, parts, st);
+        if (type == AMV_T_F16) pg_launch<AMV_T_F16, 128>(a, t, tiles, parts, st);
+        else if (type == AMV_T_Q8_0) pg_launch<AMV_T_Q8_0, 128>(a, t, tiles, parts, st);
+        else pg_launch<AMV_T_Q4_0, 128>(a, t, tiles, parts, st);
     } else {
-        if (type == AMV_T_F16) pg_launch<AMV_T_F16, 64>(a, rt, tiles, parts, st);
-        else if (type == AMV_T_Q8_0) pg_launch<AMV_T_Q8_0, 64>(a, rt, tiles, parts, st);
-        else pg_launch<AMV_T_Q4_0, 64>(a, rt, tiles, parts, st);
+        if (type == AMV_T_F16) pg_launch<AMV_T_F16, 64>(a, t, tiles, parts, st);
+        else if (type == AMV_T_Q8_0) pg_launch<AMV_T_Q8_0, 64>(a, t, tiles, parts, st);
+        else pg_launch<AMV_T_Q4_0, 64>(a, t, tiles, parts, st);
     }
 }
 
@@ -708,10 +828,10 @@ static int pg_attn(const char* what, const amv_paged_kv* kv, const amv_paged_bat
     a.list = list;
     // workspace: the weighted values of the parts of own keys (by sequence, by row) and of the prefix, then their (m, l)
     float* const acc = (float*)workspace;
-    float2* const ml = (float2*)(acc + (p.one + p.many + p.pre) * kv->D);
-    PgMerge m = {a.b, {ml, acc, p.one ? p.n_one : 0},
-                 {ml + p.one, acc + p.one * kv->D, p.many ? (n_sel > 0 ? p.n_one : p.n_find) : 0},
-                 {ml + p.one + p.many, acc + (p.one + p.many) * kv->D, p.n_pre},
+    float2* const ml = (float2*)(acc + (p.w_one + p.w_many + p.w_pre) * kv->D);
+    PgMerge m = {a.b, {ml, acc, p.w_one ? p.n_one : 0},
+                 {ml + p.w_one, acc + p.w_one * kv->D, p.w_many ? (n_sel > 0 ? p.n_one : p.n_find) : 0},
+                 {ml + p.w_one + p.w_many, acc + (p.w_one + p.w_many) * kv->D, p.n_pre},
                  out, (int)n_head, kv->n_head_kv, a.G, n_sel > 0 ? -1 : p.rows_most};
     const auto into = [&](const PgParts& parts) {
         a.ml = parts.n ? const_cast<float2*>(parts.ml) : nullptr;
@@ -724,8 +844,7 @@ static int pg_attn(const char* what, const amv_paged_kv* kv, const amv_paged_bat
         a.n_split = p.n_pre;
         a.split_len = p.len_pre;
         into(m.pre);
-        const int rt = b->n_tok * a.G > 16 ? 2 : 1;
-        pg_launch(kv->type, kv->D, a, rt, (b->n_tok * a.G + 16 * rt - 1) / (16 * rt), p.n_pre, st);
+        pg_launch(kv->type, kv->D, a, p.pre, p.pre.of(b->n_tok * a.G), p.n_pre, st);
     }
     if (p.find) {
         a.kind = PG_FIND;
@@ -733,7 +852,7 @@ static int pg_attn(const char* what, const amv_paged_kv* kv, const amv_paged_bat
         a.n_split = p.n_find;
         a.split_len = p.len_find;
         into(m.many);
-        pg_launch(kv->type, kv->D, a, 2, p.find_tiles, p.n_find, st);
+        pg_launch(kv->type, kv->D, a, PgTiles{2, 1}, p.find_tiles, p.n_find, st);
     }
     a.kind = n_sel > 0 ? PG_LIST : PG_ONE;
     a.n_list = (int)n_sel;
@@ -742,8 +861,8 @@ static int pg_attn(const char* what, const amv_paged_kv* kv, const amv_paged_bat
     a.n_split = p.n_one;
     a.split_len = p.len_one;
     into(n_sel > 0 ? m.many : m.one);
-    pg_launch(kv->type, kv->D, a, p.rt_one, (n_sel > 0 ? b->n_tok : b->n_seq) * p.ta, p.n_one, st);
-    if (p.one + p.many + p.pre) {
+    pg_launch(kv->type, kv->D, a, p.one, (n_sel > 0 ? b->n_tok : b->n_seq) * p.ta, p.n_one, st);
+    if (p.w_one + p.w_many + p.w_pre) {
         const dim3 grid((unsigned)((rows + 3) / 4));
         if (kv->D == 128) hipLaunchKernelGGL(k_paged_merge<128>, grid, dim3(256), 0, st, m);
         else hipLaunchKernelGGL(k_paged_merge<64>, grid, dim3(256), 0, st, m);

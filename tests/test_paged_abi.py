@@ -121,7 +121,7 @@ def test_sizes():
     assert [w(*refs(kv(), empty), 8, *a) for a in ((0, 0), (0, 5))] == [0, 0] and w(*refs(kv(), batch(n_tok=0, cu_q=A, max_kv=0)), 8, 9, 0) >= 0
     assert lib().amv_paged_select_workspace_bytes(*refs(kv(), empty)) == 0
     # parts of a prefix need room for every row, and the own keys' with them
-    assert w(*refs(kv(), batch()), 8, 20, 0) == (3 * 8 + 3 * 2 * 16) * (8 + 512)
+    assert w(*refs(kv(), batch()), 8, 20, 0) >= 2 * 3 * 8 * (8 + 512)
 
 
 def test_python_side():
