@@ -46,7 +46,7 @@ struct PgAttn {
     int ta;            // row tiles of a sequence (PG_ONE) or a token (PG_LIST)
     int rows_most;     // PG_ONE: sequences of at most, PG_FIND: of more than so many rows
     int n_list;        // selected pages, or the prefix's keys
-    int n_split, split_len;  // parts (blockIdx.y) of the keys and their length
+    int tiles, n_split, split_len;  // row tiles (of one KV head), parts of their keys and the parts' length
 };
 enum { PG_ONE, PG_FIND, PG_PREFIX, PG_LIST };
 
@@ -231,13 +231,152 @@ __device__ __forceinline__ float pg_dpp(float x) { return __int_as_float(amv_dpp
 __device__ __forceinline__ pg_f4 pg_mfma(pg_h8 a, pg_h8 b, pg_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ float pg_half(const uint32_t* s, int i) { return amv_h2f(s[i >> 1] >> (16 * (i & 1))); }
 
+// A tile's rows: rows r0 .. r_last of the n_rows of tokens tok0 .., row r is head r % G of token tok0 + r / G, whose place is place0 +
+// r / G; keys: how many there are to see, see_all: that each of the rows sees, see_any: that any does
+struct PgRows {
+    int tok0, r0, r_last, n_rows, place0, keys, see_all, see_any;
+    const int32_t* pages;  // the physical pages, or the sequence's table where `list` says which
+    const int32_t* list;
+    int64_t part0;         // PG_ONE: where the rows of the sequence are in ml; else -1
+    __device__ void see(const PgAttn& a, int from, int to) {
+        r0 = from;
+        r_last = to;
+        see_all = see_any = keys;
+        if (a.kind != PG_PREFIX) {
+            see_all = min(keys, place0 + r0 / a.G + 1);
+            see_any = min(keys, place0 + r_last / a.G + 1);
+        }
+    }
+};
+// the rows of tile `tile` of `rows` rows; false where there are none (the same for the whole workgroup)
+__device__ __forceinline__ bool pg_rows(const PgAttn& a, int hk, int tile, int rows, PgRows& t) {
+    t.list = nullptr;
+    t.part0 = -1;
+    int in = tile;
+    if (a.kind == PG_PREFIX) {
+        t.tok0 = 0;
+        t.n_rows = a.b.n_tok * a.G;
+        t.keys = t.place0 = a.n_list;
+        t.pages = a.list;
+    } else {
+        int s;
+        if (a.kind == PG_LIST) {
+            t.tok0 = tile / a.ta;
+            in = tile % a.ta;
+            s = pg_seq_of(a.b, t.tok0);
+        } else if (a.kind == PG_ONE) {
+            s = tile / a.ta;
+            in = tile % a.ta;
+        } else {
+            pg_find(a.b.n_seq, tile, [&](int q) {
+                const int r = (a.b.last(q) - a.b.first(q)) * a.G;
+                return r > a.rows_most ? (r + rows - 1) / rows : 0;
+            }, s, in);
+        }
+        if (s >= a.b.n_seq) return false;
+        const int first = a.b.first(s), n_q = a.b.last(s) - first;
+        t.place0 = a.b.end(s) - n_q;
+        t.keys = a.b.keys(s);
+        t.pages = a.b.table + s * a.b.table_stride;
+        if (a.kind == PG_LIST) {
+            t.place0 += t.tok0 - first;
+            t.n_rows = a.G;
+            t.list = a.list + ((int64_t)t.tok0 * a.n_head_kv + hk) * a.n_list;
+        } else {
+            t.tok0 = first;
+            t.n_rows = n_q * a.G;
+            if (a.kind == PG_ONE && t.n_rows > a.rows_most) return false;
+            if (a.kind == PG_ONE) t.part0 = ((int64_t)s * a.n_head_kv + hk) * a.rows_most;
+            if (a.kind == PG_FIND) in = (t.n_rows + rows - 1) / rows - 1 - in;  // the rows with the most keys first
+        }
+    }
+    if (in * rows >= t.n_rows) return false;
+    t.see(a, in * rows, min(in * rows + rows, t.n_rows) - 1);
+    return true;
+}
+// where keys 32 i .. 32 i + 31 are (i: uniform over the wave)
+__device__ __forceinline__ PgAt pg_where(const PgAttn& a, const int32_t* pages, int keys, int i) {
+    PgAt at;
+    at.p0 = i * 32;
+    at.p1 = at.p0 + 16;
+    at.e0 = pages[at.p0 >> a.b.pshift];
+    at.e1 = at.p1 < keys ? pages[at.p1 >> a.b.pshift] : -1;
+    if ((uint32_t)at.e0 >= (uint32_t)a.n_pages) at.e0 = -1;
+    if ((uint32_t)at.e1 >= (uint32_t)a.n_pages) at.e1 = -1;
+    return at;
+}
+// elements 32 s + 8 g .. of row r of a tile, times scale log2(e) 2^-e below 2; returns 2^e
+template <int D>
+__device__ __forceinline__ float pg_query(const PgAttn& a, const PgRows& t, int hk, int r, int g, float (&x)[D / 32][8]) {
+    const int tr = r / a.G;
+    const float* src = a.q + (t.tok0 + tr) * a.q_stride + (int64_t)(hk * a.G + r - tr * a.G) * D + 8 * g;
+    float am = 0.0f;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+        const float4 y = *reinterpret_cast<const float4*>(src + 32 * s), z = *reinterpret_cast<const float4*>(src + 32 * s + 4);
+        const float yz[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[s][j] = yz[j] * a.scale2;
+            am = fmaxf(am, fabsf(x[s][j]));
+        }
+    }
+    am = amv_max_x32(amv_max_x16(am));
+    const uint32_t e = max(1u, min(253u, __float_as_uint(am) >> 23));
+    const float down = __uint_as_float((254u - e) << 23);
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[s][j] *= down;
+    return __uint_as_float(e << 23);
+}
+// the weights w of a row's scores s, whose units are f; m the running reference, l and o the sums so far
+template <int P, int N, int T>
+__device__ __forceinline__ void pg_soften(const float (&s)[N], float f, float& m, float& l, pg_f4 (&o)[T], float (&w)[N]) {
+    float mx = s[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) mx = fmaxf(mx, s[j]);
+    if constexpr (P == 4) mx = fmaxf(mx, pg_dpp<PG_ROR8>(mx));
+    mx = amv_max_x32(amv_max_x16(mx)) * f;  // (f a power of two: exact)
+    // the reference moves when a weight would pass 2^15 (or there is none yet), to 2^-12 of the maximum; where no difference of 12 is
+    // exact, to the maximum
+    const bool grow = mx > m + 15.0f;
+    if (__builtin_amdgcn_ballot_w64(grow)) {
+        const float to = fabsf(mx) > 0x1p20f ? mx : mx - 12.0f;
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+        if (grow) m = to;
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < T; ++t) o[t] *= alpha;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        w[j] = __builtin_amdgcn_exp2f(fmaf(s[j], f, -ref));
+        sum += w[j];
+    }
+    l += sum;
+}
+// where a row's result goes: the output, or (*ml not NULL) its part z
+template <int D>
+__device__ __forceinline__ float* pg_to(const PgAttn& a, const PgRows& t, int hk, int r, int z, float2** ml) {
+    const int tr = r / a.G;
+    const int64_t row = (int64_t)(t.tok0 + tr) * a.n_head + hk * a.G + (r - tr * a.G);
+    const int64_t part = (t.part0 >= 0 ? t.part0 + r : row) * a.n_split + z;
+    *ml = a.ml ? a.ml + part : nullptr;
+    return a.ml ? a.acc + part * D : a.out + row * D;
+}
+
+// The waves of the workgroup take the tile's keys in turn, each for all its rows
 template <int TYPE, int D, int RT, int P>
-__global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
+__device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int z, float* so0, float* so1) {
     using R = PgRow<TYPE, D>;
     constexpr int NB = D / 32, T = D / 16, ROWS = 16 / P, KPL = P == 4 ? 4 : 8;
     constexpr bool QUANT = TYPE != AMV_T_F16;
     static_assert(P == 1 || RT == 1, "rows that share a product's columns are one tile");
-    __shared__ float so[4][4][T][64];  // a row tile's O^T of the four waves, [wave][register][product][lane]
+    // a row tile's O^T of waves 0 and 1, 2 and 3: [wave][register][product][lane]
+    const auto so = [&](int w, int r, int v) -> float& { return (w < 2 ? so0 : so1)[(((w & 1) * 4 + r) * T + v) * 64 + (threadIdx.x & 63)]; };
     __shared__ float sm[4][16 * RT], sl[4][16 * RT];
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     // what column c of the products is: row `col` of its tile, rounded (part 0) or the rest (part 1); u: whose keys it keeps
@@ -246,69 +385,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
     const int col = P == 4 ? (rest ? 3 - (c & 3) : c & 3) : P == 2 ? (rest ? 15 - c : c) : c;
     const float part = rest ? 1.0f : 0.0f;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int hk = (int)blockIdx.x % a.n_head_kv, tile = (int)blockIdx.x / a.n_head_kv, z = blockIdx.y;
     const int psh = a.b.pshift, ps = 1 << psh;
+    PgRows t;
+    if (!pg_rows(a, hk, tile, ROWS * RT, t)) return;
 
-    // the tile's rows: rows r0 .. of the n_rows of tokens tok0 .., row r is head r % G of token tok0 + r / G, whose place is
-    // place0 + r / G; keys: how many there are to see
-    int tok0, r0, n_rows, place0, keys;
-    const int32_t* pages;  // the physical pages, or the sequence's table where `list` says which
-    const int32_t* list = nullptr;
-    int64_t part0 = -1;  // PG_ONE: where the rows of the sequence are in ml
-    if (a.kind == PG_PREFIX) {
-        tok0 = 0;
-        r0 = tile * ROWS * RT;
-        n_rows = a.b.n_tok * a.G;
-        keys = a.n_list;
-        place0 = keys;  // (every row sees them all)
-        pages = a.list;
-    } else {
-        int s, in;
-        if (a.kind == PG_LIST) {
-            tok0 = tile / a.ta;
-            in = tile % a.ta;
-            s = pg_seq_of(a.b, tok0);
-        } else if (a.kind == PG_ONE) {
-            s = tile / a.ta;
-            in = tile % a.ta;
-        } else {
-            pg_find(a.b.n_seq, tile, [&](int q) {
-                const int r = (a.b.last(q) - a.b.first(q)) * a.G;
-                return r > a.rows_most ? (r + ROWS * RT - 1) / (ROWS * RT) : 0;
-            }, s, in);
-        }
-        if (s >= a.b.n_seq) return;
-        const int first = a.b.first(s), n_q = a.b.last(s) - first;
-        place0 = a.b.end(s) - n_q;
-        keys = a.b.keys(s);
-        pages = a.b.table + s * a.b.table_stride;
-        if (a.kind == PG_LIST) {
-            place0 += tok0 - first;
-            n_rows = a.G;
-            list = a.list + ((int64_t)tok0 * a.n_head_kv + hk) * a.n_list;
-        } else {
-            tok0 = first;
-            n_rows = n_q * a.G;
-            if (a.kind == PG_ONE && n_rows > a.rows_most) return;
-            if (a.kind == PG_ONE) part0 = ((int64_t)s * a.n_head_kv + hk) * a.rows_most;
-            if (a.kind == PG_FIND) in = (n_rows + ROWS * RT - 1) / (ROWS * RT) - 1 - in;  // the rows with the most keys first
-        }
-        r0 = in * ROWS * RT;
-        if (r0 >= n_rows) return;
-    }
-    const int r_last = min(r0 + ROWS * RT, n_rows) - 1;
-    // keys that every row of the tile sees, and the last that any does
-    int see_all = keys, see_any = keys;
-    if (a.kind != PG_PREFIX) {
-        see_all = min(keys, place0 + r0 / a.G + 1);
-        see_any = min(keys, place0 + r_last / a.G + 1);
-    }
     // the walk: 32-key tiles i = begin + w, begin + w + 4, ... of the keys (of the listed pages' keys)
-    int walk = see_any;
-    if (list) {
+    int walk = t.see_any;
+    if (t.list) {
         walk = 0;
         for (int i = lane; i < (a.n_list + 63) / 64 * 64; i += 64) {
-            const uint64_t m = __builtin_amdgcn_ballot_w64(i < a.n_list && list[min(i, a.n_list - 1)] >= 0);
+            const uint64_t m = __builtin_amdgcn_ballot_w64(i < a.n_list && t.list[min(i, a.n_list - 1)] >= 0);
             if (m) walk = ((i - lane) + 64 - __builtin_clzll(m)) << psh;
         }
         walk = __builtin_amdgcn_readfirstlane(walk);
@@ -316,21 +402,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
     const int end = (min(walk, (z + 1) * a.split_len) + 31) >> 5;
     int i = (z * a.split_len >> 5) + w;
 
-    const auto where = [&](int i) {  // i: uniform over the wave
+    const auto where = [&](int i) {
+        if (!t.list) return pg_where(a, t.pages, t.keys, i);
         PgAt at;
-        if (list) {
-            const int j0 = i * 32 >> psh, j1 = min(i * 32 + 16, walk - 1) >> psh, off = (i * 32) & (ps - 1);
-            const int l0 = list[j0], l1 = list[j1], most = (a.b.max_kv - 1) >> psh;
-            at.e0 = l0 >= 0 && l0 <= most ? pages[l0] : -1;
-            at.e1 = i * 32 + 16 < walk && l1 >= 0 && l1 <= most ? pages[l1] : -1;
-            at.p0 = (l0 << psh) + off;
-            at.p1 = psh == 4 ? l1 << psh : at.p0 + 16;
-        } else {
-            at.p0 = i * 32;
-            at.p1 = at.p0 + 16;
-            at.e0 = pages[at.p0 >> psh];
-            at.e1 = at.p1 < keys ? pages[at.p1 >> psh] : -1;
-        }
+        const int j0 = i * 32 >> psh, j1 = min(i * 32 + 16, walk - 1) >> psh, off = (i * 32) & (ps - 1);
+        const int l0 = t.list[j0], l1 = t.list[j1], most = (a.b.max_kv - 1) >> psh;
+        at.e0 = l0 >= 0 && l0 <= most ? t.pages[l0] : -1;
+        at.e1 = i * 32 + 16 < walk && l1 >= 0 && l1 <= most ? t.pages[l1] : -1;
+        at.p0 = (l0 << psh) + off;
+        at.p1 = psh == 4 ? l1 << psh : at.p0 + 16;
         if ((uint32_t)at.e0 >= (uint32_t)a.n_pages) at.e0 = -1;
         if ((uint32_t)at.e1 >= (uint32_t)a.n_pages) at.e1 = -1;
         return at;
@@ -359,28 +439,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
     int lim[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int r = min(r0 + 16 * rt + col, r_last), t = r / a.G;
-        lim[rt] = a.kind == PG_PREFIX ? keys : min(keys, place0 + t + 1);
-        const float* src = a.q + (tok0 + t) * a.q_stride + (int64_t)(hk * a.G + r - t * a.G) * D + 8 * g;
-        float x[NB][8], am = 0.0f;
+        const int r = min(t.r0 + 16 * rt + col, t.r_last);
+        lim[rt] = a.kind == PG_PREFIX ? t.keys : min(t.keys, t.place0 + r / a.G + 1);
+        float x[NB][8];
+        f[rt] = pg_query<D>(a, t, hk, r, g, x);
 #pragma unroll
         for (int s = 0; s < NB; ++s) {
-            const float4 y = *reinterpret_cast<const float4*>(src + 32 * s), z = *reinterpret_cast<const float4*>(src + 32 * s + 4);
-            const float yz[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[s][j] = yz[j] * a.scale2;
-                am = fmaxf(am, fabsf(x[s][j]));
-            }
-        }
-        am = amv_max_x32(amv_max_x16(am));
-        const uint32_t e = max(1u, min(253u, __float_as_uint(am) >> 23));
-        const float down = __uint_as_float((254u - e) << 23);
-        f[rt] = __uint_as_float(e << 23);
-#pragma unroll
-        for (int s = 0; s < NB; ++s) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[s][j] *= down;
             if constexpr (P == 1) {
                 pg_split(x[s], qa[rt][0][s], qa[rt][1][s]);
             } else {
@@ -407,7 +471,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
         m[rt] = -INFINITY;
         l[rt] = 0.0f;
 #pragma unroll
-        for (int t = 0; t < T; ++t) o[rt][t] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int v = 0; v < T; ++v) o[rt][v] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     float vref = 0.0f, vdown = 0.0f;  // the power of two that values' scales are held below, its inverse
 
@@ -437,14 +501,13 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const pg_h8 kf = pg_k_operand<TYPE, D>(tk.k[h], b);
+                if constexpr (P == 4 && QUANT) {
+                    x[0][0] = pg_mfma(kf, qa[0][h][b], x[0][0]);
+                } else {
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    if constexpr (P == 4 && QUANT) {
-                        x[rt][0] = pg_mfma(kf, qa[rt][h][b], x[rt][0]);
-                    } else {
-                        if constexpr (P == 1) x[rt][h] = pg_mfma(kf, qa[rt][1][b], x[rt][h]);
-                        x[rt][h] = pg_mfma(kf, qa[rt][0][b], x[rt][h]);
-                    }
+                    for (int k = P == 1 ? 1 : 0; k >= 0; --k)
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) x[rt][h] = pg_mfma(kf, qa[rt][k][b], x[rt][h]);
                 }
             }
             if constexpr (QUANT) {
@@ -466,7 +529,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
         // keys that are not there, or not seen by every row
         const int p = (g >= 2 ? now.p1 : now.p0) + 8 * (g & 1);
         const bool there = (g >= 2 ? now.e1 : now.e0) >= 0;
-        const bool some = now.e0 < 0 || now.e1 < 0 || max(now.p0, now.p1) + 16 > see_all;
+        const bool some = now.e0 < 0 || now.e1 < 0 || max(now.p0, now.p1) + 16 > t.see_all;
         if (some) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
@@ -474,14 +537,14 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
                 for (int j = 0; j < KPL; ++j) s[rt][j] = there && p + 4 * u + j < lim[rt] ? s[rt][j] : -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {  // what lies there must not matter, 0 times infinity is no number
-                const uint32_t keep = there && p + j < keys ? 0xFFFFFFFFu : 0u;
+                const uint32_t keep = there && p + j < t.keys ? 0xFFFFFFFFu : 0u;
 #pragma unroll
                 for (int x = 0; x < PgV<TYPE, D, KPL>::W; ++x) tv.v[j][x] &= keep;
             }
             if constexpr (QUANT) {
 #pragma unroll
                 for (int j = 0; j < KPL; ++j) {
-                    const uint32_t keep = there && p + 4 * u + j < keys ? 0xFFFFFFFFu : 0u;
+                    const uint32_t keep = there && p + 4 * u + j < t.keys ? 0xFFFFFFFFu : 0u;
 #pragma unroll
                     for (int b = 0; b < NB; b += 2) tv.s[(j * NB + b) >> 1] &= keep;
                 }
@@ -502,7 +565,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                    for (int t = 0; t < T; ++t) o[rt][t] *= by;
+                    for (int v = 0; v < T; ++v) o[rt][v] *= by;
             }
         }
         pg_h8 ph[RT], pl[RT];  // P^T operands: the weights and their rest, or (P > 1) both in one
@@ -526,30 +589,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
         };
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            float mx = s[rt][0];
-#pragma unroll
-            for (int j = 1; j < KPL; ++j) mx = fmaxf(mx, s[rt][j]);
-            if constexpr (P == 4) mx = fmaxf(mx, pg_dpp<PG_ROR8>(mx));
-            mx = amv_max_x32(amv_max_x16(mx)) * f[rt];  // (f a power of two: exact)
-            // the reference moves when a weight would pass 2^15 (or there is none yet), to 2^-12 of the maximum; where no difference
-            // of 12 is exact, to the maximum
-            const bool grow = mx > m[rt] + 15.0f;
-            if (__builtin_amdgcn_ballot_w64(grow)) {
-                const float to = fabsf(mx) > 0x1p20f ? mx : mx - 12.0f;
-                const float alpha = grow ? __builtin_amdgcn_exp2f(m[rt] - to) : 1.0f;
-                if (grow) m[rt] = to;
-                l[rt] *= alpha;
-#pragma unroll
-                for (int t = 0; t < T; ++t) o[rt][t] *= alpha;
-            }
-            const float ref = m[rt] == -INFINITY ? 0.0f : m[rt];
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < KPL; ++j) {
-                pw[rt][j] = __builtin_amdgcn_exp2f(fmaf(s[rt][j], f[rt], -ref));
-                sum += pw[rt][j];
-            }
-            l[rt] += sum;
+            pg_soften<P>(s[rt], f[rt], m[rt], l[rt], o[rt], pw[rt]);
             if constexpr (QUANT) {
 #pragma unroll
                 for (int j = 0; j < KPL; ++j) pw[rt][j] *= vdown;
@@ -558,16 +598,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
             }
         }
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const pg_h8 vf = pg_v_operand<TYPE, D>(tv, t);
+        for (int v = 0; v < T; ++v) {
+            const pg_h8 vf = pg_v_operand<TYPE, D>(tv, v);
             if constexpr (QUANT) {
-                if ((t & 1) == 0) {  // products 2 b and 2 b + 1 are block b
+                if ((v & 1) == 0) {  // products 2 b and 2 b + 1 are block b
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) {
                         float y[KPL];
 #pragma unroll
                         for (int j = 0; j < KPL; ++j) {
-                            y[j] = pw[rt][j] * pg_half(tv.s, j * NB + (t >> 1));
+                            y[j] = pw[rt][j] * pg_half(tv.s, j * NB + (v >> 1));
                             // The compiler would round the unrounded product to f16 (v_fma_mixlo_f16) but take the rest from the
                             // f16 of the rounded one; where the two differ, next to a tie, the parts do not sum to y.
                             asm("" : "+v"(y[j]));
@@ -576,11 +616,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
                     }
                 }
             }
+            if constexpr (P == 1) {
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                if constexpr (P == 1) o[rt][t] = pg_mfma(vf, pl[rt], o[rt][t]);
-                o[rt][t] = pg_mfma(vf, ph[rt], o[rt][t]);
+                for (int rt = 0; rt < RT; ++rt) o[rt][v] = pg_mfma(vf, pl[rt], o[rt][v]);
             }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) o[rt][v] = pg_mfma(vf, ph[rt], o[rt][v]);
         }
         if constexpr (more()) pg_load_v(tv, a, vc, at, ln);
     };
@@ -604,51 +645,280 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PgAttn a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int t = 0; t < T; ++t) {
-                float y = o[rt][t][r];
+            for (int v = 0; v < T; ++v) {
+                float y = o[rt][v][r];
                 if constexpr (P == 2) y += pg_dpp<PG_MIRROR>(y);  // (lanes of part 0 end with their row's)
                 if constexpr (P == 4) y += pg_dpp<PG_HALF_MIRROR>(y);
-                so[w][r][t][lane] = y * back;
+                so(w, r, v) = y * back;
             }
         __syncthreads();
-        const int r = r0 + 16 * rt + c;
+        const int r = t.r0 + 16 * rt + c;
         float M = -INFINITY, L = 0.0f, x[T];
 #pragma unroll
         for (int j = 0; j < 4; ++j) M = fmaxf(M, sm[j][16 * rt + c]);
 #pragma unroll
-        for (int t = 0; t < T; ++t) x[t] = 0.0f;
+        for (int v = 0; v < T; ++v) x[v] = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float mj = sm[j][16 * rt + c], by = mj == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mj - M);
             L = fmaf(sl[j][16 * rt + c], by, L);
 #pragma unroll
-            for (int t = 0; t < T; ++t) x[t] = fmaf(so[j][w][t][lane], by, x[t]);
+            for (int v = 0; v < T; ++v) x[v] = fmaf(so(j, w, v), by, x[v]);
         }
-        if (r < n_rows && c < ROWS) {
-            const int tr = r / a.G;
-            const int64_t row = (int64_t)(tok0 + tr) * a.n_head + hk * a.G + (r - tr * a.G);
-            float* to = a.out + row * D;
-            if (!a.ml) {
+        if (r < t.n_rows && c < ROWS) {
+            float2* ml;
+            float* to = pg_to<D>(a, t, hk, r, z, &ml);
+            if (!ml) {
                 const float inv = L > 0.0f ? 1.0f / L : L;  // (no keys: 0; a weight that is no number stays one)
 #pragma unroll
-                for (int t = 0; t < T; ++t) x[t] *= inv;
-            } else {
-                const int64_t part = (part0 >= 0 ? part0 + r : row) * a.n_split + z;
-                to = a.acc + part * D;
-                if (w == 0 && g == 0) a.ml[part] = make_float2(M, L);
+                for (int v = 0; v < T; ++v) x[v] *= inv;
+            } else if (w == 0 && g == 0) {
+                *ml = make_float2(M, L);
             }
             const int d = 4 * g + w;  // the operand row
             if constexpr (QUANT) {
 #pragma unroll
-                for (int t = 0; t < T; t += 2)
-                    *reinterpret_cast<float2*>(to + 16 * t + 2 * d) = make_float2(x[t], x[t + 1]);
+                for (int v = 0; v < T; v += 2)
+                    *reinterpret_cast<float2*>(to + 16 * v + 2 * d) = make_float2(x[v], x[v + 1]);
             } else {
 #pragma unroll
-                for (int t = 0; t < T; t += 4)
-                    *reinterpret_cast<float4*>(to + T * d + t) = make_float4(x[t], x[t + 1], x[t + 2], x[t + 3]);
+                for (int v = 0; v < T; v += 4)
+                    *reinterpret_cast<float4*>(to + T * d + v) = make_float4(x[v], x[v + 1], x[v + 2], x[v + 3]);
             }
         }
     }
+}
+
+// Many rows over f16 keys (prompts, a prefix): a tile of 128 rows, 32 of each wave, and every wave goes over all its keys, so these
+// come from memory once for the four: read by each wave for itself (pg_few), K's pieces of 16 bytes from 16 rows an instruction keep
+// the loads' address unit busy for all of the time. K and V rows of 64 keys go to LDS without registers (global_load_lds), one step
+// ahead in two buffers; the products are those of pg_few with RT = 2. The loads write LDS in lane order, so a row's pieces are
+// exchanged on the memory side: K's 16-byte pieces by a number of the key that differs among the 16 keys of an operand read, V's
+// 32-byte units by one that takes each value twice among the 16 keys of a transposing read (ds_read_b64_tr_b16: 16 lanes pointing at
+// 4 keys' 8-byte quarters of a unit get an element of the 4 keys each), so both reads meet all banks.
+typedef __attribute__((address_space(3))) void pg_lds;
+typedef __attribute__((address_space(1))) const void pg_glb;
+typedef short pg_s4 __attribute__((ext_vector_type(4)));
+typedef short pg_s8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) pg_s4 pg_lds_s4;
+// every wave's LDS accesses and vector memory loads (those into LDS too) done, then the workgroup's barrier
+#define PG_BARRIER()                        \
+    do {                                    \
+        asm volatile("" ::: "memory");      \
+        __builtin_amdgcn_s_waitcnt(0x0070); \
+        __builtin_amdgcn_s_barrier();       \
+        asm volatile("" ::: "memory");      \
+    } while (0)
+#define PG_MANY_ROWS 128
+__device__ __align__(16) const uint8_t pg_zeros[16] = {};
+
+template <int D>
+__device__ __forceinline__ void pg_many(const PgAttn& a, int hk, int tile, int z, uint16_t* sKa, uint16_t* sKb, uint16_t* sVa,
+                                        uint16_t* sVb) {
+    constexpr int NB = D / 32, T = D / 16, PIECES = D / 8;  // (of 16 bytes a row)
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ps = 1 << a.b.pshift;
+    PgRows t;
+    if (!pg_rows(a, hk, tile, PG_MANY_ROWS, t)) return;
+    // steps of 64 keys
+    const int begin = z * a.split_len >> 6, end = (min(t.see_any, (z + 1) * a.split_len) + 63) >> 6;
+    // the wave's own rows
+    const int wr0 = t.r0 + 32 * w, wr1 = min(wr0 + 31, t.r_last);
+    const bool idle = wr0 > t.r_last;
+    t.see(a, idle ? t.r_last : wr0, idle ? t.r_last : wr1);
+    const int mine = idle ? 0 : min(end, (t.see_any + 63) >> 6);  // steps that its rows see a part of
+
+    // staging: the wave's 16 rows of a step; lane: row `row` of an instruction's, place x of its pieces
+    constexpr int RPI = 64 / PIECES, LOADS = 16 / RPI;  // rows of an instruction
+    const int row = lane / PIECES, x = lane % PIECES;
+    const auto hash_k = [](int key) { return D == 128 ? ((key >> 3 & 3) << 2 | (key & 3)) : ((key >> 3 & 3) << 1 | (key >> 1 & 1)); };
+    const auto hash_v = [](int key) { return D == 128 ? ((key & 3) | (key >> 3 & 1) << 2) : ((key >> 1 & 1) | (key >> 3 & 1) << 1); };
+    uint32_t ko[LOADS], vo[LOADS];  // bytes from the wave's first row
+#pragma unroll
+    for (int y = 0; y < LOADS; ++y) {
+        const int key = 16 * w + RPI * y + row;
+        ko[y] = (RPI * y + row) * 2 * D + 16 * (x ^ hash_k(key));
+        vo[y] = (RPI * y + row) * 2 * D + 16 * ((((x >> 1) ^ hash_v(key)) << 1) | (x & 1));
+    }
+    const size_t chunk = (size_t)ps * 2 * D;
+    const uint8_t *kc = a.k + hk * chunk, *vc = a.v + hk * chunk;
+    struct Step {
+        PgAt a, b;  // its 32-key halves
+    };
+    const auto where = [&](int i) {
+        Step s;
+        s.a = pg_where(a, t.pages, t.keys, 2 * i);
+        if (64 * i + 32 < t.keys) s.b = pg_where(a, t.pages, t.keys, 2 * i + 1);
+        else s.b = {-1, -1, 64 * i + 32, 64 * i + 48};
+        return s;
+    };
+    const auto stage = [&](const Step& s, uint16_t* sK, uint16_t* sV) {
+        const int e = w == 0 ? s.a.e0 : w == 1 ? s.a.e1 : w == 2 ? s.b.e0 : s.b.e1;
+        const int64_t off = pg_off<AMV_T_F16, D>(a, e, s.a.p0 + 16 * w, false);
+        const bool whole = e >= 0 && s.a.p0 + 16 * w + 16 <= t.keys;
+        // (scalar: a base in scalar registers and the lane's bytes, not a sum for each load that is kept over the steps)
+        const int64_t so = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(off >> 32)) << 32 |
+                                     (uint32_t)__builtin_amdgcn_readfirstlane((int)off));
+        const uint8_t *ks = kc + so, *vs = vc + so;
+#pragma unroll
+        for (int y = 0; y < LOADS; ++y) {
+            asm volatile("" : "+v"(ko[y]), "+v"(vo[y]));
+            __builtin_amdgcn_global_load_lds((pg_glb*)(ks + (size_t)ko[y]), (pg_lds*)(sK + (16 * w + RPI * y) * D), 16, 0, 0);
+            if (whole) {
+                __builtin_amdgcn_global_load_lds((pg_glb*)(vs + (size_t)vo[y]), (pg_lds*)(sV + (16 * w + RPI * y) * D), 16, 0, 0);
+            } else {  // zeros where there is no key: what lies there must not matter, and 0 times infinity is no number
+                const uint8_t* from = e >= 0 && s.a.p0 + 16 * w + RPI * y + row < t.keys ? vs + vo[y] : pg_zeros;
+                __builtin_amdgcn_global_load_lds((pg_glb*)from, (pg_lds*)(sV + (16 * w + RPI * y) * D), 16, 0, 0);
+            }
+        }
+    };
+    Step at = {};
+    if (begin < end) {
+        at = where(begin);
+        stage(at, sKa, sVa);
+    }
+    pg_h8 qh[2][NB], ql[2][NB];
+    float f[2], m[2], l[2];
+    int lim[2];
+    pg_f4 o[2][T];
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+        const int r = min(t.r0 + 16 * rt + c, t.r_last);
+        lim[rt] = a.kind == PG_PREFIX ? t.keys : min(t.keys, t.place0 + r / a.G + 1);
+        float y[NB][8];
+        f[rt] = pg_query<D>(a, t, hk, r, g, y);
+#pragma unroll
+        for (int s = 0; s < NB; ++s) pg_split(y[s], qh[rt][s], ql[rt][s]);
+        m[rt] = -INFINITY;
+        l[rt] = 0.0f;
+#pragma unroll
+        for (int v = 0; v < T; ++v) o[rt][v] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // the lane's places in the rows of 32 keys: K's key of product 0 and its piece g (+ 4 b: by XOR), V's key and unit 0 (v: by XOR)
+    const int kx = (8 * (c >> 2) + (c & 3)) * D + 8 * (g ^ (D == 128 ? c : c >> 1));  // (hash_k of both products' key)
+    const int vx = (8 * g + (c >> 2)) * D + 16 * hash_v(8 * g + (c >> 2)) + 4 * (c & 3);  // (and hash_v of key + 4)
+    const auto half = [&](const PgAt& now, const uint16_t* sK, const uint16_t* sV) {  // 32 keys
+        int kx0 = kx, vx0 = vx;  // (not known to be the same each time: their sums would be kept, in registers that are not there)
+        asm volatile("" : "+v"(kx0), "+v"(vx0));
+        pg_f4 y[2][2];
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) y[rt][0] = y[rt][1] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const pg_h8 kf = *reinterpret_cast<const pg_h8*>(&sK[(kx0 ^ (32 * b)) + 4 * h * D]);
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt) y[rt][h] = pg_mfma(kf, ql[rt][b], y[rt][h]);
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt) y[rt][h] = pg_mfma(kf, qh[rt][b], y[rt][h]);
+            }
+        float s[2][8], pw[8];
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[rt][j] = y[rt][j >> 2][j & 3];
+        if (now.e0 < 0 || now.e1 < 0 || now.p1 + 16 > t.see_all) {
+            const int p = now.p0 + 8 * g;
+            const bool there = (g >= 2 ? now.e1 : now.e0) >= 0;
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[rt][j] = there && p + j < lim[rt] ? s[rt][j] : -INFINITY;
+        }
+        pg_h8 ph[2], pl[2];
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            pg_soften<1>(s[rt], f[rt], m[rt], l[rt], o[rt], pw);
+            pg_split(pw, ph[rt], pl[rt]);
+        }
+#pragma unroll
+        for (int v = 0; v < T; ++v) {
+            const uint16_t* at0 = &sV[vx0 ^ (16 * v)];
+            const pg_s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pg_lds_s4*)(__attribute__((address_space(3))) uint16_t*)at0);
+            const pg_s4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pg_lds_s4*)(__attribute__((address_space(3))) uint16_t*)(at0 + 4 * D));
+            const pg_s8 ab = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+            const pg_h8 vf = __builtin_bit_cast(pg_h8, ab);
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) o[rt][v] = pg_mfma(vf, pl[rt], o[rt][v]);
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) o[rt][v] = pg_mfma(vf, ph[rt], o[rt][v]);
+        }
+    };
+    const auto step = [&](const Step& now, const uint16_t* sK, const uint16_t* sV) {
+        half(now.a, sK, sV);
+        half(now.b, sK + 32 * D, sV + 32 * D);
+    };
+    PG_BARRIER();
+    for (int i = begin; i < end; i += 2) {
+        Step next = at;
+        if (i + 1 < end) {
+            next = where(i + 1);
+            stage(next, sKb, sVb);
+        }
+        if (i < mine) step(at, sKa, sVa);
+        PG_BARRIER();
+        if (i + 1 >= end) break;
+        if (i + 2 < end) {
+            at = where(i + 2);
+            stage(at, sKa, sVa);
+        }
+        if (i + 1 < mine) step(next, sKb, sVb);
+        PG_BARRIER();
+    }
+    if (idle) return;
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+        const float L = amv_sum_x32(amv_sum_x16(l[rt]));
+        const int r = t.r0 + 16 * rt + c;
+        if (r > t.r_last) continue;
+        float2* ml;
+        float* to = pg_to<D>(a, t, hk, r, z, &ml);
+        float inv = 1.0f;
+        if (!ml) inv = L > 0.0f ? 1.0f / L : L;
+        else if (g == 0) *ml = make_float2(m[rt], L);
+#pragma unroll
+        for (int v = 0; v < T; ++v) {
+            const pg_f4 y = o[rt][v] * inv;
+            *reinterpret_cast<pg_f4*>(to + 16 * v + 4 * g) = y;
+        }
+    }
+}
+
+// A launch has up to three jobs, one after the other over the workgroups, so that one's reading fills the other's computing: tiles of
+// many rows (of the prefix, of sequences with many tokens), then those of few.
+struct PgJobs {
+    PgAttn a[3];
+    int n[3];  // workgroups
+};
+__device__ __forceinline__ void pg_place_of(const PgAttn& a, int b, int& hk, int& tile, int& z) {
+    hk = b % a.n_head_kv;
+    b /= a.n_head_kv;
+    tile = b % a.tiles;
+    z = b / a.tiles;
+}
+template <int TYPE, int D, int RT, int P>
+__global__ __launch_bounds__(256, 2) void k_paged_few(PgJobs jobs) {  // jobs 1 and 2
+    __shared__ float so[2][32 * D];
+    const int b = (int)blockIdx.x, k = b < jobs.n[1] ? 1 : 2;
+    int hk, tile, z;
+    pg_place_of(jobs.a[k], k == 1 ? b : b - jobs.n[1], hk, tile, z);
+    pg_few<TYPE, D, RT, P>(jobs.a[k], hk, tile, z, so[0], so[1]);
+}
+template <int TYPE, int D, int RT, int P>
+__global__ __launch_bounds__(256, 2) void k_paged_many_few(PgJobs jobs) {  // jobs 0 and 1 of many rows, 2 of few
+    // buffers as variables of their own: reads of one do not wait for the loads into another
+    __shared__ __align__(16) uint16_t sKa[64 * D], sKb[64 * D], sVa[64 * D], sVb[64 * D];
+    float *so0 = reinterpret_cast<float*>(sKa), *so1 = reinterpret_cast<float*>(sKb);
+    int b = (int)blockIdx.x, hk, tile, z;
+    const int k = b < jobs.n[0] ? 0 : b < jobs.n[0] + jobs.n[1] ? 1 : 2;
+    if (k > 0) b -= jobs.n[0];
+    if (k > 1) b -= jobs.n[1];
+    pg_place_of(jobs.a[k], b, hk, tile, z);
+    if (k == 2) pg_few<TYPE, D, RT, P>(jobs.a[2], hk, tile, z, so0, so1);
+    else if constexpr (TYPE == AMV_T_F16) pg_many<D>(jobs.a[k], hk, tile, z, sKa, sKb, sVa, sVb);
+    else pg_few<TYPE, D, 2, 1>(jobs.a[k], hk, tile, z, so0, so1);
 }
 
 // out = sum_z w_z O_z / sum_z w_z l_z over the parts z of a row's keys, w_z = 2^(m_z - max m): one wave per row. A row has parts of
@@ -716,22 +986,23 @@ __global__ __launch_bounds__(256) void k_paged_merge(PgMerge a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
-// Row tiles of a launch: rt times 16 rows, or 16 / pack of them where rows are few: the products' 16 columns then hold the two f16 of
-// every row side by side, and with pack 4 the two products' keys too, so that each lane's scores are of use to half the lanes
-// rather than an eighth.
+// Row tiles: rt times 16 rows, or 16 / pack of them where rows are few: the products' 16 columns then hold the two f16 of every row side
+// by side, and with pack 4 the two products' keys too, so that each lane's scores are of use to half the lanes rather than an eighth.
 struct PgTiles {
     int rt, pack;
     int rows() const { return 16 * rt / pack; }
     int of(int64_t n) const { return (int)((n + rows() - 1) / rows()); }
 };
 static PgTiles pg_tiles(int64_t rows) { return {rows > 16 ? 2 : 1, rows <= 4 ? 4 : rows <= 8 ? 2 : 1}; }
-// How a call is launched: up to two launches over the sequences' own keys and one over the prefix, and the workspace of the parts.
+// How a call is launched, and the workspace of the parts
 struct PgPlan {
-    PgTiles one, pre;                       // sequences (or listed tokens) of few rows, ta tiles each; the prefix's
+    PgTiles few;                            // tiles of few rows: sequences (or listed tokens), ta tiles each, and a small batch's prefix
     int ta, n_one, len_one;                 // their parts
-    int find, rows_most, n_find, len_find;  // sequences of more rows than rows_most, tiles of 32
+    int many_rows;                          // rows of the other tiles
+    int find, rows_most, n_find, len_find;  // sequences of more rows than rows_most
     int64_t find_tiles;
-    int n_pre, len_pre;                     // parts of the prefix
+    bool pre_many;                          // the prefix in tiles of many rows
+    int pre_tiles, n_pre, len_pre;
     int64_t w_one, w_many, w_pre;           // parts in the workspace
     int64_t bytes(int64_t D) const { return (w_one + w_many + w_pre) * (8 + 4 * D); }
 };
@@ -748,26 +1019,30 @@ static int pg_parts(int64_t units, int64_t keys, int* len) {
 }
 static PgPlan pg_plan(const amv_paged_kv* kv, const amv_paged_batch* b, int64_t n_head, int64_t n_prefix, int64_t n_sel) {
     PgPlan p = {};
-    const int64_t G = n_head / kv->n_head_kv;
+    const int64_t G = n_head / kv->n_head_kv, all = b->n_tok * G;
     if (n_sel > 0) {
-        p.one = pg_tiles(G);
-        p.ta = p.one.of(G);
+        p.few = pg_tiles(G);
+        p.ta = p.few.of(G);
         p.n_one = pg_parts(b->n_tok * kv->n_head_kv * p.ta, n_sel * kv->page_size, &p.len_one);
         if (p.n_one > 1) p.w_many = b->n_tok * n_head * p.n_one;
         return p;
     }
     const int64_t rows = std::min(b->max_q, b->n_tok) * G;
-    p.one = pg_tiles(rows <= 32 ? rows : G);
-    p.rows_most = (int)std::max<int64_t>(p.one.rows(), G);
-    p.ta = p.one.of(p.rows_most);
+    p.many_rows = kv->type == AMV_T_F16 ? PG_MANY_ROWS : 32;
+    p.pre_many = all > 32;
+    p.few = pg_tiles(n_prefix > 0 && !p.pre_many ? all : rows <= 32 ? rows : G);
+    p.rows_most = (int)std::max<int64_t>(p.few.rows(), G);
+    p.ta = p.few.of(p.rows_most);
     p.n_one = pg_parts(b->n_seq * kv->n_head_kv * p.ta, b->max_kv, &p.len_one);
     p.find = rows > p.rows_most;
     if (p.find) {
-        p.find_tiles = b->n_tok * G / 32 + b->n_seq;
-        p.n_find = pg_parts(b->n_tok * G / 32 * kv->n_head_kv + 1, b->max_kv, &p.len_find);
+        p.find_tiles = all / p.many_rows + b->n_seq;
+        p.n_find = pg_parts(all / p.many_rows * kv->n_head_kv + 1, b->max_kv, &p.len_find);
     }
-    p.pre = pg_tiles(b->n_tok * G);
-    if (n_prefix > 0) p.n_pre = pg_parts(p.pre.of(b->n_tok * G) * kv->n_head_kv, n_prefix, &p.len_pre);
+    if (n_prefix > 0) {
+        p.pre_tiles = p.pre_many ? (int)((all + p.many_rows - 1) / p.many_rows) : p.few.of(all);
+        p.n_pre = pg_parts(p.pre_tiles * kv->n_head_kv, n_prefix, &p.len_pre);
+    }
     if (p.n_one > 1 || p.n_pre) p.w_one = b->n_seq * kv->n_head_kv * p.rows_most * p.n_one;
     if (p.find && (p.n_find > 1 || p.n_pre)) p.w_many = b->n_tok * n_head * p.n_find;
     p.w_pre = b->n_tok * n_head * p.n_pre;
@@ -780,23 +1055,28 @@ extern "C" int64_t amv_paged_attn_workspace_bytes(const amv_paged_kv* kv, const 
     return pg_plan(kv, batch, n_head, n_prefix, n_sel).bytes(kv->D);
 }
 
-template <int TYPE, int D>
-static void pg_launch(const PgAttn& a, PgTiles t, int64_t tiles, int parts, hipStream_t st) {
-    const dim3 grid((unsigned)(tiles * a.n_head_kv), (unsigned)parts);
-    if (t.pack == 4) hipLaunchKernelGGL((k_paged_attn<TYPE, D, 1, 4>), grid, dim3(256), 0, st, a);
-    else if (t.pack == 2) hipLaunchKernelGGL((k_paged_attn<TYPE, D, 1, 2>), grid, dim3(256), 0, st, a);
-    else if (t.rt == 1) hipLaunchKernelGGL((k_paged_attn<TYPE, D, 1, 1>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_paged_attn<TYPE, D, 2, 1>), grid, dim3(256), 0, st, a);
+template <int TYPE, int D, int RT, int P>
+static void pg_launch(const PgJobs& j, bool many, hipStream_t st) {
+    const dim3 grid((unsigned)(j.n[0] + j.n[1] + j.n[2]));
+    if (many) hipLaunchKernelGGL((k_paged_many_few<TYPE, D, RT, P>), grid, dim3(256), 0, st, j);
+    else hipLaunchKernelGGL((k_paged_few<TYPE, D, RT, P>), grid, dim3(256), 0, st, j);
 }
-static void pg_launch(int type, int D, const PgAttn& a, PgTiles t, int64_t tiles, int parts, hipStream_t st) {
+template <int TYPE, int D>
+static void pg_launch(const PgJobs& j, PgTiles t, bool many, hipStream_t st) {
+    if (t.pack == 4) pg_launch<TYPE, D, 1, 4>(j, many, st);
+    else if (t.pack == 2) pg_launch<TYPE, D, 1, 2>(j, many, st);
+    else if (t.rt == 1) pg_launch<TYPE, D, 1, 1>(j, many, st);
+    else pg_launch<TYPE, D, 2, 1>(j, many, st);
+}
+static void pg_launch(int type, int D, const PgJobs& j, PgTiles t, bool many, hipStream_t st) {
     if (D == 128) {
-        if (type == AMV_T_F16) pg_launch<AMV_T_F16, 128>(a, t, tiles, parts, st);
-        else if (type == AMV_T_Q8_0) pg_launch<AMV_T_Q8_0, 128>(a, t, tiles, parts, st);
-        else pg_launch<AMV_T_Q4_0, 128>(a, t, tiles, parts, st);
+        if (type == AMV_T_F16) pg_launch<AMV_T_F16, 128>(j, t, many, st);
+        else if (type == AMV_T_Q8_0) pg_launch<AMV_T_Q8_0, 128>(j, t, many, st);
+        else pg_launch<AMV_T_Q4_0, 128>(j, t, many, st);
     } else {
-        if (type == AMV_T_F16) pg_launch<AMV_T_F16, 64>(a, t, tiles, parts, st);
-        else if (type == AMV_T_Q8_0) pg_launch<AMV_T_Q8_0, 64>(a, t, tiles, parts, st);
-        else pg_launch<AMV_T_Q4_0, 64>(a, t, tiles, parts, st);
+        if (type == AMV_T_F16) pg_launch<AMV_T_F16, 64>(j, t, many, st);
+        else if (type == AMV_T_Q8_0) pg_launch<AMV_T_Q8_0, 64>(j, t, many, st);
+        else pg_launch<AMV_T_Q4_0, 64>(j, t, many, st);
     }
 }
 
@@ -833,35 +1113,26 @@ static int pg_attn(const char* what, const amv_paged_kv* kv, const amv_paged_bat
                  {ml + p.w_one, acc + p.w_one * kv->D, p.w_many ? (n_sel > 0 ? p.n_one : p.n_find) : 0},
                  {ml + p.w_one + p.w_many, acc + (p.w_one + p.w_many) * kv->D, p.n_pre},
                  out, (int)n_head, kv->n_head_kv, a.G, n_sel > 0 ? -1 : p.rows_most};
-    const auto into = [&](const PgParts& parts) {
-        a.ml = parts.n ? const_cast<float2*>(parts.ml) : nullptr;
-        a.acc = const_cast<float*>(parts.acc);
+    PgJobs jobs = {};
+    const auto job = [&](int k, int kind, int64_t tiles, int parts, int len, const PgParts& into) {
+        PgAttn& x = jobs.a[k] = a;
+        x.kind = kind;
+        x.n_list = (int)(kind == PG_PREFIX ? n_prefix : n_sel);
+        x.ta = p.ta;
+        x.rows_most = p.rows_most;
+        x.tiles = (int)tiles;
+        x.n_split = parts;
+        x.split_len = len;
+        x.ml = into.n ? const_cast<float2*>(into.ml) : nullptr;
+        x.acc = const_cast<float*>(into.acc);
+        jobs.n[k] = (int)(tiles * parts * kv->n_head_kv);
     };
+    if (p.find) job(0, PG_FIND, p.find_tiles, p.n_find, p.len_find, m.many);
+    if (p.n_pre) job(1, PG_PREFIX, p.pre_tiles, p.n_pre, p.len_pre, m.pre);
+    if (n_sel > 0) job(2, PG_LIST, b->n_tok * p.ta, p.n_one, p.len_one, m.many);
+    else job(2, PG_ONE, b->n_seq * p.ta, p.n_one, p.len_one, m.one);
     hipStream_t st = amv_stream(stream);
-    if (p.n_pre) {
-        a.kind = PG_PREFIX;
-        a.n_list = (int)n_prefix;
-        a.n_split = p.n_pre;
-        a.split_len = p.len_pre;
-        into(m.pre);
-        pg_launch(kv->type, kv->D, a, p.pre, p.pre.of(b->n_tok * a.G), p.n_pre, st);
-    }
-    if (p.find) {
-        a.kind = PG_FIND;
-        a.rows_most = p.rows_most;
-        a.n_split = p.n_find;
-        a.split_len = p.len_find;
-        into(m.many);
-        pg_launch(kv->type, kv->D, a, PgTiles{2, 1}, p.find_tiles, p.n_find, st);
-    }
-    a.kind = n_sel > 0 ? PG_LIST : PG_ONE;
-    a.n_list = (int)n_sel;
-    a.ta = p.ta;
-    a.rows_most = p.rows_most;
-    a.n_split = p.n_one;
-    a.split_len = p.len_one;
-    into(n_sel > 0 ? m.many : m.one);
-    pg_launch(kv->type, kv->D, a, p.one, (n_sel > 0 ? b->n_tok : b->n_seq) * p.ta, p.n_one, st);
+    pg_launch(kv->type, kv->D, jobs, p.few, p.find || (p.n_pre && p.pre_many), st);
     if (p.w_one + p.w_many + p.w_pre) {
         const dim3 grid((unsigned)((rows + 3) / 4));
         if (kv->D == 128) hipLaunchKernelGGL(k_paged_merge<128>, grid, dim3(256), 0, st, m);
