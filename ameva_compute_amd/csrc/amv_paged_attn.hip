@@ -1007,11 +1007,11 @@ struct PgPlan {
     int64_t bytes(int64_t D) const { return (w_one + w_many + w_pre) * (8 + 4 * D); }
 };
 // parts of `keys` keys for `units` workgroups' worth of rows: two workgroups a CU, none of less than 128 keys (a tile for each of its
-// waves). More and shorter parts cost their prologues and the merge (us at 512 / 1024 / 2048 workgroups: 64 sequences of up to 4096
+// waves), and up to 256 keys no parts, as their merge is a launch of its own. More and shorter parts cost their prologues and the merge (us at 512 / 1024 / 2048 workgroups: 64 sequences of up to 4096
 // f16 keys 136 / 147 / 144, 3 of 65536 Q8_0 keys 78 / 78 / 82, one of 777 with parts of 256 keys 9.6, of 128 9.3)
 static int pg_parts(int64_t units, int64_t keys, int* len) {
     units = std::max<int64_t>(1, units);
-    const int64_t n = std::max<int64_t>(1, std::min<int64_t>(512 / units, (keys + 127) / 128));
+    const int64_t n = keys <= 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(512 / units, (keys + 127) / 128));
     int64_t l = ((keys + n - 1) / n + 127) / 128 * 128;
     l = std::max<int64_t>(128, l);
     *len = (int)l;

@@ -8,7 +8,6 @@ there is no CPU path.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import os
@@ -600,6 +599,7 @@ class PagedKV:
                 raise ValueError("PagedKV bounds: f16 [n_pages, n_head_kv, 2, D] expected")
         self.type, self.page_size, self.n_head_kv, self.D = kv_type, page_size, n_head_kv, head_dim
         self.k, self.v, self.bounds, self.n_pages, self.device = k, v, bounds, k.shape[0], k.device
+        self.index = k.get_device()
         stride = k.stride(0) * k.element_size() if self.n_pages > 1 else n_head_kv * chunk
         self._c = PagedKVStruct(kv_type, n_head_kv, head_dim, page_size, self.n_pages, stride, k.data_ptr(), v.data_ptr(),
                                 _ptr(bounds))
@@ -638,7 +638,7 @@ class PagedBatch:
         if table.dim() != 2 or table.shape[0] != self.n_seq or (cu_q is not None and cu_q.numel() != self.n_seq + 1):
             raise ValueError("PagedBatch: table must be [n_seq, pages], cu_q [n_seq + 1]")
         self.n_tok = self.n_seq if n_tok is None else n_tok
-        self.n_kv, self.table, self.cu_q, self.max_q, self.max_kv, self.device = n_kv, table, cu_q, max_q, max_kv, n_kv.device
+        self.n_kv, self.table, self.cu_q, self.max_q, self.max_kv, self.index = n_kv, table, cu_q, max_q, max_kv, n_kv.get_device()
         self._c = PagedBatchStruct(self.n_seq, self.n_tok, max_q, max_kv, table.shape[1], _ptr(cu_q), n_kv.data_ptr(),
                                    table.data_ptr())
         self._p = ctypes.addressof(self._c)
@@ -659,15 +659,17 @@ class PagedBatch:
         return n
 
 
-def _paged_rows(kv: PagedKV, b: PagedBatch, x: torch.Tensor, heads: int | None, what: str) -> int:
-    """Checks x f32 [n_tok, heads, D] (contiguous heads, any row stride); the heads it has."""
-    if x.dim() != 3 or x.shape[0] != b.n_tok or x.shape[2] != kv.D or (heads is not None and x.shape[1] != heads):
-        raise ValueError(f"{what}: [{b.n_tok}, {'heads' if heads is None else heads}, {kv.D}] expected, got {tuple(x.shape)}")
-    if x.dtype != torch.float32 or x.device != kv.device or b.device != kv.device:
+def _paged_rows(kv: PagedKV, b: PagedBatch, x: torch.Tensor, heads: int, what: str) -> int:
+    """Checks x f32 [n_tok, heads, D] (heads 0: any; contiguous heads, any row stride); its row stride."""
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != b.n_tok or shape[2] != kv.D or (heads and shape[1] != heads):
+        raise ValueError(f"{what}: [{b.n_tok}, {heads or 'heads'}, {kv.D}] expected, got {tuple(shape)}")
+    if x.dtype is not torch.float32 or x.get_device() != kv.index or b.index != kv.index:
         raise ValueError(f"{what}: f32 on {kv.device} expected (pool, batch and rows on one GPU)")
-    if b.n_tok and (x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != kv.D)):
+    s0, s1, s2 = x.stride()
+    if b.n_tok and (s2 != 1 or (s1 != kv.D and shape[1] > 1)):
         raise ValueError(f"{what}: a row's heads must be contiguous")
-    return x.shape[1]
+    return s0 if b.n_tok > 1 else shape[1] * kv.D
 
 
 def _paged_out(out: torch.Tensor | None, shape, like: torch.Tensor, what: str, dtype=torch.float32) -> torch.Tensor:
@@ -687,13 +689,15 @@ def _paged_ws(ws: torch.Tensor | None, need: int, like: torch.Tensor, what: str)
     return ws
 
 
-def _row_stride(x: torch.Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
-
-
-def _on(device: torch.device):
-    """The device of the operands as the current one, where it is not."""
-    return contextlib.nullcontext() if device.index == _device() else torch.cuda.device(device)
+def _on_device(f):
+    """f(kv, ...) with the pool's GPU as the current one."""
+    @functools.wraps(f)
+    def g(kv, *args, **kw):
+        if kv.index == _device():
+            return f(kv, *args, **kw)
+        with torch.cuda.device(kv.device):
+            return f(kv, *args, **kw)
+    return g
 
 
 def paged_workspace_bytes(kv: PagedKV, batch: PagedBatch, n_head: int, n_prefix: int = 0, n_sel: int = 0) -> int:
@@ -701,6 +705,7 @@ def paged_workspace_bytes(kv: PagedKV, batch: PagedBatch, n_head: int, n_prefix:
     return batch._workspace(kv, n_head, n_prefix, n_sel)
 
 
+@_on_device
 def paged_rope_append(kv: PagedKV, batch: PagedBatch, qkv: torch.Tensor, n_head: int, pos: torch.Tensor | None = None,
                       n_dims: int | None = None, mode: int = 0, freq_base: float = 10000.0, freq_scale: float = 1.0,
                       attn_factor: float = 1.0, rule: int = Q8_X86, bad: torch.Tensor | None = None,
@@ -708,79 +713,78 @@ def paged_rope_append(kv: PagedKV, batch: PagedBatch, qkv: torch.Tensor, n_head:
     """ROPE of the q and k heads of qkv f32 [n_tok, n_head + 2 n_head_kv, D]; the rotated k and the v go to the pages at their
     tokens' places (and into the pool's bounds), the rotated q is returned, f32 [n_tok, n_head, D]. pos int32 [n_tok]: the
     rotation's positions (None: the places in the cache). bad int32 [1]: counts tokens and KV heads that were not stored."""
-    _paged_rows(kv, batch, qkv, n_head + 2 * kv.n_head_kv, "paged_rope_append")
-    for t, dt, n, name in ((pos, torch.int32, batch.n_tok, "pos"), (bad, torch.int32, 1, "bad")):
-        if t is not None and (t.dtype != dt or t.device != kv.device or not t.is_contiguous() or t.numel() < n):
+    stride = _paged_rows(kv, batch, qkv, n_head + 2 * kv.n_head_kv, "paged_rope_append")
+    for t, n, name in ((pos, batch.n_tok, "pos"), (bad, 1, "bad")):
+        if t is not None and (t.dtype is not torch.int32 or t.get_device() != kv.index or not t.is_contiguous() or t.numel() < n):
             raise ValueError(f"paged_rope_append: {name} must be int32 [{n}] on {kv.device}")
-    with _on(kv.device):
-        out = _paged_out(out, (batch.n_tok, n_head, kv.D), qkv, "paged_rope_append")
-        check(lib().amv_paged_rope_append(kv._p, batch._p, qkv.data_ptr(), _row_stride(qkv), n_head, _ptr(pos),
-                                          kv.D if n_dims is None else n_dims, mode, freq_base, freq_scale, attn_factor, rule,
-                                          out.data_ptr(), n_head * kv.D, _ptr(bad), _stream()), "amv_paged_rope_append")
+    out = _paged_out(out, (batch.n_tok, n_head, kv.D), qkv, "paged_rope_append")
+    check(lib().amv_paged_rope_append(kv._p, batch._p, qkv.data_ptr(), stride, n_head, _ptr(pos),
+                                      kv.D if n_dims is None else n_dims, mode, freq_base, freq_scale, attn_factor, rule,
+                                      out.data_ptr(), n_head * kv.D, _ptr(bad), _stream()), "amv_paged_rope_append")
     return out
 
 
+@_on_device
 def paged_attn(kv: PagedKV, batch: PagedBatch, q: torch.Tensor, scale: float, out: torch.Tensor | None = None,
                workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of the batch's tokens q f32 [n_tok, n_head, D] over their sequences' pages: decode steps, prompt chunks and
     both together. Returns f32 [n_tok, n_head, D]; tokens that see no key give zeros."""
-    n_head = _paged_rows(kv, batch, q, None, "paged_attn")
-    with _on(kv.device):
-        out = _paged_out(out, q.shape, q, "paged_attn")
-        need = batch._workspace(kv, n_head, 0, 0)
-        ws = _paged_ws(workspace, need, q, "paged_attn")
-        check(lib().amv_paged_attn(kv._p, batch._p, q.data_ptr(), _row_stride(q), out.data_ptr(), n_head, scale, _ptr(ws), need,
-                                   _stream()), "amv_paged_attn")
+    stride, n_head = _paged_rows(kv, batch, q, 0, "paged_attn"), q.shape[1]
+    out = _paged_out(out, q.shape, q, "paged_attn")
+    need = batch._workspace(kv, n_head, 0, 0)
+    ws = _paged_ws(workspace, need, q, "paged_attn")
+    check(lib().amv_paged_attn(kv._p, batch._p, q.data_ptr(), stride, out.data_ptr(), n_head, scale, _ptr(ws), need,
+                               _stream()), "amv_paged_attn")
     return out
 
 
+@_on_device
 def paged_attn_shared(kv: PagedKV, batch: PagedBatch, q: torch.Tensor, scale: float, prefix_table: torch.Tensor,
                       n_prefix: int, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """paged_attn of sequences that all begin with the n_prefix keys of the pages prefix_table (int32): these are read once for all
     of them. batch has the keys behind the prefix only (rotate theirs and q with pos = n_prefix + place)."""
-    n_head = _paged_rows(kv, batch, q, None, "paged_attn_shared")
+    stride, n_head = _paged_rows(kv, batch, q, 0, "paged_attn_shared"), q.shape[1]
     if prefix_table.dtype != torch.int32 or prefix_table.device != kv.device or not prefix_table.is_contiguous():
         raise ValueError(f"paged_attn_shared: prefix_table must be contiguous int32 on {kv.device}")
     if n_prefix < 0 or prefix_table.numel() * kv.page_size < n_prefix:
         raise ValueError(f"paged_attn_shared: {prefix_table.numel()} pages for a prefix of {n_prefix} keys")
-    with _on(kv.device):
-        out = _paged_out(out, q.shape, q, "paged_attn_shared")
-        need = batch._workspace(kv, n_head, n_prefix, 0)
-        ws = _paged_ws(workspace, need, q, "paged_attn_shared")
-        check(lib().amv_paged_attn_shared(kv._p, batch._p, prefix_table.data_ptr(), n_prefix, q.data_ptr(), _row_stride(q),
-                                          out.data_ptr(), n_head, scale, _ptr(ws), need, _stream()), "amv_paged_attn_shared")
+    out = _paged_out(out, q.shape, q, "paged_attn_shared")
+    need = batch._workspace(kv, n_head, n_prefix, 0)
+    ws = _paged_ws(workspace, need, q, "paged_attn_shared")
+    check(lib().amv_paged_attn_shared(kv._p, batch._p, prefix_table.data_ptr(), n_prefix, q.data_ptr(), stride,
+                                      out.data_ptr(), n_head, scale, _ptr(ws), need, _stream()), "amv_paged_attn_shared")
     return out
 
 
+@_on_device
 def paged_select(kv: PagedKV, batch: PagedBatch, q: torch.Tensor, n_sel: int, n_first: int = 1, n_last: int = 1,
                  sel: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """For each token and KV head the n_sel pages of its sequence whose bounds allow the largest sum of q . k over the group's
     heads, the first n_first and the last n_last always among them: int32 [n_tok, n_head_kv, n_sel], rising, -1 behind the last."""
-    n_head = _paged_rows(kv, batch, q, None, "paged_select")
+    stride, n_head = _paged_rows(kv, batch, q, 0, "paged_select"), q.shape[1]
     if kv.bounds is None:
         raise ValueError("paged_select: the pool has no bounds")
-    with _on(kv.device):
-        sel = _paged_out(sel, (batch.n_tok, kv.n_head_kv, n_sel), q, "paged_select", torch.int32)
-        need = batch._workspace(kv, n_head, 0, -1)
-        ws = _paged_ws(workspace, need, q, "paged_select")
-        check(lib().amv_paged_select(kv._p, batch._p, q.data_ptr(), _row_stride(q), n_head, n_sel, n_first, n_last,
-                                     sel.data_ptr(), _ptr(ws), need, _stream()), "amv_paged_select")
+    sel = _paged_out(sel, (batch.n_tok, kv.n_head_kv, n_sel), q, "paged_select", torch.int32)
+    need = batch._workspace(kv, n_head, 0, -1)
+    ws = _paged_ws(workspace, need, q, "paged_select")
+    check(lib().amv_paged_select(kv._p, batch._p, q.data_ptr(), stride, n_head, n_sel, n_first, n_last,
+                                 sel.data_ptr(), _ptr(ws), need, _stream()), "amv_paged_select")
     return sel
 
 
+@_on_device
 def paged_attn_sparse(kv: PagedKV, batch: PagedBatch, q: torch.Tensor, sel: torch.Tensor, scale: float,
                       out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """paged_attn over the pages sel (paged_select's, or any choice with each page once) of each token and KV head."""
-    n_head = _paged_rows(kv, batch, q, None, "paged_attn_sparse")
+    stride, n_head = _paged_rows(kv, batch, q, 0, "paged_attn_sparse"), q.shape[1]
     if sel.dim() != 3 or sel.shape[:2] != (batch.n_tok, kv.n_head_kv) or sel.dtype != torch.int32 or not sel.is_contiguous() or \
             sel.device != kv.device:
         raise ValueError("paged_attn_sparse: sel must be contiguous int32 [n_tok, n_head_kv, pages] on the pool's GPU")
-    with _on(kv.device):
-        out = _paged_out(out, q.shape, q, "paged_attn_sparse")
-        need = batch._workspace(kv, n_head, 0, sel.shape[2])
-        ws = _paged_ws(workspace, need, q, "paged_attn_sparse")
-        check(lib().amv_paged_attn_sparse(kv._p, batch._p, sel.data_ptr(), sel.shape[2], q.data_ptr(), _row_stride(q),
-                                          out.data_ptr(), n_head, scale, _ptr(ws), need, _stream()), "amv_paged_attn_sparse")
+    out = _paged_out(out, q.shape, q, "paged_attn_sparse")
+    need = batch._workspace(kv, n_head, 0, sel.shape[2])
+    ws = _paged_ws(workspace, need, q, "paged_attn_sparse")
+    check(lib().amv_paged_attn_sparse(kv._p, batch._p, sel.data_ptr(), sel.shape[2], q.data_ptr(), stride,
+                                      out.data_ptr(), n_head, scale, _ptr(ws), need, _stream()), "amv_paged_attn_sparse")
     return out
 
 

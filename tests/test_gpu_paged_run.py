@@ -105,12 +105,12 @@ def test_prefix_is_the_same_as_a_copy_of_it():
 def test_streams_and_two_graphs():
     """Calls on a side stream, and two captured graphs in turn, each with the workspace it was captured with."""
     from ameva_compute_amd import ops
-    kv = ops.PagedKV.alloc(F16, 80, PAGE, G, D, DEV, bounds=True)
-    table = torch.randperm(80, device=DEV).int().view(2, 40)
-    n_kv = ints([600, 333])
-    fill = ops.PagedBatch(n_kv, table, 640, 933, cu_q=ints([0, 600, 933]), max_q=600)
-    ops.paged_rope_append(kv, fill, rows(933, 1), H)
-    b = ops.PagedBatch(n_kv, table, 640)
+    kv = ops.PagedKV.alloc(F16, 800, PAGE, G, D, DEV, bounds=True)
+    table = torch.randperm(800, device=DEV).int().view(2, 400)
+    n_kv = ints([6000, 333])
+    fill = ops.PagedBatch(n_kv, table, 6400, 6333, cu_q=ints([0, 6000, 6333]), max_q=6000)
+    ops.paged_rope_append(kv, fill, rows(6333, 1), H)
+    b = ops.PagedBatch(n_kv, table, 6400)
     qs = [torch.randn(2, H, D, device=DEV) for _ in range(2)]
     want = [ops.paged_attn(kv, b, q, SCALE) for q in qs]
     wsel = [ops.paged_select(kv, b, q, 6) for q in qs]
