@@ -689,10 +689,11 @@ __device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int z,
     }
 }
 
-// Many rows over f16 keys (prompts, a prefix): a tile of 128 rows, 32 of each wave, and every wave goes over all its keys, so these
-// come from memory once for the four: read by each wave for itself (pg_few), K's pieces of 16 bytes from 16 rows an instruction keep
-// the loads' address unit busy for all of the time. K and V rows of 64 keys go to LDS without registers (global_load_lds), one step
-// ahead in two buffers; the products are those of pg_few with RT = 2. The loads write LDS in lane order, so a row's pieces are
+// Many rows over f16 keys (prompts, a prefix): tiles of 32 RW rows, 32 of each wave, whose keys come from memory once for the
+// workgroup: read by each wave for itself (pg_few), K's pieces of 16 bytes from 16 rows an instruction keep the loads' address unit busy
+// for all of the time. RW = 4: every wave goes over all keys; RW = 2: two waves a row range, each with one half of every step's keys,
+// joined at the end. K and V rows of 64 keys, a step, go to LDS without registers (global_load_lds), one step ahead in two buffers; the
+// products are those of pg_few with RT = 2. The loads write LDS in lane order, so a row's pieces are
 // exchanged on the memory side: K's 16-byte pieces by a number of the key that differs among the 16 keys of an operand read, V's
 // 32-byte units by one that takes each value twice among the 16 keys of a transposing read (ds_read_b64_tr_b16: 16 lanes pointing at
 // 4 keys' 8-byte quarters of a unit get an element of the 4 keys each), so both reads meet all banks.
@@ -709,10 +710,9 @@ typedef __attribute__((address_space(3))) pg_s4 pg_lds_s4;
         __builtin_amdgcn_s_barrier();       \
         asm volatile("" ::: "memory");      \
     } while (0)
-#define PG_MANY_ROWS 128
 __device__ __align__(16) const uint8_t pg_zeros[16] = {};
 
-template <int D>
+template <int D, int RW>
 __device__ __forceinline__ void pg_many(const PgAttn& a, int hk, int tile, int z, uint16_t* sKa, uint16_t* sKb, uint16_t* sVa,
                                         uint16_t* sVb) {
     constexpr int NB = D / 32, T = D / 16, PIECES = D / 8;  // (of 16 bytes a row)
@@ -720,11 +720,11 @@ __device__ __forceinline__ void pg_many(const PgAttn& a, int hk, int tile, int z
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ps = 1 << a.b.pshift;
     PgRows t;
-    if (!pg_rows(a, hk, tile, PG_MANY_ROWS, t)) return;
+    if (!pg_rows(a, hk, tile, 32 * RW, t)) return;
     // steps of 64 keys
     const int begin = z * a.split_len >> 6, end = (min(t.see_any, (z + 1) * a.split_len) + 63) >> 6;
-    // the wave's own rows
-    const int wr0 = t.r0 + 32 * w, wr1 = min(wr0 + 31, t.r_last);
+    // the wave's own rows, and which half of a step's keys it takes
+    const int rw = w & (RW - 1), kw = w / RW, wr0 = t.r0 + 32 * rw, wr1 = min(wr0 + 31, t.r_last);
     const bool idle = wr0 > t.r_last;
     t.see(a, idle ? t.r_last : wr0, idle ? t.r_last : wr1);
     const int mine = idle ? 0 : min(end, (t.see_any + 63) >> 6);  // steps that its rows see a part of
@@ -847,8 +847,12 @@ __device__ __forceinline__ void pg_many(const PgAttn& a, int hk, int tile, int z
         }
     };
     const auto step = [&](const Step& now, const uint16_t* sK, const uint16_t* sV) {
-        half(now.a, sK, sV);
-        half(now.b, sK + 32 * D, sV + 32 * D);
+        if constexpr (RW == 4) {
+            half(now.a, sK, sV);
+            half(now.b, sK + 32 * D, sV + 32 * D);
+        } else {
+            half(kw ? now.b : now.a, sK + 32 * D * kw, sV + 32 * D * kw);
+        }
     };
     PG_BARRIER();
     for (int i = begin; i < end; i += 2) {
@@ -867,17 +871,46 @@ __device__ __forceinline__ void pg_many(const PgAttn& a, int hk, int tile, int z
         if (i + 1 < mine) step(next, sKb, sVb);
         PG_BARRIER();
     }
+    float* const ex = reinterpret_cast<float*>(rw ? sKb : sKa) + lane;  // [row tile][product][register][lane]
+    float* const ml = reinterpret_cast<float*>(sVa) + 256 * rw + lane;  // [row tile][m, l][lane]
+    if constexpr (RW == 2) {  // the second half's sums go to the first's, through the buffers
+        if (kw) {
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) {
+                ml[128 * rt] = m[rt];
+                ml[128 * rt + 64] = l[rt];
+#pragma unroll
+                for (int v = 0; v < T; ++v)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) ex[64 * ((rt * T + v) * 4 + r)] = o[rt][v][r];
+            }
+        }
+        __syncthreads();
+        if (kw) return;
+    }
     if (idle) return;
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
-        const float L = amv_sum_x32(amv_sum_x16(l[rt]));
+        float L = l[rt];
+        if constexpr (RW == 2) {
+            const float m1 = ml[128 * rt], M = fmaxf(m[rt], m1);
+            const float f0 = m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - M);
+            const float f1 = m1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m1 - M);
+            L = fmaf(L, f0, ml[128 * rt + 64] * f1);
+            m[rt] = M;
+#pragma unroll
+            for (int v = 0; v < T; ++v)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[rt][v][r] = fmaf(o[rt][v][r], f0, ex[64 * ((rt * T + v) * 4 + r)] * f1);
+        }
+        L = amv_sum_x32(amv_sum_x16(L));
         const int r = t.r0 + 16 * rt + c;
         if (r > t.r_last) continue;
-        float2* ml;
-        float* to = pg_to<D>(a, t, hk, r, z, &ml);
+        float2* part;
+        float* to = pg_to<D>(a, t, hk, r, z, &part);
         float inv = 1.0f;
-        if (!ml) inv = L > 0.0f ? 1.0f / L : L;
-        else if (g == 0) *ml = make_float2(m[rt], L);
+        if (!part) inv = L > 0.0f ? 1.0f / L : L;
+        else if (g == 0) *part = make_float2(m[rt], L);
 #pragma unroll
         for (int v = 0; v < T; ++v) {
             const pg_f4 y = o[rt][v] * inv;
@@ -906,7 +939,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PgJobs jobs) {  // jobs 1 
     pg_place_of(jobs.a[k], k == 1 ? b : b - jobs.n[1], hk, tile, z);
     pg_few<TYPE, D, RT, P>(jobs.a[k], hk, tile, z, so[0], so[1]);
 }
-template <int TYPE, int D, int RT, int P>
+template <int TYPE, int D, int RT, int P, int RW>
 __global__ __launch_bounds__(256, 2) void k_paged_many_few(PgJobs jobs) {  // jobs 0 and 1 of many rows, 2 of few
     // buffers as variables of their own: reads of one do not wait for the loads into another
     __shared__ __align__(16) uint16_t sKa[64 * D], sKb[64 * D], sVa[64 * D], sVb[64 * D];
@@ -917,7 +950,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_many_few(PgJobs jobs) {  // jo
     if (k > 1) b -= jobs.n[1];
     pg_place_of(jobs.a[k], b, hk, tile, z);
     if (k == 2) pg_few<TYPE, D, RT, P>(jobs.a[2], hk, tile, z, so0, so1);
-    else if constexpr (TYPE == AMV_T_F16) pg_many<D>(jobs.a[k], hk, tile, z, sKa, sKb, sVa, sVb);
+    else if constexpr (TYPE == AMV_T_F16) pg_many<D, RW>(jobs.a[k], hk, tile, z, sKa, sKb, sVa, sVb);
     else pg_few<TYPE, D, 2, 1>(jobs.a[k], hk, tile, z, so0, so1);
 }
 
@@ -998,7 +1031,7 @@ static PgTiles pg_tiles(int64_t rows) { return {rows > 16 ? 2 : 1, rows <= 4 ? 4
 struct PgPlan {
     PgTiles few;                            // tiles of few rows: sequences (or listed tokens), ta tiles each, and a small batch's prefix
     int ta, n_one, len_one;                 // their parts
-    int many_rows;                          // rows of the other tiles
+    int many_rows;                          // rows of the other tiles: 64 or 128, of quantized keys 32
     int find, rows_most, n_find, len_find;  // sequences of more rows than rows_most
     int64_t find_tiles;
     bool pre_many;                          // the prefix in tiles of many rows
@@ -1009,9 +1042,9 @@ struct PgPlan {
 // parts of `keys` keys for `units` workgroups' worth of rows: two workgroups a CU, none of less than 128 keys (a tile for each of its
 // waves), and up to 256 keys no parts, as their merge is a launch of its own. More and shorter parts cost their prologues and the merge (us at 512 / 1024 / 2048 workgroups: 64 sequences of up to 4096
 // f16 keys 136 / 147 / 144, 3 of 65536 Q8_0 keys 78 / 78 / 82, one of 777 with parts of 256 keys 9.6, of 128 9.3)
-static int pg_parts(int64_t units, int64_t keys, int* len) {
+static int pg_parts(int64_t units, int64_t keys, int* len, int target = 512) {
     units = std::max<int64_t>(1, units);
-    const int64_t n = keys <= 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(512 / units, (keys + 127) / 128));
+    const int64_t n = keys <= 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(target / units, (keys + 127) / 128));
     int64_t l = ((keys + n - 1) / n + 127) / 128 * 128;
     l = std::max<int64_t>(128, l);
     *len = (int)l;
@@ -1028,20 +1061,26 @@ static PgPlan pg_plan(const amv_paged_kv* kv, const amv_paged_batch* b, int64_t 
         return p;
     }
     const int64_t rows = std::min(b->max_q, b->n_tok) * G;
-    p.many_rows = kv->type == AMV_T_F16 ? PG_MANY_ROWS : 32;
     p.pre_many = all > 32;
     p.few = pg_tiles(n_prefix > 0 && !p.pre_many ? all : rows <= 32 ? rows : G);
     p.rows_most = (int)std::max<int64_t>(p.few.rows(), G);
     p.ta = p.few.of(p.rows_most);
     p.n_one = pg_parts(b->n_seq * kv->n_head_kv * p.ta, b->max_kv, &p.len_one);
     p.find = rows > p.rows_most;
+    // Tiles of 128 rows do more with a step (8192 tokens 996 us, with 64 rows 1150; 512 after 7488 others 174 and 219; 128 sequences behind
+    // 16384 keys 107 and 119), those of 64 rows share the GPU more evenly where the larger are no more than a few for each CU and
+    // not cut into parts (2048 tokens 104 and 113, 512 28 and 35), and read a prefix for up to 64 rows as soon.
+    const int64_t large = all / 128 * kv->n_head_kv;
+    const bool even = (!p.find || b->max_kv <= 1024 || (large >= 256 && large < 1024)) && (n_prefix == 0 || all <= 64);
+    p.many_rows = kv->type != AMV_T_F16 ? 32 : even ? 64 : 128;
     if (p.find) {
         p.find_tiles = all / p.many_rows + b->n_seq;
         p.n_find = pg_parts(all / p.many_rows * kv->n_head_kv + 1, b->max_kv, &p.len_find);
     }
     if (n_prefix > 0) {
         p.pre_tiles = p.pre_many ? (int)((all + p.many_rows - 1) / p.many_rows) : p.few.of(all);
-        p.n_pre = pg_parts(p.pre_tiles * kv->n_head_kv, n_prefix, &p.len_pre);
+        // (fewer parts: each is all rows' sums again. 32 sequences behind 8192 keys 39 us with 512, 31 with 384)
+        p.n_pre = pg_parts(p.pre_tiles * kv->n_head_kv, n_prefix, &p.len_pre, p.pre_many ? 384 : 512);
     }
     if (p.n_one > 1 || p.n_pre) p.w_one = b->n_seq * kv->n_head_kv * p.rows_most * p.n_one;
     if (p.find && (p.n_find > 1 || p.n_pre)) p.w_many = b->n_tok * n_head * p.n_find;
@@ -1056,19 +1095,20 @@ extern "C" int64_t amv_paged_attn_workspace_bytes(const amv_paged_kv* kv, const 
 }
 
 template <int TYPE, int D, int RT, int P>
-static void pg_launch(const PgJobs& j, bool many, hipStream_t st) {
+static void pg_launch(const PgJobs& j, int many, hipStream_t st) {
     const dim3 grid((unsigned)(j.n[0] + j.n[1] + j.n[2]));
-    if (many) hipLaunchKernelGGL((k_paged_many_few<TYPE, D, RT, P>), grid, dim3(256), 0, st, j);
+    if (many == 64 && TYPE == AMV_T_F16) hipLaunchKernelGGL((k_paged_many_few<TYPE, D, RT, P, TYPE == AMV_T_F16 ? 2 : 4>), grid, dim3(256), 0, st, j);
+    else if (many) hipLaunchKernelGGL((k_paged_many_few<TYPE, D, RT, P, 4>), grid, dim3(256), 0, st, j);
     else hipLaunchKernelGGL((k_paged_few<TYPE, D, RT, P>), grid, dim3(256), 0, st, j);
 }
 template <int TYPE, int D>
-static void pg_launch(const PgJobs& j, PgTiles t, bool many, hipStream_t st) {
+static void pg_launch(const PgJobs& j, PgTiles t, int many, hipStream_t st) {
     if (t.pack == 4) pg_launch<TYPE, D, 1, 4>(j, many, st);
     else if (t.pack == 2) pg_launch<TYPE, D, 1, 2>(j, many, st);
     else if (t.rt == 1) pg_launch<TYPE, D, 1, 1>(j, many, st);
     else pg_launch<TYPE, D, 2, 1>(j, many, st);
 }
-static void pg_launch(int type, int D, const PgJobs& j, PgTiles t, bool many, hipStream_t st) {
+static void pg_launch(int type, int D, const PgJobs& j, PgTiles t, int many, hipStream_t st) {
     if (D == 128) {
         if (type == AMV_T_F16) pg_launch<AMV_T_F16, 128>(j, t, many, st);
         else if (type == AMV_T_Q8_0) pg_launch<AMV_T_Q8_0, 128>(j, t, many, st);
@@ -1132,7 +1172,7 @@ static int pg_attn(const char* what, const amv_paged_kv* kv, const amv_paged_bat
     if (n_sel > 0) job(2, PG_LIST, b->n_tok * p.ta, p.n_one, p.len_one, m.many);
     else job(2, PG_ONE, b->n_seq * p.ta, p.n_one, p.len_one, m.one);
     hipStream_t st = amv_stream(stream);
-    pg_launch(kv->type, kv->D, jobs, p.few, p.find || (p.n_pre && p.pre_many), st);
+    pg_launch(kv->type, kv->D, jobs, p.few, p.find || (p.n_pre && p.pre_many) ? p.many_rows : 0, st);
     if (p.w_one + p.w_many + p.w_pre) {
         const dim3 grid((unsigned)((rows + 3) / 4));
         if (kv->D == 128) hipLaunchKernelGGL(k_paged_merge<128>, grid, dim3(256), 0, st, m);
