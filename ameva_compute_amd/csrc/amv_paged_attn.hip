@@ -158,15 +158,18 @@ __device__ __forceinline__ void pg_load_v(PgV<TYPE, D, KPL>& t, const PgAttn& a,
     }
 }
 
-// integers u (value + 8 or + 128) in the low bits of a word's two halves, as f16 values times 2^-10: such a half is the f16 u 2^-24,
-// and u 2^-24 2^14 - bias 2^-10 is exact
+// Integers u = value + bias in the low bits of a word's two halves are, as they stand, the f16 u 2^-24. Values become operands times
+// 2^-10: u 2^-24 2^14 - bias 2^-10 is exact.
+template <int TYPE>
+__device__ __forceinline__ constexpr float pg_bias() { return TYPE == AMV_T_Q8_0 ? 128.0f : 8.0f; }
 template <int TYPE>
 __device__ __forceinline__ uint32_t pg_f16_of(uint32_t u) {
-    constexpr float bias = (TYPE == AMV_T_Q8_0 ? 128.0f : 8.0f) / 1024.0f;
+    constexpr float bias = pg_bias<TYPE>() / 1024.0f;
     const amv_h2 m = {(_Float16)16384.0f, (_Float16)16384.0f}, b = {(_Float16)-bias, (_Float16)-bias};
     return pg_bits(__builtin_elementwise_fma(__builtin_bit_cast(amv_h2, u), m, b));
 }
-// the operand of product s of K: 8 f16
+// The operand of product s of K: 8 f16; of quantized keys (value + bias) 2^-24, whose product begins at -bias 2^-24 times the sum of
+// q's elements, so that no instruction is spent on the bias (it rounds at the size of the biased sums: some 2 or 3 bits of the 24 more)
 template <int TYPE, int D>
 __device__ __forceinline__ pg_h8 pg_k_operand(const uint32_t* k, int s) {
     amv_v4u x;
@@ -176,15 +179,15 @@ __device__ __forceinline__ pg_h8 pg_k_operand(const uint32_t* k, int s) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t w = k[2 * s + h] ^ 0x80808080u;
-            x[2 * h] = pg_f16_of<TYPE>(__builtin_amdgcn_perm(0u, w, 0x0C010C00u));
-            x[2 * h + 1] = pg_f16_of<TYPE>(__builtin_amdgcn_perm(0u, w, 0x0C030C02u));
+            x[2 * h] = __builtin_amdgcn_perm(0u, w, 0x0C010C00u);
+            x[2 * h + 1] = __builtin_amdgcn_perm(0u, w, 0x0C030C02u);
         }
     } else {
         const uint32_t even = k[s] & 0x0F0F0F0Fu, odd = (k[s] >> 4) & 0x0F0F0F0Fu;
-        x[0] = pg_f16_of<TYPE>(__builtin_amdgcn_perm(odd, even, 0x0C040C00u));
-        x[1] = pg_f16_of<TYPE>(__builtin_amdgcn_perm(odd, even, 0x0C050C01u));
-        x[2] = pg_f16_of<TYPE>(__builtin_amdgcn_perm(odd, even, 0x0C060C02u));
-        x[3] = pg_f16_of<TYPE>(__builtin_amdgcn_perm(odd, even, 0x0C070C03u));
+        x[0] = __builtin_amdgcn_perm(odd, even, 0x0C040C00u);
+        x[1] = __builtin_amdgcn_perm(odd, even, 0x0C050C01u);
+        x[2] = __builtin_amdgcn_perm(odd, even, 0x0C060C02u);
+        x[3] = __builtin_amdgcn_perm(odd, even, 0x0C070C03u);
     }
     return __builtin_bit_cast(pg_h8, x);
 }
@@ -322,7 +325,7 @@ __device__ __forceinline__ float pg_query(const PgAttn& a, const PgRows& t, int 
         }
     }
     am = amv_max_x32(amv_max_x16(am));
-    const uint32_t e = max(1u, min(253u, __float_as_uint(am) >> 23));
+    const uint32_t e = max(1u, min(229u, __float_as_uint(am) >> 23));  // (2^e 2^24 is a number)
     const float down = __uint_as_float((254u - e) << 23);
 #pragma unroll
     for (int s = 0; s < D / 32; ++s)
@@ -432,10 +435,10 @@ __device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int z,
     // Q^T operands: values times scale log2(e) 2^-e below 2, P = 1: as f16 and the rest in two operands, P = 2: in the two halves of
     // the columns of one, P = 4 and quantized keys: of two, one for each product u, that is 0 where the columns keep the other's keys,
     // so that the products add up to what each column keeps (f16 keys may be infinite or no number where nobody sees them: 0 times
-    // them would not be 0, so there each column picks its product). f: 2^e (for quantized keys times the 2^10 that their operands
-    // lack); lim: keys the row sees
+    // them would not be 0, so there each column picks its product). f: 2^e (for quantized keys times the 2^24 that their operands
+    // lack); lim: keys the row sees; q0: where the products of quantized keys begin
     pg_h8 qa[RT][P == 2 || (P == 4 && !QUANT) ? 1 : 2][NB];
-    float f[RT];
+    float f[RT], q0[RT][QUANT ? NB : 1];
     int lim[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -460,8 +463,15 @@ __device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int z,
                     qa[rt][1][s] = __builtin_bit_cast(pg_h8, hw & ~k0);
                 }
             }
+            if constexpr (QUANT) {
+                float sum = 0.0f;  // of what the products multiply: the two parts, or the column's
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    sum += P == 2 ? (float)qa[rt][0][s][j] : (float)qa[rt][0][s][j] + (float)qa[rt][1][s][j];
+                q0[rt][s] = amv_sum_x32(amv_sum_x16(sum)) * (-pg_bias<TYPE>() * 0x1p-24f);
+            }
         }
-        if constexpr (QUANT) f[rt] *= 1024.0f;
+        if constexpr (QUANT) f[rt] *= 0x1p24f;
     }
 
     float m[RT], l[RT];
@@ -496,7 +506,10 @@ __device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int z,
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                    for (int h = 0; h < X; ++h) x[rt][h] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int h = 0; h < X; ++h) {
+                        const float y = QUANT ? q0[rt][QUANT ? b : 0] : 0.0f;
+                        x[rt][h] = pg_f4{y, y, y, y};
+                    }
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
