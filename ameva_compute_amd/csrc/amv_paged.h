@@ -3,6 +3,7 @@
 #pragma once
 #include "amv_common.h"
 
+#define PG_MAX_GROUPS (1 << 23)  // workgroups of a launch (of up to 256 threads: a grid has less than 2^32)
 #define PG_MAX_PAGES 16384  // pages of one sequence that amv_paged_select ranks (their scores are in LDS, 8 bytes each)
 
 // one key's (or value's) integers and scales in a chunk

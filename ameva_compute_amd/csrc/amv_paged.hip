@@ -32,7 +32,7 @@ int pg_check(const char* what, const amv_paged_kv* kv, const amv_paged_batch* b,
     AMV_REQUIRE(b->n_kv && b->table && b->n_seq > 0 && b->n_tok >= 0 && b->max_q > 0 && b->max_kv >= 0,
                 "%s: null lengths or table, or a bad size", what);
     AMV_REQUIRE(b->n_seq <= 65535 && b->n_tok <= (int64_t)1 << 24 && b->max_kv <= (int64_t)1 << 30 &&
-                    b->n_tok * n_head <= (int64_t)1 << 30,
+                    b->n_tok * n_head <= 4 * (int64_t)PG_MAX_GROUPS,
                 "%s: batch too large", what);
     AMV_REQUIRE(b->cu_q || (b->n_tok == b->n_seq && b->max_q == 1), "%s: without cu_q there is one token a sequence", what);
     AMV_REQUIRE(b->table_stride >= (b->max_kv + kv->page_size - 1) / kv->page_size,
@@ -272,6 +272,7 @@ extern "C" int amv_paged_rope_append(const amv_paged_kv* kv, const amv_paged_bat
                   (int)(n_head / kv->n_head_kv), n_dims, mode == 2, rule, one};
     // n tokens touch at most (n - 1) / page_size + 2 pages
     const int64_t items = one ? batch->n_seq : batch->n_tok / kv->page_size + 2 * batch->n_seq;
+    AMV_REQUIRE(items * kv->n_head_kv <= PG_MAX_GROUPS, "%s: batch too large", what);
     const dim3 grid((unsigned)(items * kv->n_head_kv)), block(one ? 64 : 256);
     const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, amv_stream(stream), a); };
     if (kv->D == 128) {
@@ -516,6 +517,7 @@ extern "C" int amv_paged_select(const amv_paged_kv* kv, const amv_paged_batch* b
     const int64_t need = batch->n_tok * kv->n_head_kv * most * 8;
     AMV_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need),
                 "%s: workspace of %lld bytes, %lld needed (16-byte aligned)", what, (long long)workspace_bytes, (long long)need);
+    AMV_REQUIRE(batch->n_tok * kv->n_head_kv <= PG_MAX_GROUPS, "%s: batch too large", what);
     PgSelect a = {pg_batch(kv, batch), q, (const uint16_t*)kv->bounds, (double*)workspace, sel, q_stride, (int)kv->n_pages,
                   kv->n_head_kv, (int)(n_head / kv->n_head_kv), (int)most, (int)n_sel, (int)n_first, (int)n_last};
     hipStream_t st = amv_stream(stream);

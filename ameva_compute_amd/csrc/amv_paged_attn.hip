@@ -216,6 +216,17 @@ __device__ __forceinline__ pg_h8 pg_v_operand(const PgV<TYPE, D, KPL>& v, int t)
     }
     return __builtin_bit_cast(pg_h8, x);
 }
+// 1 in the halves of a word that are infinite or no number
+__device__ __forceinline__ uint32_t pg_strange(uint32_t w) { return (((w & 0x7C007C00u) + 0x04000400u) >> 15) & 0x00010001u; }
+// Values that are infinite or no number, where a tile's rows see different keys: a row that does not see such a value has the weight 0
+// for it, and the product would make no number of it. Such keys (bits j: the lane's keys 8 g + j) leave the products, and a row that sees
+// one gets a sum that is no number.
+__device__ __forceinline__ uint32_t pg_row16_or(uint32_t x) {
+    x |= (uint32_t)amv_dpp_i<0xB1>((int)x);
+    x |= (uint32_t)amv_dpp_i<0x4E>((int)x);
+    x |= (uint32_t)amv_dpp_i<0x141>((int)x);
+    return x | (uint32_t)amv_dpp_i<0x140>((int)x);
+}
 // 8 values as f16 and the rest as f16
 __device__ __forceinline__ void pg_split(const float (&x)[8], pg_h8& hi, pg_h8& lo) {
 #pragma unroll
@@ -371,9 +382,9 @@ __device__ __forceinline__ float* pg_to(const PgAttn& a, const PgRows& t, int hk
     return a.ml ? a.acc + part * D : a.out + row * D;
 }
 
-// The waves of the workgroup take the tile's keys in turn, each for all its rows
+// The waves of the workgroup take the tile's keys in turn, each for all its rows: rows 16 RT / P sub .. of tile `tile` of `rows`
 template <int TYPE, int D, int RT, int P>
-__device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int z, float* so0, float* so1) {
+__device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int rows, int sub, int z, float* so0, float* so1) {
     using R = PgRow<TYPE, D>;
     constexpr int NB = D / 32, T = D / 16, ROWS = 16 / P, KPL = P == 4 ? 4 : 8;
     constexpr bool QUANT = TYPE != AMV_T_F16;
@@ -390,7 +401,12 @@ __device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int z,
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int psh = a.b.pshift, ps = 1 << psh;
     PgRows t;
-    if (!pg_rows(a, hk, tile, ROWS * RT, t)) return;
+    if (!pg_rows(a, hk, tile, rows, t)) return;
+    if (rows > ROWS * RT) {
+        const int r0 = t.r0 + ROWS * RT * sub;
+        if (r0 > t.r_last) return;
+        t.see(a, r0, min(r0 + ROWS * RT - 1, t.r_last));
+    }
 
     // the walk: 32-key tiles i = begin + w, begin + w + 4, ... of the keys (of the listed pages' keys)
     int walk = t.see_any;
@@ -550,35 +566,17 @@ __device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int z,
                 for (int j = 0; j < KPL; ++j) s[rt][j] = there && p + 4 * u + j < lim[rt] ? s[rt][j] : -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {  // what lies there must not matter, 0 times infinity is no number
-                const uint32_t keep = there && p + j < t.keys ? 0xFFFFFFFFu : 0u;
+                const uint32_t keep = there && p + j < t.see_any ? 0xFFFFFFFFu : 0u;
 #pragma unroll
                 for (int x = 0; x < PgV<TYPE, D, KPL>::W; ++x) tv.v[j][x] &= keep;
             }
             if constexpr (QUANT) {
 #pragma unroll
                 for (int j = 0; j < KPL; ++j) {
-                    const uint32_t keep = there && p + 4 * u + j < t.keys ? 0xFFFFFFFFu : 0u;
+                    const uint32_t keep = there && p + 4 * u + j < t.see_any ? 0xFFFFFFFFu : 0u;
 #pragma unroll
                     for (int b = 0; b < NB; b += 2) tv.s[(j * NB + b) >> 1] &= keep;
                 }
-            }
-        }
-        if constexpr (QUANT) {  // the values' largest scale
-            amv_h2 big = {(_Float16)0.0f, (_Float16)0.0f};
-#pragma unroll
-            for (int x = 0; x < KPL * NB / 2; ++x)
-                big = __builtin_elementwise_max(big, __builtin_bit_cast(amv_h2, tv.s[x] & 0x7FFF7FFFu));
-            float top = amv_max_x32(amv_max_x16(fmaxf((float)big.x, (float)big.y)));
-            if constexpr (P == 4) top = fmaxf(top, pg_dpp<PG_ROR8>(top));
-            if (__builtin_amdgcn_readfirstlane(top > vref)) {
-                const uint32_t e = min(253u, (__float_as_uint(top) >> 23) + 1u);
-                const float up = __uint_as_float(e << 23), by = vref * __uint_as_float((254u - e) << 23);
-                vref = up;
-                vdown = __uint_as_float((254u - e) << 23);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int v = 0; v < T; ++v) o[rt][v] *= by;
             }
         }
         pg_h8 ph[RT], pl[RT];  // P^T operands: the weights and their rest, or (P > 1) both in one
@@ -600,6 +598,58 @@ __device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int z,
                 ph[rt] = __builtin_bit_cast(pg_h8, o4);
             }
         };
+        if (some && t.see_all < t.see_any) {
+            uint32_t strange = 0;  // bits of the lane's keys
+            if constexpr (QUANT) {  // (a scale is a whole block's)
+#pragma unroll
+                for (int x = 0; x < KPL * NB / 2; ++x) {
+                    const uint32_t b = pg_strange(tv.s[x]);
+                    strange |= b ? 1u << (4 * u + 2 * x / NB) : 0u;
+                    tv.s[x] &= ~(b * 0xFFFFu);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int x = 0; x < PgV<TYPE, D, KPL>::W; ++x) {
+                        const uint32_t b = pg_strange(tv.v[j][x]);
+                        strange |= b ? 1u << j : 0u;
+                        tv.v[j][x] &= ~(b * 0xFFFFu);
+                    }
+                strange = pg_row16_or(strange);
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+                if (strange & ((1u << max(0, min(8, lim[rt] - p))) - 1)) l[rt] = __uint_as_float(0x7FC00000u);
+        }
+        if constexpr (QUANT) {  // the values' largest scale
+            amv_h2 big = {(_Float16)0.0f, (_Float16)0.0f};
+#pragma unroll
+            for (int x = 0; x < KPL * NB / 2; ++x)
+                big = __builtin_elementwise_max(big, __builtin_bit_cast(amv_h2, tv.s[x] & 0x7FFF7FFFu));
+            float top = amv_max_x32(amv_max_x16(fmaxf((float)big.x, (float)big.y)));
+            if constexpr (P == 4) top = fmaxf(top, pg_dpp<PG_ROR8>(top));
+            if (__builtin_amdgcn_readfirstlane(top == INFINITY)) {  // (it is its own rows' matter: the largest of the others)
+                float y = 0.0f;
+#pragma unroll
+                for (int x = 0; x < KPL * NB; ++x) {
+                    const float z = fabsf(pg_half(tv.s, x));
+                    y = z < INFINITY ? fmaxf(y, z) : y;
+                }
+                top = amv_max_x32(amv_max_x16(y));
+                if constexpr (P == 4) top = fmaxf(top, pg_dpp<PG_ROR8>(top));
+            }
+            if (__builtin_amdgcn_readfirstlane(top > vref)) {
+                const uint32_t e = min(253u, (__float_as_uint(top) >> 23) + 1u);
+                const float up = __uint_as_float(e << 23), by = vref * __uint_as_float((254u - e) << 23);
+                vref = up;
+                vdown = __uint_as_float((254u - e) << 23);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int v = 0; v < T; ++v) o[rt][v] *= by;
+            }
+        }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             pg_soften<P>(s[rt], f[rt], m[rt], l[rt], o[rt], pw[rt]);
@@ -725,15 +775,16 @@ typedef __attribute__((address_space(3))) pg_s4 pg_lds_s4;
     } while (0)
 __device__ __align__(16) const uint8_t pg_zeros[16] = {};
 
+// (true: nothing is written, as a sum is no number: a value that not all rows see may be the reason, which pg_few leaves out)
 template <int D, int RW>
-__device__ __forceinline__ void pg_many(const PgAttn& a, int hk, int tile, int z, uint16_t* sKa, uint16_t* sKb, uint16_t* sVa,
+__device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z, uint16_t* sKa, uint16_t* sKb, uint16_t* sVa,
                                         uint16_t* sVb) {
     constexpr int NB = D / 32, T = D / 16, PIECES = D / 8;  // (of 16 bytes a row)
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ps = 1 << a.b.pshift;
     PgRows t;
-    if (!pg_rows(a, hk, tile, 32 * RW, t)) return;
+    if (!pg_rows(a, hk, tile, 32 * RW, t)) return false;
     // steps of 64 keys
     const int begin = z * a.split_len >> 6, end = (min(t.see_any, (z + 1) * a.split_len) + 63) >> 6;
     // the wave's own rows, and which half of a step's keys it takes
@@ -886,6 +937,16 @@ __device__ __forceinline__ void pg_many(const PgAttn& a, int hk, int tile, int z
     }
     float* const ex = reinterpret_cast<float*>(rw ? sKb : sKa) + lane;  // [row tile][product][register][lane]
     float* const ml = reinterpret_cast<float*>(sVa) + 256 * rw + lane;  // [row tile][m, l][lane]
+    float sum = 0.0f;  // no number: one of the sums is none, or infinite
+    if (!idle)
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            sum = fmaf(l[rt], 0.0f, sum);
+#pragma unroll
+            for (int v = 0; v < T; ++v)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum = fmaf(o[rt][v][r], 0.0f, sum);
+        }
     if constexpr (RW == 2) {  // the second half's sums go to the first's, through the buffers
         if (kw) {
 #pragma unroll
@@ -898,10 +959,9 @@ __device__ __forceinline__ void pg_many(const PgAttn& a, int hk, int tile, int z
                     for (int r = 0; r < 4; ++r) ex[64 * ((rt * T + v) * 4 + r)] = o[rt][v][r];
             }
         }
-        __syncthreads();
-        if (kw) return;
     }
-    if (idle) return;
+    if (__syncthreads_or(sum != sum)) return true;
+    if (idle || (RW == 2 && kw)) return false;
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
         float L = l[rt];
@@ -930,6 +990,7 @@ __device__ __forceinline__ void pg_many(const PgAttn& a, int hk, int tile, int z
             *reinterpret_cast<pg_f4*>(to + 16 * v + 4 * g) = y;
         }
     }
+    return false;
 }
 
 // A launch has up to three jobs, one after the other over the workgroups, so that one's reading fills the other's computing: tiles of
@@ -950,7 +1011,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PgJobs jobs) {  // jobs 1 
     const int b = (int)blockIdx.x, k = b < jobs.n[1] ? 1 : 2;
     int hk, tile, z;
     pg_place_of(jobs.a[k], k == 1 ? b : b - jobs.n[1], hk, tile, z);
-    pg_few<TYPE, D, RT, P>(jobs.a[k], hk, tile, z, so[0], so[1]);
+    pg_few<TYPE, D, RT, P>(jobs.a[k], hk, tile, 16 * RT / P, 0, z, so[0], so[1]);
 }
 template <int TYPE, int D, int RT, int P, int RW>
 __global__ __launch_bounds__(256, 2) void k_paged_many_few(PgJobs jobs) {  // jobs 0 and 1 of many rows, 2 of few
@@ -962,9 +1023,18 @@ __global__ __launch_bounds__(256, 2) void k_paged_many_few(PgJobs jobs) {  // jo
     if (k > 0) b -= jobs.n[0];
     if (k > 1) b -= jobs.n[1];
     pg_place_of(jobs.a[k], b, hk, tile, z);
-    if (k == 2) pg_few<TYPE, D, RT, P>(jobs.a[2], hk, tile, z, so0, so1);
-    else if constexpr (TYPE == AMV_T_F16) pg_many<D, RW>(jobs.a[k], hk, tile, z, sKa, sKb, sVa, sVb);
-    else pg_few<TYPE, D, 2, 1>(jobs.a[k], hk, tile, z, so0, so1);
+    if constexpr (TYPE == AMV_T_F16) {
+        constexpr int ROWS = 16 * RT / P;
+        if (k < 2 && !pg_many<D, RW>(jobs.a[k], hk, tile, z, sKa, sKb, sVa, sVb)) return;
+        const int rows = k < 2 ? 32 * RW : ROWS;
+        for (int sub = 0; sub < rows / ROWS; ++sub) {
+            if (sub) __syncthreads();
+            pg_few<TYPE, D, RT, P>(jobs.a[k], hk, tile, rows, sub, z, so0, so1);
+        }
+    } else {
+        if (k == 2) pg_few<TYPE, D, RT, P>(jobs.a[2], hk, tile, 16 * RT / P, 0, z, so0, so1);
+        else pg_few<TYPE, D, 2, 1>(jobs.a[k], hk, tile, 32, 0, z, so0, so1);
+    }
 }
 
 // out = sum_z w_z O_z / sum_z w_z l_z over the parts z of a row's keys, w_z = 2^(m_z - max m): one wave per row. A row has parts of
@@ -1167,6 +1237,7 @@ static int pg_attn(const char* what, const amv_paged_kv* kv, const amv_paged_bat
                  {ml + p.w_one + p.w_many, acc + (p.w_one + p.w_many) * kv->D, p.n_pre},
                  out, (int)n_head, kv->n_head_kv, a.G, n_sel > 0 ? -1 : p.rows_most};
     PgJobs jobs = {};
+    int64_t groups = 0;
     const auto job = [&](int k, int kind, int64_t tiles, int parts, int len, const PgParts& into) {
         PgAttn& x = jobs.a[k] = a;
         x.kind = kind;
@@ -1179,11 +1250,13 @@ static int pg_attn(const char* what, const amv_paged_kv* kv, const amv_paged_bat
         x.ml = into.n ? const_cast<float2*>(into.ml) : nullptr;
         x.acc = const_cast<float*>(into.acc);
         jobs.n[k] = (int)(tiles * parts * kv->n_head_kv);
+        groups += tiles * parts * kv->n_head_kv;
     };
     if (p.find) job(0, PG_FIND, p.find_tiles, p.n_find, p.len_find, m.many);
     if (p.n_pre) job(1, PG_PREFIX, p.pre_tiles, p.n_pre, p.len_pre, m.pre);
     if (n_sel > 0) job(2, PG_LIST, b->n_tok * p.ta, p.n_one, p.len_one, m.many);
     else job(2, PG_ONE, b->n_seq * p.ta, p.n_one, p.len_one, m.one);
+    AMV_REQUIRE(groups <= PG_MAX_GROUPS, "%s: batch too large", what);
     hipStream_t st = amv_stream(stream);
     pg_launch(kv->type, kv->D, jobs, p.few, p.find || (p.n_pre && p.pre_many) ? p.many_rows : 0, st);
     if (p.w_one + p.w_many + p.w_pre) {

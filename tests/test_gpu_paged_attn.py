@@ -279,3 +279,70 @@ def test_all_pages_selected_is_dense():
     q = torch.randn(2, 8, 128, device=DEV)
     sel = ops.paged_select(w.cache, w.batch(), q, 30)
     assert off(ops.paged_attn_sparse(w.cache, w.batch(), q, sel, 0.09), ops.paged_attn(w.cache, w.batch(), q, 0.09).double()) < TOL
+
+
+# ------------------------------------------------------------------------------------------------- what nobody may see
+@pytest.mark.parametrize("t", [F16, Q8_0, Q4_0])
+@pytest.mark.parametrize("heads,g,d,page,n_kv,n_q", [
+    (32, 8, 128, 64, [300, 70, 40], [4, 2, 1]),
+    (8, 2, 128, 16, [700, 33, 64], [260, 33, 1]),
+    (8, 2, 128, 16, [1300, 33], [260, 33]),
+    (6, 2, 64, 32, [1200, 90], [200, 9]),
+    (40, 2, 128, 64, [100, 64], [3, 1]),
+])
+def test_later_tokens_do_not_matter(t, heads, g, d, page, n_kv, n_q):
+    """A token whose value is infinite or no number, one whose key is: tokens before it, in the same tile or not, do not see it; what
+    those behind it get there is no number, and elements and heads that it does not reach are right."""
+    from ameva_compute_amd import ops
+    w = World(t, g, d, page, n_kv, n_q, seed=n_kv[0])
+    q = torch.randn(w.first[-1], heads, d, device=DEV)
+    r = attend(w, q, d ** -0.5)
+    for s, (n, m) in enumerate(zip(n_kv, n_q)):
+        place = n - 1 - m // 2
+        e, slot = int(w.table[s, place // page]), place % page
+        if t == F16:
+            w.cache.v[e, 0, slot, 5], w.cache.v[e, 0, slot, 40] = math.nan if s & 1 else -math.inf, math.inf
+            w.cache.k[e, 1, slot, 3] = math.nan
+        else:
+            ni = page * d // (1 if t == Q8_0 else 2)
+            v, k = (x[..., ni:].view(torch.float16).view(-1, g, page, d // 32) for x in (w.cache.v, w.cache.k))
+            v[e, 0, slot, 1] = math.nan if s & 1 else math.inf
+            k[e, 1, slot, 0] = math.nan
+    y, G = ops.paged_attn(w.cache, w.batch(), q, d ** -0.5), heads // g
+    for s, (n, m) in enumerate(zip(n_kv, n_q)):
+        a, at, e = w.first[s], w.first[s] + m - 1 - m // 2, w.first[s] + m
+        if at > a:
+            assert off(y[a:at], r[a:at]) < TOL, s
+        hit = [5, 40] if t == F16 else list(range(32, 64))
+        assert not y[at:e, :G][..., hit].isfinite().any() and y[at:e, G:2 * G].isnan().all(), s
+        if g > 2:
+            assert off(y[at:e, 2 * G:], r[at:e, 2 * G:]) < TOL, s
+        if m == 1:
+            rest = [i for i in range(d) if i not in hit]
+            assert off(y[at:e, :G][..., rest], r[at:e, :G][..., rest]) < TOL, s
+
+
+@pytest.mark.parametrize("t", [F16, Q4_0])
+def test_more_sequences_than_lanes(t):
+    """150 sequences: steps, a few tokens, prompts, sequences without tokens or without keys, in no order."""
+    n_kv = [(37 * i) % 211 for i in range(150)]
+    n_q = [min(n, (0, 1, 1, 5, 40)[i * 7 % 5]) for i, n in enumerate(n_kv)]
+    w = World(t, 2, 64, 16, n_kv, n_q, seed=11)
+    y, r = run(w, 8, pad=2)
+    for s in range(150):
+        a, e = w.first[s], w.first[s + 1]
+        assert off(y[a:e], r[a:e]) < TOL, s
+
+
+@pytest.mark.parametrize("t", [F16, Q8_0])
+@pytest.mark.parametrize("heads,g,d,prefix,n,kv", [(16, 4, 128, 700, 150, 3), (8, 2, 64, 2100, 70, 40), (4, 1, 128, 1500, 40, 300)])
+def test_shared_prefix_of_many_sequences(t, heads, g, d, prefix, n, kv):
+    """More rows than 128 behind a prefix, whose last tile is not whole."""
+    from ameva_compute_amd import ops
+    n_kv, n_pre = [(kv * i) % (kv + 1) + 1 for i in range(n)], -(-prefix // 16)
+    w = World(t, g, d, 16, n_kv, seed=12, extra=n_pre)
+    pre = w.free[:n_pre].clone()
+    q = torch.randn(n, heads, d, device=DEV)
+    y = ops.paged_attn_shared(w.cache, w.batch(), q, d ** -0.5, pre, prefix)
+    kv = [x[pre.long()].transpose(0, 1).reshape(g, -1, d)[:, :prefix] for x in (w.k, w.v)]
+    assert off(y, attend(w, q, d ** -0.5, prefix=kv)) < TOL

@@ -134,3 +134,16 @@ def test_python_side():
         ops.PagedKV.alloc(F16, 2, 20, 1, 64, "cpu")
     with pytest.raises(ValueError, match="GPU"):
         ops.PagedBatch(torch.ones(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32), 16)
+
+
+def test_launches_that_would_be_too_large():
+    """More workgroups than a grid has: sequences (even empty ones) of many KV heads, rows of many heads."""
+    chunk = 16 * 256
+    many = kv(n_head_kv=1024, page_stride=1024 * chunk)
+    seqs = batch(n_seq=65535, n_tok=8, cu_q=A, max_q=1)
+    refused(attn(many, seqs, heads=1024, stride=1024 * 128), "too large")
+    refused(append(many, seqs, heads=1024, stride=3 * 1024 * 128, out_stride=1024 * 128), "too large")
+    refused(attn(kv(), batch(n_seq=1, n_tok=(1 << 22) + 1, cu_q=A, max_q=9)), "too large")
+    tokens = batch(n_seq=1, n_tok=(1 << 13) + 1, cu_q=A, max_q=9)
+    rc = lib().amv_paged_select(*refs(many, tokens), A, 1024 * 128, 1024, 4, 1, 1, A, A, 1 << 40, None)
+    refused(rc, "too large")
