@@ -773,12 +773,22 @@ typedef __attribute__((address_space(3))) pg_s4 pg_lds_s4;
         __builtin_amdgcn_s_barrier();       \
         asm volatile("" ::: "memory");      \
     } while (0)
+// the same without the loads into registers, which may still be on their way
+#define PG_BARRIER_LDS()                    \
+    do {                                    \
+        asm volatile("" ::: "memory");      \
+        __builtin_amdgcn_s_waitcnt(0xC07F); \
+        __builtin_amdgcn_s_barrier();       \
+        asm volatile("" ::: "memory");      \
+    } while (0)
 __device__ __align__(16) const uint8_t pg_zeros[16] = {};
 
 // (true: nothing is written, as a sum is no number: a value that not all rows see may be the reason, which pg_few leaves out)
-template <int D, int RW>
+template <int TYPE, int D, int RW>
 __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z, uint16_t* sKa, uint16_t* sKb, uint16_t* sVa,
                                         uint16_t* sVb) {
+    using R = PgRow<TYPE, D>;
+    constexpr bool QUANT = TYPE != AMV_T_F16;
     constexpr int NB = D / 32, T = D / 16, PIECES = D / 8;  // (of 16 bytes a row)
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -805,7 +815,7 @@ __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z
         ko[y] = (RPI * y + row) * 2 * D + 16 * (x ^ hash_k(key));
         vo[y] = (RPI * y + row) * 2 * D + 16 * ((((x >> 1) ^ hash_v(key)) << 1) | (x & 1));
     }
-    const size_t chunk = (size_t)ps * 2 * D;
+    const size_t chunk = (size_t)ps * (R::ROW + R::SC);
     const uint8_t *kc = a.k + hk * chunk, *vc = a.v + hk * chunk;
     struct Step {
         PgAt a, b;  // its 32-key halves
@@ -837,10 +847,86 @@ __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z
             }
         }
     };
+    // quantized: a lane has a quarter of a key's row (8 elements of each block) in registers, from where put() brings it to LDS
+    __shared__ float sF[QUANT ? 2 : 1][QUANT ? 64 : 1];
+    constexpr int RAW = QUANT ? R::ROW / 16 : 1, RSC = QUANT ? NB / 2 : 1;
+    uint32_t rk[RAW], rv[RAW], sk[RSC], sv[RSC];
+    const int key = 16 * w + (lane >> 2), j4 = lane & 3;
+    const auto fetch = [&](const Step& s) {
+        if constexpr (QUANT) {
+            const int e = w == 0 ? s.a.e0 : w == 1 ? s.a.e1 : w == 2 ? s.b.e0 : s.b.e1, p = s.a.p0 + 16 * w;
+            const int64_t off = pg_off<TYPE, D>(a, e, p, false) + (lane >> 2) * R::ROW + j4 * (R::ROW / 4);
+            const int64_t sof = pg_off<TYPE, D>(a, e, p, true) + (lane >> 2) * R::SC;
+            pg_load<R::ROW / 4>(rk, kc + off);
+            pg_load<R::SC>(sk, kc + sof);
+            pg_load<R::ROW / 4>(rv, vc + off);
+            pg_load<R::SC>(sv, vc + sof);
+            const uint32_t keep = e >= 0 && p + (lane >> 2) < t.keys ? 0xFFFFFFFFu : 0u;  // values of no key: 0
+#pragma unroll
+            for (int i = 0; i < RSC; ++i) sv[i] &= keep;
+        }
+    };
+    const auto put = [&]() {
+        if constexpr (QUANT) {
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const uint32_t(&x)[RAW] = v ? rv : rk;
+                const uint32_t(&sc)[RSC] = v ? sv : sk;
+                // the key's scales times the power of two that brings the largest to 2^7 .. 2^8
+                amv_h2 big = __builtin_bit_cast(amv_h2, sc[0] & 0x7FFF7FFFu);
+                if constexpr (RSC > 1) big = __builtin_elementwise_max(big, __builtin_bit_cast(amv_h2, sc[RSC - 1] & 0x7FFF7FFFu));
+                const uint32_t e = max(103u, min(142u, __float_as_uint(fmaxf((float)big.x, (float)big.y)) >> 23));
+                const float norm = __uint_as_float((261u - e) << 23);
+                if (j4 == 0) sF[v][key] = __uint_as_float((e - 7u) << 23);
+                constexpr float zero = TYPE == AMV_T_Q8_0 ? -1152.0f : -1032.0f;  // integers in the low bits of 1024 are 1024 more
+                const amv_h2 bias = {(_Float16)zero, (_Float16)zero};
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t n[4];
+                    if constexpr (TYPE == AMV_T_Q8_0) {
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            const uint32_t word = (v ? x[m * (D / 64) + (b >> 1)] : x[2 * b + (m >> 1)]) ^ 0x80808080u;
+                            n[m] = __builtin_amdgcn_perm(0x64646464u, word, ((v ? b : m) & 1) ? 0x04030402u : 0x04010400u);
+                        }
+                    } else if (v) {  // elements 0, 2, 1, 3 and 4, 6, 5, 7
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            uint32_t z;
+                            if constexpr (D == 128) {  // byte b of words 2 m and 2 m + 1
+                                z = __builtin_amdgcn_perm(x[(2 * m + 1) % RAW], x[2 * m % RAW], 0x0C040C00u + 0x00010001u * b);
+                            } else {                   // bytes b and 2 + b of word m
+                                z = (x[m] >> (8 * b)) & 0x00FF00FFu;
+                            }
+                            n[2 * m] = (z & 0x000F000Fu) | 0x64006400u;
+                            n[2 * m + 1] = ((z >> 4) & 0x000F000Fu) | 0x64006400u;
+                        }
+                    } else {  // elements 0, 4, 1, 5, 2, 6, 3, 7
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) n[m] = ((x[b] >> (4 * m)) & 0x000F000Fu) | 0x64006400u;
+                    }
+                    const _Float16 s1 = (_Float16)(pg_half(sc, b) * norm);
+                    const amv_h2 s2 = {s1, s1};
+                    amv_v4u hi, lo;
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        const amv_h2 y = __builtin_bit_cast(amv_h2, n[m]) + bias, h = y * s2;
+                        hi[m] = pg_bits(h);
+                        lo[m] = pg_bits(__builtin_elementwise_fma(y, s2, -h));
+                    }
+                    const int piece = 4 * b + j4;
+                    const int to = key * D + 8 * (v ? (((piece >> 1) ^ hash_v(key)) << 1) | (piece & 1) : piece ^ hash_k(key));
+                    *reinterpret_cast<amv_v4u*>((v ? sVa : sKa) + to) = hi;
+                    *reinterpret_cast<amv_v4u*>((v ? sVb : sKb) + to) = lo;
+                }
+            }
+        }
+    };
     Step at = {};
     if (begin < end) {
         at = where(begin);
-        stage(at, sKa, sVa);
+        if constexpr (QUANT) fetch(at);
+        else stage(at, sKa, sVa);
     }
     pg_h8 qh[2][NB], ql[2][NB];
     float f[2], m[2], l[2];
@@ -853,7 +939,14 @@ __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z
         float y[NB][8];
         f[rt] = pg_query<D>(a, t, hk, r, g, y);
 #pragma unroll
-        for (int s = 0; s < NB; ++s) pg_split(y[s], qh[rt][s], ql[rt][s]);
+        for (int s = 0; s < NB; ++s) {
+            if constexpr (TYPE == AMV_T_Q4_0) {  // in put()'s order
+                const float z[8] = {y[s][0], y[s][4], y[s][1], y[s][5], y[s][2], y[s][6], y[s][3], y[s][7]};
+                pg_split(z, qh[rt][s], ql[rt][s]);
+            } else {
+                pg_split(y[s], qh[rt][s], ql[rt][s]);
+            }
+        }
         m[rt] = -INFINITY;
         l[rt] = 0.0f;
 #pragma unroll
@@ -862,7 +955,8 @@ __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z
     // the lane's places in the rows of 32 keys: K's key of product 0 and its piece g (+ 4 b: by XOR), V's key and unit 0 (v: by XOR)
     const int kx = (8 * (c >> 2) + (c & 3)) * D + 8 * (g ^ (D == 128 ? c : c >> 1));  // (hash_k of both products' key)
     const int vx = (8 * g + (c >> 2)) * D + 16 * hash_v(8 * g + (c >> 2)) + 4 * (c & 3);  // (and hash_v of key + 4)
-    const auto half = [&](const PgAt& now, const uint16_t* sK, const uint16_t* sV) {  // 32 keys
+    float vref = 0.0f;  // quantized: the largest power of two of a key's values met
+    const auto half = [&](const PgAt& now, const uint16_t* sK, const uint16_t* sV, int h32) {  // 32 keys
         int kx0 = kx, vx0 = vx;  // (not known to be the same each time: their sums would be kept, in registers that are not there)
         asm volatile("" : "+v"(kx0), "+v"(vx0));
         pg_f4 y[2][2];
@@ -873,6 +967,11 @@ __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const pg_h8 kf = *reinterpret_cast<const pg_h8*>(&sK[(kx0 ^ (32 * b)) + 4 * h * D]);
+                if constexpr (QUANT) {
+                    const pg_h8 kr = *reinterpret_cast<const pg_h8*>(&sKb[32 * D * h32 + (kx0 ^ (32 * b)) + 4 * h * D]);
+#pragma unroll
+                    for (int rt = 0; rt < 2; ++rt) y[rt][h] = pg_mfma(kr, qh[rt][b], y[rt][h]);
+                }
 #pragma unroll
                 for (int rt = 0; rt < 2; ++rt) y[rt][h] = pg_mfma(kf, ql[rt][b], y[rt][h]);
 #pragma unroll
@@ -882,7 +981,10 @@ __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[rt][j] = y[rt][j >> 2][j & 3];
+            for (int j = 0; j < 8; ++j) {
+                s[rt][j] = y[rt][j >> 2][j & 3];
+                if constexpr (QUANT) s[rt][j] *= sF[0][32 * h32 + 8 * g + j];
+            }
         if (now.e0 < 0 || now.e1 < 0 || now.p1 + 16 > t.see_all) {
             const int p = now.p0 + 8 * g;
             const bool there = (g >= 2 ? now.e1 : now.e0) >= 0;
@@ -892,18 +994,50 @@ __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z
                 for (int j = 0; j < 8; ++j) s[rt][j] = there && p + j < lim[rt] ? s[rt][j] : -INFINITY;
         }
         pg_h8 ph[2], pl[2];
+        float fv[QUANT ? 8 : 1];
+        if constexpr (QUANT) {
+            float top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                fv[j] = sF[1][32 * h32 + 8 * g + j];
+                top = fmaxf(top, fv[j]);
+            }
+            top = amv_max_x32(amv_max_x16(top));
+            if (__builtin_amdgcn_readfirstlane(top > vref)) {
+                const float by = vref * __uint_as_float((254u << 23) - __float_as_uint(top));
+                vref = top;
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                    for (int v = 0; v < T; ++v) o[rt][v] *= by;
+            }
+            const float down = __uint_as_float((254u << 23) - __float_as_uint(vref));  // (1 / vref: powers of two)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) fv[j] *= down;
+        }
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
             pg_soften<1>(s[rt], f[rt], m[rt], l[rt], o[rt], pw);
+            if constexpr (QUANT) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) pw[j] *= fv[j];
+            }
             pg_split(pw, ph[rt], pl[rt]);
         }
 #pragma unroll
         for (int v = 0; v < T; ++v) {
-            const uint16_t* at0 = &sV[vx0 ^ (16 * v)];
-            const pg_s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pg_lds_s4*)(__attribute__((address_space(3))) uint16_t*)at0);
-            const pg_s4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pg_lds_s4*)(__attribute__((address_space(3))) uint16_t*)(at0 + 4 * D));
-            const pg_s8 ab = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-            const pg_h8 vf = __builtin_bit_cast(pg_h8, ab);
+            const auto value = [&](const uint16_t* at0) {
+                const pg_s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pg_lds_s4*)(__attribute__((address_space(3))) uint16_t*)at0);
+                const pg_s4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pg_lds_s4*)(__attribute__((address_space(3))) uint16_t*)(at0 + 4 * D));
+                const pg_s8 ab = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+                return __builtin_bit_cast(pg_h8, ab);
+            };
+            const pg_h8 vf = value(&sV[vx0 ^ (16 * v)]);
+            if constexpr (QUANT) {
+                const pg_h8 vr = value(&sVb[32 * D * h32 + (vx0 ^ (16 * v))]);
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt) o[rt][v] = pg_mfma(vr, ph[rt], o[rt][v]);
+            }
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt) o[rt][v] = pg_mfma(vf, pl[rt], o[rt][v]);
 #pragma unroll
@@ -912,14 +1046,32 @@ __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z
     };
     const auto step = [&](const Step& now, const uint16_t* sK, const uint16_t* sV) {
         if constexpr (RW == 4) {
-            half(now.a, sK, sV);
-            half(now.b, sK + 32 * D, sV + 32 * D);
+            half(now.a, sK, sV, 0);
+            half(now.b, sK + 32 * D, sV + 32 * D, 1);
         } else {
-            half(kw ? now.b : now.a, sK + 32 * D * kw, sV + 32 * D * kw);
+            half(kw ? now.b : now.a, sK + 32 * D * kw, sV + 32 * D * kw, kw);
         }
     };
-    PG_BARRIER();
-    for (int i = begin; i < end; i += 2) {
+    if constexpr (QUANT) {
+        for (int i = begin; i < end; ++i) {
+            put();
+            PG_BARRIER();
+            Step next = at;
+            if (i + 1 < end) {
+                next = where(i + 1);
+                fetch(next);
+            }
+            if (i < mine) step(at, sKa, sVa);
+            at = next;
+            PG_BARRIER_LDS();
+        }
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+            for (int v = 0; v < T; ++v) o[rt][v] *= vref;
+    }
+    if constexpr (!QUANT) PG_BARRIER();
+    for (int i = QUANT ? end : begin; i < end; i += 2) {
         Step next = at;
         if (i + 1 < end) {
             next = where(i + 1);
@@ -986,7 +1138,8 @@ __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z
         else if (g == 0) *part = make_float2(m[rt], L);
 #pragma unroll
         for (int v = 0; v < T; ++v) {
-            const pg_f4 y = o[rt][v] * inv;
+            pg_f4 y = o[rt][v] * inv;
+            if constexpr (TYPE == AMV_T_Q4_0) y = pg_f4{y.x, y.z, y.y, y.w};  // (put()'s order)
             *reinterpret_cast<pg_f4*>(to + 16 * v + 4 * g) = y;
         }
     }
@@ -1023,17 +1176,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_many_few(PgJobs jobs) {  // jo
     if (k > 0) b -= jobs.n[0];
     if (k > 1) b -= jobs.n[1];
     pg_place_of(jobs.a[k], b, hk, tile, z);
-    if constexpr (TYPE == AMV_T_F16) {
-        constexpr int ROWS = 16 * RT / P;
-        if (k < 2 && !pg_many<D, RW>(jobs.a[k], hk, tile, z, sKa, sKb, sVa, sVb)) return;
-        const int rows = k < 2 ? 32 * RW : ROWS;
-        for (int sub = 0; sub < rows / ROWS; ++sub) {
-            if (sub) __syncthreads();
-            pg_few<TYPE, D, RT, P>(jobs.a[k], hk, tile, rows, sub, z, so0, so1);
-        }
-    } else {
-        if (k == 2) pg_few<TYPE, D, RT, P>(jobs.a[2], hk, tile, 16 * RT / P, 0, z, so0, so1);
-        else pg_few<TYPE, D, 2, 1>(jobs.a[k], hk, tile, 32, 0, z, so0, so1);
+    constexpr int ROWS = 16 * RT / P;
+    if (k < 2 && !pg_many<TYPE, D, RW>(jobs.a[k], hk, tile, z, sKa, sKb, sVa, sVb)) return;
+    const int rows = k < 2 ? 32 * RW : ROWS;
+    for (int sub = 0; sub < rows / ROWS; ++sub) {
+        if (sub) __syncthreads();
+        pg_few<TYPE, D, RT, P>(jobs.a[k], hk, tile, rows, sub, z, so0, so1);
     }
 }
 
@@ -1155,7 +1303,7 @@ static PgPlan pg_plan(const amv_paged_kv* kv, const amv_paged_batch* b, int64_t 
     // not cut into parts (2048 tokens 104 and 113, 512 28 and 35), and read a prefix for up to 64 rows as soon.
     const int64_t large = all / 128 * kv->n_head_kv;
     const bool even = (!p.find || b->max_kv <= 1024 || (large >= 256 && large < 1024)) && (n_prefix == 0 || all <= 64);
-    p.many_rows = kv->type != AMV_T_F16 ? 32 : even ? 64 : 128;
+    p.many_rows = even ? 64 : 128;
     if (p.find) {
         p.find_tiles = all / p.many_rows + b->n_seq;
         p.n_find = pg_parts(all / p.many_rows * kv->n_head_kv + 1, b->max_kv, &p.len_find);
@@ -1180,7 +1328,7 @@ extern "C" int64_t amv_paged_attn_workspace_bytes(const amv_paged_kv* kv, const 
 template <int TYPE, int D, int RT, int P>
 static void pg_launch(const PgJobs& j, int many, hipStream_t st) {
     const dim3 grid((unsigned)(j.n[0] + j.n[1] + j.n[2]));
-    if (many == 64 && TYPE == AMV_T_F16) hipLaunchKernelGGL((k_paged_many_few<TYPE, D, RT, P, TYPE == AMV_T_F16 ? 2 : 4>), grid, dim3(256), 0, st, j);
+    if (many == 64) hipLaunchKernelGGL((k_paged_many_few<TYPE, D, RT, P, 2>), grid, dim3(256), 0, st, j);
     else if (many) hipLaunchKernelGGL((k_paged_many_few<TYPE, D, RT, P, 4>), grid, dim3(256), 0, st, j);
     else hipLaunchKernelGGL((k_paged_few<TYPE, D, RT, P>), grid, dim3(256), 0, st, j);
 }
