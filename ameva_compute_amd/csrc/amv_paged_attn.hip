@@ -161,15 +161,15 @@ __device__ __forceinline__ void pg_load_v(PgV<TYPE, D, KPL>& t, const PgAttn& a,
 // Integers u = value + bias in the low bits of a word's two halves are, as they stand, the f16 u 2^-24. Values become operands times
 // 2^-10: u 2^-24 2^14 - bias 2^-10 is exact.
 template <int TYPE>
-__device__ __forceinline__ constexpr float pg_bias() { return TYPE == AMV_T_Q8_0 ? 128.0f : 8.0f; }
-template <int TYPE>
 __device__ __forceinline__ uint32_t pg_f16_of(uint32_t u) {
-    constexpr float bias = pg_bias<TYPE>() / 1024.0f;
+    constexpr float bias = (TYPE == AMV_T_Q8_0 ? 128.0f : 8.0f) / 1024.0f;
     const amv_h2 m = {(_Float16)16384.0f, (_Float16)16384.0f}, b = {(_Float16)-bias, (_Float16)-bias};
     return pg_bits(__builtin_elementwise_fma(__builtin_bit_cast(amv_h2, u), m, b));
 }
-// The operand of product s of K: 8 f16; of quantized keys (value + bias) 2^-24, whose product begins at -bias 2^-24 times the sum of
-// q's elements, so that no instruction is spent on the bias (it rounds at the size of the biased sums: some 2 or 3 bits of the 24 more)
+// The operand of product s of K: 8 f16; of quantized keys (value + bias) 2^-24 (Q4_0: times 16), whose product begins at -128 2^-24
+// times the sum of q's elements, so that no instruction is spent on the bias (96 sequences of 4096 Q4_0 keys 105 us, so 100). The matrix
+// cores align such f16 by their exponent, which is the least for all of them: with Q4_0's integers in the lowest 4 of the 10 bits the
+// sums lost 6 bits (an error of 4.6e-6 for 24 selected pages), in bits 4 to 7, as with Q8_0's 8 bits, they lose 2.
 template <int TYPE, int D>
 __device__ __forceinline__ pg_h8 pg_k_operand(const uint32_t* k, int s) {
     amv_v4u x;
@@ -183,7 +183,7 @@ __device__ __forceinline__ pg_h8 pg_k_operand(const uint32_t* k, int s) {
             x[2 * h + 1] = __builtin_amdgcn_perm(0u, w, 0x0C030C02u);
         }
     } else {
-        const uint32_t even = k[s] & 0x0F0F0F0Fu, odd = (k[s] >> 4) & 0x0F0F0F0Fu;
+        const uint32_t even = (k[s] << 4) & 0xF0F0F0F0u, odd = k[s] & 0xF0F0F0F0u;
         x[0] = __builtin_amdgcn_perm(odd, even, 0x0C040C00u);
         x[1] = __builtin_amdgcn_perm(odd, even, 0x0C050C01u);
         x[2] = __builtin_amdgcn_perm(odd, even, 0x0C060C02u);
@@ -451,7 +451,7 @@ __device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int ro
     // Q^T operands: values times scale log2(e) 2^-e below 2, P = 1: as f16 and the rest in two operands, P = 2: in the two halves of
     // the columns of one, P = 4 and quantized keys: of two, one for each product u, that is 0 where the columns keep the other's keys,
     // so that the products add up to what each column keeps (f16 keys may be infinite or no number where nobody sees them: 0 times
-    // them would not be 0, so there each column picks its product). f: 2^e (for quantized keys times the 2^24 that their operands
+    // them would not be 0, so there each column picks its product). f: 2^e (for quantized keys times what their operands
     // lack); lim: keys the row sees; q0: where the products of quantized keys begin
     pg_h8 qa[RT][P == 2 || (P == 4 && !QUANT) ? 1 : 2][NB];
     float f[RT], q0[RT][QUANT ? NB : 1];
@@ -484,10 +484,10 @@ __device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int ro
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     sum += P == 2 ? (float)qa[rt][0][s][j] : (float)qa[rt][0][s][j] + (float)qa[rt][1][s][j];
-                q0[rt][s] = amv_sum_x32(amv_sum_x16(sum)) * (-pg_bias<TYPE>() * 0x1p-24f);
+                q0[rt][s] = amv_sum_x32(amv_sum_x16(sum)) * (-128.0f * 0x1p-24f);
             }
         }
-        if constexpr (QUANT) f[rt] *= 0x1p24f;
+        if constexpr (QUANT) f[rt] *= TYPE == AMV_T_Q8_0 ? 0x1p24f : 0x1p20f;
     }
 
     float m[RT], l[RT];
@@ -1292,8 +1292,11 @@ static PgPlan pg_plan(const amv_paged_kv* kv, const amv_paged_batch* b, int64_t 
         return p;
     }
     const int64_t rows = std::min(b->max_q, b->n_tok) * G;
-    p.pre_many = all > 32;
-    p.few = pg_tiles(n_prefix > 0 && !p.pre_many ? all : rows <= 32 ? rows : G);
+    // 17 to 32 rows are one tile of few rows, but not of Q8_0 keys, whose registers for it do not suffice (32 sequences of 8 tokens
+    // after 4096 keys 147 us, in half a tile of 64 rows 141; Q4_0 122 and 140)
+    const int64_t most = kv->type == AMV_T_Q8_0 ? 16 : 32;
+    p.pre_many = all > most;
+    p.few = pg_tiles(n_prefix > 0 && !p.pre_many ? all : rows <= most ? rows : G);
     p.rows_most = (int)std::max<int64_t>(p.few.rows(), G);
     p.ta = p.few.of(p.rows_most);
     p.n_one = pg_parts(b->n_seq * kv->n_head_kv * p.ta, b->max_kv, &p.len_one);
@@ -1302,7 +1305,7 @@ static PgPlan pg_plan(const amv_paged_kv* kv, const amv_paged_batch* b, int64_t 
     // 16384 keys 107 and 119), those of 64 rows share the GPU more evenly where the larger are no more than a few for each CU and
     // not cut into parts (2048 tokens 104 and 113, 512 28 and 35), and read a prefix for up to 64 rows as soon.
     const int64_t large = all / 128 * kv->n_head_kv;
-    const bool even = (!p.find || b->max_kv <= 1024 || (large >= 256 && large < 1024)) && (n_prefix == 0 || all <= 64);
+    const bool even = (!p.find || rows <= 64 || b->max_kv <= 1024 || (large >= 256 && large < 1024)) && (n_prefix == 0 || all <= 64);
     p.many_rows = even ? 64 : 128;
     if (p.find) {
         p.find_tiles = all / p.many_rows + b->n_seq;
