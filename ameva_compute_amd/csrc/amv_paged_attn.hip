@@ -1197,21 +1197,33 @@ struct PgMerge {
     PgParts one, many, pre;
     float* out;
     int n_head, n_head_kv, G, rows_most;
+    int by_seq;  // only sequences of few rows have parts: the waves go over their rows, not over all tokens'
 };
 template <int D>
 __global__ __launch_bounds__(256) void k_paged_merge(PgMerge a) {
     constexpr int E = D / 64;
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tok = (int)(row / a.n_head), h = (int)(row - (int64_t)tok * a.n_head);
-    if (tok >= a.b.n_tok) return;
-    const int s = pg_seq_of(a.b, tok);
-    if (s >= a.b.n_seq) return;
-    const int first = a.b.first(s);
-    const bool few = (a.b.last(s) - first) * a.G <= a.rows_most;
-    const PgParts own = few ? a.one : a.many;
-    if (!own.n) return;  // its workgroup wrote the row
-    const int64_t own_row = few ? ((int64_t)s * a.n_head_kv + h / a.G) * a.rows_most + (tok - first) * a.G + h % a.G : row;
+    const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int64_t row = at, own_row;
+    PgParts own = a.one;
+    if (a.by_seq) {
+        if (at >= (int64_t)a.b.n_seq * a.n_head_kv * a.rows_most) return;
+        const int hs = (int)(at / a.rows_most), r = (int)(at - (int64_t)hs * a.rows_most), s = hs / a.n_head_kv;
+        const int first = a.b.first(s), n_rows = (a.b.last(s) - first) * a.G;
+        if (n_rows > a.rows_most || r >= n_rows) return;
+        own_row = at;
+        row = (int64_t)(first + r / a.G) * a.n_head + (hs - s * a.n_head_kv) * a.G + r % a.G;
+    } else {
+        const int tok = (int)(row / a.n_head), h = (int)(row - (int64_t)tok * a.n_head);
+        if (tok >= a.b.n_tok) return;
+        const int s = pg_seq_of(a.b, tok);
+        if (s >= a.b.n_seq) return;
+        const int first = a.b.first(s);
+        const bool few = (a.b.last(s) - first) * a.G <= a.rows_most;
+        if (!few) own = a.many;
+        if (!own.n) return;  // its workgroup wrote the row
+        own_row = few ? ((int64_t)s * a.n_head_kv + h / a.G) * a.rows_most + (tok - first) * a.G + h % a.G : row;
+    }
     const float2 *ml0 = own.ml + own_row * own.n, *ml1 = a.pre.ml + row * a.pre.n;
     const float *acc0 = own.acc + own_row * own.n * D, *acc1 = a.pre.acc + row * a.pre.n * D;
     float M = -INFINITY;
@@ -1386,7 +1398,7 @@ static int pg_attn(const char* what, const amv_paged_kv* kv, const amv_paged_bat
     PgMerge m = {a.b, {ml, acc, p.w_one ? p.n_one : 0},
                  {ml + p.w_one, acc + p.w_one * kv->D, p.w_many ? (n_sel > 0 ? p.n_one : p.n_find) : 0},
                  {ml + p.w_one + p.w_many, acc + (p.w_one + p.w_many) * kv->D, p.n_pre},
-                 out, (int)n_head, kv->n_head_kv, a.G, n_sel > 0 ? -1 : p.rows_most};
+                 out, (int)n_head, kv->n_head_kv, a.G, n_sel > 0 ? -1 : p.rows_most, n_sel == 0 && !p.w_many && !p.w_pre};
     PgJobs jobs = {};
     int64_t groups = 0;
     const auto job = [&](int k, int kind, int64_t tiles, int parts, int len, const PgParts& into) {
@@ -1411,7 +1423,7 @@ static int pg_attn(const char* what, const amv_paged_kv* kv, const amv_paged_bat
     hipStream_t st = amv_stream(stream);
     pg_launch(kv->type, kv->D, jobs, p.few, p.find || (p.n_pre && p.pre_many) ? p.many_rows : 0, st);
     if (p.w_one + p.w_many + p.w_pre) {
-        const dim3 grid((unsigned)((rows + 3) / 4));
+        const dim3 grid((unsigned)(((m.by_seq ? b->n_seq * kv->n_head_kv * p.rows_most : rows) + 3) / 4));
         if (kv->D == 128) hipLaunchKernelGGL(k_paged_merge<128>, grid, dim3(256), 0, st, m);
         else hipLaunchKernelGGL(k_paged_merge<64>, grid, dim3(256), 0, st, m);
     }
