@@ -21,8 +21,17 @@
 // scale in f16's range whatever the values' size.
 //
 // Four waves of a workgroup take the 32-key tiles of a range in turn and join in LDS; ranges of a long sequence go to several
-// workgroups (blockIdx.y), joined by k_paged_merge from
-// (m, l, O) in the workspace.
+// workgroups, joined by k_paged_merge from (m, l, O) in the workspace. Tiles of many rows share K and V through LDS (pg_many).
+//
+// Measured (32 query and 8 KV heads of 128), and what bounds it:
+//   64 sequences of up to 4096 f16 keys, 684 MB: 123 us, 5.5 TB/s (equally long ones 6.6, where a copy of 4 GiB reaches 5.0): memory
+//   3 of up to 65536 Q8_0 keys, 331 MB: 66 us and 5 the merge, 4.7 TB/s (96 equal ones 6.0): memory, VALU a third of the SIMD cycles
+//   96 of 4096 Q4_0 keys: 104 us, 4.4 TB/s: VALU, as much work a key as Q8_0's for half the bytes
+//   one of 777 f16 keys: 7.7 us and 2.4 the merge: two launches, a tile's latency and the join
+//   2 x 1024 tokens, up to 3000 f16 keys: 138 us, 0.76 PFLOP/s of products, which are twice the formula's (8192 tokens 1.1, a library's
+//     product 1.17): matrix cores 30 %, VALU 38 % of the SIMD cycles at two waves a SIMD; over Q8_0 keys 232 us, Q4_0 231: half as many
+//     products again and the bringing of integers to LDS
+//   128 tokens behind 16384 shared f16 keys: 107 us and 9 the merge: the same, and the first steps of 384 workgroups
 #include "amv_paged.h"
 
 #include <algorithm>
@@ -756,8 +765,7 @@ __device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int ro
 // workgroup: read by each wave for itself (pg_few), K's pieces of 16 bytes from 16 rows an instruction keep the loads' address unit busy
 // for all of the time. RW = 4: every wave goes over all keys; RW = 2: two waves a row range, each with one half of every step's keys,
 // joined at the end. K and V rows of 64 keys, a step, go to LDS without registers (global_load_lds), one step ahead in two buffers; the
-// products are those of pg_few with RT = 2. The loads write LDS in lane order, so a row's pieces are
-// exchanged on the memory side: K's 16-byte pieces by a number of the key that differs among the 16 keys of an operand read, V's
+// products are those of pg_few with RT = 2. The loads write LDS in lane order, so a row's pieces are exchanged on the memory side: K's 16-byte pieces by a number of the key that differs among the 16 keys of an operand read, V's
 // 32-byte units by one that takes each value twice among the 16 keys of a transposing read (ds_read_b64_tr_b16: 16 lanes pointing at
 // 4 keys' 8-byte quarters of a unit get an element of the 4 keys each), so both reads meet all banks.
 typedef __attribute__((address_space(3))) void pg_lds;
@@ -783,6 +791,12 @@ typedef __attribute__((address_space(3))) pg_s4 pg_lds_s4;
     } while (0)
 __device__ __align__(16) const uint8_t pg_zeros[16] = {};
 
+// Quantized keys and values come through registers, a quarter of a key's row a lane: the integers become f16 (the low bits of 1024 plus
+// the value), times the scales in packed f16, the product rounded and the rest (exact, by an fma), each a buffer of its own in LDS, one
+// step at a time; the next step's bytes are on their way while this one is worked on. A power of two per key brings its largest scale to
+// 2^7 .. 2^8, so that blocks down to 2^-20 of it keep 20 bits; it meets the scores and the weights in f32. Three products of the parts in
+// place of two (the rests' own is below 2^-22), but the scales no longer cost an instruction for each row and block: the 2 x 1024 tokens
+// over Q8_0 keys took 418 us with every wave working from its own registers (pg_few of 32 rows).
 // (true: nothing is written, as a sum is no number: a value that not all rows see may be the reason, which pg_few leaves out)
 template <int TYPE, int D, int RW>
 __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z, uint16_t* sKa, uint16_t* sKb, uint16_t* sVa,
@@ -1186,7 +1200,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_many_few(PgJobs jobs) {  // jo
 }
 
 // out = sum_z w_z O_z / sum_z w_z l_z over the parts z of a row's keys, w_z = 2^(m_z - max m): one wave per row. A row has parts of
-// its own keys, laid out by sequence where that has at most rows_most rows and else by row, and of the prefix.
+// its own keys, laid out by sequence where that has at most rows_most rows and else by row, and of the prefix. Bound: the launch and
+// two dependent reads (2.4 us for 32 rows of 7 parts, 4.5 for 96 of 21, 9 for 4096 of the prefix' and their own).
 struct PgParts {
     const float2* ml;
     const float* acc;
@@ -1283,8 +1298,9 @@ struct PgPlan {
     int64_t bytes(int64_t D) const { return (w_one + w_many + w_pre) * (8 + 4 * D); }
 };
 // parts of `keys` keys for `units` workgroups' worth of rows: two workgroups a CU, none of less than 128 keys (a tile for each of its
-// waves), and up to 256 keys no parts, as their merge is a launch of its own. More and shorter parts cost their prologues and the merge (us at 512 / 1024 / 2048 workgroups: 64 sequences of up to 4096
-// f16 keys 136 / 147 / 144, 3 of 65536 Q8_0 keys 78 / 78 / 82, one of 777 with parts of 256 keys 9.6, of 128 9.3)
+// waves), and up to 256 keys no parts, as their merge is a launch of its own. More and shorter parts cost their prologues and the merge
+// (us at 512 / 1024 / 2048 workgroups: 64 sequences of up to 4096 f16 keys 136 / 147 / 144, 3 of 65536 Q8_0 keys 78 / 78 / 82; one of 777
+// with parts of 256 keys 9.6, of 128 9.3)
 static int pg_parts(int64_t units, int64_t keys, int* len, int target = 512) {
     units = std::max<int64_t>(1, units);
     const int64_t n = keys <= 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(target / units, (keys + 127) / 128));
@@ -1313,8 +1329,8 @@ static PgPlan pg_plan(const amv_paged_kv* kv, const amv_paged_batch* b, int64_t 
     p.ta = p.few.of(p.rows_most);
     p.n_one = pg_parts(b->n_seq * kv->n_head_kv * p.ta, b->max_kv, &p.len_one);
     p.find = rows > p.rows_most;
-    // Tiles of 128 rows do more with a step (8192 tokens 996 us, with 64 rows 1150; 512 after 7488 others 174 and 219; 128 sequences behind
-    // 16384 keys 107 and 119), those of 64 rows share the GPU more evenly where the larger are no more than a few for each CU and
+    // Tiles of 128 rows do more with a step (8192 tokens 996 us, with 64 rows 1150; 512 after 7488 others 174 and 219; 128 sequences
+    // behind 16384 keys 107 and 119), those of 64 rows share the GPU more evenly where the larger are no more than a few for each CU and
     // not cut into parts (2048 tokens 104 and 113, 512 28 and 35), and read a prefix for up to 64 rows as soon.
     const int64_t large = all / 128 * kv->n_head_kv;
     const bool even = (!p.find || rows <= 64 || b->max_kv <= 1024 || (large >= 256 && large < 1024)) && (n_prefix == 0 || all <= 64);
