@@ -278,7 +278,7 @@ __device__ __forceinline__ bool pg_rows(const PgAttn& a, int hk, int tile, int r
     int in = tile;
     if (a.kind == PG_PREFIX) {
         t.tok0 = 0;
-        t.n_rows = a.b.n_tok * a.G;
+        t.n_rows = a.b.last(a.b.n_seq - 1) * a.G;  // (not the rows behind the last sequence, whatever is in them)
         t.keys = t.place0 = a.n_list;
         t.pages = a.list;
     } else {

@@ -346,3 +346,25 @@ def test_shared_prefix_of_many_sequences(t, heads, g, d, prefix, n, kv):
     y = ops.paged_attn_shared(w.cache, w.batch(), q, d ** -0.5, pre, prefix)
     kv = [x[pre.long()].transpose(0, 1).reshape(g, -1, d)[:, :prefix] for x in (w.k, w.v)]
     assert off(y, attend(w, q, d ** -0.5, prefix=kv)) < TOL
+
+
+@pytest.mark.parametrize("t", [F16, Q4_0])
+@pytest.mark.parametrize("n,n_q", [(5, 1), (70, 1), (3, 40)])
+def test_padding_that_is_no_number(t, n, n_q):
+    """q rows behind the last sequence, fewer and more of them than a tile, hold no numbers: nobody reads them."""
+    from ameva_compute_amd import ops
+    w = World(t, 2, 128, 16, [n_q + 9] * n, [n_q] * n, seed=13, extra=30, bounds=True)
+    pre, m = w.free[:30].clone(), n * n_q
+    for pad in (3, 200):
+        b = w.batch(pad=pad)
+        q = torch.randn(m + pad, 8, 128, device=DEV)
+        q[m:] = math.nan
+        kv = [x[pre.long()].transpose(0, 1).reshape(2, -1, 128)[:, :470] for x in (w.k, w.v)]
+        out = torch.full_like(q, 7.0)
+        ops.paged_attn_shared(w.cache, b, q, 0.09, pre, 470, out=out)
+        assert off(out[:m], attend(w, q[:m], 0.09, prefix=kv)) < TOL and bool((out[m:] == 7.0).all())
+        out.fill_(7.0)
+        ops.paged_attn(w.cache, b, q, 0.09, out=out)
+        assert off(out[:m], attend(w, q[:m], 0.09)) < TOL and bool((out[m:] == 7.0).all())
+        sel = ops.paged_select(w.cache, b, q, 2)
+        assert torch.equal(sel[:m], choose(w, q[:m], 2, 1, 1))
