@@ -29,7 +29,7 @@
 //   96 of 4096 Q4_0 keys: 104 us, 4.4 TB/s: VALU, as much work a key as Q8_0's for half the bytes
 //   one of 777 f16 keys: 7.7 us and 2.4 the merge: two launches, a tile's latency and the join
 //   2 x 1024 tokens, up to 3000 f16 keys: 138 us, 0.76 PFLOP/s of products, which are twice the formula's (8192 tokens 1.1, a library's
-//     product 1.17): matrix cores 30 %, VALU 38 % of the SIMD cycles at two waves a SIMD; over Q8_0 keys 232 us, Q4_0 231: half as many
+//     product 1.17): matrix cores 30 %, VALU 35 % of the SIMD cycles at two waves a SIMD; over Q8_0 keys 232 us, Q4_0 231: half as many
 //     products again and the bringing of integers to LDS
 //   128 tokens behind 16384 shared f16 keys: 107 us and 9 the merge: the same, and the first steps of 384 workgroups
 #include "amv_paged.h"
