@@ -761,13 +761,14 @@ __device__ __forceinline__ void pg_few(const PgAttn& a, int hk, int tile, int ro
     }
 }
 
-// Many rows over f16 keys (prompts, a prefix): tiles of 32 RW rows, 32 of each wave, whose keys come from memory once for the
-// workgroup: read by each wave for itself (pg_few), K's pieces of 16 bytes from 16 rows an instruction keep the loads' address unit busy
-// for all of the time. RW = 4: every wave goes over all keys; RW = 2: two waves a row range, each with one half of every step's keys,
-// joined at the end. K and V rows of 64 keys, a step, go to LDS without registers (global_load_lds), one step ahead in two buffers; the
-// products are those of pg_few with RT = 2. The loads write LDS in lane order, so a row's pieces are exchanged on the memory side: K's 16-byte pieces by a number of the key that differs among the 16 keys of an operand read, V's
-// 32-byte units by one that takes each value twice among the 16 keys of a transposing read (ds_read_b64_tr_b16: 16 lanes pointing at
-// 4 keys' 8-byte quarters of a unit get an element of the 4 keys each), so both reads meet all banks.
+// Many rows (prompts, a prefix): tiles of 32 RW rows, 32 of each wave, whose keys come from memory once for the workgroup: read by each
+// wave for itself (pg_few), K's pieces of 16 bytes from 16 rows an instruction keep the loads' address unit busy for all of the time.
+// RW = 4: every wave goes over all keys; RW = 2: two waves a row range, each with one half of every step's keys, joined at the end. f16
+// K and V rows of 64 keys, a step, go to LDS without registers (global_load_lds), one step ahead in two buffers; the products are those
+// of pg_few with RT = 2. The loads write LDS in lane order, so a row's pieces are exchanged on the memory side: K's 16-byte pieces by a
+// number of the key that differs among the 16 keys of an operand read, V's 32-byte units by one that takes each value twice among the
+// 16 keys of a transposing read (ds_read_b64_tr_b16: 16 lanes pointing at 4 keys' 8-byte quarters of a unit get an element of the 4
+// keys each), so both reads meet all banks.
 typedef __attribute__((address_space(3))) void pg_lds;
 typedef __attribute__((address_space(1))) const void pg_glb;
 typedef short pg_s4 __attribute__((ext_vector_type(4)));
