@@ -1202,7 +1202,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_many_few(PgJobs jobs) {  // jo
 
 // out = sum_z w_z O_z / sum_z w_z l_z over the parts z of a row's keys, w_z = 2^(m_z - max m): one wave per row. A row has parts of
 // its own keys, laid out by sequence where that has at most rows_most rows and else by row, and of the prefix. Bound: the launch and
-// two dependent reads (2.4 us for 32 rows of 7 parts, 4.5 for 96 of 21, 9 for 4096 of the prefix' and their own).
+// two dependent reads (2.4 us for 32 rows of 7 parts, 4.5 for 96 of 21; reads of 8 parts at once, and 4 or 2 where no more are left,
+// are a microsecond less than always 8 for 32 rows of 6 parts).
 struct PgParts {
     const float2* ml;
     const float* acc;
@@ -1254,19 +1255,24 @@ __global__ __launch_bounds__(256) void k_paged_merge(PgMerge a) {
             L = fmaf(wz, p.y, L);
             const uint64_t has = __builtin_amdgcn_ballot_w64(p.x != -INFINITY);
             const int n_here = has ? 64 - __builtin_clzll(has) : 0;  // up to the last part that has keys
-            for (int j0 = 0; j0 < n_here; j0 += 8) {
-                float y[8][E];
+            const auto some = [&](auto width, int j0) {  // parts j0 .. j0 + width - 1, their reads on the way together
+                constexpr int W = width();
+                float y[W][E];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < W; ++j)
 #pragma unroll
                     for (int e = 0; e < E; ++e) y[j][e] = acc[(int64_t)(z0 + min(j0 + j, n_here - 1)) * D + E * lane + e];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
+                for (int j = 0; j < W; ++j) {
                     const float by = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wz), min(j0 + j, 63)));
 #pragma unroll
                     for (int e = 0; e < E; ++e) x[e] = j0 + j < n_here ? fmaf(by, y[j][e], x[e]) : x[e];
                 }
-            }
+            };
+            int j0 = 0;
+            for (; j0 + 4 < n_here; j0 += 8) some(std::integral_constant<int, 8>{}, j0);
+            if (j0 + 2 < n_here) some(std::integral_constant<int, 4>{}, j0);
+            else if (j0 < n_here) some(std::integral_constant<int, 2>{}, j0);
         }
     };
     join(ml1, acc1, a.pre.n);
