@@ -449,10 +449,10 @@ __global__ __launch_bounds__(256) void k_paged_top(PgSelect a) {
             }
         }
         __syncthreads();
-        const uint64_t from = lo + ((uint64_t)s_bin << shift), to = from + ((1ull << shift) - 1);
+        const uint64_t from = lo + ((uint64_t)s_bin << shift);
         need = s_need;
         lo = from;
-        above = to < above ? to : above;
+        if ((above - from) >> shift) above = from + ((1ull << shift) - 1);  // (where it is not past `above`: +infinity's key is near 2^64)
         const bool all = s_in == need;
         __syncthreads();
         if (all) {  // the whole range: nothing is left to be told apart
