@@ -70,7 +70,8 @@ __device__ __forceinline__ float pg_row16_max(float v) {
     return fmaxf(v, __int_as_float(amv_dpp_i<0x140>(__float_as_int(v))));
 }
 // elements 2 i, 2 i + 1 of a row (lane i of its D / 2; a block of 32 is a DPP row of 16 lanes) into row `slot` of a chunk; every lane
-// of the wave calls it, `live` ones store
+// of the wave calls it, `live` ones store. Integers cannot say that an element is no number, and the maxima pass over it: the scale of
+// its block is none instead, so that whoever reads the key or the value learns of it
 template <int TYPE, int D, bool V>
 __device__ __forceinline__ void pg_store_pair(uint8_t* chunk, int ps, int slot, int i, float x0, float x1, int rule, bool live) {
     using R = PgRow<TYPE, D>;
@@ -80,6 +81,8 @@ __device__ __forceinline__ void pg_store_pair(uint8_t* chunk, int ps, int slot, 
         if (live) *reinterpret_cast<amv_h2*>(chunk + (size_t)slot * R::ROW + 4 * i) = h;
     } else {
         uint16_t* scale = reinterpret_cast<uint16_t*>(chunk + (size_t)ps * R::ROW + (size_t)slot * R::SC) + (i >> 4);
+        const uint64_t none = __builtin_amdgcn_ballot_w64(x0 != x0 || x1 != x1);
+        const bool no_number = (none >> (threadIdx.x & 48) & 0xFFFF) != 0;  // in the lane's block
         if constexpr (TYPE == AMV_T_Q8_0) {
             const float amax = pg_row16_max(fmaxf(fabsf(x0), fabsf(x1)));
             const float d = amax / 127.0f;
@@ -91,7 +94,7 @@ __device__ __forceinline__ void pg_store_pair(uint8_t* chunk, int ps, int slot, 
             const int q1 = (int)fminf(127.0f, fmaxf(-127.0f, rule == AMV_Q8_REF ? roundf(t1) : rintf(t1)));
             if (live) {
                 *reinterpret_cast<uint16_t*>(chunk + (size_t)slot * R::ROW + at) = (uint16_t)((q0 & 0xFF) | (q1 & 0xFF) << 8);
-                if ((i & 15) == 0) *scale = amv_f2h(d);
+                if ((i & 15) == 0) *scale = no_number ? 0x7E00 : amv_f2h(d);
             }
         } else {
             // the element of largest magnitude, the first on ties
@@ -111,7 +114,7 @@ __device__ __forceinline__ void pg_store_pair(uint8_t* chunk, int ps, int slot, 
             const int q0 = min(15, max(0, (int)(x0 * id + 8.5f))), q1 = min(15, max(0, (int)(x1 * id + 8.5f)));
             if (live) {
                 chunk[(size_t)slot * R::ROW + (at >> 1)] = (uint8_t)(q0 | q1 << 4);
-                if ((i & 15) == 0) *scale = amv_f2h(d);
+                if ((i & 15) == 0) *scale = no_number ? 0x7E00 : amv_f2h(d);
             }
         }
     }

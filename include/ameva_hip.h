@@ -484,7 +484,8 @@ typedef struct amv_paged_batch {
 int64_t amv_paged_chunk_bytes(int type, int64_t D, int64_t page_size);
 /* ROPE of the q and k heads of qkv f32 [n_tok][n_head + 2 n_head_kv][D] (rows qkv_stride floats apart), the rotated q to q_out
  * f32 [n_tok][n_head][D] (both 16-byte aligned, strides multiples of 4), the rotated k and the v to the pages at their tokens'
- * places, as F16, or as ggml's Q8_0 (`rule`) or Q4_0 of the f32 values. pos int32 [n_tok]: the rotation's positions (NULL: the
+ * places, as F16, or as ggml's Q8_0 (`rule`) or Q4_0 of the f32 values, where a block with an element that is no number gets a scale
+ * that is none (ggml's loses the element). pos int32 [n_tok]: the rotation's positions (NULL: the
  * places). mode 0 NORMAL or 2 NEOX, n_dims even, the rest of a head as it is. The angles pos * freq_scale * freq_base^(-2 i / n_dims), their sines and the rotation are
  * computed in 64 bits and rounded once (amv_rope's are ggml's in 32, which have lost the angle of a far position). q_out rows are
  * out_stride floats apart; q_out == qkv with out_stride == qkv_stride rotates q in place (k and v stay as they are in qkv). With

@@ -44,3 +44,61 @@ def test_select_among_infinite_scores(pages, infinite, n_sel, n_first, n_last, h
     w.cache.bounds[w.table[0, infinite].long(), :, 1, 7] = math.inf
     sel = ops.paged_select(w.cache, w.batch(), q, n_sel, n_first, n_last)
     assert torch.equal(sel, best_pages(w, q, n_sel, n_first, n_last))
+
+
+@pytest.mark.parametrize("t", [Q8_0, Q4_0])
+@pytest.mark.parametrize("rule,d,at", [(0, 128, (2, 70)), (0, 64, (3, 33)), (1, 128, (0, 127)), (2, 64, (31, 32)), (0, 128, (14, 17))])
+def test_append_of_elements_that_are_no_number(t, rule, d, at):
+    """A block with such an element gets a scale that is no number, wherever the element stands; all other blocks are as ever, and the
+    tokens that see the key or the value get no number where the header says so."""
+    from ameva_compute_amd import ops
+    a, b, w = (World(t, 2, d, 16, [20, 9], [20, 9], seed=d + rule) for _ in "abw")
+    x = w.rand(29, 8, d)
+    y = x.clone()
+    y[6, 4, at[0]] = math.nan       # a key of KV head 0
+    y[6, 7, at[1]] = -math.nan      # a value of KV head 1
+    y[25, 4:, at[0]] = math.nan     # all that the second sequence's token 5 stores
+    y[25, 4:, at[1]] = math.nan
+    q = ops.paged_rope_append(a.cache, a.batch(), x, 4, n_dims=0, rule=rule)
+    ops.paged_rope_append(b.cache, b.batch(), y, 4, n_dims=0, rule=rule)
+    ni = 16 * d // (1 if t == Q8_0 else 2)
+    hit = {(0, 6, "k", 0): at[:1], (0, 6, "v", 1): at[1:], **{(1, 5, p, j): at for p in "kv" for j in range(2)}}
+    for p in "kv":
+        was, now = getattr(a.cache, p).clone(), getattr(b.cache, p).clone()
+        for (s, place, what, j), elements in hit.items():
+            if what != p:
+                continue
+            e, slot = int(w.table[s, place // 16]), place % 16
+            for block in {i // 32 for i in elements}:
+                c = ni + (slot * (d // 32) + block) * 2
+                assert bool(now[e, j, c:c + 2].view(torch.float16).isnan()), (p, s, j, block)
+                # (the block's integers do not matter any more)
+                row = slice(slot * (ni // 16), (slot + 1) * (ni // 16))
+                for pool in (was, now):
+                    pool[e, j, c:c + 2] = 0
+                    places = pool[e, j, row].view(*((4, d // 32, -1) if p == "k" else (16, d // 32, -1)))
+                    places[:, block] = 0
+        assert torch.equal(was, now), p
+    r = ops.paged_attn(a.cache, a.batch(), q, d ** -0.5)
+    z = ops.paged_attn(b.cache, b.batch(), q, d ** -0.5)
+    for s, place in ((0, 6), (1, 5)):
+        first, hot, end = w.first[s], w.first[s] + place, w.first[s + 1]
+        assert off(z[first:hot], r[first:hot].double()) < 2e-5
+        assert z[hot:end, :2].isnan().all()  # (heads 0 and 1 are KV head 0's)
+        block = at[1] // 32
+        assert z[hot:end, 2:, 32 * block:32 * block + 32].isnan().all()
+
+
+@pytest.mark.parametrize("mode,n_dims", [(0, 64), (2, 64), (2, 32)])
+def test_append_of_an_element_that_is_no_number_in_f16(mode, n_dims):
+    """F16 pages keep it at its pair's two elements; the bounds are those of the page's other keys there."""
+    from ameva_compute_amd import ops
+    w = World(F16, 1, 64, 16, [16], [16], seed=3, bounds=True)
+    x = w.rand(16, 3, 64)
+    x[9, 1, 5] = math.nan
+    ops.paged_rope_append(w.cache, w.batch(), x, 1, mode=mode, n_dims=n_dims)
+    k = w.cache.k[int(w.table[0, 0]), 0]
+    pair = {5, 4} if mode == 0 else {5, 5 + n_dims // 2}
+    assert set(torch.nonzero(k.isnan())[:, 1].tolist()) == pair and set(torch.nonzero(k.isnan())[:, 0].tolist()) == {9}
+    assert torch.equal(w.cache.bounds[int(w.table[0, 0]), 0],
+                       torch.stack([torch.where(k.isnan(), math.inf, k).amin(0), torch.where(k.isnan(), -math.inf, k).amax(0)]))
