@@ -354,6 +354,15 @@ __global__ __launch_bounds__(256) void k_paged_score(PgSelect a) {
         double x = 0.0;
 #pragma unroll
         for (int e = 0; e < E; ++e) x = fma(up[e], (double)(float)high[j][e], fma(down[e], (double)(float)low[j][e], x));
+        if (x != x) {  // 0 times infinity: a side without a bound, where no q asks for it, does not enter
+            const auto add = [&](double q, double b, double none) { x = q == 0.0 && b == none ? x : fma(q, b, x); };
+            x = 0.0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                add(down[e], (double)(float)low[j][e], -INFINITY);
+                add(up[e], (double)(float)high[j][e], INFINITY);
+            }
+        }
         x += amv_dpp_d<0xB1>(x);
         x += amv_dpp_d<0x4E>(x);
         x += amv_dpp_d<0x141>(x);

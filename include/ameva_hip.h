@@ -514,8 +514,8 @@ int amv_paged_attn_shared(const amv_paged_kv* kv, const amv_paged_batch* batch, 
  * indices into the sequence's table in rising order, -1 behind the last where the token sees fewer pages. The first n_first and
  * the last n_last pages that the token sees are taken (n_first + n_last <= n_sel), then those with the largest score, equal
  * ones by the lower index: the sum over the KV head's query heads of the largest q . k that the page's bounds allow,
- * sum_d (sum_h max(q_hd, 0)) high_d + (sum_h min(q_hd, 0)) low_d, computed in 64 bits. A score that is no number, and a page
- * outside the pool, come last. The pool needs bounds; at most 16384 pages in max_kv. workspace: amv_paged_select_workspace_bytes bytes, 16-byte aligned. */
+ * sum_d (sum_h max(q_hd, 0)) high_d + (sum_h min(q_hd, 0)) low_d, computed in 64 bits, where a high of infinity and a low of minus
+ * infinity (keys beyond f16) do not enter if their factor is 0. A score that is no number, and a page outside the pool, come last. The pool needs bounds; at most 16384 pages in max_kv. workspace: amv_paged_select_workspace_bytes bytes, 16-byte aligned. */
 int64_t amv_paged_select_workspace_bytes(const amv_paged_kv* kv, const amv_paged_batch* batch);
 int amv_paged_select(const amv_paged_kv* kv, const amv_paged_batch* batch, const float* q, int64_t q_stride,
                      int64_t n_head, int64_t n_sel, int64_t n_first, int64_t n_last, int32_t* sel, void* workspace,

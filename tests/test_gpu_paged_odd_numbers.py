@@ -102,3 +102,38 @@ def test_append_of_an_element_that_is_no_number_in_f16(mode, n_dims):
     assert set(torch.nonzero(k.isnan())[:, 1].tolist()) == pair and set(torch.nonzero(k.isnan())[:, 0].tolist()) == {9}
     assert torch.equal(w.cache.bounds[int(w.table[0, 0]), 0],
                        torch.stack([torch.where(k.isnan(), math.inf, k).amin(0), torch.where(k.isnan(), -math.inf, k).amax(0)]))
+
+
+@pytest.mark.parametrize("heads,g", [(1, 1), (8, 2), (6, 6)])
+def test_infinite_bounds_that_no_query_element_meets(heads, g):
+    """A bound of infinity where every query of the group has the other sign, or 0, does not enter: the page's score is a number."""
+    from ameva_compute_amd import ops
+    w = World(F16, g, 64, 16, [16 * 70], seed=heads, bounds=True)
+    q = torch.randn(1, heads, 64, device=DEV)
+    q[:, :, 3] = -q[:, :, 3].abs()
+    q[:, :, 4] = q[:, :, 4].abs()
+    q[:, :, 5] = 0.0
+    at = w.table[0, 2:60:3].long()
+    w.cache.bounds[at, :, 1, 3] = math.inf
+    w.cache.bounds[at, :, 0, 4] = -math.inf
+    w.cache.bounds[at, :, 0, 5], w.cache.bounds[at, :, 1, 5] = -math.inf, math.inf
+    w.cache.bounds[w.table[0, 30].long(), :, 1, 4] = math.inf  # this one's is infinite
+    w.cache.bounds[w.table[0, 31].long(), :, :, 9] = math.nan  # and this one's no number
+    for n_sel in (1, 9, 69):
+        assert torch.equal(ops.paged_select(w.cache, w.batch(), q, n_sel, 0, 0), best_pages(w, q, n_sel, 0, 0))
+
+
+@pytest.mark.parametrize("t", [Q8_0, Q4_0])
+def test_keys_beyond_f16_are_still_selected(t):
+    """A quantized key's element above 65504 is an ordinary number, its f16 bound infinite: the page's other elements still count."""
+    from ameva_compute_amd import ops
+    w = World(t, 1, 64, 16, [16 * 40], [16 * 40], seed=8, bounds=True)
+    x = torch.randn(16 * 40, 3, 64, device=DEV)
+    x[16 * 25 + 3, 1, 40], x[16 * 25 + 3, 1, :32] = 7e4, 5.0
+    ops.paged_rope_append(w.cache, w.batch(), x, 1, n_dims=0)
+    page = int(w.table[0, 25])
+    assert w.cache.bounds[page, 0, 1, 40] == math.inf and w.cache.bounds[page, 0, 0, 40].isfinite()
+    q = torch.ones(1, 1, 64, device=DEV)
+    q[0, 0, 40] = -1e-3
+    b = ops.PagedBatch(w.n_kv_dev, w.table, 16 * 40)
+    assert ops.paged_select(w.cache, b, q, 1, 0, 0).tolist() == [[[25]]]
