@@ -798,7 +798,7 @@ __device__ __align__(16) const uint8_t pg_zeros[16] = {};
 // 2^7 .. 2^8, so that blocks down to 2^-20 of it keep 20 bits; it meets the scores and the weights in f32. Three products of the parts in
 // place of two (the rests' own is below 2^-22), but the scales no longer cost an instruction for each row and block: the 2 x 1024 tokens
 // over Q8_0 keys took 418 us with every wave working from its own registers (pg_few of 32 rows).
-// (true: nothing is written, as a sum is no number: a value that not all rows see may be the reason, which pg_few leaves out)
+// (true: nothing is written, as a sum is no number and a value that not all rows see may be the reason, which pg_few leaves out)
 template <int TYPE, int D, int RW>
 __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z, uint16_t* sKa, uint16_t* sKb, uint16_t* sVa,
                                         uint16_t* sVb) {
@@ -812,6 +812,7 @@ __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z
     if (!pg_rows(a, hk, tile, 32 * RW, t)) return false;
     // steps of 64 keys
     const int begin = z * a.split_len >> 6, end = (min(t.see_any, (z + 1) * a.split_len) + 63) >> 6;
+    const int seen = t.see_all;  // (by all rows of the tile)
     // the wave's own rows, and which half of a step's keys it takes
     const int rw = w & (RW - 1), kw = w / RW, wr0 = t.r0 + 32 * rw, wr1 = min(wr0 + 31, t.r_last);
     const bool idle = wr0 > t.r_last;
@@ -1127,7 +1128,24 @@ __device__ __forceinline__ bool pg_many(const PgAttn& a, int hk, int tile, int z
             }
         }
     }
-    if (__syncthreads_or(sum != sum)) return true;
+    bool again = __builtin_amdgcn_readfirstlane(__syncthreads_or(sum != sum));
+    if (again) {
+        // A sum that is no number is its own rows' matter (a query, a key, a value that they see), unless a value that not all rows see
+        // is infinite or no number. Only those keys' values are looked at, a row tile's tokens and a step of them at most: 2 x 1024
+        // tokens, those of one sequence no number, take 143 us in place of 139; all of pg_few again would be 956.
+        bool strange = false;
+        constexpr int UNITS = QUANT ? 1 : PIECES;  // of a value: its scales, or 16 bytes each
+        for (int i = (int)threadIdx.x; i < (min(64 * end, t.keys) - max(64 * begin, seen)) * UNITS; i += 256) {
+            const int key = max(64 * begin, seen) + i / UNITS, e = t.pages[key >> a.b.pshift];
+            if ((uint32_t)e >= (uint32_t)a.n_pages) continue;
+            uint32_t v[QUANT ? RSC : 4];
+            pg_load<QUANT ? R::SC : 16>(v, vc + pg_off<TYPE, D>(a, e, key, QUANT) + 16 * (i % UNITS));
+#pragma unroll
+            for (int x = 0; x < (QUANT ? RSC : 4); ++x) strange |= pg_strange(v[x]) != 0;
+        }
+        again = __builtin_amdgcn_readfirstlane(__syncthreads_or(strange));
+    }
+    if (again) return true;
     if (idle || (RW == 2 && kw)) return false;
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {

@@ -137,3 +137,69 @@ def test_keys_beyond_f16_are_still_selected(t):
     q[0, 0, 40] = -1e-3
     b = ops.PagedBatch(w.n_kv_dev, w.table, 16 * 40)
     assert ops.paged_select(w.cache, b, q, 1, 0, 0).tolist() == [[[25]]]
+
+
+@pytest.mark.parametrize("t", [F16, Q8_0, Q4_0])
+@pytest.mark.parametrize("strange", ["query", "value", "both"])
+@pytest.mark.parametrize("prefix,n_kv,n_q", [(0, [700, 300, 64], [300, 90, 64]), (333, [200, 70, 9], [130, 70, 9]), (2100, [5] * 70, [1] * 70)])
+def test_rows_that_are_no_number_among_others(t, strange, prefix, n_kv, n_q):
+    """One token's query is no number in one head, one sequence's value infinite at a place that some of its tokens do not see: every
+    other row is as without them."""
+    from ameva_compute_amd import ops
+    n_pre = -(-prefix // 16)
+    w = World(t, 2, 128, 16, n_kv, n_q, seed=prefix + 17, extra=n_pre)
+    pre = w.free[:n_pre].clone()
+    q = torch.randn(w.first[-1], 8, 128, device=DEV)
+    kv = [x[pre.long()].transpose(0, 1).reshape(2, -1, 128)[:, :prefix] for x in (w.k, w.v)]
+    r = attend(w, q, 0.09, prefix=kv)
+    hit = torch.zeros(q.shape[:2], dtype=torch.bool, device=DEV)
+    if strange != "value":
+        tok = w.first[0] + n_q[0] // 3
+        q[tok, 2, 11] = math.nan
+        hit[tok, 2] = True
+    if strange != "query":
+        s = 1
+        place = n_kv[s] - 1 - n_q[s] // 2
+        e, slot = int(w.table[s, place // 16]), place % 16
+        if t == F16:
+            w.cache.v[e, 1, slot, 40] = math.inf
+        else:
+            ni = 16 * 128 // (1 if t == Q8_0 else 2)
+            w.cache.v[..., ni:].view(torch.float16).view(-1, 2, 16, 4)[e, 1, slot, 1] = math.inf
+        hit[w.first[s + 1] - 1 - n_q[s] // 2:w.first[s + 1], 4:] = True
+    b = w.batch()
+    y = ops.paged_attn_shared(w.cache, b, q, 0.09, pre, prefix) if prefix else ops.paged_attn(w.cache, b, q, 0.09)
+    assert off(y[~hit], r[~hit]) < 1e-5  # (test_gpu_paged_attn.py derives it)
+    assert not y[hit].isfinite().all(-1).any()
+
+
+@pytest.mark.parametrize("t", [F16, Q8_0])
+@pytest.mark.parametrize("prefix,n_kv,n_q", [(8192, 64, 1), (0, 1200, 700)])
+def test_a_query_that_is_no_number_costs_no_second_pass(t, prefix, n_kv, n_q):
+    """The time of a batch with such a row against the same without it (least of several; a second pass over the tile's keys in tiles of
+    4 rows took 3 to 7 times as long)."""
+    from ameva_compute_amd import ops
+    n, n_pre = (64, prefix // 64) if prefix else (2, 0)
+    kv = ops.PagedKV.alloc(t, n * -(-n_kv // 64) + n_pre, 64, 8, 128, DEV)
+    for x in (kv.k, kv.v):
+        x.zero_()
+    pages = torch.arange(kv.n_pages, device=DEV).int()
+    b = ops.PagedBatch(torch.full((n,), n_kv, device=DEV).int(), pages[n_pre:].view(n, -1).contiguous(), n_kv, n * n_q,
+                       cu_q=torch.arange(0, n * n_q + 1, n_q, device=DEV).int(), max_q=n_q)
+    q = torch.randn(n * n_q, 32, 128, device=DEV)
+    bad = q.clone()
+    bad[n * n_q // 3] = math.nan
+
+    def least(x):
+        times = []
+        for _ in range(6):
+            a, e = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(10):
+                ops.paged_attn_shared(kv, b, x, 0.1, pages[:n_pre], prefix)
+            e.record()
+            e.synchronize()
+            times.append(a.elapsed_time(e))
+        return min(times)
+    least(q)
+    assert least(bad) < 2 * least(q)
