@@ -243,7 +243,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PgAppend a) {
     }
     amv_h2* low = reinterpret_cast<amv_h2*>(a.bounds + ((size_t)phys * a.n_head_kv + hk) * 2 * D) + i;
     amv_h2* high = low + D / 2;
-    if ((p0 & (ps - 1)) != 0) {  // the page had keys before
+    if ((p0 & (ps - 1)) != 0) {  // the page had keys before (and perhaps some at these places: their bounds stay, wider than need be)
         const amv_h2 l = *low, h = *high;
         lo0 = fminf(lo0, (float)l.x);
         lo1 = fminf(lo1, (float)l.y);

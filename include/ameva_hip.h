@@ -455,8 +455,9 @@ int amv_flash_attn_prefill(const float* q, int64_t q_tok_stride, int64_t q_head_
  *   Q4_0: 4-bit integers [page_size][D], two a byte, the even place in the low bits, value + 8 | scales f16 [page_size][D / 32]
  * The integers of a key lie in an order that the matrix cores take without exchanges: element d of a K row at place
  * (d / 8 % 4) * (D / 4) + d / 32 * 8 + d % 8, of a V row at place (d % 32 / 2) * (D / 16) + d / 32 * 2 + d % 2.
- * bounds (may be NULL): f16 [n_pages][n_head_kv][2][D], the smallest and largest element d of the keys in a page, taken from
- * the rotated keys rounded to f16.
+ * bounds (may be NULL): f16 [n_pages][n_head_kv][2][D], the smallest and largest element d of the keys appended to a page since its
+ * key 0 was, taken from the rotated keys rounded to f16. Where places are written again (tokens taken back, others in their stead),
+ * they still hold for the old keys too: bounds of all keys there, but wider than need be until key 0 is appended again.
  *
  * amv_paged_batch, the sequences of a call, all in device memory but for the sizes. Sequence s has n_kv[s] keys, this call's
  * own included; key j is row j % page_size of page table[s * table_stride + j / page_size]. Its tokens of this call are

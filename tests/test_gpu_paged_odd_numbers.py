@@ -203,3 +203,29 @@ def test_a_query_that_is_no_number_costs_no_second_pass(t, prefix, n_kv, n_q):
         return min(times)
     least(q)
     assert least(bad) < 2 * least(q)
+
+
+def rows_written_again(w, b, place, x):
+    """Appends x at the places from `place` on of a cache that holds one sequence."""
+    from ameva_compute_amd import ops
+    n = x.shape[0]
+    n_kv = torch.tensor([place + n], dtype=torch.int32, device=DEV)
+    ops.paged_rope_append(w.cache, ops.PagedBatch(n_kv, w.table, b, n, cu_q=torch.tensor([0, n], dtype=torch.int32, device=DEV), max_q=n),
+                          x, 1, n_dims=0)
+
+
+@pytest.mark.parametrize("t", [F16, Q8_0])
+def test_bounds_of_places_written_again(t):
+    """Tokens taken back and others appended in their place: the page's bounds hold both, the keys there and those taken back, until
+    the page's place 0 is written again; later pages that begin anew have their own."""
+    w = World(t, 1, 64, 16, [48], seed=5, bounds=True)
+    old, new = w.rand(40, 3, 64), w.rand(14, 3, 64)
+    rows_written_again(w, 48, 0, old)
+    rows_written_again(w, 48, 20, new)  # 20 .. 33: the rest of page 1, and page 2 from its beginning
+    k, k2 = old[:, 1].half(), new[:, 1].half()
+    has = lambda *keys: torch.stack([torch.cat(keys).amin(0), torch.cat(keys).amax(0)])
+    bounds = w.cache.bounds[w.table[0].long(), 0]
+    assert torch.equal(bounds[0], has(k[:16])) and torch.equal(bounds[1], has(k[16:32], k2[:12])) and torch.equal(bounds[2], has(k2[12:]))
+    rows_written_again(w, 48, 16, torch.cat([old[16:20], new]))  # the page from its beginning
+    bounds = w.cache.bounds[w.table[0].long(), 0]
+    assert torch.equal(bounds[1], has(k[16:20], k2[:12])) and torch.equal(bounds[2], has(k2[12:]))
