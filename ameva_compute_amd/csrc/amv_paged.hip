@@ -45,8 +45,8 @@ int pg_check(const char* what, const amv_paged_kv* kv, const amv_paged_batch* b,
 // waves (one where every sequence has one token), D / 2 lanes per token, two elements a lane: the lanes' angle, sine and cosine
 // are computed once per token in f64 and used by the G query heads and the key head. Elements are rotated in f64 and rounded to
 // f32, which fixes the f32 value, and so the stored f16 or integer, up to one in 2^29 borderline cases, however a machine orders
-// the sum. What bounds it: memory (4500 tokens of 32 and 8 heads of 128 over f16 pages, 193 MB: 39.6 us, 4.9 TB/s, where a copy of
-// 4 GiB reaches 5.0), at one token a sequence the launch (48 tokens: 4.5 us).
+// the sum. What bounds it: memory (4226 tokens of 32 and 8 heads of 128 into f16 pages of 16, 193 MB: 40 us, 4.8 TB/s, where a copy
+// of 4 GiB reaches 5.0; into pages of 64, a quarter of the workgroups, 60 the call), at one token a sequence the launch (48 tokens: 4.5 us).
 struct PgAppend {
     PgBatch b;
     const float* qkv;

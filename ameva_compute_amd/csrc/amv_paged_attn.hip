@@ -13,8 +13,8 @@
 //     operand elements is all the transposing there is.
 // q and the weights are f32; f16 alone would cost them 2^-11. Each enters its product as two f16, the value rounded and the rest
 // (22 bits together): twice the matrix work, at less than a fifth of their rate where keys come from memory. q is scaled by a power
-// of two to below 2 first, so that no f32 is out of f16's range; the weights' reference is kept 12 to 15 below the running maximum, so
-// that the rest keeps its bits beside a dominating key.
+// of two to below 2 first (from 2^103 on by 2^-102, so that q times scale log2(e) leaves f16's range at 2^118); the weights' reference is
+// kept 12 to 15 below the running maximum, so that the rest keeps its bits beside a dominating key.
 // Quantized caches: the integers are exact in f16. Block b of a key is one product of K's (its own accumulator, then times the
 // block's scale in f32), and two of V's products, whose weights are multiplied by the value's scale before they are split. The
 // scales are brought to at most 1 by a power of two that follows the largest met (as the maximum does), which keeps weight times
@@ -31,7 +31,9 @@
 //   2 x 1024 tokens, up to 3000 f16 keys: 138 us, 0.76 PFLOP/s of products, which are twice the formula's (8192 tokens 1.1, a library's
 //     product 1.17): matrix cores 30 %, VALU 35 % of the SIMD cycles at two waves a SIMD; over Q8_0 keys 232 us, Q4_0 231: half as many
 //     products again and the bringing of integers to LDS
-//   128 tokens behind 16384 shared f16 keys: 107 us and 9 the merge: the same, and the first steps of 384 workgroups
+//   128 tokens behind 16384 shared f16 keys: 107 us and 7 the merge: the same, and the first steps of 384 workgroups
+//   32 sequences of up to 8 tokens after up to 4096 keys (17 to 32 rows a KV head): f16 84 us, 70 of them the bytes; Q8_0 142, half of the
+//     waves of tiles of 64 rows having no rows; Q4_0 121, VALU (29 %) and the way of 64 spilled registers
 #include "amv_paged.h"
 
 #include <algorithm>
@@ -1309,12 +1311,16 @@ struct PgTiles {
     int rows() const { return 16 * rt / pack; }
     int of(int64_t n) const { return (int)((n + rows() - 1) / rows()); }
 };
+// Two row tiles (17 to 32 rows) of heads of 128 need more than the 256 registers of two waves a SIMD: 3 are spilled over f16 keys, 64
+// over Q4_0, 86 over Q8_0, and 41, 103 and 119 in the kernels that have tiles of many rows too. 32 sequences of up to 4096 keys in
+// groups of 32 heads take 30, 42 and 54 us, their bytes 18, 5 and 10; 64 of up to 5 tokens in groups of 4 behind 8192 keys (their own up
+// to 512 in such tiles) 88 over f16 and 130 over Q4_0.
 static PgTiles pg_tiles(int64_t rows) { return {rows > 16 ? 2 : 1, rows <= 4 ? 4 : rows <= 8 ? 2 : 1}; }
 // How a call is launched, and the workspace of the parts
 struct PgPlan {
     PgTiles few;                            // tiles of few rows: sequences (or listed tokens), ta tiles each, and a small batch's prefix
     int ta, n_one, len_one;                 // their parts
-    int many_rows;                          // rows of the other tiles: 64 or 128, of quantized keys 32
+    int many_rows;                          // rows of the other tiles: 64 or 128
     int find, rows_most, n_find, len_find;  // sequences of more rows than rows_most
     int64_t find_tiles;
     bool pre_many;                          // the prefix in tiles of many rows
@@ -1345,8 +1351,8 @@ static PgPlan pg_plan(const amv_paged_kv* kv, const amv_paged_batch* b, int64_t 
         return p;
     }
     const int64_t rows = std::min(b->max_q, b->n_tok) * G;
-    // 17 to 32 rows are one tile of few rows, but not of Q8_0 keys, whose registers for it do not suffice (32 sequences of 8 tokens
-    // after 4096 keys 147 us, in half a tile of 64 rows 141; Q4_0 122 and 140)
+    // 17 to 32 rows are one tile of few rows, but not of Q8_0 keys, whose registers for it suffice least (32 sequences of up to 8 tokens
+    // after up to 4096 keys 147 us, in half a tile of 64 rows 141; Q4_0 122 and 140)
     const int64_t most = kv->type == AMV_T_Q8_0 ? 16 : 32;
     p.pre_many = all > most;
     p.few = pg_tiles(n_prefix > 0 && !p.pre_many ? all : rows <= most ? rows : G);

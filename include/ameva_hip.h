@@ -465,11 +465,11 @@ int amv_flash_attn_prefill(const float* q, int64_t q_tok_stride, int64_t q_head_
  * n_seq): the last of its keys, so token i of n_q stands at place n_kv - n_q + i and sees the keys 0 .. place. max_q >= every
  * n_q and max_kv >= every n_kv size the launches, so a captured graph replays at growing lengths; keys from place max_kv on are
  * neither stored nor seen.
- * Rows from cu_q[n_seq] on are left as they were. A table entry outside [0, n_pages) is a page without keys; entries that no
- * key needs are not looked at. What lies in a page behind a sequence's last key does not matter, and a key or value that is
- * infinite or no number reaches only the tokens that see it: with a key, their head's row is no number, with a value at least the
- * elements that it stands in (a block of 32 with a scale). n_seq is at most 65535, n_tok * n_head 2^25, max_kv 2^30; what would need
- * more than 2^23 workgroups is refused.
+ * Rows from cu_q[n_seq] on are left as they were. A table entry outside [0, n_pages) is a page without keys; entries that no key
+ * needs are not looked at. What lies in a page behind a sequence's last key does not matter, and a key or value that is infinite or
+ * no number reaches only the tokens that see it: with a key, their head's row is no number (or, where an infinite key scores minus
+ * infinity, as if it were not there), with a value at least the elements that it stands in (a block of 32 with a scale). n_seq is at
+ * most 65535, n_tok * n_head 2^25, max_kv 2^30; what would need more than 2^23 workgroups is refused.
  * ---------------------------------------------------------------------------------------------------------- */
 typedef struct amv_paged_kv {
     int32_t type, n_head_kv, D, page_size;
@@ -485,22 +485,22 @@ typedef struct amv_paged_batch {
 int64_t amv_paged_chunk_bytes(int type, int64_t D, int64_t page_size);
 /* ROPE of the q and k heads of qkv f32 [n_tok][n_head + 2 n_head_kv][D] (rows qkv_stride floats apart), the rotated q to q_out
  * f32 [n_tok][n_head][D] (both 16-byte aligned, strides multiples of 4), the rotated k and the v to the pages at their tokens'
- * places, as F16, or as ggml's Q8_0 (`rule`) or Q4_0 of the f32 values, where a block with an element that is no number gets a scale
- * that is none (ggml's loses the element). pos int32 [n_tok]: the rotation's positions (NULL: the
- * places). mode 0 NORMAL or 2 NEOX, n_dims even, the rest of a head as it is. The angles pos * freq_scale * freq_base^(-2 i / n_dims), their sines and the rotation are
- * computed in 64 bits and rounded once (amv_rope's are ggml's in 32, which have lost the angle of a far position). q_out rows are
- * out_stride floats apart; q_out == qkv with out_stride == qkv_stride rotates q in place (k and v stay as they are in qkv). With
- * bounds, those of the pages written to are brought up to date (an element that is no number does not enter); a page's begin with
- * its key 0. A token whose place is negative or from max_kv on, or whose page is outside the pool, is not stored, and adds 1 per
- * KV head to *bad (device, may be NULL). Pages that a call writes belong to one of its sequences each. */
+ * places, as F16, or as ggml's Q8_0 (`rule`) or Q4_0 of the f32 values, where a block with an element that is no number gets a
+ * scale that is none (ggml's loses the element). pos int32 [n_tok]: the rotation's positions (NULL: the places). mode 0 NORMAL or 2
+ * NEOX, n_dims even, the rest of a head as it is. The angles pos * freq_scale * freq_base^(-2 i / n_dims), their sines and the
+ * rotation are computed in 64 bits and rounded once (amv_rope's are ggml's in 32, which have lost the angle of a far position).
+ * q_out rows are out_stride floats apart; q_out == qkv with out_stride == qkv_stride rotates q in place (k and v stay as they are
+ * in qkv). With bounds, those of the pages written to are brought up to date (an element that is no number does not enter); a
+ * page's begin with its key 0. A token whose place is negative or from max_kv on, or whose page is outside the pool, is not stored,
+ * and adds 1 per KV head to *bad (device, may be NULL). Pages that a call writes belong to one of its sequences each. */
 int amv_paged_rope_append(const amv_paged_kv* kv, const amv_paged_batch* batch, const float* qkv, int64_t qkv_stride,
                           int64_t n_head, const int32_t* pos, int n_dims, int mode, float freq_base, float freq_scale,
                           float attn_factor, int rule, float* q_out, int64_t out_stride, unsigned int* bad, void* stream);
 /* Attention of the batch's tokens over their sequences' keys: out[t][h] = sum_j w_j v_j, w = softmax_j(scale * q[t][h] . k_j) over
  * the keys the token sees, head h with KV head h / (n_head / n_head_kv). q f32 [n_tok][n_head][D] (rows q_stride floats apart,
  * 16-byte aligned), out f32 [n_tok][n_head][D]; a token that sees no key gets zeros. q, the weights and the values meet in 32-bit
- * arithmetic: q and the weights are given to the f16 matrix cores as two f16 each. workspace: amv_paged_attn_workspace_bytes
- * (n_prefix and n_sel 0) bytes, 16-byte aligned. */
+ * arithmetic: q and the weights are given to the f16 matrix cores as two f16 each. A row in which |scale log2(e) q| reaches 2^118 is no
+ * number. workspace: amv_paged_attn_workspace_bytes (n_prefix and n_sel 0) bytes, 16-byte aligned. */
 int64_t amv_paged_attn_workspace_bytes(const amv_paged_kv* kv, const amv_paged_batch* batch, int64_t n_head,
                                        int64_t n_prefix, int64_t n_sel);
 int amv_paged_attn(const amv_paged_kv* kv, const amv_paged_batch* batch, const float* q, int64_t q_stride, float* out,
@@ -516,7 +516,8 @@ int amv_paged_attn_shared(const amv_paged_kv* kv, const amv_paged_batch* batch, 
  * the last n_last pages that the token sees are taken (n_first + n_last <= n_sel), then those with the largest score, equal
  * ones by the lower index: the sum over the KV head's query heads of the largest q . k that the page's bounds allow,
  * sum_d (sum_h max(q_hd, 0)) high_d + (sum_h min(q_hd, 0)) low_d, computed in 64 bits, where a high of infinity and a low of minus
- * infinity (keys beyond f16) do not enter if their factor is 0. A score that is no number, and a page outside the pool, come last. The pool needs bounds; at most 16384 pages in max_kv. workspace: amv_paged_select_workspace_bytes bytes, 16-byte aligned. */
+ * infinity (keys beyond f16) do not enter if their factor is 0. A score that is no number, and a page outside the pool, come last.
+ * The pool needs bounds; at most 16384 pages in max_kv. workspace: amv_paged_select_workspace_bytes bytes, 16-byte aligned. */
 int64_t amv_paged_select_workspace_bytes(const amv_paged_kv* kv, const amv_paged_batch* batch);
 int amv_paged_select(const amv_paged_kv* kv, const amv_paged_batch* batch, const float* q, int64_t q_stride,
                      int64_t n_head, int64_t n_sel, int64_t n_first, int64_t n_last, int32_t* sel, void* workspace,
