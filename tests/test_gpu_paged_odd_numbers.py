@@ -229,3 +229,53 @@ def test_bounds_of_places_written_again(t):
     rows_written_again(w, 48, 16, torch.cat([old[16:20], new]))  # the page from its beginning
     bounds = w.cache.bounds[w.table[0].long(), 0]
     assert torch.equal(bounds[1], has(k[16:20], k2[:12])) and torch.equal(bounds[2], has(k2[12:]))
+
+
+@pytest.mark.parametrize("t", [F16, Q8_0, Q4_0])
+@pytest.mark.parametrize("heads,g,n_kv,n_q", [(8, 2, [300, 40], [1, 1]), (8, 2, [300, 40], [2, 1]), (8, 2, [300, 70], [4, 7]),
+                                              (32, 2, [90, 64], [2, 1]), (8, 2, [700, 333], [300, 90])])
+def test_infinite_keys(t, heads, g, n_kv, n_q):
+    """A head's row that sees an infinite key is no number in all elements, or that of the other keys; the rest is as ever."""
+    from ameva_compute_amd import ops
+    w = World(t, g, 128, 16, n_kv, n_q, seed=31)
+    q = torch.randn(w.first[-1], heads, 128, device=DEV)
+    r = attend(w, q, 0.09)
+    sees = torch.zeros(w.first[-1], dtype=torch.bool, device=DEV)
+    there = []
+    for s, (n, m) in enumerate(zip(n_kv, n_q)):
+        place = n - 1 - m // 2
+        e, slot = int(w.table[s, place // 16]), place % 16
+        if t == F16:
+            w.cache.k[e, 0, slot, 9] = -math.inf if s else math.inf
+        else:
+            ni = 16 * 128 // (1 if t == Q8_0 else 2)
+            w.cache.k[..., ni:].view(torch.float16).view(-1, g, 16, 4)[e, 0, slot, 2] = math.inf
+        sees[w.first[s + 1] - 1 - m // 2:w.first[s + 1]] = True
+        there.append(torch.arange(n, device=DEV) != place)
+    other = attend(w, q, 0.09, see=lambda s, i, j: there[s])
+    y, G = ops.paged_attn(w.cache, w.batch(), q, 0.09), heads // g
+    assert off(y[~sees], r[~sees]) < 1e-5 and off(y[:, G:], r[:, G:]) < 1e-5
+    hit, without = y[sees, :G].flatten(0, 1), other[sees, :G].flatten(0, 1)
+    none = hit.isnan().all(-1)
+    assert bool(none.any()) and off(hit[~none], without[~none]) < 1e-5
+
+
+@pytest.mark.parametrize("t", [F16, Q8_0])
+@pytest.mark.parametrize("n_q", [1, 2, 4, 100])
+def test_queries_of_any_size(t, n_q):
+    """|scale log2(e) q| up to 2^117: the key of the largest score has all the weight. From 2^118 on that head's row is no number, and
+    the others are as ever."""
+    from ameva_compute_amd import ops
+    w = World(t, 2, 64, 16, [130], [n_q], seed=n_q)
+    q = torch.randn(n_q, 8, 64, device=DEV)
+    to = lambda e: 2.0 ** e / (0.125 * math.log2(math.e))
+    q[0, 1] *= to(117) / float(q[0, 1].abs().max()) * 0.9
+    q[0, 3] *= to(100) / float(q[0, 3].abs().max())
+    q[0, 2] *= 2.0 ** -120
+    r = attend(w, q, 0.125)
+    q[0, 5, 7] = to(118) * 1.01
+    y = ops.paged_attn(w.cache, w.batch(), q, 0.125)
+    assert y[0, 5].isnan().all()
+    y[0, 5] = r[0, 5].float()
+    for h in range(8):
+        assert off(y[:, h], r[:, h]) < 1e-5, h
