@@ -86,6 +86,15 @@ SIGNATURES = {
     "amv_paged_select_workspace_bytes": (I64, [P, P]),
     "amv_paged_select": (I32, [P, P, P, I64, I64, I64, I64, I64, P, P, I64, P]),
     "amv_paged_attn_sparse": (I32, [P, P, P, I64, P, I64, P, I64, F32, P, I64, P]),
+    "amv_add_rms_norm_act": (I32, [P, P, I64, I64, F32, P, P, P, P, I32, I32, P]),
+    "amv_act_values": (I32, [I32, P, I64, I64, I32, P, P]),
+    "amv_moe_route": (I32, [P, I64, I64, I64, I64, I32, P, I64, I64, I32, I32, F32, P, P, P]),
+    "amv_moe_plan_bytes": (I64, [I64, I64, I64]),
+    "amv_moe_plan": (I32, [P, I64, I64, I64, P, P]),
+    "amv_moe_gate_up_workspace_bytes": (I64, [I64, I64, I64, I32]),
+    "amv_moe_gate_up": (I32, [I32, P, P, I64, I64, I64, I64, P, I64, I64, P, P, P, P, I32, I32, P, I64, P]),
+    "amv_moe_down_workspace_bytes": (I64, [I64, I64, I64]),
+    "amv_moe_down": (I32, [I32, P, I64, I64, I64, I64, P, I64, I64, P, P, P, P, P, P, I64, P]),
     "amv_binary": (I32, [I32, P, P, P, I64, I64, I64, P]),
     "amv_set_rows_f16": (I32, [P, I64, P, I64, I64, I64, P, I32, I64, P, P]),
     "amv_i2s_gemv_acc": (I32, [P, I64, I64, P, F32, P, P]),

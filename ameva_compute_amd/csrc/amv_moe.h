@@ -1,0 +1,73 @@
+// What the kernels of a mixture of experts share: the plan of a call's (token, slot) pairs, and checks of their arguments.
+#pragma once
+#include "amv_common.h"
+
+// A plan, int32 words: tiles of up to MOE_FEW rows, tiles of up to MOE_MANY rows, then the pairs in the order of their experts
+// (in the order of their numbers within one). A tile is two words: expert | rows << 16, place of its first pair in the order;
+// rows 0: no tile. Pairs without an expert stand last, in tiles of the expert n_expert. n_used >= 1, n_expert <= MOE_MAX_EXPERTS.
+#define MOE_MAX_EXPERTS 1024
+#define MOE_MAX_USED 64
+#define MOE_MAX_PAIRS (1 << 22)
+#define MOE_FEW 16
+#define MOE_MANY 64
+// up to this many pairs one workgroup makes the plan, its tiles side by side; above it each expert has places of its own for
+// them, the unused ones among them
+#define MOE_PLAN_ONE 4096
+
+static inline int64_t moe_tiles(int64_t pairs, int64_t n_expert, int64_t rows) {
+    const int64_t e = n_expert + 1;
+    if (pairs > MOE_PLAN_ONE) return pairs / rows + e;
+    const int64_t most = pairs < e ? pairs : e;  // experts that have a pair
+    const int64_t n = (pairs + (rows - 1) * most) / rows;
+    return n < pairs ? n : pairs;
+}
+struct MoePlanView {
+    const int2* few;
+    const int2* many;
+    const int32_t* order;
+    int n_few, n_many;
+};
+static inline MoePlanView moe_plan_view(const void* plan, int64_t pairs, int64_t n_expert) {
+    MoePlanView v;
+    v.n_few = (int)moe_tiles(pairs, n_expert, MOE_FEW);
+    v.n_many = (int)moe_tiles(pairs, n_expert, MOE_MANY);
+    v.few = (const int2*)plan;
+    v.many = v.few + v.n_few;
+    v.order = (const int32_t*)(v.many + v.n_many);
+    if (!plan) {  // each pair by itself
+        v.few = nullptr;
+        v.n_few = (int)pairs;
+    }
+    return v;
+}
+
+// the experts' matrices of a product: rows x k of `type` each, `stride` bytes apart; a gate has its up beside it
+struct MoeProduct {
+    int type, n_expert, n_used;
+    int64_t rows, k, stride, n_tok;
+    const void *w0, *w1;
+    const void* act;
+    int64_t act_rows;
+    const int32_t* ids;
+    const void* plan;
+    // gate and up: f32 [pairs][rows] and / or the 8-bit output; down: f32 [pairs][rows]
+    float* out;
+    AmvActOut q;
+    hipStream_t st;
+};
+int moe_few(const MoeProduct& p);
+
+// amv_act_store4 for a block with an element that is infinite or no number: integers cannot say so and the largest value passes over
+// it, so the block's scale is made none, and whatever reads it learns of it. Called as amv_act_store4.
+__device__ __forceinline__ void moe_act_store4(const AmvActOut& o, int c, const float (&v)[4]) {
+    amv_act_store4(o, c, v);
+    const bool bad = !(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY);
+    const uint64_t any = __ballot(bad);
+    if (!any) return;
+    const int lane = threadIdx.x & 63;
+    if (o.type == AMV_T_Q8_0) {
+        if ((c & 7) == 0 && ((any >> (lane & 56)) & 0xFF)) reinterpret_cast<int2*>(o.meta)[c >> 3].x = 0x7FC00000;
+    } else if ((c & 63) == 0) {
+        reinterpret_cast<int*>(o.meta)[c >> 6] = 0x7FC00000;
+    }
+}

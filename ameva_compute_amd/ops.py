@@ -788,6 +788,200 @@ def paged_attn_sparse(kv: PagedKV, batch: PagedBatch, q: torch.Tensor, sel: torc
     return out
 
 
+# ---------------------------------------------------------------------------------------------- mixture of experts
+MOE_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+class QExperts:
+    """The matrices of n_expert experts, n_rows x k each, in the MI355X layout (QWeight's), one after the other: data uint8 [n_expert,
+    bytes], rows any multiple of 16 bytes apart."""
+
+    def __init__(self, wtype: int, n_expert: int, n_rows: int, k: int, data: torch.Tensor):
+        need = lib().amv_weight_bytes(wtype, n_rows, k)
+        _need_gpu(data, "QExperts", contiguous=False)
+        if need < 0 or data.dtype != torch.uint8 or data.dim() != 2 or data.shape[0] != n_expert or data.shape[1] < need or \
+                data.stride(1) != 1 or data.stride(0) % 16 or (n_expert > 1 and data.stride(0) < need):
+            raise ValueError(f"QExperts: type {wtype}, {n_expert} experts of {n_rows}x{k}: uint8 rows of {need} bytes, a multiple of 16 apart")
+        self.type, self.n_expert, self.n_rows, self.k, self.data = wtype, n_expert, n_rows, k, data
+        self.index, self.device = data.get_device(), data.device
+        self.stride = data.stride(0) if n_expert > 1 else (need + 15) // 16 * 16
+        self.ptr = data.data_ptr()
+
+    @classmethod
+    def from_ggml(cls, wtype: int, ggml_bytes: torch.Tensor, n_expert: int, n_rows: int, k: int) -> "QExperts":
+        """From a ggml tensor [n_expert][n_rows][k] of blocks (ffn_gate_exps, ffn_up_exps, ffn_down_exps)."""
+        _need_gpu(ggml_bytes, "QExperts.from_ggml")
+        need = lib().amv_weight_bytes(wtype, n_rows, k)
+        if need < 0 or ggml_bytes.numel() * ggml_bytes.element_size() < n_expert * need:
+            raise ValueError(f"QExperts.from_ggml: type {wtype} {n_expert}x{n_rows}x{k} needs {n_expert * need} bytes")
+        out = torch.zeros((n_expert, (need + 15) // 16 * 16), dtype=torch.uint8, device=ggml_bytes.device)
+        with torch.cuda.device(ggml_bytes.device):
+            for e in range(n_expert):
+                check(lib().amv_repack(wtype, ggml_bytes.data_ptr() + e * need, out[e].data_ptr(), n_rows, k, _stream()), "amv_repack")
+        return cls(wtype, n_expert, n_rows, k, out)
+
+
+class MoePlan:
+    """The (token, slot) pairs of ids int32 [n_tok, n_used] in the order of their experts (moe_plan), for the products on the same
+    ids; a plan of one token is its ids alone."""
+
+    def __init__(self, ids: torch.Tensor, n_expert: int, buffer: torch.Tensor | None):
+        self.ids, self.n_expert, self.buffer = ids, n_expert, buffer
+        self.n_tok, self.n_used = ids.shape
+        self.index = ids.get_device()
+
+
+def _on_device_of(f):
+    """f(x, ...) with the GPU of x (a tensor, experts or a plan) as the current one."""
+    @functools.wraps(f)
+    def g(x, *args, **kw):
+        i = x.get_device() if isinstance(x, torch.Tensor) else x.index
+        if i < 0:
+            raise ValueError(f"{f.__name__}: tensor must be on the GPU (no CPU path)")
+        if i == _device():
+            return f(x, *args, **kw)
+        with torch.cuda.device(i):
+            return f(x, *args, **kw)
+    return g
+
+
+def _f32_on(t: torch.Tensor | None, shape, index: int, what: str) -> None:
+    if t is not None and (t.shape != shape or t.dtype is not torch.float32 or t.get_device() != index or not t.is_contiguous()):
+        raise ValueError(f"{what}: contiguous f32 {tuple(shape)} on the same GPU expected")
+
+
+@_on_device_of
+def add_rms_norm(x: torch.Tensor, add: torch.Tensor, eps: float, w: torch.Tensor | None = None, act_type: int | None = None,
+                 rule: int = Q8_X86, out: torch.Tensor | None = None, normed: bool = True):
+    """The residual's addition and RMS_NORM of it in one pass: x, add f32 [..., n]. Returns (x + add (in out, which may be x or
+    add), its norm times w (None without `normed`), the norm's activation rows of act_type (None without one))."""
+    shape, index = x.shape, x.get_device()
+    if x.dtype is not torch.float32 or not x.is_contiguous() or not len(shape):
+        raise ValueError("add_rms_norm: x must be contiguous f32")
+    n = shape[-1]
+    _f32_on(add, shape, index, "add_rms_norm: add")
+    _f32_on(w, (n,), index, "add_rms_norm: w")
+    _f32_on(out, shape, index, "add_rms_norm: out")
+    rows = x.numel() // n if n else 0
+    s = torch.empty_like(x) if out is None else out
+    o = torch.empty_like(x) if normed else None
+    act = None
+    if act_type is not None:
+        if act_type not in (Q8_0, Q8_K) or n % (256 if act_type == Q8_K else 32):
+            raise ValueError(f"add_rms_norm: rows of {n} have no activation type {act_type}")
+        act = torch.empty(_act_bytes(act_type, rows, n) if rows else 0, dtype=torch.uint8, device=x.device)
+    check(lib().amv_add_rms_norm_act(x.data_ptr(), add.data_ptr(), rows, n, eps, _ptr(w), s.data_ptr(), _ptr(o), _ptr(act),
+                                     act_type or 0, rule, _stream()) if rows else 0, "amv_add_rms_norm_act")
+    return s, o, act
+
+
+@_on_device_of
+def act_values(act: torch.Tensor, act_type: int, m: int, k: int, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """The values [m, k] (f16 or f32) that activation rows of quantize_act's layout (Q8_0 or Q8_K) stand for."""
+    if dtype not in (torch.float16, torch.float32) or act_type not in (Q8_0, Q8_K) or m < 0 or k <= 0 or k % (256 if act_type == Q8_K else 32):
+        raise ValueError(f"act_values: type {act_type} {m}x{k} to {dtype} is not supported")
+    _act_holds(act, act_type, m, k, act.get_device(), "act_values")
+    out = torch.empty((m, k), dtype=dtype, device=act.device)
+    if m:
+        check(lib().amv_act_values(act_type, act.data_ptr(), m, k, F16 if dtype is torch.float16 else F32, out.data_ptr(), _stream()),
+              "amv_act_values")
+    return out
+
+
+def _act_holds(act: torch.Tensor, act_type: int, m: int, k: int, index: int, what: str) -> None:
+    if act.dtype is not torch.uint8 or act.get_device() != index or not act.is_contiguous() or (m and act.numel() < _act_bytes(act_type, m, k)):
+        raise ValueError(f"{what}: contiguous uint8 activations of type {act_type}, {m} rows of {k}, on the same GPU expected")
+
+
+@_on_device_of
+def moe_route(logits: torch.Tensor, n_used: int, score: str = "softmax", bias: torch.Tensor | None = None, n_group: int = 1,
+              top_group: int = 1, group_best: int = 1, renorm: bool = True, scale: float = 1.0):
+    """The n_used experts of each token and their weights (ids int32, weights f32, [n_tok, n_used]) from logits f32 [n_tok,
+    n_expert], rows any stride apart: include/ameva_hip.h amv_moe_route."""
+    if logits.dim() != 2 or logits.dtype is not torch.float32 or (logits.numel() and logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("moe_route: logits must be f32 [n_tok, n_expert] with contiguous rows")
+    if score not in MOE_SCORES:
+        raise ValueError(f"moe_route: score {score!r} (softmax or sigmoid)")
+    t, e = logits.shape
+    _f32_on(bias, (e,), logits.get_device(), "moe_route: bias")
+    stride = logits.stride(0) if t > 1 else e
+    ids = torch.empty((t, max(n_used, 0)), dtype=torch.int32, device=logits.device)
+    weights = torch.empty((t, max(n_used, 0)), dtype=torch.float32, device=logits.device)
+    if t:
+        check(lib().amv_moe_route(logits.data_ptr(), stride, t, e, n_used, MOE_SCORES[score], _ptr(bias), n_group, top_group, group_best,
+                                  int(renorm), scale, ids.data_ptr(), weights.data_ptr(), _stream()), "amv_moe_route")
+    return ids, weights
+
+
+@_on_device_of
+def moe_plan(ids: torch.Tensor, n_expert: int) -> MoePlan:
+    """The pairs of ids int32 [n_tok, n_used] in the order of their experts, once for moe_gate_up and moe_down of a layer."""
+    if ids.dim() != 2 or ids.dtype is not torch.int32 or not ids.is_contiguous():
+        raise ValueError("moe_plan: ids must be contiguous int32 [n_tok, n_used]")
+    t, u = ids.shape
+    n = lib().amv_moe_plan_bytes(t, u, n_expert)
+    if n < 0:
+        check(-1, "amv_moe_plan_bytes")
+    if t <= 1:
+        return MoePlan(ids, n_expert, None)
+    buf = torch.empty(n, dtype=torch.uint8, device=ids.device)
+    check(lib().amv_moe_plan(ids.data_ptr(), t, u, n_expert, buf.data_ptr(), _stream()), "amv_moe_plan")
+    return MoePlan(ids, n_expert, buf)
+
+
+def _moe_check(w: QExperts, plan: MoePlan, act: torch.Tensor, m: int, what: str) -> None:
+    if plan.index != w.index or plan.n_expert != w.n_expert:
+        raise ValueError(f"{what}: the plan is for {plan.n_expert} experts, or another GPU")
+    _act_holds(act, Q8_K if w.type in (Q4_K, Q6_K) else Q8_0, m, w.k, w.index, what)
+
+
+@_on_device_of
+def moe_gate_up(gate: QExperts, up: QExperts, act: torch.Tensor, plan: MoePlan, act_type: int | None = Q8_0, rule: int = Q8_X86,
+                eout: bool = False):
+    """silu(gate a) * (up a) of each pair's expert and its token's activation row a: the activation rows [n_tok * n_used] of
+    act_type that moe_down reads; with eout the f32 values [n_tok * n_used, n_rows] too, (act, values); act_type None: those alone."""
+    if (up.type, up.n_expert, up.n_rows, up.k, up.stride, up.index) != (gate.type, gate.n_expert, gate.n_rows, gate.k, gate.stride, gate.index):
+        raise ValueError("moe_gate_up: gate and up experts differ in type, shape or device")
+    _moe_check(gate, plan, act, plan.n_tok, "moe_gate_up")
+    F, pairs = gate.n_rows, plan.n_tok * plan.n_used
+    if act_type not in (None, Q8_0, Q8_K) or (act_type == Q8_K and F % 256):
+        raise ValueError(f"moe_gate_up: rows of {F} have no activation type {act_type}")
+    h = torch.empty((pairs, F), dtype=torch.float32, device=act.device) if eout or act_type is None else None
+    a = ws = None
+    need = 0
+    if act_type is not None:
+        a = torch.empty(_act_bytes(act_type, pairs, F) if pairs else 0, dtype=torch.uint8, device=act.device)
+        if h is None:
+            need = lib().amv_moe_gate_up_workspace_bytes(plan.n_tok, plan.n_used, F, act_type)
+            ws = torch.empty(need, dtype=torch.uint8, device=act.device) if need else None
+    if pairs:
+        check(lib().amv_moe_gate_up(gate.type, gate.ptr, up.ptr, gate.stride, gate.n_expert, F, gate.k, act.data_ptr(), plan.n_tok,
+                                    plan.n_used, plan.ids.data_ptr(), _ptr(plan.buffer), _ptr(h), _ptr(a), act_type or 0, rule, _ptr(ws),
+                                    need, _stream()), "amv_moe_gate_up")
+    return h if a is None else (a, h) if eout else a
+
+
+@_on_device_of
+def moe_down(down: QExperts, act: torch.Tensor, plan: MoePlan, weights: torch.Tensor, add: torch.Tensor | None = None,
+             out: torch.Tensor | None = None) -> torch.Tensor:
+    """f32 [n_tok, n_rows]: add (f32, or None: 0) and the sum over a token's experts of weights [n_tok, n_used] times the expert's
+    product with the pair's activation row (moe_gate_up's). out may be add."""
+    t, u, n = plan.n_tok, plan.n_used, down.n_rows
+    _moe_check(down, plan, act, t * u, "moe_down")
+    _f32_on(weights, (t, u), down.index, "moe_down: weights")
+    _f32_on(add, (t, n), down.index, "moe_down: add")
+    _f32_on(out, (t, n), down.index, "moe_down: out")
+    if out is None:
+        out = torch.empty((t, n), dtype=torch.float32, device=act.device)
+    if t:
+        need = lib().amv_moe_down_workspace_bytes(t, u, n)
+        ws = torch.empty(need, dtype=torch.uint8, device=act.device)
+        check(lib().amv_moe_down(down.type, down.ptr, down.stride, down.n_expert, n, down.k, act.data_ptr(), t, u, plan.ids.data_ptr(),
+                                 _ptr(plan.buffer), weights.data_ptr(), _ptr(add), out.data_ptr(), ws.data_ptr(), need, _stream()),
+              "amv_moe_down")
+    return out
+
+
 # ------------------------------------------------------------------------------------------------ glue ops
 def add(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     """ggml_add with b broadcast over rows (b rows divide a rows)."""

@@ -530,6 +530,64 @@ int amv_paged_attn_sparse(const amv_paged_kv* kv, const amv_paged_batch* batch, 
                           int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------
+ * The feed-forward part of a mixture of experts (no counterpart in the reference, whose MUL_MAT knows one matrix): a layer
+ * calls, from its residual to the next, amv_add_rms_norm_act, its router's MUL_MAT, amv_moe_route, amv_moe_plan,
+ * amv_moe_gate_up and amv_moe_down.
+ *
+ * Experts: n_expert matrices of rows x k, each in amv_repack's layout, expert_stride bytes apart (a multiple of 16, at least
+ * amv_weight_bytes); Q4_0, Q8_0, Q4_K or Q6_K; rows a multiple of 32. Pair t * n_used + j is token t with its j-th expert
+ * ids[t * n_used + j] (int32, device). An id outside [0, n_expert) is no expert: that pair has no product (a padded batch's tokens).
+ * An expert may be named twice by a token. At most 1024 experts, 64 a token, 2^22 pairs; pairs * max(rows, k) is less than 2^32.
+ * ---------------------------------------------------------------------------------------------------------- */
+/* sum = x + add, then amv_rms_norm_act of sum in the same pass: o = sum / sqrt(mean(sum^2) + eps) * w (w may be NULL: without the
+ * factor), act (may be NULL) = o in 8 bits, act_type 8 = Q8_0 (`rule`) or 15 = Q8_K. x, add, sum, o f32 [n_rows][n] (o may be NULL;
+ * sum may be x or add), w f32 [n]; n % 4 == 0, 16-byte aligned. A block of act with an element that is infinite or no number gets a
+ * scale that is none. */
+int amv_add_rms_norm_act(const float* x, const float* add, int64_t n_rows, int64_t n, float eps, const float* w, float* sum,
+                         float* o, void* act, int act_type, int rule, void* stream);
+/* The values that an activation buffer of amv_quantize_act's layout (act_type Q8_0 or Q8_K, m rows of k) stands for: out [m][k],
+ * out_type 0 = F32 or 1 = F16. */
+int amv_act_values(int act_type, const void* act, int64_t m, int64_t k, int out_type, void* out, void* stream);
+
+/* The experts of each token and their weights, from the router's logits f32 [n_tok][n_expert] (rows logits_stride floats
+ * apart). Scores: the row's softmax, or each logit's sigmoid. Choice: the score, with `bias` f32 [n_expert] (may be NULL) added.
+ * Of the n_group groups of n_expert / n_group experts, in order, those top_group whose sum of the group_best (1 or 2) largest
+ * choices is the largest are kept (n_group at most 64; top_group == n_group: all). ids int32 [n_tok][n_used]: the n_used largest
+ * choices of the groups kept, in falling order; weights f32 [n_tok][n_used]: their scores (without the bias), divided by their sum
+ * where renorm != 0 (0 where that is 0), times scale. All in 64 bits, equal choices (and groups) by the lower index. A softmax
+ * without bias is ordered by the logits. An expert whose logit is minus infinity or no number, or whose choice is, is not
+ * chosen; where fewer than n_used are left, the rest is id -1 and weight 0. A softmax row with a logit that is infinite or no
+ * number has weights that are none. */
+#define AMV_MOE_SOFTMAX 0
+#define AMV_MOE_SIGMOID 1
+int amv_moe_route(const float* logits, int64_t logits_stride, int64_t n_tok, int64_t n_expert, int64_t n_used, int score,
+                  const float* bias, int64_t n_group, int64_t top_group, int group_best, int renorm, float scale, int32_t* ids,
+                  float* weights, void* stream);
+/* The pairs in the order of their experts, for the products of both amv_moe_gate_up and amv_moe_down on the same ids.
+ * plan: amv_moe_plan_bytes bytes of device memory, 8-byte aligned; its contents are this library's own. */
+int64_t amv_moe_plan_bytes(int64_t n_tok, int64_t n_used, int64_t n_expert);
+int amv_moe_plan(const int32_t* ids, int64_t n_tok, int64_t n_used, int64_t n_expert, void* plan, void* stream);
+/* The experts' gate and up products with SWIGLU: h[p] = silu(W_gate a) * (W_up a) of pair p's expert and its token's row a of act
+ * (amv_quantize_act's layout of n_tok rows of k: Q8_0 for Q4_0 / Q8_0 weights, Q8_K for Q4_K / Q6_K; exact block integers as
+ * amv_mul_mat_q). eout f32 [pairs][rows] and act_out, h in 8 bits (act_type 8 = Q8_0 with `rule`, or 15 = Q8_K for rows % 256 == 0; the
+ * layout of `pairs` rows of `rows`): either may be NULL. Pairs without an expert get zeros; a block with an element that is
+ * infinite or no number gets a scale that is none. plan: amv_moe_plan's of the same ids, n_used and n_expert, or NULL: each pair is
+ * then a product by itself (a single token; at most 65535 pairs). workspace: amv_moe_gate_up_workspace_bytes bytes (0: may be
+ * NULL), 16-byte aligned. */
+int64_t amv_moe_gate_up_workspace_bytes(int64_t n_tok, int64_t n_used, int64_t rows, int act_type);
+int amv_moe_gate_up(int wtype, const void* w_gate, const void* w_up, int64_t expert_stride, int64_t n_expert, int64_t rows,
+                    int64_t k, const void* act, int64_t n_tok, int64_t n_used, const int32_t* ids, const void* plan, float* eout,
+                    void* act_out, int act_type, int rule, void* workspace, int64_t workspace_bytes, void* stream);
+/* The experts' down product, summed over a token's experts: dst[t] = add[t] + sum_j weights[t][j] (W h[t * n_used + j]), act the
+ * rows h (amv_moe_gate_up's act_out: Q8_0 for Q4_0 / Q8_0 weights, Q8_K for Q4_K / Q6_K), weights f32 [n_tok][n_used], add f32
+ * [n_tok][rows] or NULL (may be dst). The sum starts with add and goes in the order of j; pairs without an expert are left out,
+ * whatever their weight and row. workspace: amv_moe_down_workspace_bytes bytes, 16-byte aligned. */
+int64_t amv_moe_down_workspace_bytes(int64_t n_tok, int64_t n_used, int64_t rows);
+int amv_moe_down(int wtype, const void* w, int64_t expert_stride, int64_t n_expert, int64_t rows, int64_t k, const void* act,
+                 int64_t n_tok, int64_t n_used, const int32_t* ids, const void* plan, const float* weights, const float* add,
+                 float* dst, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------
  * Glue ops of the decoder graph (ameva_binary.comp, ameva_cpy.comp, ameva_set_rows.comp, ameva_get_rows(_q).comp).
  * ---------------------------------------------------------------------------------------------------------- */
 /* ADD (op 0) / MUL (op 1), f32: dst[r][i] = a[r][i] op b[r % b_rows][i] for n_rows rows of n elements. */
