@@ -55,7 +55,11 @@ struct MoeProduct {
     AmvActOut q;
     hipStream_t st;
 };
-int moe_few(const MoeProduct& p);
+int moe_few(const MoeProduct& p);   // amv_moe_few.hip
+int moe_many(const MoeProduct& p);  // amv_moe_many.hip (with a plan)
+
+// four int32 at an address of any whole int32 (a Q8_K buffer's sums begin where its scales end)
+typedef int moe_i4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // amv_act_store4 for a block with an element that is infinite or no number: integers cannot say so and the largest value passes over
 // it, so the block's scale is made none, and whatever reads it learns of it. Called as amv_act_store4.

@@ -465,6 +465,12 @@ __global__ __launch_bounds__(256) void k_moe_quantize(const float4* __restrict__
     moe_act_store4(amv_act_row(act, r, 4 * (int64_t)n4), (int)(i - r * n4), h);
 }
 
+static int moe_product(const MoeProduct& p) {
+    // tiles of many rows where an expert has more than a few of them
+    const bool many = p.plan && p.n_tok * p.n_used >= (int64_t)MOE_FEW * p.n_expert;
+    return many ? moe_many(p) : moe_few(p);
+}
+
 static int moe_check_product(const char* what, const MoeProduct& p) {
     const int rc = moe_check_pairs(what, p.n_tok, p.n_used, p.n_expert);
     if (rc) return rc;
@@ -513,7 +519,7 @@ extern "C" int amv_moe_gate_up(int wtype, const void* w_gate, const void* w_up, 
         p.out = (float*)workspace;
     }
     if (act_out && !late) p.q = amv_act_out(act_out, rows, act_type, rule, pairs);
-    const int r = moe_few(p);
+    const int r = moe_product(p);
     if (r || !late) return r;
     const int64_t total4 = pairs * rows / 4;
     k_moe_quantize<<<(unsigned)((total4 + 255) / 256), 256, 0, p.st>>>((const float4*)p.out, total4, (int)(rows / 4),
@@ -559,7 +565,7 @@ extern "C" int amv_moe_down(int wtype, const void* w, int64_t expert_stride, int
     AMV_REQUIRE(workspace && workspace_bytes >= need, "%s: a workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes,
                 (long long)need);
     p.w1 = nullptr;
-    const int r = moe_few(p);
+    const int r = moe_product(p);
     if (r) return r;
     const int n4 = (int)(rows / 4);
     for (int64_t t0 = 0; t0 < n_tok; t0 += 65535) {

@@ -112,10 +112,10 @@ struct Mf<AMV_T_Q4_K> {
         const uint4 z = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) a.q[i] = diag ? p[i] : z;
-        const int4* u = reinterpret_cast<const int4*>(act.s16 + (row * nsb + s) * 16);
+        const moe_i4* u = reinterpret_cast<const moe_i4*>(act.s16 + (row * nsb + s) * 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int4 v = u[i];
+            const moe_i4 v = u[i];
             a.u[2 * i] = v.x + v.y;
             a.u[2 * i + 1] = v.z + v.w;
         }

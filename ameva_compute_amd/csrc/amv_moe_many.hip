@@ -1,0 +1,605 @@
+// The experts' products with many rows each (prompts): tiles of 64 or 128 rows (pairs) of one expert on v_mfma_i32_32x32x32_i8, as
+// the dense products of amv_qgemm.hip, with the rows gathered through the plan's order and gate and up side by side.
+//
+// Operands: A = rows, B = weight rows; lane l has row l % 32 and 16 bytes l / 32 of a 32-block; result D of lane l: weight row
+// l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4. A workgroup's tile is 64 WM rows x 128 weight rows, a wave's 64 x 32; for gate and up, the
+// waves of weight rows take them in turn, so that 64 columns of both meet in the workgroup. Steps of 128 k go from memory to LDS without
+// registers, one step ahead; the 16-byte pieces of an LDS row are exchanged by an XOR with the row index on the memory side, so that
+// the fragments' reads hit all banks. Rows past the end of a buffer read as zero (the buffers' own range check).
+// The work beside the matrix core bounds these kernels: of a 32-block's 32 x 32 integers, each is converted and added with its
+// scale (Q4_0, Q8_0; the scale products are one outer product on the matrix core), or multiplied by its unit's scale (K-quants).
+#include "amv_moe.h"
+
+#include <algorithm>
+
+typedef int mm_v4i __attribute__((ext_vector_type(4)));
+typedef int mm_v16i __attribute__((ext_vector_type(16)));
+typedef _Float16 mm_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 mm_h2 __attribute__((ext_vector_type(2)));
+typedef float mm_f16v __attribute__((ext_vector_type(16)));
+typedef float mm_f32v __attribute__((ext_vector_type(32)));
+typedef __attribute__((address_space(3))) void mm_lds;
+#define MM_RSRC(p, bytes) __builtin_amdgcn_make_buffer_rsrc((void*)(p), 0, (uint32_t)(bytes), 0x00027000)
+// wait for every vector memory load (the other counters are left alone)
+#define MM_WAIT_LOADS() __builtin_amdgcn_s_waitcnt(0x0f70)
+
+// 16 bytes a lane from byte `off` of a buffer to LDS, the wave's 64 side by side from `to` on
+__device__ __forceinline__ void mm_to_lds(__amdgpu_buffer_rsrc_t from, uint4* to, uint32_t off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (mm_lds*)to, 16, off, 0, 0, 0);
+}
+
+#define MM_BN 128  // weight rows of a workgroup (gate and up: 64 of each)
+
+struct MmArgs {
+    const uint8_t *w0, *w1;
+    int64_t stride;
+    int rows, n_k, n_expert, act_div, n_tw, n_tiles;
+    const int8_t* aq;       // integers [act_rows][k]
+    const uint8_t* meta;    // Q8_0: {d, sum} [act_rows][k / 32]; Q8_K: d [act_rows][k / 256], sums [act_rows][k / 16]
+    int64_t act_rows;
+    const int2* tiles;
+    const int32_t* order;
+    float* out;
+    AmvActOut q;
+};
+
+// what a workgroup works on: its tile of rows and its weight rows; LDS: the rows' pairs
+struct MmTile {
+    int e, count, n0;  // n0: first weight row (gate and up: of each)
+};
+template <int BM, bool GU>
+__device__ __forceinline__ MmTile mm_tile(const MmArgs& p, int* s_pair) {
+    // the row tiles of a weight tile one after another on one XCD: its weights stay in that XCD's L2
+    const int T = amv_xcd_tile(blockIdx.x, p.n_tw * p.n_tiles);
+    MmTile m;
+    const int2 t = p.tiles[T / p.n_tw];
+    m.e = t.x & 0xFFFF;
+    m.count = t.x >> 16;
+    m.n0 = (T % p.n_tw) * (GU ? MM_BN / 2 : MM_BN);
+    if (m.count && (int)threadIdx.x < BM) s_pair[threadIdx.x] = p.order[t.y + min((int)threadIdx.x, m.count - 1)];
+    return m;
+}
+
+// The end of a tile. acc[i][r] of wave (wm, wn): row 64 wm + 32 i + 8 (r / 4) + 4 h + r % 4, weight row 32 wn + l % 32.
+// Down: stored as they lie, 32 lanes a row's 32 floats. Gate and up: 32 rows of each 64 at a time through LDS (s: 2 x 32 WM x 68 floats),
+// where four columns of a row come to a thread: h = silu(g) u, its store and its block's quantization (8 lanes).
+template <int WM, bool GU>
+__device__ __forceinline__ void mm_finish(const MmArgs& p, const MmTile& tile, const int* s_pair, float* s, const mm_f16v (&acc)[2], int wm,
+                                          int wn) {
+    const int lane = threadIdx.x & 63, c32 = lane & 31, h = lane >> 5;
+    if constexpr (!GU) {
+        const int n = tile.n0 + 32 * wn + c32;
+        if (n >= p.rows) return;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int m = 64 * wm + 32 * i + 8 * (r >> 2) + 4 * h + (r & 3);
+                if (m < tile.count) p.out[(int64_t)s_pair[m] * p.rows + n] = acc[i][r];
+            }
+    } else {
+        constexpr int LD = 68, NT = 256 * WM;
+        float* const half = s + (wn & 1) * (32 * WM * LD);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < 16; ++r) half[(32 * wm + 8 * (r >> 2) + 4 * h + (r & 3)) * LD + 32 * (wn >> 1) + c32] = acc[i][r];
+            __syncthreads();
+            for (int x = threadIdx.x; x < 32 * WM * 16; x += NT) {
+                const int lr = x >> 4, c = x & 15, m = 64 * (lr >> 5) + 32 * i + (lr & 31), col = tile.n0 + 4 * c;
+                if (m >= tile.count || col >= p.rows) continue;  // (eight lanes at a time: columns come in blocks of 32)
+                const float4 g = *reinterpret_cast<const float4*>(&s[lr * LD + 4 * c]);
+                const float4 u = *reinterpret_cast<const float4*>(&s[32 * WM * LD + lr * LD + 4 * c]);
+                const float v[4] = {g.x / (1.0f + expf(-g.x)) * u.x, g.y / (1.0f + expf(-g.y)) * u.y, g.z / (1.0f + expf(-g.z)) * u.z,
+                                    g.w / (1.0f + expf(-g.w)) * u.w};
+                const int64_t pr = s_pair[m];
+                if (p.out) *reinterpret_cast<float4*>(p.out + pr * p.rows + col) = make_float4(v[0], v[1], v[2], v[3]);
+                if (p.q.type) moe_act_store4(amv_act_row(p.q, pr, p.rows), col / 4, v);
+            }
+        }
+    }
+}
+
+// pairs without an expert: zeros from gate and up, nothing from down (their rows are left out of the sum)
+template <int WM, bool GU>
+__device__ __forceinline__ void mm_none(const MmArgs& p, const MmTile& tile, const int* s_pair, float* s) {
+    mm_f16v z[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[i][r] = 0.0f;
+    const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if constexpr (GU) mm_finish<WM, GU>(p, tile, s_pair, s, z, wv >> 2, wv & 3);
+}
+
+// byte-wise n - 8 of nibbles n in 0..15 (no carry crosses a byte: n + 0x78 <= 0x87)
+__device__ __forceinline__ uint32_t mm_m8(uint32_t v) { return (v + 0x78787878u) ^ 0x80808080u; }
+
+// ---------------------------------------------------------------------------------------------------------------- Q4_0, Q8_0
+template <int WT, int WM, bool GU>
+__global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) void k_moe_many(const MmArgs p) {
+    constexpr bool Q4 = WT == AMV_T_Q4_0;
+    constexpr int BM = 64 * WM, BN = MM_BN, NT = 256 * WM;
+    constexpr int WB = Q4 ? 16 : 32, WP = 4 * WB / 16;          // bytes of a weight block, 16-byte pieces of a step's row
+    constexpr int RA = BM * 8 / NT, RW = BN * WP / NT;          // rounds of the threads over a step's pieces
+    constexpr int RDW = BN * 4 / NT;                            // and over its weight scales (its rows': one)
+    constexpr int LA = BM * 8, LW = BN * WP, LEND = 2 * 32 * WM * 68 / 4;
+    // the buffers of even and odd steps, then (in the same place) what the end of a tile needs
+    __shared__ __align__(16) uint4 sm[(2 * (LA + LW) > LEND || !GU) ? 2 * (LA + LW) : LEND];
+    __shared__ __align__(16) float sDa[2][4 * BM], sDw[2][4 * BN];
+    __shared__ int s_pair[BM];
+    uint4 *const sAa = sm, *const sAb = sm + LA, *const sWa = sm + 2 * LA, *const sWb = sm + 2 * LA + LW;
+    const MmTile tile = mm_tile<BM, GU>(p, s_pair);
+    if (!tile.count) return;
+    __syncthreads();
+    if (tile.e >= p.n_expert) return mm_none<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm));
+    const int t = threadIdx.x, lane = t & 63, c32 = lane & 31, h = lane >> 5;
+    const int wv = __builtin_amdgcn_readfirstlane(t >> 6), wm = wv >> 2, wn = wv & 3;
+    const int nb = p.n_k, N = p.rows, nsteps = (nb + 3) / 4;
+    const uint32_t K = 32u * nb;
+
+    const uint8_t* const m0 = p.w0 + tile.e * p.stride;
+    const uint8_t* const m1 = GU ? p.w1 + tile.e * p.stride : m0;
+    const uint32_t wbytes = (uint32_t)N * nb * WB;
+    const __amdgpu_buffer_rsrc_t ra = MM_RSRC(p.aq, p.act_rows * K), rw0 = MM_RSRC(m0, wbytes), rw1 = MM_RSRC(m1, wbytes);
+    // weight row of a tile's row r (past the last one: none, which reads as zero)
+    const auto wrow = [&](int r) { return GU ? tile.n0 + 32 * (r >> 6) + (r & 31) : tile.n0 + r; };
+    uint32_t oa[RA], ow[RW];
+#pragma unroll
+    for (int i = 0; i < RA; ++i)
+        oa[i] = (uint32_t)(s_pair[(t >> 3) + NT / 8 * i] / p.act_div) * K + 16 * ((t & 7) ^ ((t >> 4) & 7));
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+        const int r = t / WP + NT / WP * i, n = wrow(r);
+        ow[i] = n < N ? (uint32_t)n * (nb * WB) + 16 * (Q4 ? (t & 3) ^ ((t >> 4) & 3) : (t & 7) ^ ((t >> 4) & 7)) : 0x80000000u;
+    }
+    const auto load = [&](uint4* sA, uint4* sW, int b) {
+#pragma unroll
+        for (int i = 0; i < RA; ++i)
+            mm_to_lds(ra, sA + NT * i + 64 * wv, oa[i] + 32u * b);
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            const bool up = GU && (((NT * i + 64 * wv) / WP) & 32);
+            if (up) mm_to_lds(rw1, sW + NT * i + 64 * wv, ow[i] + (uint32_t)WB * b);
+            else mm_to_lds(rw0, sW + NT * i + 64 * wv, ow[i] + (uint32_t)WB * b);
+        }
+    };
+    // scales, through registers: row x / 4 of the block x % 4 of the step; 0 past the last block
+    const float2* const pda = reinterpret_cast<const float2*>(p.meta) + (int64_t)(s_pair[t >> 2] / p.act_div) * nb;
+    float da;
+    uint32_t dw[RDW];
+    const uint16_t* pdw[RDW];
+#pragma unroll
+    for (int i = 0; i < RDW; ++i) {
+        const int r = (t + NT * i) >> 2, n = min(wrow(r), N - 1);
+        const uint16_t* d = reinterpret_cast<const uint16_t*>((GU && (r & 32) ? m1 : m0) + wbytes);
+        pdw[i] = Q4 ? d + (size_t)(n >> 1) * nb * 2 + (n & 1) : d + (size_t)n * nb;
+    }
+    const auto load_s = [&](int b) {
+        const int bb = min(b + (t & 3), nb - 1);
+        da = pda[bb].x;
+#pragma unroll
+        for (int i = 0; i < RDW; ++i) dw[i] = pdw[i][Q4 ? 2 * bb : bb];
+    };
+    const auto store_s = [&](int b, int buf) {
+        const bool in = b + (t & 3) < nb;
+        sDa[buf][(t & 3) * BM + (t >> 2)] = in ? da : 0.0f;
+#pragma unroll
+        for (int i = 0; i < RDW; ++i) {
+            const int x = t + NT * i;
+            sDw[buf][(x & 3) * BN + (x >> 2)] = in ? amv_h2f((uint16_t)dw[i]) : 0.0f;
+        }
+    };
+
+    mm_f16v acc[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
+    const int ar = 64 * wm + c32, wr = 32 * wn + c32;
+    const int ax = (c32 >> 1) & 7, wx = Q4 ? (c32 >> 2) & 3 : ax;  // the rows' XOR (64 wm, 32 i, 32 wn do not change them)
+    const auto compute = [&](const uint4* sA, const uint4* sW, int buf) {
+#pragma unroll
+        for (int bl = 0; bl < 4; ++bl) {
+            const mm_f32v zero = {};
+            const mm_f32v o = __builtin_amdgcn_mfma_f32_32x32x1f32(sDa[buf][bl * BM + 64 * wm + lane], sDw[buf][bl * BN + wr], zero, 0, 0, 0);
+            mm_v4i B;
+            if constexpr (Q4) {  // element e < 16: low nibble of byte e (lane half 0); 16 + e: its high nibble (half 1)
+                const uint4 x = sW[wr * 4 + (bl ^ wx)];
+                const int s = 4 * h;
+                B = mm_v4i{(int)mm_m8((x.x >> s) & 0x0F0F0F0Fu), (int)mm_m8((x.y >> s) & 0x0F0F0F0Fu),
+                           (int)mm_m8((x.z >> s) & 0x0F0F0F0Fu), (int)mm_m8((x.w >> s) & 0x0F0F0F0Fu)};
+            } else {
+                const uint4 x = sW[wr * 8 + ((2 * bl + h) ^ wx)];
+                B = mm_v4i{(int)x.x, (int)x.y, (int)x.z, (int)x.w};
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint4 a = sA[(ar + 32 * i) * 8 + ((2 * bl + h) ^ ax)];
+                const mm_v16i z = {};
+                const mm_v16i C = __builtin_amdgcn_mfma_i32_32x32x32_i8(mm_v4i{(int)a.x, (int)a.y, (int)a.z, (int)a.w}, B, z, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][r] = fmaf((float)C[r], o[16 * i + r], acc[i][r]);
+            }
+            // one block's results at a time (more do not fit the registers), added up here (the compiler would move the
+            // additions behind the next barrier and keep the results until then)
+            asm volatile("" : "+v"(acc[0]), "+v"(acc[1]));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    load(sAa, sWa, 0);
+    load_s(0);
+    store_s(0, 0);
+    MM_WAIT_LOADS();
+    __syncthreads();
+    for (int s = 0;; s += 2) {
+        const bool more = s + 1 < nsteps, again = s + 2 < nsteps;
+        if (more) {
+            load(sAb, sWb, 4 * (s + 1));
+            load_s(4 * (s + 1));
+        }
+        compute(sAa, sWa, 0);
+        if (!more) break;
+        store_s(4 * (s + 1), 1);
+        MM_WAIT_LOADS();
+        __syncthreads();
+        if (again) {
+            load(sAa, sWa, 4 * (s + 2));
+            load_s(4 * (s + 2));
+        }
+        compute(sAb, sWb, 1);
+        if (!again) break;
+        store_s(4 * (s + 2), 0);
+        MM_WAIT_LOADS();
+        __syncthreads();
+    }
+    mm_finish<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm), acc, wm, wn);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- Q4_K
+// Steps of half a super-block. Heads go to LDS with the first half, the activation sums per 16 (as f16, exact) and scales through
+// registers; the mins' sum is one f16 matrix product of the units' mins against the sums, exact in f32.
+__device__ __forceinline__ uint32_t mm_h2bits(int a, int b) {
+    return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(float)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(float)b) << 16);
+}
+
+template <int WM, bool GU>
+__global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) void k_moe_many_q4k(const MmArgs p) {
+    constexpr int BM = 64 * WM, BN = MM_BN, NT = 256 * WM;
+    constexpr int RA = BM * 8 / NT, RW = BN * 4 / NT;
+    constexpr int LA = BM * 8, LW = BN * 4, LEND = 2 * 32 * WM * 68 / 4;
+    __shared__ __align__(16) uint4 sm[(2 * (LA + LW) > LEND || !GU) ? 2 * (LA + LW) : LEND];
+    __shared__ __align__(16) uint4 sHd[BN];
+    __shared__ __align__(16) uint2 sBs[BM * 4];
+    __shared__ __align__(16) float sDa[BM];
+    __shared__ int s_pair[BM];
+    uint4 *const sAa = sm, *const sAb = sm + LA, *const sWa = sm + 2 * LA, *const sWb = sm + 2 * LA + LW;
+    const MmTile tile = mm_tile<BM, GU>(p, s_pair);
+    if (!tile.count) return;
+    __syncthreads();
+    if (tile.e >= p.n_expert) return mm_none<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm));
+    const int t = threadIdx.x, lane = t & 63, c32 = lane & 31, h = lane >> 5;
+    const int wv = __builtin_amdgcn_readfirstlane(t >> 6), wm = wv >> 2, wn = wv & 3;
+    const int nsb = p.n_k, N = p.rows;
+    const uint32_t K = 256u * nsb;
+
+    const uint8_t* const m0 = p.w0 + tile.e * p.stride;
+    const uint8_t* const m1 = GU ? p.w1 + tile.e * p.stride : m0;
+    const uint32_t wbytes = (uint32_t)N * nsb * 128;
+    const __amdgpu_buffer_rsrc_t ra = MM_RSRC(p.aq, p.act_rows * K);
+    const __amdgpu_buffer_rsrc_t rw0 = MM_RSRC(m0, wbytes), rw1 = MM_RSRC(m1, wbytes);
+    const __amdgpu_buffer_rsrc_t rh0 = MM_RSRC(m0 + wbytes, N * nsb * 16);
+    const auto wrow = [&](int r) { return GU ? tile.n0 + 32 * (r >> 6) + (r & 31) : tile.n0 + r; };
+    uint32_t oa[RA], ow[RW];
+#pragma unroll
+    for (int i = 0; i < RA; ++i)
+        oa[i] = (uint32_t)(s_pair[(t >> 3) + NT / 8 * i] / p.act_div) * K + 16 * ((t & 7) ^ ((t >> 4) & 7));
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+        const int n = wrow((t >> 2) + NT / 4 * i);
+        ow[i] = n < N ? (uint32_t)n * (nsb * 128) + 16 * ((t & 3) ^ ((t >> 4) & 3)) : 0x80000000u;
+    }
+    const auto load = [&](uint4* sA, uint4* sW, int j, int half) {
+#pragma unroll
+        for (int i = 0; i < RA; ++i)
+            mm_to_lds(ra, sA + NT * i + 64 * wv, oa[i] + 256u * j + 128 * half);
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            if (GU && (((NT * i + 64 * wv) / 4) & 32))
+                mm_to_lds(rw1, sW + NT * i + 64 * wv, ow[i] + 128u * j + 64 * half);
+            else
+                mm_to_lds(rw0, sW + NT * i + 64 * wv, ow[i] + 128u * j + 64 * half);
+        }
+    };
+    // a row's head is loaded by lane r % 64 of wave r / 64: of gate and up, 32 lanes each
+    const int hn = wrow(min(t, BN - 1));
+    const uint32_t oh = hn < N ? (uint32_t)hn * (nsb * 16) : 0x80000000u;
+    const uint8_t* const ph = (GU && (t & 32) ? m1 : m0) + wbytes;
+    const auto load_head = [&](int j) {
+        if (wv < BN / 64) {
+            if constexpr (GU) sHd[t] = hn < N ? *reinterpret_cast<const uint4*>(ph + oh + 16 * j) : make_uint4(0, 0, 0, 0);
+            else mm_to_lds(rh0, sHd + 64 * wv, oh + 16u * j);
+        }
+    };
+    // activation sums (thread: row t / 4, 4 of the 16) and scale of super-block j, through registers
+    const moe_i4* const ps = reinterpret_cast<const moe_i4*>(p.meta + p.act_rows * nsb * 4) + (int64_t)(s_pair[t >> 2] / p.act_div) * nsb * 4 + (t & 3);
+    const float* const pd = reinterpret_cast<const float*>(p.meta) + (int64_t)(s_pair[min(t, BM - 1)] / p.act_div) * nsb;
+    moe_i4 bs;
+    float da0;
+    const auto load_sb = [&](int j) {
+        bs = ps[4 * j];
+        da0 = pd[j];
+    };
+    const auto store_sb = [&]() {
+        sBs[t] = make_uint2(mm_h2bits(bs.x, bs.y), mm_h2bits(bs.z, bs.w));
+        if (t < BM) sDa[t] = da0;
+    };
+
+    mm_f16v acc[2];
+    mm_v16i I1[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
+    const int ar = 64 * wm + c32, wr = 32 * wn + c32;
+    const int ax = (c32 >> 1) & 7, wx = (c32 >> 2) & 3;
+    const auto half_step = [&](const uint4* sA, const uint4* sW, uint32_t scw, bool first) {
+#pragma unroll
+        for (int cp = 0; cp < 2; ++cp) {
+            const uint4 x = sW[wr * 4 + ((2 * cp + h) ^ wx)];
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const int u = 2 * cp + v, s = 4 * v;
+                const mm_v4i B = mm_v4i{(int)((x.x >> s) & 0x0F0F0F0Fu), (int)((x.y >> s) & 0x0F0F0F0Fu), (int)((x.z >> s) & 0x0F0F0F0Fu),
+                                        (int)((x.w >> s) & 0x0F0F0F0Fu)};
+                const int sc = (int)((scw >> (8 * u)) & 0xFFu);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint4 a = sA[(ar + 32 * i) * 8 + ((2 * u + h) ^ ax)];
+                    const mm_v16i z = {};
+                    const mm_v16i C = __builtin_amdgcn_mfma_i32_32x32x32_i8(mm_v4i{(int)a.x, (int)a.y, (int)a.z, (int)a.w}, B, z, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) I1[i][r] = first && u == 0 ? __mul24(C[r], sc) : I1[i][r] + __mul24(C[r], sc);
+                }
+                asm volatile("" : "+v"(I1[0]), "+v"(I1[1]));  // (as in k_moe_many)
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+
+    load_head(0);
+    load(sAa, sWa, 0, 0);
+    load_sb(0);
+    MM_WAIT_LOADS();
+    __syncthreads();
+    for (int j = 0; j < nsb; ++j) {
+        const int jn = min(j + 1, nsb - 1);
+        load(sAb, sWb, j, 1);
+        const uint4 hd = sHd[wr];
+        // scales and mins of units 0-3 and 4-7, one per byte
+        const uint32_t sc0 = hd.y & 0x3F3F3F3Fu, sc1 = (hd.w & 0x0F0F0F0Fu) | ((hd.y >> 2) & 0x30303030u);
+        const uint32_t mw = h ? ((hd.w >> 4) & 0x0F0F0F0Fu) | ((hd.z >> 2) & 0x30303030u) : hd.z & 0x3F3F3F3Fu;
+        half_step(sAa, sWa, sc0, true);
+        store_sb();
+        MM_WAIT_LOADS();
+        __syncthreads();
+        load(sAa, sWa, jn, 0);
+        load_head(jn);
+        load_sb(jn);
+        half_step(sAb, sWb, sc1, false);
+        // the mins, each on its unit's two 16-sum slots, against the sums
+        mm_h8 Bmn;
+        {
+            const uint32_t off = 0xE400E400u;  // -1024, -1024: 0x6400 | m is the f16 1024 + m
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t q = __builtin_amdgcn_perm(0x64646464u, mw, 0x04000400u + 0x00010001u * e);
+                const mm_h2 v = __builtin_bit_cast(mm_h2, q) + __builtin_bit_cast(mm_h2, off);
+                Bmn[2 * e] = v.x;
+                Bmn[2 * e + 1] = v.y;
+            }
+        }
+        const float d = amv_h2f(hd.x), dm = amv_h2f(hd.x >> 16);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int tl = 64 * wm + 32 * i;
+            const mm_h8 Abs = *reinterpret_cast<const mm_h8*>(&sBs[(tl + c32) * 4 + 2 * h]);
+            const mm_f16v zf = {};
+            const mm_f16v I2 = __builtin_amdgcn_mfma_f32_32x32x16_f16(Abs, Bmn, zf, 0, 0, 0);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 v = *reinterpret_cast<const float4*>(&sDa[tl + 4 * h + 8 * q]);
+                const float da[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    acc[i][4 * q + r] = fmaf(fmaf(d, (float)I1[i][4 * q + r], -(dm * I2[4 * q + r])), da[r], acc[i][4 * q + r]);
+            }
+        }
+        MM_WAIT_LOADS();
+        __syncthreads();
+    }
+    mm_finish<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm), acc, wm, wn);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- Q6_K
+// Steps of half a super-block: elements 128 n + {l, 32 + l, 64 + l, 96 + l} (l < 32) from the low nibbles of ql[l], ql[32 + l], then the
+// high ones, with bits 0-1, 2-3, 4-5, 6-7 of qh[l]; sub-blocks of 16 have scales of their own, so the matrix core takes 16 k at a time
+// (v_mfma_i32_32x32x16_i8, lane half h the bytes 8 h .. 8 h + 7 of a sub-block).
+template <int WM, bool GU>
+__global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 1 ? 3 : 4))) void k_moe_many_q6k(const MmArgs p) {
+    constexpr int BM = 64 * WM, BN = MM_BN, NT = 256 * WM;
+    constexpr int RA = BM * 8 / NT, RW = BN * 4 / NT;
+    constexpr int LA = BM * 8, LW = BN * 4, LH = BN * 2, LEND = 2 * 32 * WM * 68 / 4;
+    __shared__ __align__(16) uint4 sm[(2 * (LA + LW + LH) > LEND || !GU) ? 2 * (LA + LW + LH) : LEND];
+    __shared__ __align__(16) uint4 sSc[2][BN];
+    __shared__ __align__(16) float sD[2][BN], sDa[2][BM];
+    __shared__ int s_pair[BM];
+    const MmTile tile = mm_tile<BM, GU>(p, s_pair);
+    if (!tile.count) return;
+    __syncthreads();
+    if (tile.e >= p.n_expert) return mm_none<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm));
+    uint4 *const sAa = sm, *const sAb = sm + LA, *const sWa = sm + 2 * LA, *const sWb = sWa + LW, *const sHa = sWb + LW, *const sHb = sHa + LH;
+    const int t = threadIdx.x, lane = t & 63, c32 = lane & 31, h = lane >> 5;
+    const int wv = __builtin_amdgcn_readfirstlane(t >> 6), wm = wv >> 2, wn = wv & 3;
+    const int nsb = p.n_k, N = p.rows;
+    const uint32_t K = 256u * nsb;
+
+    const uint8_t* const m0 = p.w0 + tile.e * p.stride;
+    const uint8_t* const m1 = GU ? p.w1 + tile.e * p.stride : m0;
+    const uint32_t nblk = (uint32_t)N * nsb;
+    const __amdgpu_buffer_rsrc_t ra = MM_RSRC(p.aq, p.act_rows * K);
+    const __amdgpu_buffer_rsrc_t rw0 = MM_RSRC(m0, nblk * 128), rw1 = MM_RSRC(m1, nblk * 128);
+    const __amdgpu_buffer_rsrc_t rq0 = MM_RSRC(m0 + nblk * 128, nblk * 64), rq1 = MM_RSRC(m1 + nblk * 128, nblk * 64);
+    const auto wrow = [&](int r) { return GU ? tile.n0 + 32 * (r >> 6) + (r & 31) : tile.n0 + r; };
+    uint32_t oa[RA], ow[RW];
+#pragma unroll
+    for (int i = 0; i < RA; ++i)
+        oa[i] = (uint32_t)(s_pair[(t >> 3) + NT / 8 * i] / p.act_div) * K + 16 * ((t & 7) ^ ((t >> 4) & 7));
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+        const int n = wrow((t >> 2) + NT / 4 * i);
+        ow[i] = n < N ? (uint32_t)n * (nsb * 128) + 16 * ((t & 3) ^ ((t >> 4) & 3)) : 0x80000000u;
+    }
+    // qh: two pieces a row, the first 2 BN threads
+    const int qn = wrow(min(t >> 1, BN - 1));
+    const uint32_t oq = qn < N ? (uint32_t)qn * (nsb * 64) + 16 * ((t & 1) ^ ((t >> 3) & 1)) : 0x80000000u;
+    const auto load = [&](uint4* sA, uint4* sW, uint4* sH, int j, int half) {
+#pragma unroll
+        for (int i = 0; i < RA; ++i)
+            mm_to_lds(ra, sA + NT * i + 64 * wv, oa[i] + 256u * j + 128 * half);
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            if (GU && (((NT * i + 64 * wv) / 4) & 32))
+                mm_to_lds(rw1, sW + NT * i + 64 * wv, ow[i] + 128u * j + 64 * half);
+            else
+                mm_to_lds(rw0, sW + NT * i + 64 * wv, ow[i] + 128u * j + 64 * half);
+        }
+        if (wv < BN * 2 / 64) {
+            if (GU && (wv & 1)) mm_to_lds(rq1, sH + 64 * wv, oq + 64u * j + 32 * half);
+            else mm_to_lds(rq0, sH + 64 * wv, oq + 64u * j + 32 * half);
+        }
+    };
+    // scales of super-block j: 16 bytes and d of the first BN threads' weight rows, d of the first BM threads' rows, through registers
+    const int sr = min(t, BN - 1), sn = min(wrow(sr), N - 1);
+    const uint8_t* const ms = GU && (sr & 32) ? m1 : m0;
+    const uint4* const psc = reinterpret_cast<const uint4*>(ms + (size_t)nblk * 192) + (size_t)sn * nsb;
+    const uint16_t* const pd = reinterpret_cast<const uint16_t*>(ms + (size_t)nblk * 208) + (size_t)sn * nsb;
+    const float* const pda = reinterpret_cast<const float*>(p.meta) + (int64_t)(s_pair[min(t, BM - 1)] / p.act_div) * nsb;
+    uint4 scr;
+    uint32_t dr;
+    float dar;
+    const auto load_sb = [&](int j) {
+        scr = psc[j];
+        dr = pd[j];
+        dar = pda[j];
+    };
+    const auto store_sb = [&](int buf) {
+        if (t < BN) {
+            sSc[buf][t] = scr;
+            sD[buf][t] = amv_h2f(dr);
+        }
+        if (t < BM) sDa[buf][t] = dar;
+    };
+
+    mm_f16v acc[2];
+    mm_v16i I[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            acc[i][r] = 0.0f;
+            I[i][r] = 0;
+        }
+    const int ar = 64 * wm + c32, wr = 32 * wn + c32;
+    const int ax = (c32 >> 1) & 7, wx = (c32 >> 2) & 3, hx = (c32 >> 2) & 1;
+    // sw: the half's eight scales (bytes 2 e + pp: sub-block of elements 32 e + 16 pp ..)
+    const auto half_step = [&](const uint4* sA, const uint4* sW, const uint4* sH, uint32_t s0, uint32_t s1) {
+#pragma unroll
+        for (int pp = 0; pp < 2; ++pp) {
+            const uint2 l0 = reinterpret_cast<const uint2*>(sW + wr * 4 + (pp ^ wx))[h];
+            const uint2 l1 = reinterpret_cast<const uint2*>(sW + wr * 4 + ((2 + pp) ^ wx))[h];
+            const uint2 qh = reinterpret_cast<const uint2*>(sH + wr * 2 + (pp ^ hx))[h];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint2 l = e & 1 ? l1 : l0;
+                const int s = e < 2 ? 0 : 4;
+                const auto q6 = [&](uint32_t lo, uint32_t hi) {
+                    return ((((lo >> s) & 0x0F0F0F0Fu) | (((hi >> (2 * e)) & 0x03030303u) << 4)) + 0x60606060u) ^ 0x80808080u;
+                };
+                const uint2 b = make_uint2(q6(l.x, qh.x), q6(l.y, qh.y));
+                const int sub = 2 * e + pp, sc = (int)(int8_t)((sub < 4 ? s0 : s1) >> (8 * (sub & 3)));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint2 a = reinterpret_cast<const uint2*>(sA + (ar + 32 * i) * 8 + ((2 * e + pp) ^ ax))[h];
+                    const mm_v16i z = {};
+                    const mm_v16i C = __builtin_amdgcn_mfma_i32_32x32x16_i8(__builtin_bit_cast(long, a), __builtin_bit_cast(long, b), z, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) I[i][r] += __mul24(C[r], sc);
+                }
+                asm volatile("" : "+v"(I[0]), "+v"(I[1]));  // (as in k_moe_many)
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+
+    load(sAa, sWa, sHa, 0, 0);
+    load_sb(0);
+    store_sb(0);
+    MM_WAIT_LOADS();
+    __syncthreads();
+    for (int j = 0; j < nsb; ++j) {
+        const int jn = min(j + 1, nsb - 1), buf = j & 1;
+        load(sAb, sWb, sHb, j, 1);
+        load_sb(jn);
+        const uint4 sc = sSc[buf][wr];
+        half_step(sAa, sWa, sHa, sc.x, sc.y);
+        store_sb(buf ^ 1);
+        MM_WAIT_LOADS();
+        __syncthreads();
+        load(sAa, sWa, sHa, jn, 0);
+        half_step(sAb, sWb, sHb, sc.z, sc.w);
+        const float d = sD[buf][wr];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 v = *reinterpret_cast<const float4*>(&sDa[buf][64 * wm + 32 * i + 4 * h + 8 * q]);
+                const float da[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    acc[i][4 * q + r] = fmaf(d * da[r], (float)I[i][4 * q + r], acc[i][4 * q + r]);
+                    I[i][4 * q + r] = 0;
+                }
+            }
+        MM_WAIT_LOADS();
+        __syncthreads();
+    }
+    mm_finish<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm), acc, wm, wn);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+int moe_many(const MoeProduct& p) {
+    const int64_t pairs = p.n_tok * p.n_used;
+    const MoePlanView v = moe_plan_view(p.plan, pairs, p.n_expert);
+    const bool kq = p.type == AMV_T_Q4_K || p.type == AMV_T_Q6_K, gu = p.w1 != nullptr;
+    const int8_t* aq = (const int8_t*)p.act;
+    MmArgs a{(const uint8_t*)p.w0, (const uint8_t*)p.w1, p.stride, (int)p.rows, (int)(p.k / (kq ? 256 : 32)), p.n_expert, gu ? p.n_used : 1,
+             0, v.n_many, aq, (const uint8_t*)aq + p.act_rows * p.k, p.act_rows, v.many, v.order, p.out, p.q};
+    a.n_tw = (int)((p.rows + (gu ? MM_BN / 2 : MM_BN) - 1) / (gu ? MM_BN / 2 : MM_BN));
+    AMV_REQUIRE((int64_t)a.n_tw * a.n_tiles < (int64_t)1 << 31, "moe: too many tiles");
+    const unsigned grid = (unsigned)((int64_t)a.n_tw * a.n_tiles);
+    constexpr int WM = MOE_MANY / 64;
+#define GO(KERNEL) hipLaunchKernelGGL((gu ? KERNEL(true) : KERNEL(false)), dim3(grid), dim3(256 * WM), 0, p.st, a)
+#define K40(G) k_moe_many<AMV_T_Q4_0, WM, G>
+#define K80(G) k_moe_many<AMV_T_Q8_0, WM, G>
+#define K4K(G) k_moe_many_q4k<WM, G>
+#define K6K(G) k_moe_many_q6k<WM, G>
+    if (p.type == AMV_T_Q4_0) GO(K40);
+    else if (p.type == AMV_T_Q8_0) GO(K80);
+    else if (p.type == AMV_T_Q4_K) GO(K4K);
+    else GO(K6K);
+#undef GO
+    return amv_check_launch("amv_moe products");
+}
