@@ -9,6 +9,7 @@
 #include "amv_moe.h"
 
 #include <algorithm>
+#include <type_traits>
 
 typedef int mf_v4i __attribute__((ext_vector_type(4)));
 typedef short mf_s2 __attribute__((ext_vector_type(2)));
@@ -33,6 +34,12 @@ __device__ __forceinline__ void mf_quarters(uint32_t x, uint32_t (&o)[4]) {
     o[3] = b[1];
 }
 
+#define MF_RSRC(p, bytes) __builtin_amdgcn_make_buffer_rsrc((void*)(p), 0, (uint32_t)(bytes), 0x00027000)
+__device__ __forceinline__ uint4 mf_load(__amdgpu_buffer_rsrc_t r, uint32_t off) {  // 0 past the buffer's end
+    const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 // the activation rows of a call: integers, and scales (Q8_0: {d, sum} per block; Q8_K: d per super-block) and sums per 16 (Q8_K)
 struct MfAct {
     const int8_t* q;
@@ -41,40 +48,33 @@ struct MfAct {
     const int32_t* s16;
 };
 
-// Per weight type: a step (STEP k) is four blocks of 32 or a super-block; U steps are loaded at once (struct W, one matrix). The
-// activations come from LDS: rows of integers LD bytes apart, their scales at s (float [row][STEPS * 4 or 1]), unit sums at u.
-template <int WT>
+// Per weight type: a step (STEP k) is four blocks of 32 or a super-block, U steps are loaded at once (struct W) of row n of the matrix at
+// m (buffer r). The activations come from LDS: a row's integers of the step, the lane's own quarter of them, at p, its scales at s, its
+// sums at u.
+template <int WT, int U>
 struct Mf32 {  // Q4_0, Q8_0
     static constexpr bool Q4 = WT == AMV_T_Q4_0;
-    static constexpr int STEP = 128, U = Q4 ? 4 : 2, PER = 4;  // PER: scales of a row and step
+    static constexpr int STEP = 128, PER = 4;      // PER: scales of a row and step
+    static constexpr int SUMS = 0, AT = 32;  // SUMS: words of sums of a row and step; AT: bytes between the quarters' integers
+    static_assert(!Q4 || U == 4, "a quarter of the wave holds a step's scales");
     struct W {
         uint4 q[U][Q4 ? 1 : 2];
-        uint2 d[Q4 ? 1 : U];  // four f16; Q4_0: quarter j of the wave holds step j's
+        std::conditional_t<Q4, uint4, uint2> d[Q4 ? 1 : U];  // four f16; Q4_0: four pairs, quarter j of the wave holds step j's
     };
-    // steps s .. of weight row n of a matrix of `rows`; blocks past the end: another block's integers, scales 0
-    static __device__ __forceinline__ void load(W& w, const uint8_t* m, int rows, int nb, int n, int q, int s) {
-        const uint8_t* const d = m + (size_t)rows * nb * (Q4 ? 16 : 32);
+    // blocks past the end: other integers (their activations are zeros) and scales 0
+    static __device__ __forceinline__ void load(W& w, __amdgpu_buffer_rsrc_t r, const uint8_t* m, int rows, int nb, int n, int q, int s) {
+        const uint32_t at = ((uint32_t)n * nb + 4 * s + q) * (Q4 ? 16 : 32);
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const uint4* p = reinterpret_cast<const uint4*>(m + ((size_t)n * nb + min(4 * (s + j) + q, nb - 1)) * (Q4 ? 16 : 32));
-            w.q[j][0] = p[0];
-            if constexpr (!Q4) w.q[j][1] = p[1];
+            w.q[j][0] = mf_load(r, at + j * (Q4 ? 64 : 128));
+            if constexpr (!Q4) w.q[j][1] = mf_load(r, at + j * 128 + 16);
         }
         if constexpr (Q4) {
-            // the scales of rows 2 p and 2 p + 1 side by side: lane quarter q takes blocks 4 (s + q) .. + 3, its own row's halves
-            const uint32_t* p = reinterpret_cast<const uint32_t*>(d) + (size_t)(n >> 1) * nb;
-            uint32_t x[4];
-            if (4 * (s + 4) <= nb) {
-                const mf_u4 v = *reinterpret_cast<const mf_u4*>(p + 4 * (s + q));
-                x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = 4 * (s + q) + i < nb ? p[min(4 * (s + q) + i, nb - 1)] : 0u;
-            }
-            const uint32_t sel = n & 1 ? 0x07060302u : 0x05040100u;  // the upper or the lower halves of two words
-            w.d[0] = make_uint2(__builtin_amdgcn_perm(x[1], x[0], sel), __builtin_amdgcn_perm(x[3], x[2], sel));
+            // the scales of rows 2 p and 2 p + 1 side by side: lane quarter q takes blocks 4 (s + q) .. + 3 (of both rows: what is done
+            // to them here would wait for them)
+            w.d[0] = mf_load(r, (uint32_t)rows * nb * 16 + ((uint32_t)(n >> 1) * nb + 4 * (s + q)) * 4);
         } else {
-            const uint16_t* p = reinterpret_cast<const uint16_t*>(d) + (size_t)n * nb;
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(m + (size_t)rows * nb * 32) + (size_t)n * nb;
 #pragma unroll
             for (int j = 0; j < U; ++j) {
                 if (4 * (s + j + 1) <= nb) {
@@ -89,7 +89,7 @@ struct Mf32 {  // Q4_0, Q8_0
             }
         }
     }
-    // what the steps need of the weights alone, once for all tokens: operands and scales of step j
+    // what a step needs of the weights alone, once for all tokens
     struct B {
         uint4 q[2];
         float d[4];
@@ -97,10 +97,15 @@ struct Mf32 {  // Q4_0, Q8_0
     struct Scales {
         uint32_t lo[4], hi[4];
     };
-    static __device__ __forceinline__ void scales(const W& w, Scales& c) {
+    static __device__ __forceinline__ void scales(const W& w, Scales& c, int nb, int n, int q, int s) {
         if constexpr (Q4) {
-            mf_quarters(w.d[0].x, c.lo);
-            mf_quarters(w.d[0].y, c.hi);
+            uint32_t x[4] = {w.d[0].x, w.d[0].y, w.d[0].z, w.d[0].w};
+            if (4 * (s + 4) > nb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = 4 * (s + q) + i < nb ? x[i] : 0u;
+            const uint32_t sel = n & 1 ? 0x07060302u : 0x05040100u;  // the upper or the lower halves of two words
+            mf_quarters(__builtin_amdgcn_perm(x[1], x[0], sel), c.lo);
+            mf_quarters(__builtin_amdgcn_perm(x[3], x[2], sel), c.hi);
         } else {
 #pragma unroll
             for (int j = 0; j < U; ++j) {
@@ -122,176 +127,169 @@ struct Mf32 {  // Q4_0, Q8_0
         o.d[2] = amv_h2f(c.hi[j]);
         o.d[3] = amv_h2f(c.hi[j] >> 16);
     }
-    struct A {
-        uint4 q[2];
-        float4 d;
-    };
-    // a: the lane's integers of the step (or zeros, `on` 0), s: its token's scales of the step
-    static __device__ __forceinline__ void read(A& a, const uint8_t* p, int on, int q, const float* s, const int16_t*) {
-        const uint4* v = reinterpret_cast<const uint4*>(p + on * 32 * q);
-        a.q[0] = v[0];
-        a.q[1] = v[1];
-        a.d = *reinterpret_cast<const float4*>(s);
-    }
-    static __device__ __forceinline__ float add(const B& w, const A& a, float acc) {
+    static __device__ __forceinline__ float add(const B& w, const uint8_t* p, const float* s, const int*, float acc) {
+        const uint4* v = reinterpret_cast<const uint4*>(p);
+        const float4 d = *reinterpret_cast<const float4*>(s);
         mf_v4i c = {0, 0, 0, 0};
-        c = mf_mma(a.q[0], w.q[0], c);
-        c = mf_mma(a.q[1], w.q[1], c);
-        acc = fmaf((float)c[0], w.d[0] * a.d.x, acc);
-        acc = fmaf((float)c[1], w.d[1] * a.d.y, acc);
-        acc = fmaf((float)c[2], w.d[2] * a.d.z, acc);
-        return fmaf((float)c[3], w.d[3] * a.d.w, acc);
+        c = mf_mma(v[0], w.q[0], c);
+        c = mf_mma(v[1], w.q[1], c);
+        acc = fmaf((float)c[0], w.d[0] * d.x, acc);
+        acc = fmaf((float)c[1], w.d[1] * d.y, acc);
+        acc = fmaf((float)c[2], w.d[2] * d.z, acc);
+        return fmaf((float)c[3], w.d[3] * d.w, acc);
     }
 };
-template <int WT>
-struct Mf : Mf32<WT> {};
+template <int WT, int U>
+struct Mf : Mf32<WT, U> {};
 
 // Q4_K: quarter q has the 32 bytes of units 2 q (low nibbles) and 2 q + 1 (high) of a super-block
-template <>
-struct Mf<AMV_T_Q4_K> {
-    static constexpr int STEP = 256, U = 2, PER = 1;
+template <int U>
+struct Mf<AMV_T_Q4_K, U> {
+    static constexpr int STEP = 256, PER = 1, SUMS = 4, AT = 64;
     struct W {
         uint4 q[U][2], head[U];
     };
-    static __device__ __forceinline__ void load(W& w, const uint8_t* m, int rows, int nsb, int n, int q, int s) {
+    static __device__ __forceinline__ void load(W& w, __amdgpu_buffer_rsrc_t r, const uint8_t*, int rows, int nsb, int n, int q, int s) {
+        const uint32_t sb = (uint32_t)n * nsb + s, h = (uint32_t)rows * nsb * 128;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const size_t sb = (size_t)n * nsb + min(s + j, nsb - 1);
-            const uint4* p = reinterpret_cast<const uint4*>(m) + sb * 8 + 2 * q;
-            w.q[j][0] = p[0];
-            w.q[j][1] = p[1];
-            w.head[j] = reinterpret_cast<const uint4*>(m)[(size_t)rows * nsb * 8 + sb];
+            w.q[j][0] = mf_load(r, (sb + j) * 128 + 32 * q);
+            w.q[j][1] = mf_load(r, (sb + j) * 128 + 32 * q + 16);
+            w.head[j] = mf_load(r, h + (sb + j) * 16);
         }
     }
     struct B {
-        uint4 lo[2], hi[2];
-        int sc[8];
+        uint4 q[2];
+        uint32_t sc[2];
         mf_s2 mn[4];
         float d, dm;
     };
     struct Scales {};
-    static __device__ __forceinline__ void scales(const W&, Scales&) {}
+    static __device__ __forceinline__ void scales(const W&, Scales&, int, int, int, int) {}
     static __device__ __forceinline__ void operands(const W& w, const Scales&, int j, B& o) {
         const uint4 h = w.head[j];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            o.lo[i] = mf_each(w.q[j][i], [](uint32_t v) { return v & 0x0F0F0F0Fu; });
-            o.hi[i] = mf_each(w.q[j][i], [](uint32_t v) { return (v >> 4) & 0x0F0F0F0Fu; });
-        }
+        o.q[0] = w.q[j][0];
+        o.q[1] = w.q[j][1];
         // scales and mins of units 0-3 and 4-7, one per byte
-        const uint32_t sc[2] = {h.y & 0x3F3F3F3Fu, (h.w & 0x0F0F0F0Fu) | ((h.y >> 2) & 0x30303030u)};
+        o.sc[0] = h.y & 0x3F3F3F3Fu;
+        o.sc[1] = (h.w & 0x0F0F0F0Fu) | ((h.y >> 2) & 0x30303030u);
         const uint32_t mn[2] = {h.z & 0x3F3F3F3Fu, ((h.w >> 4) & 0x0F0F0F0Fu) | ((h.z >> 2) & 0x30303030u)};
-#pragma unroll
-        for (int u = 0; u < 8; ++u) o.sc[u] = (int)((sc[u >> 2] >> (8 * (u & 3))) & 0xFF);
 #pragma unroll
         for (int u = 0; u < 4; ++u)  // bytes 2 u, 2 u + 1 as two 16-bit numbers
             o.mn[u] = __builtin_bit_cast(mf_s2, __builtin_amdgcn_perm(0u, mn[u >> 1], u & 1 ? 0x0C030C02u : 0x0C010C00u));
         o.d = amv_h2f(h.x);
         o.dm = amv_h2f(h.x >> 16);
     }
-    struct A {
-        uint4 q[4], u;
-        float d;
-    };
-    static __device__ __forceinline__ void read(A& a, const uint8_t* p, int on, int q, const float* s, const int16_t* u) {
-        const uint4* v = reinterpret_cast<const uint4*>(p + on * 64 * q);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a.q[i] = v[on * i];
-        a.u = *reinterpret_cast<const uint4*>(u);
-        a.d = *s;
-    }
-    static __device__ __forceinline__ float add(const B& w, const A& a, float acc) {
+    static __device__ __forceinline__ float add(const B& w, const uint8_t* p, const float* s, const int* u, float acc) {
+        const uint4* v = reinterpret_cast<const uint4*>(p);
         mf_v4i lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            lo = mf_mma(a.q[i], w.lo[i], lo);
-            hi = mf_mma(a.q[2 + i], w.hi[i], hi);
+            lo = mf_mma(v[i], mf_each(w.q[i], [](uint32_t x) { return x & 0x0F0F0F0Fu; }), lo);
+            hi = mf_mma(v[2 + i], mf_each(w.q[i], [](uint32_t x) { return (x >> 4) & 0x0F0F0F0Fu; }), hi);
         }
-        const uint32_t us[4] = {a.u.x, a.u.y, a.u.z, a.u.w};
+        const uint4 us = *reinterpret_cast<const uint4*>(u);
+        const uint32_t uw[4] = {us.x, us.y, us.z, us.w};
         int I1 = 0, I2 = 0;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            I1 += __mul24(lo[u], w.sc[2 * u]);
-            I1 += __mul24(hi[u], w.sc[2 * u + 1]);
-            I2 = __builtin_amdgcn_sdot2(__builtin_bit_cast(mf_s2, us[u]), w.mn[u], I2, false);
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t c = w.sc[i >> 1] >> (16 * (i & 1));
+            I1 += __mul24(lo[i], (int)(c & 0xFF));
+            I1 += __mul24(hi[i], (int)((c >> 8) & 0xFF));
+            I2 = __builtin_amdgcn_sdot2(__builtin_bit_cast(mf_s2, uw[i]), w.mn[i], I2, false);
         }
-        return fmaf(fmaf(w.d, (float)I1, -(w.dm * (float)I2)), a.d, acc);
+        return fmaf(fmaf(w.d, (float)I1, -(w.dm * (float)I2)), *s, acc);
     }
 };
 
 // Q6_K: quarter q = 2 h + p has elements 128 h + 16 p + {0, 32, 64, 96} .. + 15, four sub-blocks of 16
-template <>
-struct Mf<AMV_T_Q6_K> {
-    static constexpr int STEP = 256, U = 1, PER = 1;
+template <int U>
+struct Mf<AMV_T_Q6_K, U> {
+    static constexpr int STEP = 256, PER = 1, SUMS = 0, AT = 0;
     struct W {
         uint4 l0[U], l1[U], h[U], sc[U];
         uint32_t d[U];
     };
-    static __device__ __forceinline__ void load(W& w, const uint8_t* m, int rows, int nsb, int n, int q, int s) {
-        const size_t all = (size_t)rows * nsb;
+    static __device__ __forceinline__ void load(W& w, __amdgpu_buffer_rsrc_t r, const uint8_t* m, int rows, int nsb, int n, int q, int s) {
+        const uint32_t all = (uint32_t)rows * nsb, sb = (uint32_t)n * nsb + s;
+        const uint16_t* d = reinterpret_cast<const uint16_t*>(m + (size_t)all * 208);
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const size_t sb = (size_t)n * nsb + min(s + j, nsb - 1);
-            const uint4* l = reinterpret_cast<const uint4*>(m) + sb * 8 + 4 * (q >> 1) + (q & 1);
-            w.l0[j] = l[0];
-            w.l1[j] = l[2];
-            w.h[j] = reinterpret_cast<const uint4*>(m)[all * 8 + sb * 4 + q];
-            w.sc[j] = reinterpret_cast<const uint4*>(m)[all * 12 + sb];
-            w.d[j] = reinterpret_cast<const uint16_t*>(m + all * 208)[sb];
+            w.l0[j] = mf_load(r, (sb + j) * 128 + 64 * (q >> 1) + 16 * (q & 1));
+            w.l1[j] = mf_load(r, (sb + j) * 128 + 64 * (q >> 1) + 16 * (q & 1) + 32);
+            w.h[j] = mf_load(r, all * 128 + (sb + j) * 64 + 16 * q);
+            w.sc[j] = mf_load(r, all * 192 + (sb + j) * 16);
+            w.d[j] = d[min(sb + j, all - 1)];
         }
     }
     struct B {
-        uint4 q[4], sc;
+        uint4 l0, l1, h, sc;
         float d;
     };
     struct Scales {};
-    static __device__ __forceinline__ void scales(const W&, Scales&) {}
+    static __device__ __forceinline__ void scales(const W&, Scales&, int, int, int, int) {}
     static __device__ __forceinline__ void operands(const W& w, const Scales&, int j, B& o) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {  // elements 32 e: low (e < 2) or high nibbles of l0 or l1, bits 2 e of h; minus 32
-            const uint4 l = e & 1 ? w.l1[j] : w.l0[j];
-            const auto one = [&](uint32_t x, uint32_t y) {
-                return ((((x >> (e < 2 ? 0 : 4)) & 0x0F0F0F0Fu) | (((y >> (2 * e)) & 0x03030303u) << 4)) + 0x60606060u) ^ 0x80808080u;
-            };
-            o.q[e] = make_uint4(one(l.x, w.h[j].x), one(l.y, w.h[j].y), one(l.z, w.h[j].z), one(l.w, w.h[j].w));
-        }
+        o.l0 = w.l0[j];
+        o.l1 = w.l1[j];
+        o.h = w.h[j];
         o.sc = w.sc[j];
         o.d = amv_h2f(w.d[j]);
     }
-    struct A {
-        uint4 q[4];
-        float d;
-    };
-    static __device__ __forceinline__ void read(A& a, const uint8_t* p, int on, int q, const float* s, const int16_t*) {
-        const uint4* v = reinterpret_cast<const uint4*>(p + on * (128 * (q >> 1) + 16 * (q & 1)));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a.q[i] = v[on * 2 * i];
-        a.d = *s;
-    }
-    static __device__ __forceinline__ float add(const B& w, const A& a, float acc) {
+    static __device__ __forceinline__ float add(const B& w, const uint8_t* p, const float* s, const int*, float acc) {
+        const uint4* v = reinterpret_cast<const uint4*>(p);
         const uint32_t S[4] = {w.sc.x, w.sc.y, w.sc.z, w.sc.w};
         const mf_v4i z = {0, 0, 0, 0};
         int I = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const mf_v4i c = mf_mma(a.q[e], w.q[e], z);
+        for (int e = 0; e < 4; ++e) {  // elements 32 e: low (e < 2) or high nibbles of l0 or l1, bits 2 e of h; minus 32
+            const uint4 l = e & 1 ? w.l1 : w.l0;
+            const auto one = [&](uint32_t x, uint32_t y) {
+                return ((((x >> (e < 2 ? 0 : 4)) & 0x0F0F0F0Fu) | (((y >> (2 * e)) & 0x03030303u) << 4)) + 0x60606060u) ^ 0x80808080u;
+            };
+            const mf_v4i c = mf_mma(v[2 * e], make_uint4(one(l.x, w.h.x), one(l.y, w.h.y), one(l.z, w.h.z), one(l.w, w.h.w)), z);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {  // sub-block 8 (i / 2) + 2 e + i % 2
                 const int sub = 8 * (i >> 1) + 2 * e + (i & 1);
                 I += __mul24(c[i], (int)(int8_t)(S[sub >> 2] >> (8 * (sub & 3))));
             }
         }
-        return fmaf(a.d * w.d, (float)I, acc);
+        return fmaf(*s * w.d, (float)I, acc);
     }
 };
 
-// Workgroup: eight waves, NW = 8 / KG of them side by side (16 weight rows each, of NM matrices: gate and up, or one), KG on parts of k.
-// The tile's activation rows go to LDS, MF_KC k at a time (all of k in most models), where every wave takes a part of it; the waves'
-// weights are loaded U steps ahead of their use, the first of them before the rows. The parts' sums meet in LDS.
+// Q8_0 of a block of 32 that 32 lanes hold, an element each: amv_q8_0_lanes32's rules and bytes, the largest and the sum by DPP; a block
+// with an element that is infinite or no number gets a scale that is none (moe_act_store4)
+__device__ __forceinline__ void mf_q8_0(float v, int rule, int j, int8_t* qs, int2* meta) {
+    float a = fabsf(v);
+    a = fmaxf(a, __int_as_float(amv_dpp_i<0xB1>(__float_as_int(a))));
+    a = fmaxf(a, __int_as_float(amv_dpp_i<0x4E>(__float_as_int(a))));
+    a = fmaxf(a, __int_as_float(amv_dpp_i<0x141>(__float_as_int(a))));
+    a = fmaxf(a, __int_as_float(amv_dpp_i<0x140>(__float_as_int(a))));
+    a = amv_max_x16(a);
+    const float d = a / 127.0f;
+    const float id = rule == AMV_Q8_X86 ? (a != 0.0f ? 127.0f / a : 0.0f) : (d != 0.0f ? 1.0f / d : 0.0f);
+    const float t = v * id;
+    const int q = (int)fminf(127.0f, fmaxf(-127.0f, rule == AMV_Q8_REF ? roundf(t) : rintf(t)));
+    int s = q;
+    s += amv_dpp_i<0xB1>(s);
+    s += amv_dpp_i<0x4E>(s);
+    s += amv_dpp_i<0x141>(s);
+    s += amv_dpp_i<0x140>(s);
+    const auto o = __builtin_amdgcn_permlane16_swap((uint32_t)s, (uint32_t)s, false, false);
+    const uint64_t bad = __ballot(!(fabsf(v) < INFINITY));
+    qs[j] = (int8_t)q;
+    if (j == 0)
+        *meta = make_int2((uint32_t)(bad >> (threadIdx.x & 32)) ? 0x7FC00000 : __float_as_int(amv_h2f(amv_f2h(d))), (int)(o[0] + o[1]));
+}
+
+// Workgroup: one tile (or, where k is long, R of its rows) and NW groups of 16 weight rows (gate and up: half of them each), a wave a
+// group on one of KG parts of k. The rows go to LDS, KC k at a time (all of k but where that is very long), a wave's first weights
+// are on their way meanwhile; then a wave goes through its weights by itself, and the parts' sums meet in LDS. What carries it is
+// several workgroups on a CU, whose chains (tile, order, rows; weights; sums) overlap: so few registers, one buffer of weights a wave.
 struct MfArgs {
     const uint8_t *w0, *w1;
-    int64_t stride;
-    int rows, n_k, n_expert, act_div;
+    int64_t stride, bytes;
+    int rows, n_k, n_expert, act_div, n_tiles, n_cols, kc;
     MfAct act;
     const int32_t* ids;
     const int2* tiles;
@@ -299,155 +297,206 @@ struct MfArgs {
     float* out;
     AmvActOut q;
 };
+// LDS, in bytes: a row of zeros and the rows' integers, their scales, their sums, the parts' sums
+struct MfLds {
+    int ld, ls, d, u, red, total;
+};
+template <int STEP, int PER, int SUMS>
+__host__ __device__ inline MfLds mf_lds(int kc, int r, int kg, int nw) {
+    MfLds l;
+    const int cs = kc / STEP;
+    l.ld = kc + 32;
+    l.ls = cs * PER + 4;
+    l.d = (r + 1) * l.ld;
+    l.u = l.d + 4 * r * l.ls;
+    l.red = l.u + 4 * SUMS * r * (cs + 1);
+    l.total = l.red + 4 * kg * r * nw * 17;
+    return l;
+}
 
-template <int WT, int NM, int KG, int G>
-__global__ __launch_bounds__(512) void k_moe_few(const MfArgs p) {
-    using T = Mf<WT>;
-    constexpr int NW = 8 / KG, KC = G == 1 ? 8192 : 4096, CS = KC / T::STEP, LD = KC + 32, LS = CS * T::PER + 4;
-    constexpr int R = 4 * G, COLS = 16 * NW;
-    constexpr bool SUMS = WT == AMV_T_Q4_K, KQ = T::STEP == 256;
-    __shared__ __align__(16) uint8_t s_q[32 + R * LD];  // 32 zeros, then the rows
-    __shared__ __align__(16) float s_d[R * LS];
-    __shared__ __align__(16) int16_t s_u[SUMS ? R * CS * 8 : 8];
-    float(*const s_red)[NM][R][COLS + 1] = reinterpret_cast<float(*)[NM][R][COLS + 1]>(s_q);  // when the rows are done with
-    static_assert(sizeof(float[KG][NM][R][COLS + 1]) <= 32 + R * LD, "the parts' sums take the rows' place");
-    __shared__ int s_pair[R];
+// ONE: without a plan, a pair is a tile of one row
+template <int WT, int U, bool GU, int NW, int KG, int G, bool ONE>
+__global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4))) void k_moe_few(const MfArgs p) {
+    using T = Mf<WT, U>;
+    constexpr int R = ONE ? 1 : 4 * G, SUB = ONE ? 1 : MOE_FEW / R, NT = 64 * NW * KG, COLS = 16 * (GU ? NW / 2 : NW);
+    constexpr bool KQ = T::STEP == 256;
+    constexpr int SUMS = T::SUMS;
+    extern __shared__ __align__(16) uint8_t s_mem[];
+    const MfLds L = mf_lds<T::STEP, T::PER, SUMS>(p.kc, R, KG, NW);
+    float* const s_d = reinterpret_cast<float*>(s_mem + L.d);
+    int* const s_u = reinterpret_cast<int*>(s_mem + L.u);
+    float(*const s_red)[NW][R][17] = reinterpret_cast<float(*)[NW][R][17]>(s_mem + L.red);
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = wv % NW, kw = wv / NW, c16 = lane & 15, q = lane >> 4;
+    // The workgroups of a tile's columns one after another over the XCDs (an XCD's own run of them would be the busier the fewer of the
+    // plan's last tiles are taken: 64 experts of 1024 x 2048 Q4_0, 48 tokens x 8: 63 us, so 50), but the parts of a tile's rows, which
+    // read the same weights, on one XCD
+    const int unit = blockIdx.x / (8 * SUB) * 8 + (blockIdx.x & 7), sub = blockIdx.x / 8 % SUB;
+    const int col = unit % p.n_cols, tile = unit / p.n_cols, n0 = col * COLS;
+    if (tile >= p.n_tiles) return;
     int e, first, count;
-    if (p.tiles) {
-        const int2 tile = p.tiles[blockIdx.y];
-        e = tile.x & 0xFFFF;
-        count = tile.x >> 16;
-        first = tile.y;
-        if (!count) return;
-    } else {
-        e = p.ids[blockIdx.y];
+    if constexpr (ONE) {
+        e = p.ids[tile];
         e = e >= 0 && e < p.n_expert ? e : p.n_expert;
-        first = blockIdx.y;
+        first = tile;
         count = 1;
+    } else {
+        const int2 t = p.tiles[tile];
+        e = t.x & 0xFFFF;
+        first = t.y + R * sub;
+        count = min(R, (t.x >> 16) - R * sub);
+        if (count <= 0) return;
     }
-    const int n0 = blockIdx.x * COLS, n_g = (count + 3) >> 2;
-    float acc[NM][G];
+    const int n_g = (count + 3) >> 2;
+    const auto pair = [&](int i) { return ONE ? first : p.order[first + i]; };
+    float acc[G];
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int m = 0; m < NM; ++m) acc[m][g] = 0.0f;
-    if (tid < R) s_pair[tid] = p.tiles ? p.order[first + min(tid, count - 1)] : first;
+    for (int g = 0; g < G; ++g) acc[g] = 0.0f;
     if (e < p.n_expert) {
-        const uint8_t* const m[2] = {p.w0 + e * p.stride, NM == 2 ? p.w1 + e * p.stride : nullptr};
-        const int n = n0 + 16 * nw + c16, nc = min(n, p.rows - 1);
-        const int steps = KQ ? p.n_k : (p.n_k + 3) / 4;
+        const uint8_t* const m = (GU && nw >= NW / 2 ? p.w1 : p.w0) + e * p.stride;
+        const __amdgpu_buffer_rsrc_t buf = MF_RSRC(m, p.bytes);
+        const int n = min(n0 + 16 * (GU ? nw % (NW / 2) : nw) + c16, p.rows - 1);
+        const int steps = KQ ? p.n_k : (p.n_k + 3) / 4, cs = p.kc / T::STEP;
         const int64_t k = (int64_t)p.n_k * (KQ ? 256 : 32);
         const int t4 = c16 >> 2, on = (c16 & 3) == q;
-        if (tid < 2) reinterpret_cast<uint4*>(s_q)[tid] = make_uint4(0, 0, 0, 0);
-        for (int c0 = 0; c0 < steps; c0 += CS) {
-            const int ns = min(CS, steps - c0), per = (ns + KG - 1) / KG, s0 = kw * per, s1 = min(ns, s0 + per);
-            typename T::W wa[NM], wb[NM];
-            const auto load = [&](typename T::W (&w)[NM], int s) {
-#pragma unroll
-                for (int i = 0; i < NM; ++i) T::load(w[i], m[i], p.rows, p.n_k, nc, q, c0 + s);
-            };
-            if (s0 < s1) load(wa, s0);
-            __syncthreads();  // (the first time: the pairs; then the rows before these are read)
-            // rows c0 .. c0 + ns of the tile: integers in pieces of 16, zeros past k
-            const int pieces = ns * (T::STEP / 16), k_left = (int)min((int64_t)KC, k - (int64_t)c0 * T::STEP) / 16;
-            for (int r = wv; r < count; r += 8) {
-                const int64_t row = s_pair[r] / p.act_div;
-                const uint4* src = reinterpret_cast<const uint4*>(p.act.q + row * k + (int64_t)c0 * T::STEP);
-                for (int i = lane; i < pieces; i += 64)
-                    *reinterpret_cast<uint4*>(s_q + 32 + r * LD + 16 * i) = i < k_left ? src[i] : make_uint4(0, 0, 0, 0);
-            }
-            for (int x = tid; x < 4 * n_g * ns * T::PER; x += 512) {
-                const int r = x / (ns * T::PER), b = x % (ns * T::PER), at = c0 * T::PER + b;
-                const int64_t i = (int64_t)(s_pair[r] / p.act_div) * p.n_k + min(at, p.n_k - 1);
-                const bool in = r < count && at < p.n_k;
-                s_d[r * LS + b] = in ? (KQ ? p.act.dk[i] : p.act.d0[i].x) : 0.0f;
-                if constexpr (SUMS) {
-                    const moe_i4* u = reinterpret_cast<const moe_i4*>(p.act.s16 + i * 16);
-                    uint32_t o[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const moe_i4 v = u[j];
-                        o[j] = (uint32_t)((v.x + v.y) & 0xFFFF) | (uint32_t)(v.z + v.w) << 16;
+        for (int i = tid; i < L.ld / 16; i += NT) reinterpret_cast<uint4*>(s_mem)[i] = make_uint4(0, 0, 0, 0);
+        for (int c0 = 0; c0 < steps; c0 += cs) {
+            const int ns = min(cs, steps - c0), per = (ns + KG - 1) / KG, s0 = kw * per, s1 = min(ns, s0 + per);
+            typename T::W w;
+            if (s0 < s1) T::load(w, buf, m, p.rows, p.n_k, n, q, c0 + s0);
+            if (c0) __syncthreads();  // (the rows before these are read)
+            // steps c0 .. c0 + ns of the rows, a wave a row: integers in pieces of 16 (zeros past k), scales, sums of the units
+            const int pieces = ns * (T::STEP / 16), k_left = (int)min((int64_t)p.kc, k - (int64_t)c0 * T::STEP) / 16;
+            for (int r = wv; r < 4 * n_g && r < R; r += NT / 64) {
+                const bool in = r < count;
+                const int64_t row = pair(in ? r : 0) / p.act_div;
+                if (in) {
+                    const uint4* src = reinterpret_cast<const uint4*>(p.act.q + row * k + (int64_t)c0 * T::STEP);
+                    for (int i = lane; i < pieces; i += 64)
+                        *reinterpret_cast<uint4*>(s_mem + (r + 1) * L.ld + 16 * i) = i < k_left ? src[i] : make_uint4(0, 0, 0, 0);
+                }
+                for (int b = lane; b < ns * T::PER; b += 64) {
+                    const int blk = c0 * T::PER + b;
+                    const int64_t i = row * p.n_k + min(blk, p.n_k - 1);
+                    const bool has = in && blk < p.n_k;
+                    if constexpr (KQ) {
+                        s_d[r * L.ls + b] = has ? p.act.dk[i] : 0.0f;
+                    } else {
+                        s_d[r * L.ls + b] = has ? p.act.d0[i].x : 0.0f;
                     }
-                    reinterpret_cast<uint4*>(s_u)[r * CS + b] = make_uint4(o[0], o[1], o[2], o[3]);
+                    if constexpr (KQ && SUMS) {  // the units' sums, two in a word
+                        const moe_i4* u = reinterpret_cast<const moe_i4*>(p.act.s16 + i * 16);
+                        uint32_t o[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const moe_i4 v = u[j];
+                            o[j] = (uint32_t)((v.x + v.y) & 0xFFFF) | (uint32_t)(v.z + v.w) << 16;
+                        }
+                        reinterpret_cast<uint4*>(s_u)[r * (cs + 1) + b] = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
                 }
             }
             __syncthreads();
-            const auto compute = [&](const typename T::W (&w)[NM], int s) {
-                typename T::Scales c[NM];
+            // all steps for n groups of four rows, two groups at a time side by side (one after the other, a chain of a row's read, its
+            // products and its sums would be waited for at every turn; more than two take too many registers)
+            const auto go = [&](auto n_groups) {
+                constexpr int NG = decltype(n_groups)::value;
+                // where the lane's integers are (in the row of zeros, for the quarters that are not its block's), its row's scales and sums
+                const uint8_t* a[NG];
 #pragma unroll
-                for (int i = 0; i < NM; ++i) T::scales(w[i], c[i]);
+                for (int g = 0; g < NG; ++g) {
+                    const int at = T::AT ? T::AT * q : 128 * (q >> 1) + 16 * (q & 1);
+                    a[g] = s_mem + (on && 4 * g + t4 < count ? (4 * g + t4 + 1) * L.ld + at : 0) + s0 * T::STEP;
+                }
+                const int r0 = ONE ? 0 : q;
+                const float* d = s_d + r0 * L.ls + s0 * T::PER;
+                const int* u = s_u + (r0 * (cs + 1) + s0) * SUMS;
+                for (int s = s0; s < s1; s += U) {
+                    if (s > s0) T::load(w, buf, m, p.rows, p.n_k, n, q, c0 + s);
+                    typename T::Scales c;
+                    T::scales(w, c, p.n_k, n, q, c0 + s);
 #pragma unroll
-                for (int j = 0; j < T::U; ++j) {
-                    if (s + j >= s1) break;
-                    typename T::B b[NM];
+                    for (int j = 0; j < U; ++j) {
+                        if (s + j >= s1) break;
+                        typename T::B b;
+                        T::operands(w, c, j, b);
 #pragma unroll
-                    for (int i = 0; i < NM; ++i) T::operands(w[i], c[i], j, b[i]);
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        if (g >= n_g) break;
-                        typename T::A a;
-                        const int live = on & (4 * g + t4 < count);
-                        T::read(a, live ? s_q + 32 + (4 * g + t4) * LD + (s + j) * T::STEP : s_q, live, q,
-                                s_d + (4 * g + q) * LS + (s + j) * T::PER, SUMS ? s_u + ((4 * g + q) * CS + s + j) * 8 : nullptr);
-#pragma unroll
-                        for (int i = 0; i < NM; ++i) acc[i][g] = T::add(b[i], a, acc[i][g]);
+                        for (int g = 0; g < NG; ++g) {
+                            acc[g] = T::add(b, a[g] + j * T::STEP, d + 4 * g * L.ls + j * T::PER, u + (4 * g * (cs + 1) + j) * SUMS, acc[g]);
+                            if (NG > 2 && (g & 1)) __builtin_amdgcn_sched_barrier(0);
+                        }
                     }
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) a[g] += U * T::STEP;
+                    d += U * T::PER;
+                    u += U * SUMS;
                 }
             };
-            for (int s = s0; s < s1; s += 2 * T::U) {
-                if (s + T::U < s1) load(wb, s + T::U);
-                compute(wa, s);
-                if (s + T::U >= s1) break;
-                if (s + 2 * T::U < s1) load(wa, s + 2 * T::U);
-                compute(wb, s + T::U);
-            }
+            if (G == 1 || n_g == 1) go(std::integral_constant<int, 1>());
+            else if (G == 2 || n_g == 2) go(std::integral_constant<int, G < 2 ? G : 2>());
+            else if (n_g == 3) go(std::integral_constant<int, G < 3 ? G : 3>());
+            else go(std::integral_constant<int, G>());
         }
     }
-    __syncthreads();
+    if constexpr (ONE) {
+        if (q == 0) s_red[kw][nw][0][c16] = acc[0];
+    } else {
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int i = 0; i < NM; ++i) s_red[kw][i][4 * g + q][16 * nw + c16] = acc[i][g];
+        for (int g = 0; g < G; ++g) s_red[kw][nw][4 * g + q][c16] = acc[g];
+    }
     __syncthreads();
-    // thread: token i and column f (a block of the 8-bit output is 32 lanes)
-    constexpr int PW = 512 / COLS;
-    for (int i = tid / COLS; i < count; i += PW) {
+    // thread: row i and column f (a block of the 8-bit output is 32 lanes)
+    for (int i = tid / COLS; i < count; i += NT / COLS) {
         const int f = tid % COLS;
-        float v[NM];
+        if (n0 + f >= p.rows) continue;  // (columns come in blocks of 32)
+        float v[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int j = 0; j < NM; ++j) {
-            v[j] = 0.0f;
+        for (int j = 0; j < (GU ? 2 : 1); ++j)
 #pragma unroll
-            for (int z = 0; z < KG; ++z) v[j] += s_red[z][j][i][f];
-        }
-        const int64_t pr = s_pair[i];
-        if constexpr (NM == 2) {
-            if (n0 + f >= p.rows) continue;  // (whole blocks of 32)
-            const float h = v[0] / (1.0f + expf(-v[0])) * v[NM - 1];
+            for (int z = 0; z < KG; ++z) v[j] += s_red[z][j * (NW / 2) + (f >> 4)][i][f & 15];
+        const int64_t pr = pair(i);
+        if constexpr (GU) {
+            const float h = v[0] / (1.0f + expf(-v[0])) * v[1];
             if (p.out) p.out[pr * p.rows + n0 + f] = h;
             if (p.q.type) {
                 const AmvActOut o = amv_act_row(p.q, pr, p.rows);
-                int2* const meta = reinterpret_cast<int2*>(o.meta) + (n0 + f) / 32;
-                amv_q8_0_lanes32(h, o.rule, f & 31, o.qs + n0 + (f & ~31), meta);
-                // (a scale that is none where an element is: moe_act_store4)
-                const uint64_t bad = __ballot(!(fabsf(h) < INFINITY));
-                if ((f & 31) == 0 && (uint32_t)(bad >> (lane & 32))) meta->x = 0x7FC00000;
+                mf_q8_0(h, o.rule, f & 31, o.qs + n0 + (f & ~31), reinterpret_cast<int2*>(o.meta) + (n0 + f) / 32);
             }
-        } else if (e < p.n_expert && n0 + f < p.rows) {
+        } else if (e < p.n_expert) {
             p.out[pr * p.rows + n0 + f] = v[0];
         }
     }
 }
 
-template <int WT, int NM, int KG>
-static void mf_go(const MfArgs& a, int n_tiles, hipStream_t st) {
-    constexpr int COLS = 16 * (8 / KG);
-    const dim3 grid((unsigned)((a.rows + COLS - 1) / COLS), (unsigned)n_tiles);
-    if (!a.tiles) k_moe_few<WT, NM, KG, 1><<<grid, 512, 0, st>>>(a);
-    else k_moe_few<WT, NM, KG, 4><<<grid, 512, 0, st>>>(a);
+template <int WT, int U, bool GU, int NW, int KG, int G, bool ONE>
+static void mf_go(MfArgs a, int64_t tiles, int64_t k, hipStream_t st) {
+    using T = Mf<WT, U>;
+    constexpr int R = ONE ? 1 : 4 * G, SUB = ONE ? 1 : MOE_FEW / R, COLS = 16 * (GU ? NW / 2 : NW);
+    a.n_tiles = (int)tiles;
+    a.n_cols = (a.rows + COLS - 1) / COLS;
+    // all of k, in whole steps, up to what 64 KB of LDS hold
+    constexpr int most = R == 16 ? 2560 : R == 8 ? 5632 : R == 4 ? 11264 : 16384;
+    a.kc = (int)std::min<int64_t>(most, (k + T::STEP - 1) / T::STEP * T::STEP);
+    const MfLds l = mf_lds<T::STEP, T::PER, T::SUMS>(a.kc, R, KG, NW);
+    k_moe_few<WT, U, GU, NW, KG, G, ONE><<<(unsigned)((tiles * a.n_cols + 7) / 8 * 8 * SUB), 64 * NW * KG, l.total, st>>>(a);
+}
+template <int WT>
+static void mf_type(const MfArgs& a, int64_t tiles, int64_t k, bool gu, hipStream_t st) {
+    constexpr int U = WT == AMV_T_Q4_0 ? 4 : WT == AMV_T_Q8_0 ? 2 : 1;
+    if (!a.tiles) {
+        constexpr int U1 = WT == AMV_T_Q6_K ? 2 : 4;
+        if (gu) mf_go<WT, U1, true, 4, 4, 1, true>(a, tiles, k, st);
+        else mf_go<WT, U1, false, 2, 8, 1, true>(a, tiles, k, st);
+    } else if (k <= 2560) {
+        if (gu) mf_go<WT, U, true, 8, 1, 4, false>(a, tiles, k, st);
+        else mf_go<WT, U, false, 8, 1, 4, false>(a, tiles, k, st);
+    } else if (k <= 5632) {
+        if (gu) mf_go<WT, U, true, 8, 1, 2, false>(a, tiles, k, st);
+        else mf_go<WT, U, false, 8, 1, 2, false>(a, tiles, k, st);
+    } else {
+        if (gu) mf_go<WT, U, true, 8, 1, 1, false>(a, tiles, k, st);
+        else mf_go<WT, U, false, 8, 1, 1, false>(a, tiles, k, st);
+    }
 }
 
 int moe_few(const MoeProduct& p) {
@@ -456,18 +505,14 @@ int moe_few(const MoeProduct& p) {
     const bool kq = p.type == AMV_T_Q4_K || p.type == AMV_T_Q6_K, gu = p.w1 != nullptr;
     const int8_t* aq = (const int8_t*)p.act;
     const int8_t* meta = aq + p.act_rows * p.k;
-    MfArgs a{(const uint8_t*)p.w0, (const uint8_t*)p.w1, p.stride, (int)p.rows, (int)(p.k / (kq ? 256 : 32)), p.n_expert, gu ? p.n_used : 1,
-             {aq, (const float2*)meta, (const float*)meta, (const int32_t*)(meta + p.act_rows * (p.k / 64))}, p.ids, v.few, v.order, p.out, p.q};
-    AMV_REQUIRE(p.plan || v.n_few <= 65535, "moe: %d pairs without a plan", v.n_few);
-    for (int64_t t0 = 0; t0 < v.n_few; t0 += 65535) {
-        const int n = (int)std::min<int64_t>(65535, v.n_few - t0);
-        if (p.plan) a.tiles = v.few + t0;
-#define GO(T) (gu ? mf_go<T, 2, 4>(a, n, p.st) : mf_go<T, 1, 4>(a, n, p.st))
-        if (p.type == AMV_T_Q4_0) GO(AMV_T_Q4_0);
-        else if (p.type == AMV_T_Q8_0) GO(AMV_T_Q8_0);
-        else if (p.type == AMV_T_Q4_K) GO(AMV_T_Q4_K);
-        else GO(AMV_T_Q6_K);
-#undef GO
-    }
+    const MfArgs a{(const uint8_t*)p.w0, (const uint8_t*)p.w1, p.stride, amv_weight_bytes(p.type, p.rows, p.k), (int)p.rows,
+                   (int)(p.k / (kq ? 256 : 32)), p.n_expert, gu ? p.n_used : 1, 0, 0, 0,
+                   {aq, (const float2*)meta, (const float*)meta, (const int32_t*)(meta + p.act_rows * (p.k / 64))}, p.ids, v.few, v.order,
+                   p.out, p.q};
+    AMV_REQUIRE((int64_t)v.n_few * (p.rows / 16) * MOE_FEW < (int64_t)1 << 31, "moe: too many tiles");
+    if (p.type == AMV_T_Q4_0) mf_type<AMV_T_Q4_0>(a, v.n_few, p.k, gu, p.st);
+    else if (p.type == AMV_T_Q8_0) mf_type<AMV_T_Q8_0>(a, v.n_few, p.k, gu, p.st);
+    else if (p.type == AMV_T_Q4_K) mf_type<AMV_T_Q4_K>(a, v.n_few, p.k, gu, p.st);
+    else mf_type<AMV_T_Q6_K>(a, v.n_few, p.k, gu, p.st);
     return amv_check_launch("amv_moe products");
 }
