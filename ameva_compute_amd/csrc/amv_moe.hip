@@ -467,7 +467,7 @@ __global__ __launch_bounds__(256) void k_moe_quantize(const float4* __restrict__
 
 static int moe_product(const MoeProduct& p) {
     // tiles of many rows where an expert has more than a few of them
-    const bool many = p.plan && p.n_tok * p.n_used >= (int64_t)32 * p.n_expert;
+    const bool many = p.plan && p.n_tok * p.n_used >= (int64_t)16 * p.n_expert;
     return many ? moe_many(p) : moe_few(p);
 }
 

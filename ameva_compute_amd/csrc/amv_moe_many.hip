@@ -11,6 +11,7 @@
 #include "amv_moe.h"
 
 #include <algorithm>
+#include <type_traits>
 
 typedef int mm_v4i __attribute__((ext_vector_type(4)));
 typedef int mm_v16i __attribute__((ext_vector_type(16)));
@@ -33,7 +34,7 @@ __device__ __forceinline__ void mm_to_lds(__amdgpu_buffer_rsrc_t from, uint4* to
 struct MmArgs {
     const uint8_t *w0, *w1;
     int64_t stride;
-    int rows, n_k, n_expert, act_div, n_tw, n_tiles;
+    int rows, n_k, n_expert, act_div, n_tw;
     const int8_t* aq;       // integers [act_rows][k]
     const uint8_t* meta;    // Q8_0: {d, sum} [act_rows][k / 32]; Q8_K: d [act_rows][k / 256], sums [act_rows][k / 16]
     int64_t act_rows;
@@ -49,13 +50,16 @@ struct MmTile {
 };
 template <int BM, bool GU>
 __device__ __forceinline__ MmTile mm_tile(const MmArgs& p, int* s_pair) {
-    // the row tiles of a weight tile one after another on one XCD: its weights stay in that XCD's L2
-    const int T = amv_xcd_tile(blockIdx.x, p.n_tw * p.n_tiles);
+    // An XCD (workgroup i runs on XCD i % 8) takes every eighth column tile of all row tiles, so the row tiles of an expert read a column
+    // tile's weights from one L2; which column tiles these are turns with the expert, as their number need not be a multiple of eight.
+    // (A run of tiles for each XCD leaves the last ones idle, where a plan's last tiles are not taken.)
+    const int x = blockIdx.x & 7, j = blockIdx.x >> 3, per = (p.n_tw + 7) >> 3;
     MmTile m;
-    const int2 t = p.tiles[T / p.n_tw];
+    const int2 t = p.tiles[j / per];
     m.e = t.x & 0xFFFF;
-    m.count = t.x >> 16;
-    m.n0 = (T % p.n_tw) * (GU ? MM_BN / 2 : MM_BN);
+    const int col = 8 * (j % per) + ((x + m.e) & 7);
+    m.count = col < p.n_tw ? t.x >> 16 : 0;
+    m.n0 = col * (GU ? MM_BN / 2 : MM_BN);
     if (m.count && (int)threadIdx.x < BM) s_pair[threadIdx.x] = p.order[t.y + min((int)threadIdx.x, m.count - 1)];
     return m;
 }
@@ -101,6 +105,13 @@ __device__ __forceinline__ void mm_finish(const MmArgs& p, const MmTile& tile, c
     }
 }
 
+// f with the number of 32-row halves of a wave's 64 rows that hold rows: the second half's products are half the work
+template <int WM, typename F>
+__device__ __forceinline__ void mm_halves(const MmTile& tile, F f) {
+    if (WM > 1 || tile.count > 32) f(std::integral_constant<int, 2>());
+    else f(std::integral_constant<int, 1>());
+}
+
 // pairs without an expert: zeros from gate and up, nothing from down (their rows are left out of the sum)
 template <int WM, bool GU>
 __device__ __forceinline__ void mm_none(const MmArgs& p, const MmTile& tile, const int* s_pair, float* s) {
@@ -127,7 +138,8 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     constexpr int LA = BM * 8, LW = BN * WP, LEND = 2 * 32 * WM * 68 / 4;
     // the buffers of even and odd steps, then (in the same place) what the end of a tile needs
     __shared__ __align__(16) uint4 sm[(2 * (LA + LW) > LEND || !GU) ? 2 * (LA + LW) : LEND];
-    __shared__ __align__(16) float sDa[2][4 * BM], sDw[2][4 * BN];
+    __shared__ __align__(16) float sDa[2][4 * BM];
+    __shared__ __align__(16) uint16_t sDw[2][4 * BN];  // (f16: three workgroups of Q8_0 on a CU)
     __shared__ int s_pair[BM];
     uint4 *const sAa = sm, *const sAb = sm + LA, *const sWa = sm + 2 * LA, *const sWb = sm + 2 * LA + LW;
     const MmTile tile = mm_tile<BM, GU>(p, s_pair);
@@ -145,6 +157,8 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     const __amdgpu_buffer_rsrc_t ra = MM_RSRC(p.aq, p.act_rows * K), rw0 = MM_RSRC(m0, wbytes), rw1 = MM_RSRC(m1, wbytes);
     // weight row of a tile's row r (past the last one: none, which reads as zero)
     const auto wrow = [&](int r) { return GU ? tile.n0 + 32 * (r >> 6) + (r & 31) : tile.n0 + r; };
+    const bool half_only = WM == 1 && tile.count <= 32;  // (the second round loads the second half's rows)
+    static_assert(RA == 2 && BM * 4 == NT, "a round loads half of the rows");
     uint32_t oa[RA], ow[RW];
 #pragma unroll
     for (int i = 0; i < RA; ++i)
@@ -157,7 +171,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     const auto load = [&](uint4* sA, uint4* sW, int b) {
 #pragma unroll
         for (int i = 0; i < RA; ++i)
-            mm_to_lds(ra, sA + NT * i + 64 * wv, oa[i] + 32u * b);
+            if (!i || !half_only) mm_to_lds(ra, sA + NT * i + 64 * wv, oa[i] + 32u * b);
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
             const bool up = GU && (((NT * i + 64 * wv) / WP) & 32);
@@ -188,7 +202,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
 #pragma unroll
         for (int i = 0; i < RDW; ++i) {
             const int x = t + NT * i;
-            sDw[buf][(x & 3) * BN + (x >> 2)] = in ? amv_h2f((uint16_t)dw[i]) : 0.0f;
+            sDw[buf][(x & 3) * BN + (x >> 2)] = in ? (uint16_t)dw[i] : (uint16_t)0;
         }
     };
 
@@ -199,11 +213,11 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
     const int ar = 64 * wm + c32, wr = 32 * wn + c32;
     const int ax = (c32 >> 1) & 7, wx = Q4 ? (c32 >> 2) & 3 : ax;  // the rows' XOR (64 wm, 32 i, 32 wn do not change them)
-    const auto compute = [&](const uint4* sA, const uint4* sW, int buf) {
+    const auto compute = [&](auto ni, const uint4* sA, const uint4* sW, int buf) {
 #pragma unroll
         for (int bl = 0; bl < 4; ++bl) {
             const mm_f32v zero = {};
-            const mm_f32v o = __builtin_amdgcn_mfma_f32_32x32x1f32(sDa[buf][bl * BM + 64 * wm + lane], sDw[buf][bl * BN + wr], zero, 0, 0, 0);
+            const mm_f32v o = __builtin_amdgcn_mfma_f32_32x32x1f32(sDa[buf][bl * BM + 64 * wm + lane], amv_h2f(sDw[buf][bl * BN + wr]), zero, 0, 0, 0);
             mm_v4i B;
             if constexpr (Q4) {  // element e < 16: low nibble of byte e (lane half 0); 16 + e: its high nibble (half 1)
                 const uint4 x = sW[wr * 4 + (bl ^ wx)];
@@ -215,7 +229,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
                 B = mm_v4i{(int)x.x, (int)x.y, (int)x.z, (int)x.w};
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < decltype(ni)::value; ++i) {
                 const uint4 a = sA[(ar + 32 * i) * 8 + ((2 * bl + h) ^ ax)];
                 const mm_v16i z = {};
                 const mm_v16i C = __builtin_amdgcn_mfma_i32_32x32x32_i8(mm_v4i{(int)a.x, (int)a.y, (int)a.z, (int)a.w}, B, z, 0, 0, 0);
@@ -234,27 +248,30 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     store_s(0, 0);
     MM_WAIT_LOADS();
     __syncthreads();
-    for (int s = 0;; s += 2) {
-        const bool more = s + 1 < nsteps, again = s + 2 < nsteps;
-        if (more) {
-            load(sAb, sWb, 4 * (s + 1));
-            load_s(4 * (s + 1));
+    const auto steps = [&](auto ni) {
+        for (int s = 0;; s += 2) {
+            const bool more = s + 1 < nsteps, again = s + 2 < nsteps;
+            if (more) {
+                load(sAb, sWb, 4 * (s + 1));
+                load_s(4 * (s + 1));
+            }
+            compute(ni, sAa, sWa, 0);
+            if (!more) break;
+            store_s(4 * (s + 1), 1);
+            MM_WAIT_LOADS();
+            __syncthreads();
+            if (again) {
+                load(sAa, sWa, 4 * (s + 2));
+                load_s(4 * (s + 2));
+            }
+            compute(ni, sAb, sWb, 1);
+            if (!again) break;
+            store_s(4 * (s + 2), 0);
+            MM_WAIT_LOADS();
+            __syncthreads();
         }
-        compute(sAa, sWa, 0);
-        if (!more) break;
-        store_s(4 * (s + 1), 1);
-        MM_WAIT_LOADS();
-        __syncthreads();
-        if (again) {
-            load(sAa, sWa, 4 * (s + 2));
-            load_s(4 * (s + 2));
-        }
-        compute(sAb, sWb, 1);
-        if (!again) break;
-        store_s(4 * (s + 2), 0);
-        MM_WAIT_LOADS();
-        __syncthreads();
-    }
+    };
+    mm_halves<WM>(tile, steps);
     mm_finish<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm), acc, wm, wn);
 }
 
@@ -292,6 +309,8 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     const __amdgpu_buffer_rsrc_t rw0 = MM_RSRC(m0, wbytes), rw1 = MM_RSRC(m1, wbytes);
     const __amdgpu_buffer_rsrc_t rh0 = MM_RSRC(m0 + wbytes, N * nsb * 16);
     const auto wrow = [&](int r) { return GU ? tile.n0 + 32 * (r >> 6) + (r & 31) : tile.n0 + r; };
+    const bool half_only = WM == 1 && tile.count <= 32;  // (the second round loads the second half's rows)
+    static_assert(RA == 2 && BM * 4 == NT, "a round loads half of the rows");
     uint32_t oa[RA], ow[RW];
 #pragma unroll
     for (int i = 0; i < RA; ++i)
@@ -304,7 +323,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     const auto load = [&](uint4* sA, uint4* sW, int j, int half) {
 #pragma unroll
         for (int i = 0; i < RA; ++i)
-            mm_to_lds(ra, sA + NT * i + 64 * wv, oa[i] + 256u * j + 128 * half);
+            if (!i || !half_only) mm_to_lds(ra, sA + NT * i + 64 * wv, oa[i] + 256u * j + 128 * half);
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
             if (GU && (((NT * i + 64 * wv) / 4) & 32))
@@ -345,7 +364,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
     const int ar = 64 * wm + c32, wr = 32 * wn + c32;
     const int ax = (c32 >> 1) & 7, wx = (c32 >> 2) & 3;
-    const auto half_step = [&](const uint4* sA, const uint4* sW, uint32_t scw, bool first) {
+    const auto half_step = [&](auto ni, const uint4* sA, const uint4* sW, uint32_t scw, bool first) {
 #pragma unroll
         for (int cp = 0; cp < 2; ++cp) {
             const uint4 x = sW[wr * 4 + ((2 * cp + h) ^ wx)];
@@ -356,7 +375,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
                                         (int)((x.w >> s) & 0x0F0F0F0Fu)};
                 const int sc = (int)((scw >> (8 * u)) & 0xFFu);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < decltype(ni)::value; ++i) {
                     const uint4 a = sA[(ar + 32 * i) * 8 + ((2 * u + h) ^ ax)];
                     const mm_v16i z = {};
                     const mm_v16i C = __builtin_amdgcn_mfma_i32_32x32x32_i8(mm_v4i{(int)a.x, (int)a.y, (int)a.z, (int)a.w}, B, z, 0, 0, 0);
@@ -374,52 +393,55 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     load_sb(0);
     MM_WAIT_LOADS();
     __syncthreads();
-    for (int j = 0; j < nsb; ++j) {
-        const int jn = min(j + 1, nsb - 1);
-        load(sAb, sWb, j, 1);
-        const uint4 hd = sHd[wr];
-        // scales and mins of units 0-3 and 4-7, one per byte
-        const uint32_t sc0 = hd.y & 0x3F3F3F3Fu, sc1 = (hd.w & 0x0F0F0F0Fu) | ((hd.y >> 2) & 0x30303030u);
-        const uint32_t mw = h ? ((hd.w >> 4) & 0x0F0F0F0Fu) | ((hd.z >> 2) & 0x30303030u) : hd.z & 0x3F3F3F3Fu;
-        half_step(sAa, sWa, sc0, true);
-        store_sb();
-        MM_WAIT_LOADS();
-        __syncthreads();
-        load(sAa, sWa, jn, 0);
-        load_head(jn);
-        load_sb(jn);
-        half_step(sAb, sWb, sc1, false);
-        // the mins, each on its unit's two 16-sum slots, against the sums
-        mm_h8 Bmn;
-        {
-            const uint32_t off = 0xE400E400u;  // -1024, -1024: 0x6400 | m is the f16 1024 + m
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t q = __builtin_amdgcn_perm(0x64646464u, mw, 0x04000400u + 0x00010001u * e);
-                const mm_h2 v = __builtin_bit_cast(mm_h2, q) + __builtin_bit_cast(mm_h2, off);
-                Bmn[2 * e] = v.x;
-                Bmn[2 * e + 1] = v.y;
+    const auto steps = [&](auto ni) {
+        for (int j = 0; j < nsb; ++j) {
+            const int jn = min(j + 1, nsb - 1);
+            load(sAb, sWb, j, 1);
+            const uint4 hd = sHd[wr];
+            // scales and mins of units 0-3 and 4-7, one per byte
+            const uint32_t sc0 = hd.y & 0x3F3F3F3Fu, sc1 = (hd.w & 0x0F0F0F0Fu) | ((hd.y >> 2) & 0x30303030u);
+            const uint32_t mw = h ? ((hd.w >> 4) & 0x0F0F0F0Fu) | ((hd.z >> 2) & 0x30303030u) : hd.z & 0x3F3F3F3Fu;
+            half_step(ni, sAa, sWa, sc0, true);
+            store_sb();
+            MM_WAIT_LOADS();
+            __syncthreads();
+            load(sAa, sWa, jn, 0);
+            load_head(jn);
+            load_sb(jn);
+            half_step(ni, sAb, sWb, sc1, false);
+            // the mins, each on its unit's two 16-sum slots, against the sums
+            mm_h8 Bmn;
+            {
+                const uint32_t off = 0xE400E400u;  // -1024, -1024: 0x6400 | m is the f16 1024 + m
+    #pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t q = __builtin_amdgcn_perm(0x64646464u, mw, 0x04000400u + 0x00010001u * e);
+                    const mm_h2 v = __builtin_bit_cast(mm_h2, q) + __builtin_bit_cast(mm_h2, off);
+                    Bmn[2 * e] = v.x;
+                    Bmn[2 * e + 1] = v.y;
+                }
             }
-        }
-        const float d = amv_h2f(hd.x), dm = amv_h2f(hd.x >> 16);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int tl = 64 * wm + 32 * i;
-            const mm_h8 Abs = *reinterpret_cast<const mm_h8*>(&sBs[(tl + c32) * 4 + 2 * h]);
-            const mm_f16v zf = {};
-            const mm_f16v I2 = __builtin_amdgcn_mfma_f32_32x32x16_f16(Abs, Bmn, zf, 0, 0, 0);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float4 v = *reinterpret_cast<const float4*>(&sDa[tl + 4 * h + 8 * q]);
-                const float da[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    acc[i][4 * q + r] = fmaf(fmaf(d, (float)I1[i][4 * q + r], -(dm * I2[4 * q + r])), da[r], acc[i][4 * q + r]);
+            const float d = amv_h2f(hd.x), dm = amv_h2f(hd.x >> 16);
+    #pragma unroll
+            for (int i = 0; i < decltype(ni)::value; ++i) {
+                const int tl = 64 * wm + 32 * i;
+                const mm_h8 Abs = *reinterpret_cast<const mm_h8*>(&sBs[(tl + c32) * 4 + 2 * h]);
+                const mm_f16v zf = {};
+                const mm_f16v I2 = __builtin_amdgcn_mfma_f32_32x32x16_f16(Abs, Bmn, zf, 0, 0, 0);
+    #pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float4 v = *reinterpret_cast<const float4*>(&sDa[tl + 4 * h + 8 * q]);
+                    const float da[4] = {v.x, v.y, v.z, v.w};
+    #pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        acc[i][4 * q + r] = fmaf(fmaf(d, (float)I1[i][4 * q + r], -(dm * I2[4 * q + r])), da[r], acc[i][4 * q + r]);
+                }
             }
+            MM_WAIT_LOADS();
+            __syncthreads();
         }
-        MM_WAIT_LOADS();
-        __syncthreads();
-    }
+    };
+    mm_halves<WM>(tile, steps);
     mm_finish<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm), acc, wm, wn);
 }
 
@@ -453,6 +475,8 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 
     const __amdgpu_buffer_rsrc_t rw0 = MM_RSRC(m0, nblk * 128), rw1 = MM_RSRC(m1, nblk * 128);
     const __amdgpu_buffer_rsrc_t rq0 = MM_RSRC(m0 + nblk * 128, nblk * 64), rq1 = MM_RSRC(m1 + nblk * 128, nblk * 64);
     const auto wrow = [&](int r) { return GU ? tile.n0 + 32 * (r >> 6) + (r & 31) : tile.n0 + r; };
+    const bool half_only = WM == 1 && tile.count <= 32;  // (the second round loads the second half's rows)
+    static_assert(RA == 2 && BM * 4 == NT, "a round loads half of the rows");
     uint32_t oa[RA], ow[RW];
 #pragma unroll
     for (int i = 0; i < RA; ++i)
@@ -468,7 +492,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 
     const auto load = [&](uint4* sA, uint4* sW, uint4* sH, int j, int half) {
 #pragma unroll
         for (int i = 0; i < RA; ++i)
-            mm_to_lds(ra, sA + NT * i + 64 * wv, oa[i] + 256u * j + 128 * half);
+            if (!i || !half_only) mm_to_lds(ra, sA + NT * i + 64 * wv, oa[i] + 256u * j + 128 * half);
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
             if (GU && (((NT * i + 64 * wv) / 4) & 32))
@@ -515,7 +539,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 
     const int ar = 64 * wm + c32, wr = 32 * wn + c32;
     const int ax = (c32 >> 1) & 7, wx = (c32 >> 2) & 3, hx = (c32 >> 2) & 1;
     // sw: the half's eight scales (bytes 2 e + pp: sub-block of elements 32 e + 16 pp ..)
-    const auto half_step = [&](const uint4* sA, const uint4* sW, const uint4* sH, uint32_t s0, uint32_t s1) {
+    const auto half_step = [&](auto ni, const uint4* sA, const uint4* sW, const uint4* sH, uint32_t s0, uint32_t s1) {
 #pragma unroll
         for (int pp = 0; pp < 2; ++pp) {
             const uint2 l0 = reinterpret_cast<const uint2*>(sW + wr * 4 + (pp ^ wx))[h];
@@ -531,7 +555,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 
                 const uint2 b = make_uint2(q6(l.x, qh.x), q6(l.y, qh.y));
                 const int sub = 2 * e + pp, sc = (int)(int8_t)((sub < 4 ? s0 : s1) >> (8 * (sub & 3)));
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < decltype(ni)::value; ++i) {
                     const uint2 a = reinterpret_cast<const uint2*>(sA + (ar + 32 * i) * 8 + ((2 * e + pp) ^ ax))[h];
                     const mm_v16i z = {};
                     const mm_v16i C = __builtin_amdgcn_mfma_i32_32x32x16_i8(__builtin_bit_cast(long, a), __builtin_bit_cast(long, b), z, 0, 0, 0);
@@ -549,33 +573,36 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 
     store_sb(0);
     MM_WAIT_LOADS();
     __syncthreads();
-    for (int j = 0; j < nsb; ++j) {
-        const int jn = min(j + 1, nsb - 1), buf = j & 1;
-        load(sAb, sWb, sHb, j, 1);
-        load_sb(jn);
-        const uint4 sc = sSc[buf][wr];
-        half_step(sAa, sWa, sHa, sc.x, sc.y);
-        store_sb(buf ^ 1);
-        MM_WAIT_LOADS();
-        __syncthreads();
-        load(sAa, sWa, sHa, jn, 0);
-        half_step(sAb, sWb, sHb, sc.z, sc.w);
-        const float d = sD[buf][wr];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float4 v = *reinterpret_cast<const float4*>(&sDa[buf][64 * wm + 32 * i + 4 * h + 8 * q]);
-                const float da[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    acc[i][4 * q + r] = fmaf(d * da[r], (float)I[i][4 * q + r], acc[i][4 * q + r]);
-                    I[i][4 * q + r] = 0;
+    const auto steps = [&](auto ni) {
+        for (int j = 0; j < nsb; ++j) {
+            const int jn = min(j + 1, nsb - 1), buf = j & 1;
+            load(sAb, sWb, sHb, j, 1);
+            load_sb(jn);
+            const uint4 sc = sSc[buf][wr];
+            half_step(ni, sAa, sWa, sHa, sc.x, sc.y);
+            store_sb(buf ^ 1);
+            MM_WAIT_LOADS();
+            __syncthreads();
+            load(sAa, sWa, sHa, jn, 0);
+            half_step(ni, sAb, sWb, sHb, sc.z, sc.w);
+            const float d = sD[buf][wr];
+    #pragma unroll
+            for (int i = 0; i < decltype(ni)::value; ++i)
+    #pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float4 v = *reinterpret_cast<const float4*>(&sDa[buf][64 * wm + 32 * i + 4 * h + 8 * q]);
+                    const float da[4] = {v.x, v.y, v.z, v.w};
+    #pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        acc[i][4 * q + r] = fmaf(d * da[r], (float)I[i][4 * q + r], acc[i][4 * q + r]);
+                        I[i][4 * q + r] = 0;
+                    }
                 }
-            }
-        MM_WAIT_LOADS();
-        __syncthreads();
-    }
+            MM_WAIT_LOADS();
+            __syncthreads();
+        }
+    };
+    mm_halves<WM>(tile, steps);
     mm_finish<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm), acc, wm, wn);
 }
 
@@ -586,10 +613,11 @@ int moe_many(const MoeProduct& p) {
     const bool kq = p.type == AMV_T_Q4_K || p.type == AMV_T_Q6_K, gu = p.w1 != nullptr;
     const int8_t* aq = (const int8_t*)p.act;
     MmArgs a{(const uint8_t*)p.w0, (const uint8_t*)p.w1, p.stride, (int)p.rows, (int)(p.k / (kq ? 256 : 32)), p.n_expert, gu ? p.n_used : 1,
-             0, v.n_many, aq, (const uint8_t*)aq + p.act_rows * p.k, p.act_rows, v.many, v.order, p.out, p.q};
+             0, aq, (const uint8_t*)aq + p.act_rows * p.k, p.act_rows, v.many, v.order, p.out, p.q};
     a.n_tw = (int)((p.rows + (gu ? MM_BN / 2 : MM_BN) - 1) / (gu ? MM_BN / 2 : MM_BN));
-    AMV_REQUIRE((int64_t)a.n_tw * a.n_tiles < (int64_t)1 << 31, "moe: too many tiles");
-    const unsigned grid = (unsigned)((int64_t)a.n_tw * a.n_tiles);
+    const int64_t wgs = (int64_t)((a.n_tw + 7) / 8 * 8) * v.n_many;
+    AMV_REQUIRE(wgs < (int64_t)1 << 31, "moe: too many tiles");
+    const unsigned grid = (unsigned)wgs;
     constexpr int WM = MOE_MANY / 64;
 #define GO(KERNEL) hipLaunchKernelGGL((gu ? KERNEL(true) : KERNEL(false)), dim3(grid), dim3(256 * WM), 0, p.st, a)
 #define K40(G) k_moe_many<AMV_T_Q4_0, WM, G>
