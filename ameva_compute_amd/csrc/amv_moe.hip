@@ -465,9 +465,17 @@ __global__ __launch_bounds__(256) void k_moe_quantize(const float4* __restrict__
     moe_act_store4(amv_act_row(act, r, 4 * (int64_t)n4), (int)(i - r * n4), h);
 }
 
+// Tiles of many rows from so many rows an expert on that their products beside the weights' bytes cost less than the few rows' kernel,
+// which does four times the matrix work; later where the tiles are too few to fill the GPU (us, few / many, at the rows an expert below
+// and above the choice): 64 experts of gate and up 1024 x 2048 Q4_0 12: 57 / 59, 24: 81 / 74; Q8_0 6: 68 / 74, 12: 84 / 79; Q4_K 6: 47 /
+// 49, 12: 60 / 56; Q6_K 12: 75 / 88, 24: 103 / 97; down 2048 x 1024 Q4_0 12: 36 / 40, 24: 46 / 45; Q8_0 6: 43 / 43, 12: 54 / 47; Q4_K 6: 27 /
+// 30, 12: 39 / 36; Q6_K 12: 49 / 51, 24: 60 / 56; 8 experts of 4096 x 6144 Q4_0 24: 68 / 89, 48: 115 / 96; Q8_0 16: 85 / 93, 32: 123 / 102;
+// Q4_K 24: 67 / 80, 32: 87 / 82; Q6_K 24: 85 / 111, 48: 137 / 115; of 4096 x 14336 Q6_K 24: 188 / 244, 48: 300 / 252
 static int moe_product(const MoeProduct& p) {
-    // tiles of many rows where an expert has more than a few of them
-    const bool many = p.plan && p.n_tok * p.n_used >= (int64_t)16 * p.n_expert;
+    const int64_t wgs = p.n_expert * ((p.rows + (p.w1 ? 63 : 127)) / (p.w1 ? 64 : 128));
+    const int rows = p.type == AMV_T_Q4_0 ? (wgs >= 512 ? 16 : 32) : p.type == AMV_T_Q8_0 ? (wgs >= 512 ? 8 : 24)
+                     : p.type == AMV_T_Q4_K ? (wgs >= 512 ? 8 : 28) : (wgs >= 512 ? 14 : 32);
+    const bool many = p.plan && p.n_tok * p.n_used >= (int64_t)rows * p.n_expert;
     return many ? moe_many(p) : moe_few(p);
 }
 

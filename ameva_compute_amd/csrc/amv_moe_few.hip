@@ -282,14 +282,14 @@ __device__ __forceinline__ void mf_q8_0(float v, int rule, int j, int8_t* qs, in
         *meta = make_int2((uint32_t)(bad >> (threadIdx.x & 32)) ? 0x7FC00000 : __float_as_int(amv_h2f(amv_f2h(d))), (int)(o[0] + o[1]));
 }
 
-// Workgroup: one tile (or, where k is long, R of its rows) and NW groups of 16 weight rows (gate and up: half of them each), a wave a
+// Workgroup: one tile and NW groups of 16 weight rows (gate and up: half of them each), a wave a
 // group on one of KG parts of k. The rows go to LDS, KC k at a time (all of k but where that is very long), a wave's first weights
 // are on their way meanwhile; then a wave goes through its weights by itself, and the parts' sums meet in LDS. What carries it is
 // several workgroups on a CU, whose chains (tile, order, rows; weights; sums) overlap: so few registers, one buffer of weights a wave.
 struct MfArgs {
     const uint8_t *w0, *w1;
     int64_t stride, bytes;
-    int rows, n_k, n_expert, act_div, n_tiles, n_cols, kc;
+    int rows, n_k, n_expert, act_div, n_cols, kc;
     MfAct act;
     const int32_t* ids;
     const int2* tiles;
@@ -315,10 +315,10 @@ __host__ __device__ inline MfLds mf_lds(int kc, int r, int kg, int nw) {
 }
 
 // ONE: without a plan, a pair is a tile of one row
-template <int WT, int U, bool GU, int NW, int KG, int G, bool ONE>
+template <int WT, int U, bool GU, int NW, int KG, bool ONE>
 __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4))) void k_moe_few(const MfArgs p) {
     using T = Mf<WT, U>;
-    constexpr int R = ONE ? 1 : 4 * G, SUB = ONE ? 1 : MOE_FEW / R, NT = 64 * NW * KG, COLS = 16 * (GU ? NW / 2 : NW);
+    constexpr int G = ONE ? 1 : MOE_FEW / 4, R = ONE ? 1 : MOE_FEW, NT = 64 * NW * KG, COLS = 16 * (GU ? NW / 2 : NW);
     constexpr bool KQ = T::STEP == 256;
     constexpr int SUMS = T::SUMS;
     extern __shared__ __align__(16) uint8_t s_mem[];
@@ -328,12 +328,9 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
     float(*const s_red)[NW][R][17] = reinterpret_cast<float(*)[NW][R][17]>(s_mem + L.red);
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = wv % NW, kw = wv / NW, c16 = lane & 15, q = lane >> 4;
-    // The workgroups of a tile's columns one after another over the XCDs (an XCD's own run of them would be the busier the fewer of the
-    // plan's last tiles are taken: 64 experts of 1024 x 2048 Q4_0, 48 tokens x 8: 63 us, so 50), but the parts of a tile's rows, which
-    // read the same weights, on one XCD
-    const int unit = blockIdx.x / (8 * SUB) * 8 + (blockIdx.x & 7), sub = blockIdx.x / 8 % SUB;
-    const int col = unit % p.n_cols, tile = unit / p.n_cols, n0 = col * COLS;
-    if (tile >= p.n_tiles) return;
+    // the workgroups of a tile's columns one after another over the XCDs (a run of tiles for each XCD leaves the last ones idle, where a
+    // plan's last tiles are not taken: 48 tokens x 8 of 64 experts of 1024 x 2048 Q4_0 63 us, so 50)
+    const int col = blockIdx.x % p.n_cols, tile = blockIdx.x / p.n_cols, n0 = col * COLS;
     int e, first, count;
     if constexpr (ONE) {
         e = p.ids[tile];
@@ -343,9 +340,9 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
     } else {
         const int2 t = p.tiles[tile];
         e = t.x & 0xFFFF;
-        first = t.y + R * sub;
-        count = min(R, (t.x >> 16) - R * sub);
-        if (count <= 0) return;
+        first = t.y;
+        count = t.x >> 16;
+        if (!count) return;
     }
     const int n_g = (count + 3) >> 2;
     const auto pair = [&](int i) { return ONE ? first : p.order[first + i]; };
@@ -432,9 +429,9 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
                     u += U * SUMS;
                 }
             };
-            if (G == 1 || n_g == 1) go(std::integral_constant<int, 1>());
-            else if (G == 2 || n_g == 2) go(std::integral_constant<int, G < 2 ? G : 2>());
-            else if (n_g == 3) go(std::integral_constant<int, G < 3 ? G : 3>());
+            if (ONE || n_g == 1) go(std::integral_constant<int, 1>());
+            else if (n_g == 2) go(std::integral_constant<int, ONE ? 1 : 2>());
+            else if (n_g == 3) go(std::integral_constant<int, ONE ? 1 : 3>());
             else go(std::integral_constant<int, G>());
         }
     }
@@ -468,34 +465,32 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
     }
 }
 
-template <int WT, int U, bool GU, int NW, int KG, int G, bool ONE>
+// k that a workgroup's LDS holds of a tile's rows
+#define MF_KC 3584
+
+template <int WT, int U, bool GU, int NW, int KG, bool ONE>
 static void mf_go(MfArgs a, int64_t tiles, int64_t k, hipStream_t st) {
     using T = Mf<WT, U>;
-    constexpr int R = ONE ? 1 : 4 * G, SUB = ONE ? 1 : MOE_FEW / R, COLS = 16 * (GU ? NW / 2 : NW);
-    a.n_tiles = (int)tiles;
+    constexpr int R = ONE ? 1 : MOE_FEW, COLS = 16 * (GU ? NW / 2 : NW);
     a.n_cols = (a.rows + COLS - 1) / COLS;
-    // all of k, in whole steps, up to what 64 KB of LDS hold
-    constexpr int most = R == 16 ? 2560 : R == 8 ? 5632 : R == 4 ? 11264 : 16384;
-    a.kc = (int)std::min<int64_t>(most, (k + T::STEP - 1) / T::STEP * T::STEP);
+    // all of k, or even parts of it, in whole steps
+    const int64_t steps = (k + T::STEP - 1) / T::STEP, most = (ONE ? 16384 : MF_KC) / T::STEP, parts = (steps + most - 1) / most;
+    a.kc = (int)((steps + parts - 1) / parts * T::STEP);
     const MfLds l = mf_lds<T::STEP, T::PER, T::SUMS>(a.kc, R, KG, NW);
-    k_moe_few<WT, U, GU, NW, KG, G, ONE><<<(unsigned)((tiles * a.n_cols + 7) / 8 * 8 * SUB), 64 * NW * KG, l.total, st>>>(a);
+    k_moe_few<WT, U, GU, NW, KG, ONE><<<(unsigned)(tiles * a.n_cols), 64 * NW * KG, l.total, st>>>(a);
 }
 template <int WT>
 static void mf_type(const MfArgs& a, int64_t tiles, int64_t k, bool gu, hipStream_t st) {
-    constexpr int U = WT == AMV_T_Q4_0 ? 4 : WT == AMV_T_Q8_0 ? 2 : 1;
+    constexpr int U = WT == AMV_T_Q4_0 ? 4 : WT == AMV_T_Q8_0 ? 2 : 1, U1 = WT == AMV_T_Q6_K ? 2 : 4;
     if (!a.tiles) {
-        constexpr int U1 = WT == AMV_T_Q6_K ? 2 : 4;
-        if (gu) mf_go<WT, U1, true, 4, 4, 1, true>(a, tiles, k, st);
-        else mf_go<WT, U1, false, 2, 8, 1, true>(a, tiles, k, st);
+        if (gu) mf_go<WT, U1, true, 4, 4, true>(a, tiles, k, st);
+        else mf_go<WT, U1, false, 2, 8, true>(a, tiles, k, st);
     } else if (k <= 2560) {
-        if (gu) mf_go<WT, U, true, 8, 1, 4, false>(a, tiles, k, st);
-        else mf_go<WT, U, false, 8, 1, 4, false>(a, tiles, k, st);
-    } else if (k <= 5632) {
-        if (gu) mf_go<WT, U, true, 8, 1, 2, false>(a, tiles, k, st);
-        else mf_go<WT, U, false, 8, 1, 2, false>(a, tiles, k, st);
+        if (gu) mf_go<WT, U, true, 8, 1, false>(a, tiles, k, st);
+        else mf_go<WT, U, false, 8, 1, false>(a, tiles, k, st);
     } else {
-        if (gu) mf_go<WT, U, true, 8, 1, 1, false>(a, tiles, k, st);
-        else mf_go<WT, U, false, 8, 1, 1, false>(a, tiles, k, st);
+        if (gu) mf_go<WT, U, true, 4, 2, false>(a, tiles, k, st);
+        else mf_go<WT, U, false, 4, 2, false>(a, tiles, k, st);
     }
 }
 
@@ -506,10 +501,10 @@ int moe_few(const MoeProduct& p) {
     const int8_t* aq = (const int8_t*)p.act;
     const int8_t* meta = aq + p.act_rows * p.k;
     const MfArgs a{(const uint8_t*)p.w0, (const uint8_t*)p.w1, p.stride, amv_weight_bytes(p.type, p.rows, p.k), (int)p.rows,
-                   (int)(p.k / (kq ? 256 : 32)), p.n_expert, gu ? p.n_used : 1, 0, 0, 0,
+                   (int)(p.k / (kq ? 256 : 32)), p.n_expert, gu ? p.n_used : 1, 0, 0,
                    {aq, (const float2*)meta, (const float*)meta, (const int32_t*)(meta + p.act_rows * (p.k / 64))}, p.ids, v.few, v.order,
                    p.out, p.q};
-    AMV_REQUIRE((int64_t)v.n_few * (p.rows / 16) * MOE_FEW < (int64_t)1 << 31, "moe: too many tiles");
+    AMV_REQUIRE((int64_t)v.n_few * (p.rows / 16) < (int64_t)1 << 31, "moe: too many tiles");
     if (p.type == AMV_T_Q4_0) mf_type<AMV_T_Q4_0>(a, v.n_few, p.k, gu, p.st);
     else if (p.type == AMV_T_Q8_0) mf_type<AMV_T_Q8_0>(a, v.n_few, p.k, gu, p.st);
     else if (p.type == AMV_T_Q4_K) mf_type<AMV_T_Q4_K>(a, v.n_few, p.k, gu, p.st);

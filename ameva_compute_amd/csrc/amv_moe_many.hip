@@ -213,7 +213,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
     const int ar = 64 * wm + c32, wr = 32 * wn + c32;
     const int ax = (c32 >> 1) & 7, wx = Q4 ? (c32 >> 2) & 3 : ax;  // the rows' XOR (64 wm, 32 i, 32 wn do not change them)
-    const auto compute = [&](auto ni, const uint4* sA, const uint4* sW, int buf) {
+    const auto compute = [&](auto ni, const uint4* sA, const uint4* sW, int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int bl = 0; bl < 4; ++bl) {
             const mm_f32v zero = {};
@@ -248,7 +248,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     store_s(0, 0);
     MM_WAIT_LOADS();
     __syncthreads();
-    const auto steps = [&](auto ni) {
+    const auto steps = [&](auto ni) __attribute__((always_inline)) {
         for (int s = 0;; s += 2) {
             const bool more = s + 1 < nsteps, again = s + 2 < nsteps;
             if (more) {
@@ -364,7 +364,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
     const int ar = 64 * wm + c32, wr = 32 * wn + c32;
     const int ax = (c32 >> 1) & 7, wx = (c32 >> 2) & 3;
-    const auto half_step = [&](auto ni, const uint4* sA, const uint4* sW, uint32_t scw, bool first) {
+    const auto half_step = [&](auto ni, const uint4* sA, const uint4* sW, uint32_t scw, bool first) __attribute__((always_inline)) {
 #pragma unroll
         for (int cp = 0; cp < 2; ++cp) {
             const uint4 x = sW[wr * 4 + ((2 * cp + h) ^ wx)];
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     load_sb(0);
     MM_WAIT_LOADS();
     __syncthreads();
-    const auto steps = [&](auto ni) {
+    const auto steps = [&](auto ni) __attribute__((always_inline)) {
         for (int j = 0; j < nsb; ++j) {
             const int jn = min(j + 1, nsb - 1);
             load(sAb, sWb, j, 1);
@@ -539,7 +539,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 
     const int ar = 64 * wm + c32, wr = 32 * wn + c32;
     const int ax = (c32 >> 1) & 7, wx = (c32 >> 2) & 3, hx = (c32 >> 2) & 1;
     // sw: the half's eight scales (bytes 2 e + pp: sub-block of elements 32 e + 16 pp ..)
-    const auto half_step = [&](auto ni, const uint4* sA, const uint4* sW, const uint4* sH, uint32_t s0, uint32_t s1) {
+    const auto half_step = [&](auto ni, const uint4* sA, const uint4* sW, const uint4* sH, uint32_t s0, uint32_t s1) __attribute__((always_inline)) {
 #pragma unroll
         for (int pp = 0; pp < 2; ++pp) {
             const uint2 l0 = reinterpret_cast<const uint2*>(sW + wr * 4 + (pp ^ wx))[h];
@@ -573,7 +573,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 
     store_sb(0);
     MM_WAIT_LOADS();
     __syncthreads();
-    const auto steps = [&](auto ni) {
+    const auto steps = [&](auto ni) __attribute__((always_inline)) {
         for (int j = 0; j < nsb; ++j) {
             const int jn = min(j + 1, nsb - 1), buf = j & 1;
             load(sAb, sWb, sHb, j, 1);
