@@ -34,10 +34,6 @@ static inline MoePlanView moe_plan_view(const void* plan, int64_t pairs, int64_t
     v.few = (const int2*)plan;
     v.many = v.few + v.n_few;
     v.order = (const int32_t*)(v.many + v.n_many);
-    if (!plan) {  // each pair by itself
-        v.few = nullptr;
-        v.n_few = (int)pairs;
-    }
     return v;
 }
 
@@ -50,13 +46,15 @@ struct MoeProduct {
     int64_t act_rows;
     const int32_t* ids;
     const void* plan;
-    // gate and up: f32 [pairs][rows] and / or the 8-bit output; down: f32 [pairs][rows]
+    // gate and up: f32 [pairs][rows] and / or the 8-bit output; down: f32 [pairs][rows], but moe_one's f32 [n_tok][rows], the sum
     float* out;
     AmvActOut q;
+    const float *weights, *add;  // of moe_one's sum
     hipStream_t st;
 };
+int moe_one(const MoeProduct& p);   // amv_moe_few.hip: without a plan
 int moe_few(const MoeProduct& p);   // amv_moe_few.hip
-int moe_many(const MoeProduct& p);  // amv_moe_many.hip (with a plan)
+int moe_many(const MoeProduct& p);  // amv_moe_many.hip
 
 // four int32 at an address of any whole int32 (a Q8_K buffer's sums begin where its scales end)
 typedef int moe_i4 __attribute__((ext_vector_type(4), aligned(4)));

@@ -472,10 +472,11 @@ __global__ __launch_bounds__(256) void k_moe_quantize(const float4* __restrict__
 // 30, 12: 39 / 36; Q6_K 12: 49 / 51, 24: 60 / 56; 8 experts of 4096 x 6144 Q4_0 24: 68 / 89, 48: 115 / 96; Q8_0 16: 85 / 93, 32: 123 / 102;
 // Q4_K 24: 67 / 80, 32: 87 / 82; Q6_K 24: 85 / 111, 48: 137 / 115; of 4096 x 14336 Q6_K 24: 188 / 244, 48: 300 / 252
 static int moe_product(const MoeProduct& p) {
+    if (!p.plan) return moe_one(p);
     const int64_t wgs = p.n_expert * ((p.rows + (p.w1 ? 63 : 127)) / (p.w1 ? 64 : 128));
     const int rows = p.type == AMV_T_Q4_0 ? (wgs >= 512 ? 16 : 32) : p.type == AMV_T_Q8_0 ? (wgs >= 512 ? 8 : 24)
                      : p.type == AMV_T_Q4_K ? (wgs >= 512 ? 8 : 28) : (wgs >= 512 ? 14 : 32);
-    const bool many = p.plan && p.n_tok * p.n_used >= (int64_t)rows * p.n_expert;
+    const bool many = p.n_tok * p.n_used >= (int64_t)rows * p.n_expert;
     return many ? moe_many(p) : moe_few(p);
 }
 
@@ -508,7 +509,7 @@ extern "C" int amv_moe_gate_up(int wtype, const void* w_gate, const void* w_up, 
                                float* eout, void* act_out, int act_type, int rule, void* workspace, int64_t workspace_bytes,
                                void* stream) {
     MoeProduct p{wtype, (int)std::min<int64_t>(n_expert, INT32_MAX), (int)std::min<int64_t>(n_used, INT32_MAX), rows, k, expert_stride,
-                 n_tok, w_gate, w_up, act, n_tok, ids, plan, eout, {}, amv_stream(stream)};
+                 n_tok, w_gate, w_up, act, n_tok, ids, plan, eout, {}, nullptr, nullptr, amv_stream(stream)};
     const char* what = "amv_moe_gate_up";
     const int rc = moe_check_product(what, p);
     if (rc) return rc;
@@ -562,7 +563,7 @@ extern "C" int amv_moe_down(int wtype, const void* w, int64_t expert_stride, int
                             int64_t n_tok, int64_t n_used, const int32_t* ids, const void* plan, const float* weights,
                             const float* add, float* dst, void* workspace, int64_t workspace_bytes, void* stream) {
     MoeProduct p{wtype, (int)std::min<int64_t>(n_expert, INT32_MAX), (int)std::min<int64_t>(n_used, INT32_MAX), rows, k, expert_stride,
-                 n_tok, w, w, act, n_tok * n_used, ids, plan, (float*)workspace, {}, amv_stream(stream)};
+                 n_tok, w, w, act, n_tok * n_used, ids, plan, plan ? (float*)workspace : dst, {}, weights, add, amv_stream(stream)};
     const char* what = "amv_moe_down";
     const int rc = moe_check_product(what, p);
     if (rc) return rc;
@@ -570,11 +571,11 @@ extern "C" int amv_moe_down(int wtype, const void* w, int64_t expert_stride, int
                 "%s: null weights or dst, or a buffer that is not 16-byte aligned", what);
     const int64_t need = amv_moe_down_workspace_bytes(n_tok, n_used, rows);
     if (!n_tok) return AMV_OK;
-    AMV_REQUIRE(workspace && workspace_bytes >= need, "%s: a workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes,
-                (long long)need);
+    AMV_REQUIRE(!plan || (workspace && workspace_bytes >= need), "%s: a workspace of %lld bytes, %lld needed", what,
+                (long long)workspace_bytes, (long long)need);
     p.w1 = nullptr;
     const int r = moe_product(p);
-    if (r) return r;
+    if (r || !plan) return r;
     const int n4 = (int)(rows / 4);
     for (int64_t t0 = 0; t0 < n_tok; t0 += 65535) {
         const int64_t n = std::min<int64_t>(65535, n_tok - t0);

@@ -291,7 +291,6 @@ struct MfArgs {
     int64_t stride, bytes;
     int rows, n_k, n_expert, act_div, n_cols, kc;
     MfAct act;
-    const int32_t* ids;
     const int2* tiles;
     const int32_t* order;
     float* out;
@@ -314,11 +313,10 @@ __host__ __device__ inline MfLds mf_lds(int kc, int r, int kg, int nw) {
     return l;
 }
 
-// ONE: without a plan, a pair is a tile of one row
-template <int WT, int U, bool GU, int NW, int KG, bool ONE>
+template <int WT, int U, bool GU, int NW, int KG>
 __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4))) void k_moe_few(const MfArgs p) {
     using T = Mf<WT, U>;
-    constexpr int G = ONE ? 1 : MOE_FEW / 4, R = ONE ? 1 : MOE_FEW, NT = 64 * NW * KG, COLS = 16 * (GU ? NW / 2 : NW);
+    constexpr int G = MOE_FEW / 4, R = MOE_FEW, NT = 64 * NW * KG, COLS = 16 * (GU ? NW / 2 : NW);
     constexpr bool KQ = T::STEP == 256;
     constexpr int SUMS = T::SUMS;
     extern __shared__ __align__(16) uint8_t s_mem[];
@@ -331,21 +329,11 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
     // the workgroups of a tile's columns one after another over the XCDs (a run of tiles for each XCD leaves the last ones idle, where a
     // plan's last tiles are not taken: 48 tokens x 8 of 64 experts of 1024 x 2048 Q4_0 63 us, so 50)
     const int col = blockIdx.x % p.n_cols, tile = blockIdx.x / p.n_cols, n0 = col * COLS;
-    int e, first, count;
-    if constexpr (ONE) {
-        e = p.ids[tile];
-        e = e >= 0 && e < p.n_expert ? e : p.n_expert;
-        first = tile;
-        count = 1;
-    } else {
-        const int2 t = p.tiles[tile];
-        e = t.x & 0xFFFF;
-        first = t.y;
-        count = t.x >> 16;
-        if (!count) return;
-    }
+    const int2 t = p.tiles[tile];
+    const int e = t.x & 0xFFFF, count = t.x >> 16;
+    if (!count) return;
     const int n_g = (count + 3) >> 2;
-    const auto pair = [&](int i) { return ONE ? first : p.order[first + i]; };
+    const auto pair = [&](int i) { return p.order[t.y + i]; };
     float acc[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) acc[g] = 0.0f;
@@ -405,9 +393,8 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
                     const int at = T::AT ? T::AT * q : 128 * (q >> 1) + 16 * (q & 1);
                     a[g] = s_mem + (on && 4 * g + t4 < count ? (4 * g + t4 + 1) * L.ld + at : 0) + s0 * T::STEP;
                 }
-                const int r0 = ONE ? 0 : q;
-                const float* d = s_d + r0 * L.ls + s0 * T::PER;
-                const int* u = s_u + (r0 * (cs + 1) + s0) * SUMS;
+                const float* d = s_d + q * L.ls + s0 * T::PER;
+                const int* u = s_u + (q * (cs + 1) + s0) * SUMS;
                 for (int s = s0; s < s1; s += U) {
                     if (s > s0) T::load(w, buf, m, p.rows, p.n_k, n, q, c0 + s);
                     typename T::Scales c;
@@ -429,18 +416,14 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
                     u += U * SUMS;
                 }
             };
-            if (ONE || n_g == 1) go(std::integral_constant<int, 1>());
-            else if (n_g == 2) go(std::integral_constant<int, ONE ? 1 : 2>());
-            else if (n_g == 3) go(std::integral_constant<int, ONE ? 1 : 3>());
+            if (n_g == 1) go(std::integral_constant<int, 1>());
+            else if (n_g == 2) go(std::integral_constant<int, 2>());
+            else if (n_g == 3) go(std::integral_constant<int, 3>());
             else go(std::integral_constant<int, G>());
         }
     }
-    if constexpr (ONE) {
-        if (q == 0) s_red[kw][nw][0][c16] = acc[0];
-    } else {
 #pragma unroll
-        for (int g = 0; g < G; ++g) s_red[kw][nw][4 * g + q][c16] = acc[g];
-    }
+    for (int g = 0; g < G; ++g) s_red[kw][nw][4 * g + q][c16] = acc[g];
     __syncthreads();
     // thread: row i and column f (a block of the 8-bit output is 32 lanes)
     for (int i = tid / COLS; i < count; i += NT / COLS) {
@@ -468,30 +451,172 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
 // k that a workgroup's LDS holds of a tile's rows
 #define MF_KC 3584
 
-template <int WT, int U, bool GU, int NW, int KG, bool ONE>
+template <int WT, int U, bool GU, int NW, int KG>
 static void mf_go(MfArgs a, int64_t tiles, int64_t k, hipStream_t st) {
     using T = Mf<WT, U>;
-    constexpr int R = ONE ? 1 : MOE_FEW, COLS = 16 * (GU ? NW / 2 : NW);
+    constexpr int COLS = 16 * (GU ? NW / 2 : NW);
     a.n_cols = (a.rows + COLS - 1) / COLS;
     // all of k, or even parts of it, in whole steps
-    const int64_t steps = (k + T::STEP - 1) / T::STEP, most = (ONE ? 16384 : MF_KC) / T::STEP, parts = (steps + most - 1) / most;
+    const int64_t steps = (k + T::STEP - 1) / T::STEP, most = MF_KC / T::STEP, parts = (steps + most - 1) / most;
     a.kc = (int)((steps + parts - 1) / parts * T::STEP);
-    const MfLds l = mf_lds<T::STEP, T::PER, T::SUMS>(a.kc, R, KG, NW);
-    k_moe_few<WT, U, GU, NW, KG, ONE><<<(unsigned)(tiles * a.n_cols), 64 * NW * KG, l.total, st>>>(a);
+    const MfLds l = mf_lds<T::STEP, T::PER, T::SUMS>(a.kc, MOE_FEW, KG, NW);
+    k_moe_few<WT, U, GU, NW, KG><<<(unsigned)(tiles * a.n_cols), 64 * NW * KG, l.total, st>>>(a);
 }
 template <int WT>
 static void mf_type(const MfArgs& a, int64_t tiles, int64_t k, bool gu, hipStream_t st) {
-    constexpr int U = WT == AMV_T_Q4_0 ? 4 : WT == AMV_T_Q8_0 ? 2 : 1, U1 = WT == AMV_T_Q6_K ? 2 : 4;
-    if (!a.tiles) {
-        if (gu) mf_go<WT, U1, true, 4, 4, true>(a, tiles, k, st);
-        else mf_go<WT, U1, false, 2, 8, true>(a, tiles, k, st);
-    } else if (k <= 2560) {
-        if (gu) mf_go<WT, U, true, 8, 1, false>(a, tiles, k, st);
-        else mf_go<WT, U, false, 8, 1, false>(a, tiles, k, st);
+    constexpr int U = WT == AMV_T_Q4_0 ? 4 : WT == AMV_T_Q8_0 ? 2 : 1;
+    if (k <= 2560) {
+        if (gu) mf_go<WT, U, true, 8, 1>(a, tiles, k, st);
+        else mf_go<WT, U, false, 8, 1>(a, tiles, k, st);
     } else {
-        if (gu) mf_go<WT, U, true, 4, 2, false>(a, tiles, k, st);
-        else mf_go<WT, U, false, 4, 2, false>(a, tiles, k, st);
+        if (gu) mf_go<WT, U, true, 4, 2>(a, tiles, k, st);
+        else mf_go<WT, U, false, 4, 2>(a, tiles, k, st);
     }
+}
+
+// Without a plan (a token by itself): each pair is a product of one row, which a wave's lanes load where they need it, with the weights.
+// Gate and up: a workgroup has 32 columns of a pair, four waves of 16 weight rows on each of four parts of k. Down: a workgroup has 16
+// columns of a token, its waves the token's experts and KP parts of k of each, and adds the weighted products up: no second launch.
+// At one token a launch's latency is half of the time: the chain is ids, weights and row, products, sums.
+struct MoArgs {
+    const uint8_t *w0, *w1;
+    int64_t stride, bytes;
+    int rows, n_k, n_expert, n_used, n_cols, kp;
+    MfAct act;
+    const int32_t* ids;
+    const float *weights, *add;
+    float* out;
+    AmvActOut q;
+};
+
+template <int WT, int U, bool GU>
+__global__ __launch_bounds__(1024) void k_moe_one(const MoArgs p) {
+    using T = Mf<WT, U>;
+    constexpr bool KQ = T::STEP == 256;
+    __shared__ float s_red[GU ? 16 : MOE_MAX_USED][17];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, q = lane >> 4;
+    const int col = blockIdx.x % p.n_cols, of = blockIdx.x / p.n_cols, n0 = col * (GU ? 32 : 16);  // of: pair, or token
+    const int steps = KQ ? p.n_k : (p.n_k + 3) / 4, kp = GU ? 4 : p.kp;
+    const int64_t k = (int64_t)p.n_k * (KQ ? 256 : 32);
+    const bool live = c16 == q;  // (A row b of the row's four: its integers in quarter b)
+    // gate and up: wave = part * 4 + matrix * 2 + 16 columns; down: expert * parts + part, in turns where there are more
+    for (int job = wv; job < (GU ? 16 : p.n_used * kp); job += blockDim.x >> 6) {
+        const int part = GU ? job >> 2 : job % kp, pair = GU ? of : of * p.n_used + job / kp;
+        const int e = p.ids[pair];
+        float acc = 0.0f;
+        if (e >= 0 && e < p.n_expert) {
+            const uint8_t* const m = (GU && (job & 2) ? p.w1 : p.w0) + e * p.stride;
+            const __amdgpu_buffer_rsrc_t buf = MF_RSRC(m, p.bytes);
+            const int n = n0 + (GU ? 16 * (job & 1) : 0) + c16;
+            const int64_t row = GU ? pair / p.n_used : pair;
+            const int8_t* const aq = p.act.q + row * k + (T::AT ? T::AT * q : 128 * (q >> 1) + 16 * (q & 1));
+            const int per = (steps + kp - 1) / kp, s0 = part * per, s1 = min(steps, s0 + per);
+            for (int s = s0; s < s1; s += U) {
+                typename T::W w;
+                T::load(w, buf, m, p.rows, p.n_k, n, q, s);
+                // the row: integers of the lane's own block (zeros in the others, and past k), scales and sums
+                uint4 a[U][8];
+                float4 d[U];
+                int4 u[U];
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    const bool in = s + j < s1 && (KQ || 4 * (s + j) + q < p.n_k);
+                    const uint4* src = reinterpret_cast<const uint4*>(aq + (int64_t)(s + j) * T::STEP);
+#pragma unroll
+                    for (int i = 0; i < (KQ ? 4 : 2); ++i) {
+                        const int at = T::AT ? i : 2 * i;
+                        a[j][at] = make_uint4(0, 0, 0, 0);
+                        if (live && in) a[j][at] = src[at];
+                    }
+                    u[j] = make_int4(0, 0, 0, 0);
+                    if constexpr (KQ) {
+                        const int64_t sb = row * p.n_k + min(s + j, p.n_k - 1);
+                        d[j].x = p.act.dk[sb];
+                        if constexpr (T::SUMS) {
+                            const moe_i4* x = reinterpret_cast<const moe_i4*>(p.act.s16 + sb * 16);
+                            int o[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const moe_i4 v = x[i];
+                                o[i] = (int)((uint32_t)((v.x + v.y) & 0xFFFF) | (uint32_t)(v.z + v.w) << 16);
+                            }
+                            u[j] = make_int4(o[0], o[1], o[2], o[3]);
+                        }
+                    } else {
+                        const float2* x = p.act.d0 + row * p.n_k;
+                        const int b = 4 * (s + j);
+                        d[j] = make_float4(x[min(b, p.n_k - 1)].x, x[min(b + 1, p.n_k - 1)].x, x[min(b + 2, p.n_k - 1)].x, x[min(b + 3, p.n_k - 1)].x);
+                    }
+                }
+                typename T::Scales c;
+                T::scales(w, c, p.n_k, n, q, s);
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    if (s + j >= s1) break;
+                    typename T::B b;
+                    T::operands(w, c, j, b);
+                    acc = T::add(b, reinterpret_cast<const uint8_t*>(a[j]), reinterpret_cast<const float*>(&d[j]),
+                                 reinterpret_cast<const int*>(&u[j]), acc);
+                }
+            }
+        }
+        if (q == 0) s_red[job][c16] = acc;
+    }
+    __syncthreads();
+    if (tid >= (GU ? 32 : 16)) return;
+    const int f = tid;
+    if constexpr (GU) {
+        float v[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int z = 0; z < 4; ++z) v[j] += s_red[4 * z + 2 * j + (f >> 4)][f & 15];
+        const float h = v[0] / (1.0f + expf(-v[0])) * v[1];
+        const int64_t pr = of;
+        if (p.out) p.out[pr * p.rows + n0 + f] = h;
+        if (p.q.type) {
+            const AmvActOut o = amv_act_row(p.q, pr, p.rows);
+            mf_q8_0(h, o.rule, f, o.qs + n0, reinterpret_cast<int2*>(o.meta) + n0 / 32);
+        }
+    } else {
+        const int64_t at = (int64_t)of * p.rows + n0 + f;
+        float v = p.add ? p.add[at] : 0.0f;
+        for (int j = 0; j < p.n_used; ++j) {
+            const int e = p.ids[of * p.n_used + j];
+            if (e < 0 || e >= p.n_expert) continue;
+            float y = 0.0f;
+            for (int z = 0; z < kp; ++z) y += s_red[j * kp + z][f];
+            v = fmaf(p.weights[of * p.n_used + j], y, v);
+        }
+        p.out[at] = v;
+    }
+}
+
+template <int WT>
+static void mo_go(MoArgs a, int64_t n, bool gu, hipStream_t st) {
+    constexpr int U = WT == AMV_T_Q4_0 ? 4 : 2;
+    a.n_cols = a.rows / (gu ? 32 : 16);
+    a.kp = gu ? 4 : std::max(1, 16 / a.n_used);
+    const unsigned grid = (unsigned)(n * a.n_cols);
+    if (gu) k_moe_one<WT, U, true><<<grid, 1024, 0, st>>>(a);
+    else k_moe_one<WT, U, false><<<grid, 64 * std::min(16, a.n_used * a.kp), 0, st>>>(a);
+}
+
+int moe_one(const MoeProduct& p) {
+    const bool kq = p.type == AMV_T_Q4_K || p.type == AMV_T_Q6_K, gu = p.w1 != nullptr;
+    const int8_t* aq = (const int8_t*)p.act;
+    const int8_t* meta = aq + p.act_rows * p.k;
+    const int64_t n = gu ? p.n_tok * p.n_used : p.n_tok;
+    AMV_REQUIRE(n * (p.rows / 16) < (int64_t)1 << 31, "moe: %lld pairs without a plan are too many", (long long)n);
+    const MoArgs a{(const uint8_t*)p.w0, (const uint8_t*)p.w1, p.stride, amv_weight_bytes(p.type, p.rows, p.k), (int)p.rows,
+                   (int)(p.k / (kq ? 256 : 32)), p.n_expert, p.n_used, 0, 0,
+                   {aq, (const float2*)meta, (const float*)meta, (const int32_t*)(meta + p.act_rows * (p.k / 64))}, p.ids, p.weights, p.add,
+                   p.out, p.q};
+    if (p.type == AMV_T_Q4_0) mo_go<AMV_T_Q4_0>(a, n, gu, p.st);
+    else if (p.type == AMV_T_Q8_0) mo_go<AMV_T_Q8_0>(a, n, gu, p.st);
+    else if (p.type == AMV_T_Q4_K) mo_go<AMV_T_Q4_K>(a, n, gu, p.st);
+    else mo_go<AMV_T_Q6_K>(a, n, gu, p.st);
+    return amv_check_launch("amv_moe products");
 }
 
 int moe_few(const MoeProduct& p) {
@@ -502,7 +627,7 @@ int moe_few(const MoeProduct& p) {
     const int8_t* meta = aq + p.act_rows * p.k;
     const MfArgs a{(const uint8_t*)p.w0, (const uint8_t*)p.w1, p.stride, amv_weight_bytes(p.type, p.rows, p.k), (int)p.rows,
                    (int)(p.k / (kq ? 256 : 32)), p.n_expert, gu ? p.n_used : 1, 0, 0,
-                   {aq, (const float2*)meta, (const float*)meta, (const int32_t*)(meta + p.act_rows * (p.k / 64))}, p.ids, v.few, v.order,
+                   {aq, (const float2*)meta, (const float*)meta, (const int32_t*)(meta + p.act_rows * (p.k / 64))}, v.few, v.order,
                    p.out, p.q};
     AMV_REQUIRE((int64_t)v.n_few * (p.rows / 16) < (int64_t)1 << 31, "moe: too many tiles");
     if (p.type == AMV_T_Q4_0) mf_type<AMV_T_Q4_0>(a, v.n_few, p.k, gu, p.st);

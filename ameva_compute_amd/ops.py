@@ -974,10 +974,10 @@ def moe_down(down: QExperts, act: torch.Tensor, plan: MoePlan, weights: torch.Te
     if out is None:
         out = torch.empty((t, n), dtype=torch.float32, device=act.device)
     if t:
-        need = lib().amv_moe_down_workspace_bytes(t, u, n)
-        ws = torch.empty(need, dtype=torch.uint8, device=act.device)
+        need = 0 if plan.buffer is None else lib().amv_moe_down_workspace_bytes(t, u, n)
+        ws = torch.empty(need, dtype=torch.uint8, device=act.device) if need else None
         check(lib().amv_moe_down(down.type, down.ptr, down.stride, down.n_expert, n, down.k, act.data_ptr(), t, u, plan.ids.data_ptr(),
-                                 _ptr(plan.buffer), weights.data_ptr(), _ptr(add), out.data_ptr(), ws.data_ptr(), need, _stream()),
+                                 _ptr(plan.buffer), weights.data_ptr(), _ptr(add), out.data_ptr(), _ptr(ws), need, _stream()),
               "amv_moe_down")
     return out
 

@@ -581,7 +581,7 @@ int amv_moe_gate_up(int wtype, const void* w_gate, const void* w_up, int64_t exp
 /* The experts' down product, summed over a token's experts: dst[t] = add[t] + sum_j weights[t][j] (W h[t * n_used + j]), act the
  * rows h (amv_moe_gate_up's act_out: Q8_0 for Q4_0 / Q8_0 weights, Q8_K for Q4_K / Q6_K), weights f32 [n_tok][n_used], add f32
  * [n_tok][rows] or NULL (may be dst). The sum starts with add and goes in the order of j; pairs without an expert are left out,
- * whatever their weight and row. workspace: amv_moe_down_workspace_bytes bytes, 16-byte aligned. */
+ * whatever their weight and row. workspace: amv_moe_down_workspace_bytes bytes, 16-byte aligned (without a plan none is needed). */
 int64_t amv_moe_down_workspace_bytes(int64_t n_tok, int64_t n_used, int64_t rows);
 int amv_moe_down(int wtype, const void* w, int64_t expert_stride, int64_t n_expert, int64_t rows, int64_t k, const void* act,
                  int64_t n_tok, int64_t n_used, const int32_t* ids, const void* plan, const float* weights, const float* add,
