@@ -3,7 +3,7 @@
 #include "amv_common.h"
 
 // A plan, int32 words: tiles of up to MOE_FEW rows, tiles of up to MOE_MANY rows, then the pairs in the order of their experts
-// (in the order of their numbers within one). A tile is two words: expert | rows << 16, place of its first pair in the order;
+// (those of one in any order: a tile's rows are computed alike, each by itself). A tile is two words: expert | rows << 16, place of its first pair in the order;
 // rows 0: no tile. Pairs without an expert stand last, in tiles of the expert n_expert. n_used >= 1, n_expert <= MOE_MAX_EXPERTS.
 #define MOE_MAX_EXPERTS 1024
 #define MOE_MAX_USED 64

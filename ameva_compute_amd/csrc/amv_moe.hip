@@ -47,7 +47,7 @@ __global__ __launch_bounds__(NT) void k_add_rms_norm(const float* x, const float
     for (int i = 0; i < NT / 64; ++i) tot += s_part[i];
     const float scale = amv_rms_scale(tot, 4 * n4, eps);
     const AmvActOut q = amv_act_row(act, row, 4 * (int64_t)n4);
-    const auto finish = [&](int c, const float4& s, const float4& g) {
+    const auto finish = [&](int c, const float4& s, const float4& g) __attribute__((always_inline)) {
         float y[4] = {s.x * scale, s.y * scale, s.z * scale, s.w * scale};
         if (w) {
             y[0] *= g.x;
@@ -84,7 +84,12 @@ extern "C" int amv_add_rms_norm_act(const float* x, const float* add, int64_t n_
     const AmvActOut q = amv_act_out(act, n, act ? act_type : 0, rule, n_rows);
     const int n4 = (int)(n / 4);
     const dim3 grid((unsigned)n_rows);
+    // few rows: as many threads a row as load it at once; many: the waves of several rows on a CU hide one another's latencies, so fewer
+    // (4096 rows of 4096, us: 1024 threads 71, 256 threads of 4 chunks 68)
     if (n4 <= 256) k_add_rms_norm<256, 1><<<grid, 256, 0, amv_stream(stream)>>>(x, add, n4, eps, w, sum, o, q);
+    else if (n_rows >= 1024 && n4 <= 512) k_add_rms_norm<256, 2><<<grid, 256, 0, amv_stream(stream)>>>(x, add, n4, eps, w, sum, o, q);
+    else if (n_rows >= 1024 && n4 <= 1024) k_add_rms_norm<256, 4><<<grid, 256, 0, amv_stream(stream)>>>(x, add, n4, eps, w, sum, o, q);
+    else if (n4 > 1024 && n4 <= 4096) k_add_rms_norm<1024, 4><<<grid, 1024, 0, amv_stream(stream)>>>(x, add, n4, eps, w, sum, o, q);
     else k_add_rms_norm<1024, 1><<<grid, 1024, 0, amv_stream(stream)>>>(x, add, n4, eps, w, sum, o, q);
     return amv_check_launch("amv_add_rms_norm");
 }
@@ -367,53 +372,69 @@ __global__ __launch_bounds__(1024) void k_moe_plan_one(const int32_t* __restrict
     for (int p = tid; p < pairs; p += 1024) order[atomicAdd(&s_first[s_id[p]], 1)] = p;
 }
 
-// Many pairs: workgroup e reads all of them, counts those of lower experts and its own, and puts its own at their places.
+// Many pairs: workgroup e reads all of them, counts those of lower experts and its own, and puts its own at their places. A lane has
+// 4 consecutive pairs of each of B runs of 256, all loaded at once: 32768 pairs of 128 experts are one round trip (11 us; 23 with 64
+// pairs a load and a ballot for each).
 __global__ __launch_bounds__(1024) void k_moe_plan(const int32_t* __restrict__ ids, int pairs, int n_expert, int2* few, int2* many,
                                                    int32_t* __restrict__ order) {
+    constexpr int B = 8;
     __shared__ int s_low[16], s_own[16];
     const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    // wave w: pairs from w * per on, per a multiple of 64
-    const int per = ((pairs + 15) / 16 + 63) / 64 * 64, p0 = wv * per, p1 = min(pairs, p0 + per);
-    const auto expert = [&](int p) {
-        const int i = p < p1 ? ids[p] : -2;
-        return p >= p1 ? -1 : i >= 0 && i < n_expert ? i : n_expert;
-    };
-    constexpr int B = 8;  // loads at once
-    int low = 0, own = 0;
-    for (int p = p0; p < p1; p += 64 * B) {
-        int i[B];
-#pragma unroll
-        for (int b = 0; b < B; ++b) i[b] = expert(p + 64 * b + lane);
+    // wave w: pairs from w * per on, per a multiple of 256
+    const int per = ((pairs + 15) / 16 + 255) / 256 * 256, p0 = wv * per, p1 = min(pairs, p0 + per);
+    int id[B][4];
+    const auto load = [&](int p) {  // the experts of 256 B pairs from p on, -1 past p1
 #pragma unroll
         for (int b = 0; b < B; ++b) {
-            low += __popcll(__ballot(i[b] >= 0 && i[b] < e));
-            own += __popcll(__ballot(i[b] == e));
+            const int at = p + 256 * b + 4 * lane;
+            moe_i4 v = {0, 0, 0, 0};
+            if (at + 3 < p1) v = *reinterpret_cast<const moe_i4*>(ids + at);
+            else
+#pragma unroll
+                for (int c = 0; c < 4; ++c) v[c] = at + c < p1 ? ids[at + c] : 0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) id[b][c] = at + c >= p1 ? -1 : v[c] >= 0 && v[c] < n_expert ? v[c] : n_expert;
         }
+    };
+    int low = 0, own = 0;
+    for (int p = p0; p < p1; p += 256 * B) {
+        load(p);
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                low += id[b][c] >= 0 && id[b][c] < e;
+                own += id[b][c] == e;
+            }
     }
-    if (lane == 0) {
-        s_low[wv] = low;
-        s_own[wv] = own;
+    int before = own;  // the own pairs of the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(before, o, 64);
+        before += lane >= o ? u : 0;
     }
+    const int wave_low = amv_wave_sum_i_u(low);
+    if (lane == 63) {
+        s_low[wv] = wave_low;
+        s_own[wv] = before;
+    }
+    before -= own;
     __syncthreads();
-    int first = 0, before = 0, count = 0;
+    int first = 0, count = 0;
     for (int j = 0; j < 16; ++j) {
         first += s_low[j];
         before += j < wv ? s_own[j] : 0;
         count += s_own[j];
     }
     int at = first + before;
-    if (own)
-        for (int p = p0; p < p1; p += 64 * B) {
-            int i[B];
+    for (int p = p0; p < p1; p += 256 * B) {
+        if (p1 - p0 > 256 * B) load(p);  // (else they are still here)
 #pragma unroll
-            for (int b = 0; b < B; ++b) i[b] = expert(p + 64 * b + lane);
+        for (int b = 0; b < B; ++b)
 #pragma unroll
-            for (int b = 0; b < B; ++b) {
-                const uint64_t mine = __ballot(i[b] == e);
-                if (i[b] == e) order[at + __popcll(mine & (((uint64_t)1 << lane) - 1))] = p + 64 * b + lane;
-                at += __popcll(mine);
-            }
-        }
+            for (int c = 0; c < 4; ++c)
+                if (id[b][c] == e) order[at++] = p + 256 * b + 4 * lane + c;
+    }
     // places for tiles: enough of them for any counts, the same ones by every workgroup's reckoning
     const auto places = [&](int2* tiles, int rows) {
         const int t0 = first / rows + e, t1 = (first + count) / rows + e + 1, n = (count + rows - 1) / rows;

@@ -148,12 +148,14 @@ def ids_for(g, t, used, n, kind="skewed"):
 SHAPES = [  # tokens, experts, used, rows, k in blocks, kind
     (1, 4, 2, 32, 1, "skewed"), (1, 8, 8, 96, 5, "skewed"), (1, 3, 1, 256, 3, "holes"), (2, 8, 2, 64, 2, "skewed"), (3, 40, 4, 32, 9, "skewed"),
     (6, 5, 3, 288, 4, "holes"), (17, 3, 1, 64, 7, "one"), (40, 16, 2, 160, 6, "holes"), (65, 2, 2, 32, 33, "skewed"), (200, 3, 2, 96, 5, "holes"),
-    (333, 60, 4, 64, 2, "skewed"), (130, 2, 1, 352, 17, "one"), (1100, 7, 4, 32, 1, "holes"), (700, 5, 1, 544, 3, "skewed")]
+    (333, 60, 4, 64, 2, "skewed"), (9, 4, 2, 96, 57, "holes"), (130, 2, 1, 352, 17, "one"), (1100, 7, 4, 32, 1, "holes"), (700, 5, 1, 544, 3, "skewed")]
 
 
 def make(t, shape, seed=0):
     tok, n, used, rows, kb, kind = shape
     k = kb * (32 if t in (Q4_0, Q8_0) else 256)
+    if kb == 57:  # longer than what LDS holds of a tile's rows: parts of it, the last one not whole
+        k = 7264 if t in (Q4_0, Q8_0) else 7424
     g = gen(seed + tok + rows)
     return ids_for(g, tok, used, n, kind), k, g
 
