@@ -1,8 +1,8 @@
-// The experts' products with many rows each (prompts): tiles of 64 or 128 rows (pairs) of one expert on v_mfma_i32_32x32x32_i8, as
+// The experts' products with many rows each (prompts): tiles of 64 rows (pairs) of one expert on v_mfma_i32_32x32x32_i8, as
 // the dense products of amv_qgemm.hip, with the rows gathered through the plan's order and gate and up side by side.
 //
 // Operands: A = rows, B = weight rows; lane l has row l % 32 and 16 bytes l / 32 of a 32-block; result D of lane l: weight row
-// l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4. A workgroup's tile is 64 WM rows x 128 weight rows, a wave's 64 x 32; for gate and up, the
+// l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4. A workgroup's tile is 64 rows x 128 weight rows, a wave's 64 x 32; for gate and up, the
 // waves of weight rows take them in turn, so that 64 columns of both meet in the workgroup. Steps of 128 k go from memory to LDS without
 // registers, one step ahead; the 16-byte pieces of an LDS row are exchanged by an XOR with the row index on the memory side, so that
 // the fragments' reads hit all banks. Rows past the end of a buffer read as zero (the buffers' own range check).
@@ -10,7 +10,6 @@
 // scale (Q4_0, Q8_0; the scale products are one outer product on the matrix core), or multiplied by its unit's scale (K-quants).
 #include "amv_moe.h"
 
-#include <algorithm>
 #include <type_traits>
 
 typedef int mm_v4i __attribute__((ext_vector_type(4)));
@@ -29,6 +28,7 @@ __device__ __forceinline__ void mm_to_lds(__amdgpu_buffer_rsrc_t from, uint4* to
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (mm_lds*)to, 16, off, 0, 0, 0);
 }
 
+#define MM_BM MOE_MANY
 #define MM_BN 128  // weight rows of a workgroup (gate and up: 64 of each)
 
 struct MmArgs {
@@ -48,7 +48,7 @@ struct MmArgs {
 struct MmTile {
     int e, count, n0;  // n0: first weight row (gate and up: of each)
 };
-template <int BM, bool GU>
+template <bool GU>
 __device__ __forceinline__ MmTile mm_tile(const MmArgs& p, int* s_pair) {
     // An XCD (workgroup i runs on XCD i % 8) takes every eighth column tile of all row tiles, so the row tiles of an expert read a column
     // tile's weights from one L2; which column tiles these are turns with the expert, as their number need not be a multiple of eight.
@@ -60,17 +60,16 @@ __device__ __forceinline__ MmTile mm_tile(const MmArgs& p, int* s_pair) {
     const int col = 8 * (j % per) + ((x + m.e) & 7);
     m.count = col < p.n_tw ? t.x >> 16 : 0;
     m.n0 = col * (GU ? MM_BN / 2 : MM_BN);
-    if (m.count && (int)threadIdx.x < BM) s_pair[threadIdx.x] = p.order[t.y + min((int)threadIdx.x, m.count - 1)];
+    if (m.count && (int)threadIdx.x < MM_BM) s_pair[threadIdx.x] = p.order[t.y + min((int)threadIdx.x, m.count - 1)];
     return m;
 }
 
-// The end of a tile. acc[i][r] of wave (wm, wn): row 64 wm + 32 i + 8 (r / 4) + 4 h + r % 4, weight row 32 wn + l % 32.
-// Down: stored as they lie, 32 lanes a row's 32 floats. Gate and up: 32 rows of each 64 at a time through LDS (s: 2 x 32 WM x 68 floats),
+// The end of a tile. acc[i][r] of wave wn: row 32 i + 8 (r / 4) + 4 h + r % 4, weight row 32 wn + l % 32.
+// Down: stored as they lie, 32 lanes a row's 32 floats. Gate and up: 16 rows at a time through LDS (the first A buffer, free by then),
 // where four columns of a row come to a thread: h = silu(g) u, its store and its block's quantization (8 lanes).
-template <int WM, bool GU>
-__device__ __forceinline__ void mm_finish(const MmArgs& p, const MmTile& tile, const int* s_pair, float* s, const mm_f16v (&acc)[2], int wm,
-                                          int wn) {
-    const int lane = threadIdx.x & 63, c32 = lane & 31, h = lane >> 5;
+template <bool GU>
+__device__ __forceinline__ void mm_finish(const MmArgs& p, const MmTile& tile, const int* s_pair, uint4* sA, mm_f16v (&acc)[2], int wn) {
+    const int t = threadIdx.x, lane = t & 63, c32 = lane & 31, h = lane >> 5;
     if constexpr (!GU) {
         const int n = tile.n0 + 32 * wn + c32;
         if (n >= p.rows) return;
@@ -78,23 +77,21 @@ __device__ __forceinline__ void mm_finish(const MmArgs& p, const MmTile& tile, c
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int m = 64 * wm + 32 * i + 8 * (r >> 2) + 4 * h + (r & 3);
+                const int m = 32 * i + 8 * (r >> 2) + 4 * h + (r & 3);
                 if (m < tile.count) p.out[(int64_t)s_pair[m] * p.rows + n] = acc[i][r];
             }
     } else {
-        constexpr int LD = 68, NT = 256 * WM;
-        float* const half = s + (wn & 1) * (32 * WM * LD);
+        float* const s = reinterpret_cast<float*>(sA);  // gate [16][64], up [16][64]
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int q = 0; q < 4; ++q) {
             __syncthreads();
 #pragma unroll
-            for (int r = 0; r < 16; ++r) half[(32 * wm + 8 * (r >> 2) + 4 * h + (r & 3)) * LD + 32 * (wn >> 1) + c32] = acc[i][r];
+            for (int r = 0; r < 8; ++r)
+                s[(wn & 1) * 1024 + (8 * (r >> 2) + 4 * h + (r & 3)) * 64 + 32 * (wn >> 1) + c32] = acc[q >> 1][8 * (q & 1) + r];
             __syncthreads();
-            for (int x = threadIdx.x; x < 32 * WM * 16; x += NT) {
-                const int lr = x >> 4, c = x & 15, m = 64 * (lr >> 5) + 32 * i + (lr & 31), col = tile.n0 + 4 * c;
-                if (m >= tile.count || col >= p.rows) continue;  // (eight lanes at a time: columns come in blocks of 32)
-                const float4 g = *reinterpret_cast<const float4*>(&s[lr * LD + 4 * c]);
-                const float4 u = *reinterpret_cast<const float4*>(&s[32 * WM * LD + lr * LD + 4 * c]);
+            const int lr = t >> 4, c = t & 15, m = 16 * q + lr, col = tile.n0 + 4 * c;
+            if (m < tile.count && col < p.rows) {  // (eight lanes at a time: columns come in blocks of 32)
+                const float4 g = reinterpret_cast<const float4*>(s)[lr * 16 + c], u = reinterpret_cast<const float4*>(s)[256 + lr * 16 + c];
                 const float v[4] = {g.x / (1.0f + expf(-g.x)) * u.x, g.y / (1.0f + expf(-g.y)) * u.y, g.z / (1.0f + expf(-g.z)) * u.z,
                                     g.w / (1.0f + expf(-g.w)) * u.w};
                 const int64_t pr = s_pair[m];
@@ -105,49 +102,51 @@ __device__ __forceinline__ void mm_finish(const MmArgs& p, const MmTile& tile, c
     }
 }
 
-// f with the number of 32-row halves of a wave's 64 rows that hold rows: the second half's products are half the work
-template <int WM, typename F>
+// f with the number of 32-row halves of the tile that hold rows: the second half's products are half the work
+template <typename F>
 __device__ __forceinline__ void mm_halves(const MmTile& tile, F f) {
-    if (WM > 1 || tile.count > 32) f(std::integral_constant<int, 2>());
+    if (tile.count > 32) f(std::integral_constant<int, 2>());
     else f(std::integral_constant<int, 1>());
 }
 
 // pairs without an expert: zeros from gate and up, nothing from down (their rows are left out of the sum)
-template <int WM, bool GU>
-__device__ __forceinline__ void mm_none(const MmArgs& p, const MmTile& tile, const int* s_pair, float* s) {
-    mm_f16v z[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) z[i][r] = 0.0f;
-    const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    if constexpr (GU) mm_finish<WM, GU>(p, tile, s_pair, s, z, wv >> 2, wv & 3);
+template <bool GU>
+__device__ __forceinline__ void mm_none(const MmArgs& p, const MmTile& tile, const int* s_pair) {
+    if constexpr (GU) {
+        const int lane = threadIdx.x & 63;
+        for (int m = threadIdx.x >> 6; m < tile.count; m += blockDim.x >> 6)
+            if (lane < 16 && tile.n0 + 4 * lane < p.rows) {
+                const int64_t pr = s_pair[m];
+                const float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (p.out) *reinterpret_cast<float4*>(p.out + pr * p.rows + tile.n0 + 4 * lane) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (p.q.type) moe_act_store4(amv_act_row(p.q, pr, p.rows), tile.n0 / 4 + lane, v);
+            }
+    }
 }
 
 // byte-wise n - 8 of nibbles n in 0..15 (no carry crosses a byte: n + 0x78 <= 0x87)
 __device__ __forceinline__ uint32_t mm_m8(uint32_t v) { return (v + 0x78787878u) ^ 0x80808080u; }
 
 // ---------------------------------------------------------------------------------------------------------------- Q4_0, Q8_0
-template <int WT, int WM, bool GU>
-__global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) void k_moe_many(const MmArgs p) {
+template <int WT, bool GU>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void k_moe_many(const MmArgs p) {
     constexpr bool Q4 = WT == AMV_T_Q4_0;
-    constexpr int BM = 64 * WM, BN = MM_BN, NT = 256 * WM;
+    constexpr int BM = MM_BM, BN = MM_BN, NT = 256;
     constexpr int WB = Q4 ? 16 : 32, WP = 4 * WB / 16;          // bytes of a weight block, 16-byte pieces of a step's row
     constexpr int RA = BM * 8 / NT, RW = BN * WP / NT;          // rounds of the threads over a step's pieces
     constexpr int RDW = BN * 4 / NT;                            // and over its weight scales (its rows': one)
-    constexpr int LA = BM * 8, LW = BN * WP, LEND = 2 * 32 * WM * 68 / 4;
-    // the buffers of even and odd steps, then (in the same place) what the end of a tile needs
-    __shared__ __align__(16) uint4 sm[(2 * (LA + LW) > LEND || !GU) ? 2 * (LA + LW) : LEND];
+    constexpr int LA = BM * 8, LW = BN * WP;
+    // the buffers of even and odd steps are variables of their own: reads of one do not wait for the loads into the other
+    __shared__ __align__(16) uint4 sAa[LA], sAb[LA], sWa[LW], sWb[LW];
     __shared__ __align__(16) float sDa[2][4 * BM];
     __shared__ __align__(16) uint16_t sDw[2][4 * BN];  // (f16: three workgroups of Q8_0 on a CU)
     __shared__ int s_pair[BM];
-    uint4 *const sAa = sm, *const sAb = sm + LA, *const sWa = sm + 2 * LA, *const sWb = sm + 2 * LA + LW;
-    const MmTile tile = mm_tile<BM, GU>(p, s_pair);
+    const MmTile tile = mm_tile<GU>(p, s_pair);
     if (!tile.count) return;
     __syncthreads();
-    if (tile.e >= p.n_expert) return mm_none<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm));
+    if (tile.e >= p.n_expert) return mm_none<GU>(p, tile, s_pair);
     const int t = threadIdx.x, lane = t & 63, c32 = lane & 31, h = lane >> 5;
-    const int wv = __builtin_amdgcn_readfirstlane(t >> 6), wm = wv >> 2, wn = wv & 3;
+    const int wv = __builtin_amdgcn_readfirstlane(t >> 6), wn = wv;
     const int nb = p.n_k, N = p.rows, nsteps = (nb + 3) / 4;
     const uint32_t K = 32u * nb;
 
@@ -157,8 +156,8 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     const __amdgpu_buffer_rsrc_t ra = MM_RSRC(p.aq, p.act_rows * K), rw0 = MM_RSRC(m0, wbytes), rw1 = MM_RSRC(m1, wbytes);
     // weight row of a tile's row r (past the last one: none, which reads as zero)
     const auto wrow = [&](int r) { return GU ? tile.n0 + 32 * (r >> 6) + (r & 31) : tile.n0 + r; };
-    const bool half_only = WM == 1 && tile.count <= 32;  // (the second round loads the second half's rows)
-    static_assert(RA == 2 && BM * 4 == NT, "a round loads half of the rows");
+    const bool half_only = tile.count <= 32;  // (the second round loads the second half's rows)
+    static_assert(RA == 2, "a round loads half of the rows");
     uint32_t oa[RA], ow[RW];
 #pragma unroll
     for (int i = 0; i < RA; ++i)
@@ -211,13 +210,13 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
-    const int ar = 64 * wm + c32, wr = 32 * wn + c32;
-    const int ax = (c32 >> 1) & 7, wx = Q4 ? (c32 >> 2) & 3 : ax;  // the rows' XOR (64 wm, 32 i, 32 wn do not change them)
+    const int ar = c32, wr = 32 * wn + c32;
+    const int ax = (c32 >> 1) & 7, wx = Q4 ? (c32 >> 2) & 3 : ax;  // the rows' XOR (32 i, 32 wn do not change them)
     const auto compute = [&](auto ni, const uint4* sA, const uint4* sW, int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int bl = 0; bl < 4; ++bl) {
             const mm_f32v zero = {};
-            const mm_f32v o = __builtin_amdgcn_mfma_f32_32x32x1f32(sDa[buf][bl * BM + 64 * wm + lane], amv_h2f(sDw[buf][bl * BN + wr]), zero, 0, 0, 0);
+            const mm_f32v o = __builtin_amdgcn_mfma_f32_32x32x1f32(sDa[buf][bl * BM + lane], amv_h2f(sDw[buf][bl * BN + wr]), zero, 0, 0, 0);
             mm_v4i B;
             if constexpr (Q4) {  // element e < 16: low nibble of byte e (lane half 0); 16 + e: its high nibble (half 1)
                 const uint4 x = sW[wr * 4 + (bl ^ wx)];
@@ -271,8 +270,8 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
             __syncthreads();
         }
     };
-    mm_halves<WM>(tile, steps);
-    mm_finish<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm), acc, wm, wn);
+    mm_halves(tile, steps);
+    mm_finish<GU>(p, tile, s_pair, sAa, acc, wn);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- Q4_K
@@ -282,24 +281,24 @@ __device__ __forceinline__ uint32_t mm_h2bits(int a, int b) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(float)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(float)b) << 16);
 }
 
-template <int WM, bool GU>
-__global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) void k_moe_many_q4k(const MmArgs p) {
-    constexpr int BM = 64 * WM, BN = MM_BN, NT = 256 * WM;
+template <bool GU>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void k_moe_many_q4k(const MmArgs p) {
+    constexpr int BM = MM_BM, BN = MM_BN, NT = 256;
     constexpr int RA = BM * 8 / NT, RW = BN * 4 / NT;
-    constexpr int LA = BM * 8, LW = BN * 4, LEND = 2 * 32 * WM * 68 / 4;
-    __shared__ __align__(16) uint4 sm[(2 * (LA + LW) > LEND || !GU) ? 2 * (LA + LW) : LEND];
+    constexpr int LA = BM * 8, LW = BN * 4;
+    // the buffers of even and odd steps are variables of their own: reads of one do not wait for the loads into the other
+    __shared__ __align__(16) uint4 sAa[LA], sAb[LA], sWa[LW], sWb[LW];
     __shared__ __align__(16) uint4 sHd[BN];
     __shared__ __align__(16) uint2 sBs[BM * 4];
     __shared__ __align__(16) float sDa[BM];
     __shared__ int s_pair[BM];
-    uint4 *const sAa = sm, *const sAb = sm + LA, *const sWa = sm + 2 * LA, *const sWb = sm + 2 * LA + LW;
-    const MmTile tile = mm_tile<BM, GU>(p, s_pair);
+    const MmTile tile = mm_tile<GU>(p, s_pair);
     if (!tile.count) return;
     __syncthreads();
-    if (tile.e >= p.n_expert) return mm_none<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm));
+    if (tile.e >= p.n_expert) return mm_none<GU>(p, tile, s_pair);
     const int t = threadIdx.x, lane = t & 63, c32 = lane & 31, h = lane >> 5;
-    const int wv = __builtin_amdgcn_readfirstlane(t >> 6), wm = wv >> 2, wn = wv & 3;
-    const int nsb = p.n_k, N = p.rows;
+    const int wv = __builtin_amdgcn_readfirstlane(t >> 6), wn = wv;
+    const int nsb = p.n_k, N = p.rows, j_last = nsb - 1;
     const uint32_t K = 256u * nsb;
 
     const uint8_t* const m0 = p.w0 + tile.e * p.stride;
@@ -309,8 +308,8 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     const __amdgpu_buffer_rsrc_t rw0 = MM_RSRC(m0, wbytes), rw1 = MM_RSRC(m1, wbytes);
     const __amdgpu_buffer_rsrc_t rh0 = MM_RSRC(m0 + wbytes, N * nsb * 16);
     const auto wrow = [&](int r) { return GU ? tile.n0 + 32 * (r >> 6) + (r & 31) : tile.n0 + r; };
-    const bool half_only = WM == 1 && tile.count <= 32;  // (the second round loads the second half's rows)
-    static_assert(RA == 2 && BM * 4 == NT, "a round loads half of the rows");
+    const bool half_only = tile.count <= 32;  // (the second round loads the second half's rows)
+    static_assert(RA == 2, "a round loads half of the rows");
     uint32_t oa[RA], ow[RW];
 #pragma unroll
     for (int i = 0; i < RA; ++i)
@@ -343,13 +342,13 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
         }
     };
     // activation sums (thread: row t / 4, 4 of the 16) and scale of super-block j, through registers
-    const moe_i4* const ps = reinterpret_cast<const moe_i4*>(p.meta + p.act_rows * nsb * 4) + (int64_t)(s_pair[t >> 2] / p.act_div) * nsb * 4 + (t & 3);
-    const float* const pd = reinterpret_cast<const float*>(p.meta) + (int64_t)(s_pair[min(t, BM - 1)] / p.act_div) * nsb;
+    const uint8_t* const sums = p.meta + p.act_rows * nsb * 4;
+    const uint32_t os = (uint32_t)(s_pair[t >> 2] / p.act_div) * (nsb * 64) + 16 * (t & 3), od = (uint32_t)(s_pair[min(t, BM - 1)] / p.act_div) * (nsb * 4);
     moe_i4 bs;
     float da0;
     const auto load_sb = [&](int j) {
-        bs = ps[4 * j];
-        da0 = pd[j];
+        bs = *reinterpret_cast<const moe_i4*>(sums + (os + 64u * j));
+        da0 = *reinterpret_cast<const float*>(p.meta + (od + 4u * j));
     };
     const auto store_sb = [&]() {
         sBs[t] = make_uint2(mm_h2bits(bs.x, bs.y), mm_h2bits(bs.z, bs.w));
@@ -362,7 +361,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
-    const int ar = 64 * wm + c32, wr = 32 * wn + c32;
+    const int ar = c32, wr = 32 * wn + c32;
     const int ax = (c32 >> 1) & 7, wx = (c32 >> 2) & 3;
     const auto half_step = [&](auto ni, const uint4* sA, const uint4* sW, uint32_t scw, bool first) __attribute__((always_inline)) {
 #pragma unroll
@@ -390,13 +389,13 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
 
     load_head(0);
     load(sAa, sWa, 0, 0);
-    load_sb(0);
     MM_WAIT_LOADS();
     __syncthreads();
     const auto steps = [&](auto ni) __attribute__((always_inline)) {
         for (int j = 0; j < nsb; ++j) {
-            const int jn = min(j + 1, nsb - 1);
+            const int jn = min(j + 1, j_last);
             load(sAb, sWb, j, 1);
+            load_sb(j);
             const uint4 hd = sHd[wr];
             // scales and mins of units 0-3 and 4-7, one per byte
             const uint32_t sc0 = hd.y & 0x3F3F3F3Fu, sc1 = (hd.w & 0x0F0F0F0Fu) | ((hd.y >> 2) & 0x30303030u);
@@ -407,13 +406,12 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
             __syncthreads();
             load(sAa, sWa, jn, 0);
             load_head(jn);
-            load_sb(jn);
             half_step(ni, sAb, sWb, sc1, false);
             // the mins, each on its unit's two 16-sum slots, against the sums
             mm_h8 Bmn;
             {
                 const uint32_t off = 0xE400E400u;  // -1024, -1024: 0x6400 | m is the f16 1024 + m
-    #pragma unroll
+#pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t q = __builtin_amdgcn_perm(0x64646464u, mw, 0x04000400u + 0x00010001u * e);
                     const mm_h2 v = __builtin_bit_cast(mm_h2, q) + __builtin_bit_cast(mm_h2, off);
@@ -422,17 +420,17 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
                 }
             }
             const float d = amv_h2f(hd.x), dm = amv_h2f(hd.x >> 16);
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < decltype(ni)::value; ++i) {
-                const int tl = 64 * wm + 32 * i;
+                const int tl = 32 * i;
                 const mm_h8 Abs = *reinterpret_cast<const mm_h8*>(&sBs[(tl + c32) * 4 + 2 * h]);
                 const mm_f16v zf = {};
                 const mm_f16v I2 = __builtin_amdgcn_mfma_f32_32x32x16_f16(Abs, Bmn, zf, 0, 0, 0);
-    #pragma unroll
+#pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const float4 v = *reinterpret_cast<const float4*>(&sDa[tl + 4 * h + 8 * q]);
                     const float da[4] = {v.x, v.y, v.z, v.w};
-    #pragma unroll
+#pragma unroll
                     for (int r = 0; r < 4; ++r)
                         acc[i][4 * q + r] = fmaf(fmaf(d, (float)I1[i][4 * q + r], -(dm * I2[4 * q + r])), da[r], acc[i][4 * q + r]);
                 }
@@ -441,31 +439,31 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(4))) v
             __syncthreads();
         }
     };
-    mm_halves<WM>(tile, steps);
-    mm_finish<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm), acc, wm, wn);
+    mm_halves(tile, steps);
+    mm_finish<GU>(p, tile, s_pair, sAa, acc, wn);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- Q6_K
 // Steps of half a super-block: elements 128 n + {l, 32 + l, 64 + l, 96 + l} (l < 32) from the low nibbles of ql[l], ql[32 + l], then the
 // high ones, with bits 0-1, 2-3, 4-5, 6-7 of qh[l]; sub-blocks of 16 have scales of their own, so the matrix core takes 16 k at a time
 // (v_mfma_i32_32x32x16_i8, lane half h the bytes 8 h .. 8 h + 7 of a sub-block).
-template <int WM, bool GU>
-__global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 1 ? 3 : 4))) void k_moe_many_q6k(const MmArgs p) {
-    constexpr int BM = 64 * WM, BN = MM_BN, NT = 256 * WM;
+template <bool GU>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k_moe_many_q6k(const MmArgs p) {
+    constexpr int BM = MM_BM, BN = MM_BN, NT = 256;
     constexpr int RA = BM * 8 / NT, RW = BN * 4 / NT;
-    constexpr int LA = BM * 8, LW = BN * 4, LH = BN * 2, LEND = 2 * 32 * WM * 68 / 4;
-    __shared__ __align__(16) uint4 sm[(2 * (LA + LW + LH) > LEND || !GU) ? 2 * (LA + LW + LH) : LEND];
+    constexpr int LA = BM * 8, LW = BN * 4, LH = BN * 2;
+    // the buffers of even and odd steps are variables of their own: reads of one do not wait for the loads into the other
+    __shared__ __align__(16) uint4 sAa[LA], sAb[LA], sWa[LW], sWb[LW], sHa[LH], sHb[LH];
     __shared__ __align__(16) uint4 sSc[2][BN];
     __shared__ __align__(16) float sD[2][BN], sDa[2][BM];
     __shared__ int s_pair[BM];
-    const MmTile tile = mm_tile<BM, GU>(p, s_pair);
+    const MmTile tile = mm_tile<GU>(p, s_pair);
     if (!tile.count) return;
     __syncthreads();
-    if (tile.e >= p.n_expert) return mm_none<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm));
-    uint4 *const sAa = sm, *const sAb = sm + LA, *const sWa = sm + 2 * LA, *const sWb = sWa + LW, *const sHa = sWb + LW, *const sHb = sHa + LH;
+    if (tile.e >= p.n_expert) return mm_none<GU>(p, tile, s_pair);
     const int t = threadIdx.x, lane = t & 63, c32 = lane & 31, h = lane >> 5;
-    const int wv = __builtin_amdgcn_readfirstlane(t >> 6), wm = wv >> 2, wn = wv & 3;
-    const int nsb = p.n_k, N = p.rows;
+    const int wv = __builtin_amdgcn_readfirstlane(t >> 6), wn = wv;
+    const int nsb = p.n_k, N = p.rows, j_last = nsb - 1;
     const uint32_t K = 256u * nsb;
 
     const uint8_t* const m0 = p.w0 + tile.e * p.stride;
@@ -475,8 +473,8 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 
     const __amdgpu_buffer_rsrc_t rw0 = MM_RSRC(m0, nblk * 128), rw1 = MM_RSRC(m1, nblk * 128);
     const __amdgpu_buffer_rsrc_t rq0 = MM_RSRC(m0 + nblk * 128, nblk * 64), rq1 = MM_RSRC(m1 + nblk * 128, nblk * 64);
     const auto wrow = [&](int r) { return GU ? tile.n0 + 32 * (r >> 6) + (r & 31) : tile.n0 + r; };
-    const bool half_only = WM == 1 && tile.count <= 32;  // (the second round loads the second half's rows)
-    static_assert(RA == 2 && BM * 4 == NT, "a round loads half of the rows");
+    const bool half_only = tile.count <= 32;  // (the second round loads the second half's rows)
+    static_assert(RA == 2, "a round loads half of the rows");
     uint32_t oa[RA], ow[RW];
 #pragma unroll
     for (int i = 0; i < RA; ++i)
@@ -536,7 +534,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 
             acc[i][r] = 0.0f;
             I[i][r] = 0;
         }
-    const int ar = 64 * wm + c32, wr = 32 * wn + c32;
+    const int ar = c32, wr = 32 * wn + c32;
     const int ax = (c32 >> 1) & 7, wx = (c32 >> 2) & 3, hx = (c32 >> 2) & 1;
     // sw: the half's eight scales (bytes 2 e + pp: sub-block of elements 32 e + 16 pp ..)
     const auto half_step = [&](auto ni, const uint4* sA, const uint4* sW, const uint4* sH, uint32_t s0, uint32_t s1) __attribute__((always_inline)) {
@@ -575,7 +573,7 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 
     __syncthreads();
     const auto steps = [&](auto ni) __attribute__((always_inline)) {
         for (int j = 0; j < nsb; ++j) {
-            const int jn = min(j + 1, nsb - 1), buf = j & 1;
+            const int jn = min(j + 1, j_last), buf = j & 1;
             load(sAb, sWb, sHb, j, 1);
             load_sb(jn);
             const uint4 sc = sSc[buf][wr];
@@ -586,13 +584,13 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 
             load(sAa, sWa, sHa, jn, 0);
             half_step(ni, sAb, sWb, sHb, sc.z, sc.w);
             const float d = sD[buf][wr];
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < decltype(ni)::value; ++i)
-    #pragma unroll
+#pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const float4 v = *reinterpret_cast<const float4*>(&sDa[buf][64 * wm + 32 * i + 4 * h + 8 * q]);
+                    const float4 v = *reinterpret_cast<const float4*>(&sDa[buf][32 * i + 4 * h + 8 * q]);
                     const float da[4] = {v.x, v.y, v.z, v.w};
-    #pragma unroll
+#pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         acc[i][4 * q + r] = fmaf(d * da[r], (float)I[i][4 * q + r], acc[i][4 * q + r]);
                         I[i][4 * q + r] = 0;
@@ -602,8 +600,8 @@ __global__ __launch_bounds__(256 * WM) __attribute__((amdgpu_waves_per_eu(WM == 
             __syncthreads();
         }
     };
-    mm_halves<WM>(tile, steps);
-    mm_finish<WM, GU>(p, tile, s_pair, reinterpret_cast<float*>(sm), acc, wm, wn);
+    mm_halves(tile, steps);
+    mm_finish<GU>(p, tile, s_pair, sAa, acc, wn);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -618,16 +616,11 @@ int moe_many(const MoeProduct& p) {
     const int64_t wgs = (int64_t)((a.n_tw + 7) / 8 * 8) * v.n_many;
     AMV_REQUIRE(wgs < (int64_t)1 << 31, "moe: too many tiles");
     const unsigned grid = (unsigned)wgs;
-    constexpr int WM = MOE_MANY / 64;
-#define GO(KERNEL) hipLaunchKernelGGL((gu ? KERNEL(true) : KERNEL(false)), dim3(grid), dim3(256 * WM), 0, p.st, a)
-#define K40(G) k_moe_many<AMV_T_Q4_0, WM, G>
-#define K80(G) k_moe_many<AMV_T_Q8_0, WM, G>
-#define K4K(G) k_moe_many_q4k<WM, G>
-#define K6K(G) k_moe_many_q6k<WM, G>
-    if (p.type == AMV_T_Q4_0) GO(K40);
-    else if (p.type == AMV_T_Q8_0) GO(K80);
-    else if (p.type == AMV_T_Q4_K) GO(K4K);
-    else GO(K6K);
+#define GO(GATE_UP, DOWN) hipLaunchKernelGGL((gu ? GATE_UP : DOWN), dim3(grid), dim3(256), 0, p.st, a)
+    if (p.type == AMV_T_Q4_0) GO((k_moe_many<AMV_T_Q4_0, true>), (k_moe_many<AMV_T_Q4_0, false>));
+    else if (p.type == AMV_T_Q8_0) GO((k_moe_many<AMV_T_Q8_0, true>), (k_moe_many<AMV_T_Q8_0, false>));
+    else if (p.type == AMV_T_Q4_K) GO(k_moe_many_q4k<true>, k_moe_many_q4k<false>);
+    else GO(k_moe_many_q6k<true>, k_moe_many_q6k<false>);
 #undef GO
     return amv_check_launch("amv_moe products");
 }
