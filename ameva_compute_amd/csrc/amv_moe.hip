@@ -72,7 +72,7 @@ __global__ __launch_bounds__(NT) void k_add_rms_norm(const float* x, const float
 extern "C" int amv_add_rms_norm_act(const float* x, const float* add, int64_t n_rows, int64_t n, float eps, const float* w,
                                     float* sum, float* o, void* act, int act_type, int rule, void* stream) {
     AMV_REQUIRE(x && add && sum, "amv_add_rms_norm: null input or sum");
-    AMV_REQUIRE(n_rows >= 0 && n > 0 && n_rows <= INT32_MAX && n <= 1 << 24, "amv_add_rms_norm: bad shape");
+    AMV_REQUIRE(n_rows >= 0 && n > 0 && n_rows < 1 << 22 && n <= 1 << 24, "amv_add_rms_norm: bad shape");
     AMV_REQUIRE(n % 4 == 0, "amv_add_rms_norm: n %% 4 != 0");
     AMV_REQUIRE((((uintptr_t)x | (uintptr_t)add | (uintptr_t)w | (uintptr_t)sum | (uintptr_t)o | (uintptr_t)act) & 15) == 0,
                 "amv_add_rms_norm: buffers must be 16-byte aligned");
@@ -113,7 +113,7 @@ extern "C" int amv_act_values(int act_type, const void* act, int64_t m, int64_t 
     AMV_REQUIRE(act_type == AMV_T_Q8_0 || act_type == AMV_T_Q8_K, "amv_act_values: type %d (Q8_0 or Q8_K)", act_type);
     const bool kq = act_type == AMV_T_Q8_K;
     AMV_REQUIRE(m >= 0 && k > 0 && k % (kq ? 256 : 32) == 0 && k <= INT32_MAX && m <= INT32_MAX, "amv_act_values: bad shape");
-    AMV_REQUIRE(m * k / 1024 < INT32_MAX, "amv_act_values: too many values");
+    AMV_REQUIRE(m * k < (int64_t)1 << 34, "amv_act_values: too many values");
     AMV_REQUIRE(out_type == AMV_T_F32 || out_type == AMV_T_F16, "amv_act_values: output type %d (F32 or F16)", out_type);
     AMV_REQUIRE((((uintptr_t)act | (uintptr_t)out) & 7) == 0, "amv_act_values: buffers must be 8-byte aligned");
     if (!m) return AMV_OK;
@@ -290,7 +290,7 @@ extern "C" int amv_moe_route(const float* logits, int64_t logits_stride, int64_t
                 (long long)n_tok, (long long)n_expert, MOE_MAX_EXPERTS);
     AMV_REQUIRE(n_used > 0 && n_used <= MOE_MAX_USED && n_used <= n_expert, "amv_moe_route: %lld of %lld experts a token (up to %d)",
                 (long long)n_used, (long long)n_expert, MOE_MAX_USED);
-    AMV_REQUIRE(n_tok * n_used <= MOE_MAX_PAIRS, "amv_moe_route: more than %d pairs", MOE_MAX_PAIRS);
+    AMV_REQUIRE(n_tok <= MOE_MAX_PAIRS / n_used, "amv_moe_route: more than %d pairs", MOE_MAX_PAIRS);
     AMV_REQUIRE(logits_stride >= n_expert || n_tok <= 1, "amv_moe_route: row stride < n_expert");
     AMV_REQUIRE(score == AMV_MOE_SOFTMAX || score == AMV_MOE_SIGMOID, "amv_moe_route: score %d", score);
     AMV_REQUIRE(n_group > 0 && n_group <= 64 && n_expert % n_group == 0 && top_group > 0 && top_group <= n_group,
@@ -488,15 +488,16 @@ __global__ __launch_bounds__(256) void k_moe_quantize(const float4* __restrict__
 
 // Tiles of many rows from so many rows an expert on that their products beside the weights' bytes cost less than the few rows' kernel,
 // which does four times the matrix work; later where the tiles are too few to fill the GPU (us, few / many, at the rows an expert below
-// and above the choice): 64 experts of gate and up 1024 x 2048 Q4_0 12: 57 / 59, 24: 81 / 74; Q8_0 6: 68 / 74, 12: 84 / 79; Q4_K 6: 47 /
-// 49, 12: 60 / 56; Q6_K 12: 75 / 88, 24: 103 / 97; down 2048 x 1024 Q4_0 12: 36 / 40, 24: 46 / 45; Q8_0 6: 43 / 43, 12: 54 / 47; Q4_K 6: 27 /
-// 30, 12: 39 / 36; Q6_K 12: 49 / 51, 24: 60 / 56; 8 experts of 4096 x 6144 Q4_0 24: 68 / 89, 48: 115 / 96; Q8_0 16: 85 / 93, 32: 123 / 102;
-// Q4_K 24: 67 / 80, 32: 87 / 82; Q6_K 24: 85 / 111, 48: 137 / 115; of 4096 x 14336 Q6_K 24: 188 / 244, 48: 300 / 252
+// and above the choice): 64 experts of gate and up 1024 x 2048 Q4_0 8: 50 / 51, 16: 65 / 60; Q8_0 4: 61 / 66, 8: 75 / 71; Q4_K 4: 44 / 46,
+// 8: 54 / 50; Q6_K 8: 67 / 74, 16: 83 / 82; down 2048 x 1024 Q4_0 6: 28 / 30, 12: 36 / 33; Q8_0 4: 38 / 38, 8: 45 / 40; Q4_K 4: 25 / 26,
+// 6: 28 / 25; Q6_K 8: 40 / 42, 12: 44 / 43; 8 experts of 4096 x 6144 Q4_0 24: 68 / 75, 32: 87 / 78; Q8_0 8: 65 / 64, 16: 85 / 79; Q4_K 8:
+// 43 / 45, 24: 67 / 60; Q6_K 8: 57 / 62, 16: 78 / 74; of gate and up 2048 x 4096 Q4_K 16: 38 / 43, 32: 59 / 51; of 4096 x 14336 Q6_K 8:
+// 126 / 136, 16: 168 / 160
 static int moe_product(const MoeProduct& p) {
     if (!p.plan) return moe_one(p);
     const int64_t wgs = p.n_expert * ((p.rows + (p.w1 ? 63 : 127)) / (p.w1 ? 64 : 128));
-    const int rows = p.type == AMV_T_Q4_0 ? (wgs >= 512 ? 16 : 32) : p.type == AMV_T_Q8_0 ? (wgs >= 512 ? 8 : 24)
-                     : p.type == AMV_T_Q4_K ? (wgs >= 512 ? 8 : 28) : (wgs >= 512 ? 14 : 32);
+    const int rows = p.type == AMV_T_Q4_0 ? (wgs >= 512 ? 10 : 28) : p.type == AMV_T_Q8_0 ? (wgs >= 512 ? 6 : 8)
+                     : p.type == AMV_T_Q4_K ? (wgs >= 512 ? 5 : 20) : (wgs >= 512 ? 12 : 16);
     const bool many = p.n_tok * p.n_used >= (int64_t)rows * p.n_expert;
     return many ? moe_many(p) : moe_few(p);
 }

@@ -607,7 +607,8 @@ int moe_one(const MoeProduct& p) {
     const int8_t* aq = (const int8_t*)p.act;
     const int8_t* meta = aq + p.act_rows * p.k;
     const int64_t n = gu ? p.n_tok * p.n_used : p.n_tok;
-    AMV_REQUIRE(n * (p.rows / 16) < (int64_t)1 << 31, "moe: %lld pairs without a plan are too many", (long long)n);
+    AMV_REQUIRE(p.n_tok * p.n_used * p.rows < 1 << 26, "moe: %lld pairs of %lld without a plan are too many", (long long)(p.n_tok * p.n_used),
+                (long long)p.rows);
     const MoArgs a{(const uint8_t*)p.w0, (const uint8_t*)p.w1, p.stride, amv_weight_bytes(p.type, p.rows, p.k), (int)p.rows,
                    (int)(p.k / (kq ? 256 : 32)), p.n_expert, p.n_used, 0, 0,
                    {aq, (const float2*)meta, (const float*)meta, (const int32_t*)(meta + p.act_rows * (p.k / 64))}, p.ids, p.weights, p.add,
@@ -629,7 +630,7 @@ int moe_few(const MoeProduct& p) {
                    (int)(p.k / (kq ? 256 : 32)), p.n_expert, gu ? p.n_used : 1, 0, 0,
                    {aq, (const float2*)meta, (const float*)meta, (const int32_t*)(meta + p.act_rows * (p.k / 64))}, v.few, v.order,
                    p.out, p.q};
-    AMV_REQUIRE((int64_t)v.n_few * (p.rows / 16) < (int64_t)1 << 31, "moe: too many tiles");
+    AMV_REQUIRE((int64_t)v.n_few * ((p.rows + 31) / 32) < 1 << 23, "moe: %d tiles of %lld columns are too many", v.n_few, (long long)p.rows);
     if (p.type == AMV_T_Q4_0) mf_type<AMV_T_Q4_0>(a, v.n_few, p.k, gu, p.st);
     else if (p.type == AMV_T_Q8_0) mf_type<AMV_T_Q8_0>(a, v.n_few, p.k, gu, p.st);
     else if (p.type == AMV_T_Q4_K) mf_type<AMV_T_Q4_K>(a, v.n_few, p.k, gu, p.st);

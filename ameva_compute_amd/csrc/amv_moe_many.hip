@@ -614,7 +614,7 @@ int moe_many(const MoeProduct& p) {
              0, aq, (const uint8_t*)aq + p.act_rows * p.k, p.act_rows, v.many, v.order, p.out, p.q};
     a.n_tw = (int)((p.rows + (gu ? MM_BN / 2 : MM_BN) - 1) / (gu ? MM_BN / 2 : MM_BN));
     const int64_t wgs = (int64_t)((a.n_tw + 7) / 8 * 8) * v.n_many;
-    AMV_REQUIRE(wgs < (int64_t)1 << 31, "moe: too many tiles");
+    AMV_REQUIRE(wgs < 1 << 24, "moe: %d tiles of %lld columns are too many", v.n_many, (long long)p.rows);
     const unsigned grid = (unsigned)wgs;
 #define GO(GATE_UP, DOWN) hipLaunchKernelGGL((gu ? GATE_UP : DOWN), dim3(grid), dim3(256), 0, p.st, a)
     if (p.type == AMV_T_Q4_0) GO((k_moe_many<AMV_T_Q4_0, true>), (k_moe_many<AMV_T_Q4_0, false>));

@@ -541,12 +541,12 @@ int amv_paged_attn_sparse(const amv_paged_kv* kv, const amv_paged_batch* batch, 
  * ---------------------------------------------------------------------------------------------------------- */
 /* sum = x + add, then amv_rms_norm_act of sum in the same pass: o = sum / sqrt(mean(sum^2) + eps) * w (w may be NULL: without the
  * factor), act (may be NULL) = o in 8 bits, act_type 8 = Q8_0 (`rule`) or 15 = Q8_K. x, add, sum, o f32 [n_rows][n] (o may be NULL;
- * sum may be x or add), w f32 [n]; n % 4 == 0, 16-byte aligned. A block of act with an element that is infinite or no number gets a
+ * sum may be x or add), w f32 [n]; n % 4 == 0, 16-byte aligned, n_rows less than 2^22. A block of act with an element that is infinite or no number gets a
  * scale that is none. */
 int amv_add_rms_norm_act(const float* x, const float* add, int64_t n_rows, int64_t n, float eps, const float* w, float* sum,
                          float* o, void* act, int act_type, int rule, void* stream);
 /* The values that an activation buffer of amv_quantize_act's layout (act_type Q8_0 or Q8_K, m rows of k) stands for: out [m][k],
- * out_type 0 = F32 or 1 = F16. */
+ * out_type 0 = F32 or 1 = F16; less than 2^34 values. */
 int amv_act_values(int act_type, const void* act, int64_t m, int64_t k, int out_type, void* out, void* stream);
 
 /* The experts of each token and their weights, from the router's logits f32 [n_tok][n_expert] (rows logits_stride floats
@@ -572,8 +572,8 @@ int amv_moe_plan(const int32_t* ids, int64_t n_tok, int64_t n_used, int64_t n_ex
  * amv_mul_mat_q). eout f32 [pairs][rows] and act_out, h in 8 bits (act_type 8 = Q8_0 with `rule`, or 15 = Q8_K for rows % 256 == 0; the
  * layout of `pairs` rows of `rows`): either may be NULL. Pairs without an expert get zeros; a block with an element that is
  * infinite or no number gets a scale that is none. plan: amv_moe_plan's of the same ids, n_used and n_expert, or NULL: each pair is
- * then a product by itself (a single token; at most 65535 pairs). workspace: amv_moe_gate_up_workspace_bytes bytes (0: may be
- * NULL), 16-byte aligned. */
+ * then a product by itself (a single token; pairs * rows less than 2^26). workspace: amv_moe_gate_up_workspace_bytes bytes (0: may be
+ * NULL), 16-byte aligned. Outputs and workspaces overlap neither each other nor an input, here and below, but where it says so. */
 int64_t amv_moe_gate_up_workspace_bytes(int64_t n_tok, int64_t n_used, int64_t rows, int act_type);
 int amv_moe_gate_up(int wtype, const void* w_gate, const void* w_up, int64_t expert_stride, int64_t n_expert, int64_t rows,
                     int64_t k, const void* act, int64_t n_tok, int64_t n_used, const int32_t* ids, const void* plan, float* eout,

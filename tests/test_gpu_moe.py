@@ -148,7 +148,9 @@ def ids_for(g, t, used, n, kind="skewed"):
 SHAPES = [  # tokens, experts, used, rows, k in blocks, kind
     (1, 4, 2, 32, 1, "skewed"), (1, 8, 8, 96, 5, "skewed"), (1, 3, 1, 256, 3, "holes"), (2, 8, 2, 64, 2, "skewed"), (3, 40, 4, 32, 9, "skewed"),
     (6, 5, 3, 288, 4, "holes"), (17, 3, 1, 64, 7, "one"), (40, 16, 2, 160, 6, "holes"), (65, 2, 2, 32, 33, "skewed"), (200, 3, 2, 96, 5, "holes"),
-    (333, 60, 4, 64, 2, "skewed"), (9, 4, 2, 96, 57, "holes"), (130, 2, 1, 352, 17, "one"), (1100, 7, 4, 32, 1, "holes"), (700, 5, 1, 544, 3, "skewed")]
+    (333, 60, 4, 64, 2, "skewed"), (9, 4, 2, 96, 57, "holes"), (130, 2, 1, 352, 17, "one"), (1100, 7, 4, 32, 1, "holes"), (700, 5, 1, 544, 3, "skewed"),
+    # more experts a token than a workgroup has waves; a plan of more than 4096 pairs with few of them an expert
+    (1, 70, 20, 64, 3, "skewed"), (1, 64, 64, 32, 6, "skewed"), (3, 70, 64, 32, 2, "skewed"), (700, 1024, 8, 32, 1, "holes")]
 
 
 def make(t, shape, seed=0):
@@ -212,6 +214,32 @@ def test_down(t, shape):
     assert torch.equal(out[gone], add[gone])
     again = add.clone()
     assert ops.moe_down(down.gpu, act, plan, weights, add=again, out=again) is again and torch.equal(again, out)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_tokens_without_a_plan(t):
+    """Several tokens through the products that need no plan (the C entries' plan NULL), as bounded as with one."""
+    from ameva_compute_amd import ops
+    shape = (7, 9, 3, 64, 5, "holes")
+    tok, n, used, rows, _, _ = shape
+    ids, k, g = make(t, shape, 3)
+    gate, up, down = Experts(t, n, rows, k, 1), Experts(t, n, rows, k, 2), Experts(t, n, rows, k, 3)
+    act = ops.quantize_act(torch.randn(tok, k, generator=g, device=DEV), ACT[t])[0]
+    a = ops.act_values(act, ACT[t], tok, k, torch.float32).double().repeat_interleave(used, 0)
+    flat, plan = ids.flatten(), ops.MoePlan(ids, n, None)
+    (yg, sg), (yu, su) = product(a, gate, flat), product(a, up, flat)
+    ref = yg * torch.sigmoid(yg) * yu
+    h = ops.moe_gate_up(gate.gpu, up.gpu, act, plan, act_type=None)
+    # as in test_gate_up and test_down
+    lim = rounding(gate) * (1.1 * sg * yu.abs() + (yg * torch.sigmoid(yg)).abs() * su + 1.1 * sg * su * rounding(gate)) + 8 * 2.0 ** -24 * ref.abs() + 1e-30
+    assert bool(((h.double() - ref).abs() <= lim).all())
+    hact = ops.quantize_act(torch.randn(tok * used, k, generator=g, device=DEV), ACT[t])[0]
+    weights, add = torch.rand(tok, used, generator=g, device=DEV) * 2 - 0.5, torch.randn(tok, rows, generator=g, device=DEV)
+    y, size = (v.view(tok, used, rows) for v in product(ops.act_values(hact, ACT[t], tok * used, k, torch.float32).double(), down, flat))
+    w = weights.double()[..., None]
+    out = ops.moe_down(down.gpu, hact, plan, weights, add=add)
+    ref, parts = add.double() + (w * y).sum(1), (w * y).abs().sum(1) + add.double().abs()
+    assert bool(((out.double() - ref).abs() <= rounding(down) * (w.abs() * size).sum(1) + used * 2.0 ** -24 * parts * 1.01 + 1e-30).all())
 
 
 @pytest.mark.parametrize("t", TYPES)

@@ -37,7 +37,7 @@ def down(t=Q4_0, w=A, stride=None, n=8, rows=256, k=512, act=A, tok=3, used=2, i
 def test_norm():
     for bad in (dict(x=None), dict(add=None), dict(out=None)):
         refused(norm(**bad), "null")
-    for bad in (dict(rows=-1), dict(n=0), dict(n=(1 << 24) + 4)):
+    for bad in (dict(rows=-1), dict(rows=1 << 22), dict(n=0), dict(n=(1 << 24) + 4)):
         refused(norm(**bad), "bad shape")
     refused(norm(n=510, act=None), "n % 4")
     for name in ("x", "add", "w", "out", "o", "act"):
@@ -56,6 +56,7 @@ def test_act_values():
     refused(f(Q8_0, A, 1, 33, 0, A, None), "bad shape")
     refused(f(Q8_K, A, 1, 32, 0, A, None), "bad shape")
     refused(f(Q8_0, A, -1, 32, 0, A, None), "bad shape")
+    refused(f(Q8_0, A, 1 << 29, 32, 0, A, None), "too many")
     refused(f(Q8_0, A, 1, 32, 2, A, None), "output type")
     refused(f(Q8_0, A + 4, 1, 32, 0, A, None), "aligned")
     assert f(Q8_0, A, 0, 32, 0, A, None) == 0
@@ -68,7 +69,8 @@ def test_route():
         refused(route(**bad), "experts (1 to")
     for bad in (dict(used=0), dict(used=65, n=128), dict(used=9, n=8), dict(used=-1)):
         refused(route(**bad), "experts a token")
-    refused(route(tok=1 << 22), "pairs")
+    for tok in (1 << 22, 1 << 62):
+        refused(route(tok=tok), "pairs")
     refused(route(stride=63), "stride")
     refused(route(score=2), "score")
     for bad in (dict(groups=0), dict(groups=65, n=650, stride=650), dict(groups=3), dict(groups=4, top=0), dict(groups=4, top=5)):
@@ -110,6 +112,8 @@ def test_products(call):
     for bad in (dict(act=None), dict(act=A + 4), dict(p=A + 4)):
         refused(call(**bad), "activations or plan")
     refused(call(tok=1 << 20, rows=1 << 12), "too many")
+    refused(call(tok=1 << 17, p=None), "without a plan")
+    refused(call(tok=512, n=1024, rows=1 << 20, k=512, stride=1 << 40), "tiles of")
     assert call(tok=0) == 0
 
 
