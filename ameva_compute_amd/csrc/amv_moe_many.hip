@@ -124,8 +124,14 @@ __device__ __forceinline__ void mm_none(const MmArgs& p, const MmTile& tile, con
     }
 }
 
-// byte-wise n - 8 of nibbles n in 0..15 (no carry crosses a byte: n + 0x78 <= 0x87)
-__device__ __forceinline__ uint32_t mm_m8(uint32_t v) { return (v + 0x78787878u) ^ 0x80808080u; }
+// byte-wise 16 (n - 8) of the nibbles n that are the bytes' high halves (one v_bitop3; n - 8 itself takes two operations more)
+__device__ __forceinline__ int mm_m8(uint32_t v) { return (int)((v & 0xF0F0F0F0u) ^ 0x80808080u); }
+
+// Q8_0's integers as floats: the product's C operand is the word of 1 / (2 pi), whose mantissa leaves room for sums of 520192 on both
+// sides, so its bits plus the sum are a float of the same binade, and the float less 1 / (2 pi) is 2^-26 times the sum, exactly. A
+// subtraction is half of a conversion's time (8 experts of 4096 x 6144, 256 rows each, us: 655 with conversions, 635 so). Q4_0's
+// kernel has no registers for that operand at four waves a SIMD (it spills, or at three waves loses more than it gains).
+#define MM_ORIGIN 0x3E22F983
 
 // ---------------------------------------------------------------------------------------------------------------- Q4_0, Q8_0
 template <int WT, bool GU>
@@ -220,9 +226,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void k
             mm_v4i B;
             if constexpr (Q4) {  // element e < 16: low nibble of byte e (lane half 0); 16 + e: its high nibble (half 1)
                 const uint4 x = sW[wr * 4 + (bl ^ wx)];
-                const int s = 4 * h;
-                B = mm_v4i{(int)mm_m8((x.x >> s) & 0x0F0F0F0Fu), (int)mm_m8((x.y >> s) & 0x0F0F0F0Fu),
-                           (int)mm_m8((x.z >> s) & 0x0F0F0F0Fu), (int)mm_m8((x.w >> s) & 0x0F0F0F0Fu)};
+                const int s = 4 - 4 * h;
+                B = mm_v4i{mm_m8(x.x << s), mm_m8(x.y << s), mm_m8(x.z << s), mm_m8(x.w << s)};
             } else {
                 const uint4 x = sW[wr * 8 + ((2 * bl + h) ^ wx)];
                 B = mm_v4i{(int)x.x, (int)x.y, (int)x.z, (int)x.w};
@@ -230,10 +235,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void k
 #pragma unroll
             for (int i = 0; i < decltype(ni)::value; ++i) {
                 const uint4 a = sA[(ar + 32 * i) * 8 + ((2 * bl + h) ^ ax)];
-                const mm_v16i z = {};
+                mm_v16i z;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) z[r] = Q4 ? 0 : MM_ORIGIN;
                 const mm_v16i C = __builtin_amdgcn_mfma_i32_32x32x32_i8(mm_v4i{(int)a.x, (int)a.y, (int)a.z, (int)a.w}, B, z, 0, 0, 0);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][r] = fmaf((float)C[r], o[16 * i + r], acc[i][r]);
+                for (int r = 0; r < 16; ++r)
+                    acc[i][r] = fmaf(Q4 ? (float)C[r] : __int_as_float(C[r]) - __int_as_float(MM_ORIGIN), o[16 * i + r], acc[i][r]);
             }
             // one block's results at a time (more do not fit the registers), added up here (the compiler would move the
             // additions behind the next barrier and keep the results until then)
@@ -271,6 +279,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void k
         }
     };
     mm_halves(tile, steps);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] *= Q4 ? 0x1p-4f : 0x1p26f;
     mm_finish<GU>(p, tile, s_pair, sAa, acc, wn);
 }
 
@@ -520,7 +532,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k
     const auto store_sb = [&](int buf) {
         if (t < BN) {
             sSc[buf][t] = scr;
-            sD[buf][t] = amv_h2f(dr);
+            sD[buf][t] = 0.25f * amv_h2f(dr);  // (the integers are four times q - 32)
         }
         if (t < BM) sDa[buf][t] = dar;
     };
@@ -542,13 +554,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k
         for (int pp = 0; pp < 2; ++pp) {
             const uint2 l0 = reinterpret_cast<const uint2*>(sW + wr * 4 + (pp ^ wx))[h];
             const uint2 l1 = reinterpret_cast<const uint2*>(sW + wr * 4 + ((2 + pp) ^ wx))[h];
-            const uint2 qh = reinterpret_cast<const uint2*>(sH + wr * 2 + (pp ^ hx))[h];
+            uint2 qh = reinterpret_cast<const uint2*>(sH + wr * 2 + (pp ^ hx))[h];
+            qh = make_uint2(qh.x ^ 0xAAAAAAAAu, qh.y ^ 0xAAAAAAAAu);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint2 l = e & 1 ? l1 : l0;
-                const int s = e < 2 ? 0 : 4;
+                // 4 (q - 32): the six bits at the byte's top, the highest one turned over (above, for all e)
                 const auto q6 = [&](uint32_t lo, uint32_t hi) {
-                    return ((((lo >> s) & 0x0F0F0F0Fu) | (((hi >> (2 * e)) & 0x03030303u) << 4)) + 0x60606060u) ^ 0x80808080u;
+                    return ((e < 2 ? lo << 2 : lo >> 2) & 0x3C3C3C3Cu) | ((hi << (6 - 2 * e)) & 0xC0C0C0C0u);
                 };
                 const uint2 b = make_uint2(q6(l.x, qh.x), q6(l.y, qh.y));
                 const int sub = 2 * e + pp, sc = (int)(int8_t)((sub < 4 ? s0 : s1) >> (8 * (sub & 3)));
