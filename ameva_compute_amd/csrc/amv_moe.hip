@@ -136,23 +136,33 @@ __device__ __forceinline__ uint64_t moe_key(double v) {  // NaN and minus infini
     const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);  // (-0 and 0 are one)
     return v > -INFINITY ? ((b >> 63) ? ~b : b | ((uint64_t)1 << 63)) : 0;
 }
-template <int CTRL>
-__device__ __forceinline__ uint64_t moe_dpp(uint64_t v) {
-    return (uint64_t)(uint32_t)amv_dpp_i<CTRL>((int)(uint32_t)v) | (uint64_t)(uint32_t)amv_dpp_i<CTRL>((int)(v >> 32)) << 32;
-}
 __device__ __forceinline__ uint64_t moe_lane(uint64_t v, int lane) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane) |
            (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32;
 }
-__device__ __forceinline__ uint64_t moe_wave_max(uint64_t v) {
-    const auto up = [&](uint64_t o) { v = o > v ? o : v; };
-    up(moe_dpp<0xB1>(v));
-    up(moe_dpp<0x4E>(v));
-    up(moe_dpp<0x141>(v));
-    up(moe_dpp<0x140>(v));
-    const uint64_t a = moe_lane(v, 0), b = moe_lane(v, 16), c = moe_lane(v, 32), d = moe_lane(v, 48);
-    const uint64_t ab = a > b ? a : b, cd = c > d ? c : d;
-    return ab > cd ? ab : cd;
+__device__ __forceinline__ uint32_t moe_wave_max(uint32_t v) {
+    v = max(v, (uint32_t)amv_dpp_i<0xB1>((int)v));
+    v = max(v, (uint32_t)amv_dpp_i<0x4E>((int)v));
+    v = max(v, (uint32_t)amv_dpp_i<0x141>((int)v));
+    v = max(v, (uint32_t)amv_dpp_i<0x140>((int)v));
+    const auto lane = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+    return max(max(lane(0), lane(16)), max(lane(32), lane(48)));
+}
+// the lanes with the largest key, none where all are 0 (a key that is not 0 has an upper half that is not 0: others are no number)
+__device__ __forceinline__ uint64_t moe_largest(uint64_t key) {
+    const uint32_t hi = (uint32_t)(key >> 32), m = moe_wave_max(hi);
+    if (!m) return 0;
+    const uint64_t who = __ballot(hi == m);
+    if (!(who & (who - 1))) return who;
+    const uint32_t lo = hi == m ? (uint32_t)key : 0u, l = moe_wave_max(lo);
+    return __ballot(hi == m && lo == l);
+}
+// b0, b1: the two largest so far (a c that is no number is in no comparison the larger)
+__device__ __forceinline__ void moe_take(double& b0, double& b1, double c) {
+    const bool up = c > b0;
+    const double low = up ? b0 : c;
+    b0 = up ? c : b0;
+    b1 = low > b1 ? low : b1;
 }
 __device__ __forceinline__ double moe_lane_d(double v, int lane) {
     return __longlong_as_double((long long)moe_lane((uint64_t)__double_as_longlong(v), lane));
@@ -208,33 +218,33 @@ __global__ __launch_bounds__(64) void k_moe_route(const MoeRoute a) {
     }
     if constexpr (GROUPS) {
         const int size = a.n_expert / a.n_group;
+        const float inv = 1.0f / (float)size;
 #pragma unroll
         for (int v = 0; v < PER; ++v) s_choice[64 * v + lane] = key[v] ? choice[v] : __longlong_as_double(0x7FF8000000000000ll);
         __syncthreads();
-        // lane g: the sum of group g's best choices
+        // 2^sh lanes for a group, then its first one: the sum of the group's best choices
+        const int sh = __builtin_clz(a.n_group - 1) - 26, per = 1 << sh, group = lane >> sh;
         double b0 = -INFINITY, b1 = -INFINITY;
-        if (lane < a.n_group)
-            for (int i = 0; i < size; ++i) {
-                const double c = s_choice[lane * size + i];  // (no number: in no comparison the larger)
-                if (c > b0) {
-                    b1 = b0;
-                    b0 = c;
-                } else if (c > b1) {
-                    b1 = c;
-                }
-            }
-        uint64_t g = moe_key(a.group_best == 2 && b1 > -INFINITY ? b0 + b1 : b0), kept = 0;
+        if (group < a.n_group)
+            for (int i = lane & (per - 1); i < size; i += per) moe_take(b0, b1, s_choice[group * size + i]);
+        for (int o = 1; o < per; o <<= 1) {
+            const double c0 = __shfl_xor(b0, o, 64), c1 = __shfl_xor(b1, o, 64);
+            moe_take(b0, b1, c0);
+            moe_take(b0, b1, c1);
+        }
+        uint64_t g = lane & (per - 1) ? 0 : moe_key(a.group_best == 2 && b1 > -INFINITY ? b0 + b1 : b0), kept = 0;
         for (int i = 0; i < a.top_group; ++i) {
-            const uint64_t m = moe_wave_max(g);
-            if (!m) break;
-            const int first = __builtin_ctzll(__ballot(g == m));
-            kept |= (uint64_t)1 << first;
+            const uint64_t who = moe_largest(g);
+            if (!who) break;
+            const int first = __builtin_ctzll(who);
+            kept |= (uint64_t)1 << (first >> sh);
             if (lane == first) g = 0;
         }
 #pragma unroll
         for (int v = 0; v < PER; ++v) {
             const int e = 64 * v + lane;
-            if (e < a.n_expert && !((kept >> (e / size)) & 1)) key[v] = 0;
+            const int of = (int)(((float)e + 0.5f) * inv);  // e / size: at least 1 / (2 size) from a whole number, off by 2^-22 of itself
+            if (!((kept >> (of & 63)) & 1)) key[v] = 0;
         }
     }
     // lane i keeps the i-th choice
@@ -249,9 +259,8 @@ __global__ __launch_bounds__(64) void k_moe_route(const MoeRoute a) {
                 best = key[v];
                 at = v;
             }
-        const uint64_t m = moe_wave_max(best);
-        if (!m) break;
-        uint64_t who = __ballot(best == m);
+        const uint64_t who = moe_largest(best);
+        if (!who) break;
         int first = __builtin_ctzll(who), v_at = __builtin_amdgcn_readlane(at, first);
         if (who & (who - 1)) {  // equal ones: the lowest index, so the lowest v first
             for (uint64_t rest = who & (who - 1); rest; rest &= rest - 1) {
