@@ -6,6 +6,9 @@
 // tokens and four blocks, each comes out as an integer of its own, exact. Weights go from memory to the lanes as they lie (16 bytes a
 // lane), and one instruction in four would do for the arithmetic, but these products are bound by the weights' bytes.
 // Result D of lane l: weight row l % 16, token l / 16, blocks 0..3 in its four registers: the block epilogue is a sum within the lane.
+// Measured, with cold weights: gate and up of 48 tokens with 8 of 64 experts of 1024 x 2048 Q4_0 40 us, 3.8 TB/s; down of 40 tokens,
+// 2048 x 1408 Q8_0, 43 us, 4.6 TB/s; one token, two experts of 4096 x 14336 Q6_K, 27.6 us, 3.5 TB/s; its gate and up, eight of 1024 x
+// 2048 Q4_K, 7.9 us, of which 4 are the bytes: a chain of ids, weights and sums.
 #include "amv_moe.h"
 
 #include <algorithm>

@@ -8,6 +8,10 @@
 // the fragments' reads hit all banks. Rows past the end of a buffer read as zero (the buffers' own range check).
 // The work beside the matrix core bounds these kernels: of a 32-block's 32 x 32 integers, each is converted and added with its
 // scale (Q4_0, Q8_0; the scale products are one outer product on the matrix core), or multiplied by its unit's scale (K-quants).
+// Measured: gate and up of 4096 tokens with 8 of 128 experts of 1024 x 2048 Q4_0 463 us, 594 TFLOP/s (vector instructions 88 % of the
+// cycles, the matrix core 29 %, 0.9 GB read); down of the same pairs, 2048 x 1024 Q4_K, 215 us, of which memory 105 (0.5 GB of weights and
+// sums for the next launch); 1200 pairs of 8 experts of 4096 x 6144 Q4_0 129 us. Not faster: tiles of 128 rows, workgroups that
+// go on to further tiles, a start of k that turns with the workgroup, two sets of waves on halves of k (but for a dozen rows an expert).
 #include "amv_moe.h"
 
 #include <type_traits>
