@@ -6,7 +6,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
-from moe_ref import ACT, DEV, Q4_0, Q4_K, Q6_K, Q8_0, Q8_K, TYPES, Experts, product, rounding, route  # noqa: E402
+from moe_ref import ACT, DEV, Q4_0, Q4_K, Q6_K, Q8_0, Q8_K, TYPES, UNIT, Experts, product, rounding, route  # noqa: E402
 
 
 def gen(seed):
@@ -150,12 +150,16 @@ SHAPES = [  # tokens, experts, used, rows, k in blocks, kind
     (6, 5, 3, 288, 4, "holes"), (17, 3, 1, 64, 7, "one"), (40, 16, 2, 160, 6, "holes"), (65, 2, 2, 32, 33, "skewed"), (200, 3, 2, 96, 5, "holes"),
     (333, 60, 4, 64, 2, "skewed"), (9, 4, 2, 96, 57, "holes"), (130, 2, 1, 352, 17, "one"), (1100, 7, 4, 32, 1, "holes"), (700, 5, 1, 544, 3, "skewed"),
     # more experts a token than a workgroup has waves; a plan of more than 4096 pairs with few of them an expert
-    (1, 70, 20, 64, 3, "skewed"), (1, 64, 64, 32, 6, "skewed"), (3, 70, 64, 32, 2, "skewed"), (700, 1024, 8, 32, 1, "holes")]
+    (1, 70, 20, 64, 3, "skewed"), (1, 64, 64, 32, 6, "skewed"), (3, 70, 64, 32, 2, "skewed"), (700, 1024, 8, 32, 1, "holes"),
+    # the most of a tile's rows that LDS holds at once
+    (13, 4, 2, 96, 14, "holes")]
 
 
 def make(t, shape, seed=0):
     tok, n, used, rows, kb, kind = shape
     k = kb * (32 if t in (Q4_0, Q8_0) else 256)
+    if kb == 14:
+        k = 3584
     if kb == 57:  # longer than what LDS holds of a tile's rows: parts of it, the last one not whole
         k = 7264 if t in (Q4_0, Q8_0) else 7424
     g = gen(seed + tok + rows)
@@ -391,3 +395,94 @@ def test_experts_apart_and_back():
         assert torch.equal(ops.moe_gate_up(e.gpu, e.gpu, a, plan, act_type=None), ops.moe_gate_up(far, far, a, plan, act_type=None))
     with pytest.raises(ValueError, match="differ"):
         ops.moe_gate_up(e.gpu, far, act, ops.moe_plan(ids, 5))
+
+
+# ---------------------------------------------------------------------------------------------------- ends of the ranges
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tok", [1, 30, 300])
+def test_largest_integers(t, tok):
+    """Weights and activations whose integers and scales are all at their ends, one sign or in turn: no sum of a block or super-block
+    leaves what the kernels hold it in."""
+    import oracle
+    from ameva_compute_amd import ops
+    n, used, rows, k = 3, 2, 64, 1024
+    d = np.float16(0.01).tobytes()
+    block = {Q8_0: d + b"\x80" * 32, Q4_0: d + b"\x00" * 16, Q4_K: d + d + b"\xff" * 140, Q6_K: b"\x00" * 192 + b"\x80" * 16 + d}[t]
+    raw = np.frombuffer(block * (n * rows * k // UNIT[t]), dtype=np.uint8).copy()
+    e = Experts(t, n, rows, k, 1)
+    e.gpu = ops.QExperts.from_ggml(t, torch.from_numpy(raw).to(DEV), n, rows, k)
+    e.w = torch.from_numpy(oracle.dequantize(t, raw, k).reshape(n, rows, k).astype(np.float64)).to(DEV)
+    e.size = e.w.abs() * (1.15 if t == Q4_K else 1)  # (63 * 15 - 63 of the parts 63 * 15 + 63)
+    x = torch.ones(tok * used, k, device=DEV)
+    x[1::2, 1::2] = -1
+    ids = torch.tensor([[0, 2]], dtype=torch.int32, device=DEV).repeat(tok, 1)
+    act = ops.quantize_act(x, ACT[t])[0]
+    a = ops.act_values(act, ACT[t], tok * used, k, torch.float32).double()
+    weights = torch.ones(tok, used, device=DEV)
+    y, size = (v.view(tok, used, rows) for v in product(a, e, ids.flatten()))
+    plan = ops.moe_plan(ids, n)
+    out = ops.moe_down(e.gpu, act, plan, weights)
+    assert bool(((out.double() - y.sum(1)).abs() <= rounding(e) * size.sum(1) + used * 2.0 ** -24 * y.abs().sum(1) * 1.01).all())
+    one = x[:tok].contiguous()
+    act = ops.quantize_act(one, ACT[t])[0]
+    yg, sg = product(ops.act_values(act, ACT[t], tok, k, torch.float32).double().repeat_interleave(used, 0), e, ids.flatten())
+    h = ops.moe_gate_up(e.gpu, e.gpu, act, plan, act_type=None)
+    ref = yg * torch.sigmoid(yg) * yg
+    # as in test_gate_up, with one product twice
+    lim = rounding(e) * sg * (1.1 * yg.abs() + (yg * torch.sigmoid(yg)).abs() + 1.1 * sg * rounding(e)) + 8 * 2.0 ** -24 * ref.abs() + 1e-30
+    assert bool(((h.double() - ref).abs() <= lim).all())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tok", [1, 20, 400])
+def test_experts_beyond_32_bits(t, tok):
+    """Experts 2.2 GB apart (all but their own bytes never written) give what they give side by side."""
+    from ameva_compute_amd import ops
+    n, used, rows, k = 4, 2, 64, 512
+    e = Experts(t, n, rows, k, 3)
+    need = e.gpu.data.shape[1]
+    wide = torch.empty((n, 2200000000 // 16 * 16), dtype=torch.uint8, device=DEV)
+    wide[:, :need] = e.gpu.data
+    far = ops.QExperts(t, n, rows, k, wide)
+    g = gen(tok)
+    ids = torch.stack([torch.randint(0, 2, (tok,), generator=g, device=DEV), torch.randint(2, 4, (tok,), generator=g, device=DEV)], 1).int()
+    plan, weights = ops.moe_plan(ids, n), torch.rand(tok, used, generator=g, device=DEV)
+    act = ops.quantize_act(torch.randn(tok, k, generator=g, device=DEV), ACT[t])[0]
+    hact = ops.quantize_act(torch.randn(tok * used, k, generator=g, device=DEV), ACT[t])[0]
+    assert torch.equal(ops.moe_gate_up(far, far, act, plan, act_type=None), ops.moe_gate_up(e.gpu, e.gpu, act, plan, act_type=None))
+    assert torch.equal(ops.moe_down(far, hact, plan, weights), ops.moe_down(e.gpu, hact, plan, weights))
+
+
+def test_outputs_beyond_32_bits():
+    """2^20 pairs of 1088 columns (4.6 GB of products) and of 4064 k (4.3 GB of activations): the last tokens' results are what the same
+    tokens get by themselves, within the roundings."""
+    from ameva_compute_amd import ops
+    tok, n, used, last = 1 << 17, 8, 8, 16
+    g = gen(8)
+    ids = torch.randint(0, n, (tok, used), generator=g, device=DEV).int()
+    gate, up = Experts(Q8_0, n, 1088, 32, 1), Experts(Q8_0, n, 1088, 32, 2)
+    x = torch.randn(tok, 32, generator=g, device=DEV)
+    act, tail = ops.quantize_act(x, Q8_0)[0], ops.quantize_act(x[-last:].contiguous(), Q8_0)[0]
+    plan, few = ops.moe_plan(ids, n), ops.moe_plan(ids[-last:].contiguous(), n)
+    h = ops.moe_gate_up(gate.gpu, up.gpu, act, plan, act_type=None)[-last * used:].double()
+    ref = ops.moe_gate_up(gate.gpu, up.gpu, tail, few, act_type=None).double()
+    a, flat = ops.act_values(tail, Q8_0, last, 32, torch.float32).double().repeat_interleave(used, 0), ids[-last:].flatten()
+    (yg, sg), (yu, su) = product(a, gate, flat), product(a, up, flat)
+    r = rounding(gate)
+    lim = 2 * (r * (1.1 * sg * yu.abs() + (yg * torch.sigmoid(yg)).abs() * su + 1.1 * sg * su * r) + 8 * 2.0 ** -24 * ref.abs() + 1e-30)
+    assert bool(((h - ref).abs() <= lim).all())
+    del h, act, x
+    # the down product's rows: zeros but for the last tokens'
+    k, rows, pairs = 4064, 32, tok * used
+    down = Experts(Q8_0, n, rows, k, 3)
+    small = ops.quantize_act(torch.randn(last * used, k, generator=g, device=DEV), Q8_0)[0]
+    big = torch.zeros(pairs * k + pairs * k // 32 * 8, dtype=torch.uint8, device=DEV)
+    q, m = last * used * k, last * used * k // 32 * 8
+    big[pairs * k - q:pairs * k], big[-m:] = small[:q], small[q:q + m]
+    weights = torch.rand(tok, used, generator=g, device=DEV)
+    y = ops.moe_down(down.gpu, big, plan, weights)
+    assert not bool(y[:-last].any())
+    p, size = (v.view(last, used, rows) for v in product(ops.act_values(small, Q8_0, last * used, k, torch.float32).double(), down, flat))
+    w = weights[-last:].double()[..., None]
+    lim = rounding(down) * (w * size).sum(1) + used * 2.0 ** -24 * (w * p).abs().sum(1) * 1.01 + 1e-30
+    assert bool(((y[-last:].double() - (w * p).sum(1)).abs() <= lim).all())
