@@ -881,7 +881,7 @@ def act_values(act: torch.Tensor, act_type: int, m: int, k: int, dtype: torch.dt
     if dtype not in (torch.float16, torch.float32) or act_type not in (Q8_0, Q8_K) or m < 0 or k <= 0 or k % (256 if act_type == Q8_K else 32):
         raise ValueError(f"act_values: type {act_type} {m}x{k} to {dtype} is not supported")
     _act_holds(act, act_type, m, k, act.get_device(), "act_values")
-    out = torch.empty((m, k), dtype=dtype, device=act.device)
+    out = act.new_empty((m, k), dtype=dtype)
     if m:
         check(lib().amv_act_values(act_type, act.data_ptr(), m, k, F16 if dtype is torch.float16 else F32, out.data_ptr(), _stream()),
               "amv_act_values")
@@ -905,8 +905,8 @@ def moe_route(logits: torch.Tensor, n_used: int, score: str = "softmax", bias: t
     t, e = logits.shape
     _f32_on(bias, (e,), logits.get_device(), "moe_route: bias")
     stride = logits.stride(0) if t > 1 else e
-    ids = torch.empty((t, max(n_used, 0)), dtype=torch.int32, device=logits.device)
-    weights = torch.empty((t, max(n_used, 0)), dtype=torch.float32, device=logits.device)
+    weights = logits.new_empty((t, max(n_used, 0)))
+    ids = torch.empty_like(weights, dtype=torch.int32)
     if t:
         check(lib().amv_moe_route(logits.data_ptr(), stride, t, e, n_used, MOE_SCORES[score], _ptr(bias), n_group, top_group, group_best,
                                   int(renorm), scale, ids.data_ptr(), weights.data_ptr(), _stream()), "amv_moe_route")
