@@ -18,7 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libameva_hip.so")
 SOURCES = ["amv_runtime.hip", "amv_quant.hip", "amv_mmv.hip", "amv_i2s.hip", "amv_norm.hip", "amv_attn.hip", "amv_fa_prefill.hip", "amv_mmq.hip", "amv_mmq16.hip", "amv_qgemm.hip", "amv_elem.hip", "amv_bitnet.hip",
-           "amv_paged.hip", "amv_paged_attn.hip", "amv_moe.hip", "amv_moe_few.hip", "amv_moe_many.hip"]
+           "amv_paged.hip", "amv_paged_attn.hip", "amv_moe.hip", "amv_moe_one.hip", "amv_moe_few.hip", "amv_moe_many.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

@@ -52,7 +52,7 @@ struct MoeProduct {
     const float *weights, *add;  // of moe_one's sum
     hipStream_t st;
 };
-int moe_one(const MoeProduct& p);   // amv_moe_few.hip: without a plan
+int moe_one(const MoeProduct& p);   // amv_moe_one.hip: without a plan
 int moe_few(const MoeProduct& p);   // amv_moe_few.hip
 int moe_many(const MoeProduct& p);  // amv_moe_many.hip
 
@@ -72,4 +72,29 @@ __device__ __forceinline__ void moe_act_store4(const AmvActOut& o, int c, const 
     } else if ((c & 63) == 0) {
         reinterpret_cast<int*>(o.meta)[c >> 6] = 0x7FC00000;
     }
+}
+
+// Q8_0 of a block of 32 that 32 lanes hold, an element each: amv_q8_0_lanes32's rules and bytes, the largest and the sum by DPP; a block
+// with an element that is infinite or no number gets a scale that is none (moe_act_store4)
+__device__ __forceinline__ void moe_q8_0(float v, int rule, int j, int8_t* qs, int2* meta) {
+    float a = fabsf(v);
+    a = fmaxf(a, __int_as_float(amv_dpp_i<0xB1>(__float_as_int(a))));
+    a = fmaxf(a, __int_as_float(amv_dpp_i<0x4E>(__float_as_int(a))));
+    a = fmaxf(a, __int_as_float(amv_dpp_i<0x141>(__float_as_int(a))));
+    a = fmaxf(a, __int_as_float(amv_dpp_i<0x140>(__float_as_int(a))));
+    a = amv_max_x16(a);
+    const float d = a / 127.0f;
+    const float id = rule == AMV_Q8_X86 ? (a != 0.0f ? 127.0f / a : 0.0f) : (d != 0.0f ? 1.0f / d : 0.0f);
+    const float t = v * id;
+    const int q = (int)fminf(127.0f, fmaxf(-127.0f, rule == AMV_Q8_REF ? roundf(t) : rintf(t)));
+    int s = q;
+    s += amv_dpp_i<0xB1>(s);
+    s += amv_dpp_i<0x4E>(s);
+    s += amv_dpp_i<0x141>(s);
+    s += amv_dpp_i<0x140>(s);
+    const auto o = __builtin_amdgcn_permlane16_swap((uint32_t)s, (uint32_t)s, false, false);
+    const uint64_t bad = __ballot(!(fabsf(v) < INFINITY));
+    qs[j] = (int8_t)q;
+    if (j == 0)
+        *meta = make_int2((uint32_t)(bad >> (threadIdx.x & 32)) ? 0x7FC00000 : __float_as_int(amv_h2f(amv_f2h(d))), (int)(o[0] + o[1]));
 }

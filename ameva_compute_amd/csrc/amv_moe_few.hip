@@ -7,11 +7,9 @@
 // lane), and one instruction in four would do for the arithmetic, but these products are bound by the weights' bytes.
 // Result D of lane l: weight row l % 16, token l / 16, blocks 0..3 in its four registers: the block epilogue is a sum within the lane.
 // Measured, with cold weights: gate and up of 48 tokens with 8 of 64 experts of 1024 x 2048 Q4_0 40 us, 3.8 TB/s; down of 40 tokens,
-// 2048 x 1408 Q8_0, 43 us, 4.6 TB/s; one token, two experts of 4096 x 14336 Q6_K, 27.6 us, 3.5 TB/s; its gate and up, eight of 1024 x
-// 2048 Q4_K, 7.9 us, of which 4 are the bytes: a chain of ids, weights and sums.
+// 2048 x 1408 Q8_0, 43 us, 4.6 TB/s.
 #include "amv_moe.h"
 
-#include <algorithm>
 #include <type_traits>
 
 typedef int mf_v4i __attribute__((ext_vector_type(4)));
@@ -260,31 +258,6 @@ struct Mf<AMV_T_Q6_K, U> {
     }
 };
 
-// Q8_0 of a block of 32 that 32 lanes hold, an element each: amv_q8_0_lanes32's rules and bytes, the largest and the sum by DPP; a block
-// with an element that is infinite or no number gets a scale that is none (moe_act_store4)
-__device__ __forceinline__ void mf_q8_0(float v, int rule, int j, int8_t* qs, int2* meta) {
-    float a = fabsf(v);
-    a = fmaxf(a, __int_as_float(amv_dpp_i<0xB1>(__float_as_int(a))));
-    a = fmaxf(a, __int_as_float(amv_dpp_i<0x4E>(__float_as_int(a))));
-    a = fmaxf(a, __int_as_float(amv_dpp_i<0x141>(__float_as_int(a))));
-    a = fmaxf(a, __int_as_float(amv_dpp_i<0x140>(__float_as_int(a))));
-    a = amv_max_x16(a);
-    const float d = a / 127.0f;
-    const float id = rule == AMV_Q8_X86 ? (a != 0.0f ? 127.0f / a : 0.0f) : (d != 0.0f ? 1.0f / d : 0.0f);
-    const float t = v * id;
-    const int q = (int)fminf(127.0f, fmaxf(-127.0f, rule == AMV_Q8_REF ? roundf(t) : rintf(t)));
-    int s = q;
-    s += amv_dpp_i<0xB1>(s);
-    s += amv_dpp_i<0x4E>(s);
-    s += amv_dpp_i<0x141>(s);
-    s += amv_dpp_i<0x140>(s);
-    const auto o = __builtin_amdgcn_permlane16_swap((uint32_t)s, (uint32_t)s, false, false);
-    const uint64_t bad = __ballot(!(fabsf(v) < INFINITY));
-    qs[j] = (int8_t)q;
-    if (j == 0)
-        *meta = make_int2((uint32_t)(bad >> (threadIdx.x & 32)) ? 0x7FC00000 : __float_as_int(amv_h2f(amv_f2h(d))), (int)(o[0] + o[1]));
-}
-
 // Workgroup: one tile and NW groups of 16 weight rows (gate and up: half of them each), a wave a
 // group on one of KG parts of k. The rows go to LDS, KC k at a time (all of k but where that is very long), a wave's first weights
 // are on their way meanwhile; then a wave goes through its weights by itself, and the parts' sums meet in LDS. What carries it is
@@ -443,7 +416,7 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
             if (p.out) p.out[pr * p.rows + n0 + f] = h;
             if (p.q.type) {
                 const AmvActOut o = amv_act_row(p.q, pr, p.rows);
-                mf_q8_0(h, o.rule, f & 31, o.qs + n0 + (f & ~31), reinterpret_cast<int2*>(o.meta) + (n0 + f) / 32);
+                moe_q8_0(h, o.rule, f & 31, o.qs + n0 + (f & ~31), reinterpret_cast<int2*>(o.meta) + (n0 + f) / 32);
             }
         } else if (e < p.n_expert) {
             p.out[pr * p.rows + n0 + f] = v[0];
@@ -475,152 +448,6 @@ static void mf_type(const MfArgs& a, int64_t tiles, int64_t k, bool gu, hipStrea
         if (gu) mf_go<WT, U, true, 4, 2>(a, tiles, k, st);
         else mf_go<WT, U, false, 4, 2>(a, tiles, k, st);
     }
-}
-
-// Without a plan (a token by itself): each pair is a product of one row, which a wave's lanes load where they need it, with the weights.
-// Gate and up: a workgroup has 32 columns of a pair, four waves of 16 weight rows on each of four parts of k. Down: a workgroup has 16
-// columns of a token, its waves the token's experts and KP parts of k of each, and adds the weighted products up: no second launch.
-// At one token a launch's latency is half of the time: the chain is ids, weights and row, products, sums.
-struct MoArgs {
-    const uint8_t *w0, *w1;
-    int64_t stride, bytes;
-    int rows, n_k, n_expert, n_used, n_cols, kp;
-    MfAct act;
-    const int32_t* ids;
-    const float *weights, *add;
-    float* out;
-    AmvActOut q;
-};
-
-template <int WT, int U, bool GU>
-__global__ __launch_bounds__(1024) void k_moe_one(const MoArgs p) {
-    using T = Mf<WT, U>;
-    constexpr bool KQ = T::STEP == 256;
-    __shared__ float s_red[GU ? 16 : MOE_MAX_USED][17];
-    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, q = lane >> 4;
-    const int col = blockIdx.x % p.n_cols, of = blockIdx.x / p.n_cols, n0 = col * (GU ? 32 : 16);  // of: pair, or token
-    const int steps = KQ ? p.n_k : (p.n_k + 3) / 4, kp = GU ? 4 : p.kp;
-    const int64_t k = (int64_t)p.n_k * (KQ ? 256 : 32);
-    const bool live = c16 == q;  // (A row b of the row's four: its integers in quarter b)
-    // gate and up: wave = part * 4 + matrix * 2 + 16 columns; down: expert * parts + part, in turns where there are more
-    for (int job = wv; job < (GU ? 16 : p.n_used * kp); job += blockDim.x >> 6) {
-        const int part = GU ? job >> 2 : job % kp, pair = GU ? of : of * p.n_used + job / kp;
-        const int e = p.ids[pair];
-        float acc = 0.0f;
-        if (e >= 0 && e < p.n_expert) {
-            const uint8_t* const m = (GU && (job & 2) ? p.w1 : p.w0) + e * p.stride;
-            const __amdgpu_buffer_rsrc_t buf = MF_RSRC(m, p.bytes);
-            const int n = n0 + (GU ? 16 * (job & 1) : 0) + c16;
-            const int64_t row = GU ? pair / p.n_used : pair;
-            const int8_t* const aq = p.act.q + row * k + (T::AT ? T::AT * q : 128 * (q >> 1) + 16 * (q & 1));
-            const int per = (steps + kp - 1) / kp, s0 = part * per, s1 = min(steps, s0 + per);
-            for (int s = s0; s < s1; s += U) {
-                typename T::W w;
-                T::load(w, buf, m, p.rows, p.n_k, n, q, s);
-                // the row: integers of the lane's own block (zeros in the others, and past k), scales and sums
-                uint4 a[U][8];
-                float4 d[U];
-                int4 u[U];
-#pragma unroll
-                for (int j = 0; j < U; ++j) {
-                    const bool in = s + j < s1 && (KQ || 4 * (s + j) + q < p.n_k);
-                    const uint4* src = reinterpret_cast<const uint4*>(aq + (int64_t)(s + j) * T::STEP);
-#pragma unroll
-                    for (int i = 0; i < (KQ ? 4 : 2); ++i) {
-                        const int at = T::AT ? i : 2 * i;
-                        a[j][at] = make_uint4(0, 0, 0, 0);
-                        if (live && in) a[j][at] = src[at];
-                    }
-                    u[j] = make_int4(0, 0, 0, 0);
-                    if constexpr (KQ) {
-                        const int64_t sb = row * p.n_k + min(s + j, p.n_k - 1);
-                        d[j].x = p.act.dk[sb];
-                        if constexpr (T::SUMS) {
-                            const moe_i4* x = reinterpret_cast<const moe_i4*>(p.act.s16 + sb * 16);
-                            int o[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const moe_i4 v = x[i];
-                                o[i] = (int)((uint32_t)((v.x + v.y) & 0xFFFF) | (uint32_t)(v.z + v.w) << 16);
-                            }
-                            u[j] = make_int4(o[0], o[1], o[2], o[3]);
-                        }
-                    } else {
-                        const float2* x = p.act.d0 + row * p.n_k;
-                        const int b = 4 * (s + j);
-                        d[j] = make_float4(x[min(b, p.n_k - 1)].x, x[min(b + 1, p.n_k - 1)].x, x[min(b + 2, p.n_k - 1)].x, x[min(b + 3, p.n_k - 1)].x);
-                    }
-                }
-                typename T::Scales c;
-                T::scales(w, c, p.n_k, n, q, s);
-#pragma unroll
-                for (int j = 0; j < U; ++j) {
-                    if (s + j >= s1) break;
-                    typename T::B b;
-                    T::operands(w, c, j, b);
-                    acc = T::add(b, reinterpret_cast<const uint8_t*>(a[j]), reinterpret_cast<const float*>(&d[j]),
-                                 reinterpret_cast<const int*>(&u[j]), acc);
-                }
-            }
-        }
-        if (q == 0) s_red[job][c16] = acc;
-    }
-    __syncthreads();
-    if (tid >= (GU ? 32 : 16)) return;
-    const int f = tid;
-    if constexpr (GU) {
-        float v[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int z = 0; z < 4; ++z) v[j] += s_red[4 * z + 2 * j + (f >> 4)][f & 15];
-        const float h = v[0] / (1.0f + expf(-v[0])) * v[1];
-        const int64_t pr = of;
-        if (p.out) p.out[pr * p.rows + n0 + f] = h;
-        if (p.q.type) {
-            const AmvActOut o = amv_act_row(p.q, pr, p.rows);
-            mf_q8_0(h, o.rule, f, o.qs + n0, reinterpret_cast<int2*>(o.meta) + n0 / 32);
-        }
-    } else {
-        const int64_t at = (int64_t)of * p.rows + n0 + f;
-        float v = p.add ? p.add[at] : 0.0f;
-        for (int j = 0; j < p.n_used; ++j) {
-            const int e = p.ids[of * p.n_used + j];
-            if (e < 0 || e >= p.n_expert) continue;
-            float y = 0.0f;
-            for (int z = 0; z < kp; ++z) y += s_red[j * kp + z][f];
-            v = fmaf(p.weights[of * p.n_used + j], y, v);
-        }
-        p.out[at] = v;
-    }
-}
-
-template <int WT>
-static void mo_go(MoArgs a, int64_t n, bool gu, hipStream_t st) {
-    constexpr int U = WT == AMV_T_Q4_0 ? 4 : 2;
-    a.n_cols = a.rows / (gu ? 32 : 16);
-    a.kp = gu ? 4 : std::max(1, 16 / a.n_used);
-    const unsigned grid = (unsigned)(n * a.n_cols);
-    if (gu) k_moe_one<WT, U, true><<<grid, 1024, 0, st>>>(a);
-    else k_moe_one<WT, U, false><<<grid, 64 * std::min(16, a.n_used * a.kp), 0, st>>>(a);
-}
-
-int moe_one(const MoeProduct& p) {
-    const bool kq = p.type == AMV_T_Q4_K || p.type == AMV_T_Q6_K, gu = p.w1 != nullptr;
-    const int8_t* aq = (const int8_t*)p.act;
-    const int8_t* meta = aq + p.act_rows * p.k;
-    const int64_t n = gu ? p.n_tok * p.n_used : p.n_tok;
-    AMV_REQUIRE(p.n_tok * p.n_used * p.rows < 1 << 26, "moe: %lld pairs of %lld without a plan are too many", (long long)(p.n_tok * p.n_used),
-                (long long)p.rows);
-    const MoArgs a{(const uint8_t*)p.w0, (const uint8_t*)p.w1, p.stride, amv_weight_bytes(p.type, p.rows, p.k), (int)p.rows,
-                   (int)(p.k / (kq ? 256 : 32)), p.n_expert, p.n_used, 0, 0,
-                   {aq, (const float2*)meta, (const float*)meta, (const int32_t*)(meta + p.act_rows * (p.k / 64))}, p.ids, p.weights, p.add,
-                   p.out, p.q};
-    if (p.type == AMV_T_Q4_0) mo_go<AMV_T_Q4_0>(a, n, gu, p.st);
-    else if (p.type == AMV_T_Q8_0) mo_go<AMV_T_Q8_0>(a, n, gu, p.st);
-    else if (p.type == AMV_T_Q4_K) mo_go<AMV_T_Q4_K>(a, n, gu, p.st);
-    else mo_go<AMV_T_Q6_K>(a, n, gu, p.st);
-    return amv_check_launch("amv_moe products");
 }
 
 int moe_few(const MoeProduct& p) {
