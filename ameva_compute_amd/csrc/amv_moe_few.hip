@@ -8,7 +8,7 @@
 // Result D of lane l: weight row l % 16, token l / 16, blocks 0..3 in its four registers: the block epilogue is a sum within the lane.
 // Measured, with cold weights: gate and up of 48 tokens with 8 of 64 experts of 1024 x 2048 Q4_0 40 us, 3.8 TB/s; down of 40 tokens,
 // 2048 x 1408 Q8_0, 43 us, 4.6 TB/s.
-#include "amv_moe.h"
+#include "amv_moe_dot.h"
 
 #include <type_traits>
 
@@ -265,7 +265,7 @@ struct Mf<AMV_T_Q6_K, U> {
 struct MfArgs {
     const uint8_t *w0, *w1;
     int64_t stride, bytes;
-    int rows, n_k, n_expert, act_div, n_cols, kc;
+    int rows, n_k, n_expert, act_div, n_cols, kc, dot;  // dot: tiles of up to so many rows by dot products
     MfAct act;
     const int2* tiles;
     const int32_t* order;
@@ -287,6 +287,61 @@ __host__ __device__ inline MfLds mf_lds(int kc, int r, int kg, int nw) {
     l.red = l.u + 4 * SUMS * r * (cs + 1);
     l.total = l.red + 4 * kg * r * nw * 17;
     return l;
+}
+
+// v[0], v[2], v[1], v[3] summed over the wave in its four rows of 16 lanes
+__device__ __forceinline__ float mf_sum4(const float (&v)[4]) {
+    const auto half = [](float x, float y) {  // x in the lower half, y in the upper one
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    };
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(half(v[0], v[1])), __float_as_uint(half(v[2], v[3])), false, false);
+    return amv_row16_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// A tile of up to NR rows by dot products, lanes along the weight rows: its loads are runs of 1 KB where the matrix core's operand wants 64 bytes of
+// 16 rows, but each row costs vector work, so it is for one or two rows (Q8_0, without nibbles to take apart: four), and for a k that fills the
+// lanes. us, matrix core / dot products: 64 experts of gate and up 1024 x 2048, 16 tokens x 8, Q4_0 34 / 28, Q4_K 36 / 30, Q6_K 48 / 44, Q8_0 54 /
+// 51; 8 experts of 6144 x 4096, 6 x 2, Q4_0 45 / 35, Q6_K 67 / 55; with tiles of up to four rows Q4_0 32, Q4_K 36; with k of 1024, half
+// of the lanes, 8 tokens' down Q4_K 18 / 24. A wave has WR weight rows, four at a time (gate and up: two columns of both), over all of k;
+// sums to red[group of 16 weight rows][row][weight row % 16].
+template <int WT, int NR, bool GU, int NW, int WR>
+__device__ __forceinline__ void mf_dot(const uint8_t* m0, const uint8_t* m1, int rows, int units, int n0, int wave, const MoAct& act, const int32_t* order,
+                                       int count, int act_div, float (*red)[MOE_FEW][17]) {
+    using T = Mo<WT>;
+    const int lane = threadIdx.x & 63;
+    int row[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) row[r] = order[min(r, count - 1)] / act_div;
+    for (int g = wave * (WR / 4); g < (wave + 1) * (WR / 4); ++g) {
+        const uint8_t* const m[2] = {m0, GU ? m1 : m0};
+        const int n[2] = {min(GU ? n0 + 2 * g : n0 + 4 * g, rows - 2), min(GU ? n0 + 2 * g : n0 + 4 * g + 2, rows - 2)};
+        float acc[NR][4];
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[r][i] = 0.0f;
+        for (int s = 0; s < units; s += 64) {
+            const int j = min(s + lane, units - 1);
+            typename T::W w[2];
+            typename T::A a[NR];
+            T::load(w[0], m[0], rows, units, n[0], j);
+            T::load(w[1], m[1], rows, units, n[1], j);
+#pragma unroll
+            for (int r = 0; r < NR; ++r) T::load(a[r], act, row[r], units, j);
+            __builtin_amdgcn_sched_barrier(0);  // (all loads before the first product)
+            if (s + lane < units)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) T::add(w[i], a, j, acc, 2 * i);
+        }
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const float v = mf_sum4(acc[r]);
+            const int at = ((lane >> 4) & 1) * 2 + (lane >> 5);  // which of the four
+            const int c = GU ? (at >> 1) * (8 * NW) + 2 * g + (at & 1) : 4 * g + at;
+            if ((lane & 15) == 0) red[c >> 4][r][c & 15] = v;
+        }
+    }
 }
 
 template <int WT, int U, bool GU, int NW, int KG>
@@ -313,7 +368,21 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
     float acc[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) acc[g] = 0.0f;
-    if (e < p.n_expert) {
+    constexpr int WR = 16 * NW / (NW * KG);  // weight rows of a wave
+    const bool dot = count <= p.dot && e < p.n_expert;
+    if (dot) {
+        const MoAct act{p.act.q, reinterpret_cast<const int2*>(p.act.d0), p.act.dk, p.act.s16};
+        const uint8_t *const m0 = p.w0 + e * p.stride, *const m1 = GU ? p.w1 + e * p.stride : m0;
+        const int units = KQ ? 8 * p.n_k : p.n_k;
+        const auto go = [&](auto nr) __attribute__((always_inline)) {
+            mf_dot<WT, decltype(nr)::value, GU, NW, WR>(m0, m1, p.rows, units, n0, wv, act, p.order + t.y, count, p.act_div, s_red[0]);
+        };
+        if (count == 1) go(std::integral_constant<int, 1>());
+        else if (count == 2) go(std::integral_constant<int, 2>());
+        else if constexpr (WT == AMV_T_Q8_0) go(std::integral_constant<int, 4>());
+        if constexpr (KG > 1)
+            for (int i = tid; i < (KG - 1) * NW * R * 17; i += NT) (&s_red[1][0][0][0])[i] = 0.0f;
+    } else if (e < p.n_expert) {
         const uint8_t* const m = (GU && nw >= NW / 2 ? p.w1 : p.w0) + e * p.stride;
         const __amdgpu_buffer_rsrc_t buf = MF_RSRC(m, p.bytes);
         const int n = min(n0 + 16 * (GU ? nw % (NW / 2) : nw) + c16, p.rows - 1);
@@ -398,8 +467,9 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
             else go(std::integral_constant<int, G>());
         }
     }
+    if (!dot)
 #pragma unroll
-    for (int g = 0; g < G; ++g) s_red[kw][nw][4 * g + q][c16] = acc[g];
+        for (int g = 0; g < G; ++g) s_red[kw][nw][4 * g + q][c16] = acc[g];
     __syncthreads();
     // thread: row i and column f (a block of the 8-bit output is 32 lanes)
     for (int i = tid / COLS; i < count; i += NT / COLS) {
@@ -456,8 +526,10 @@ int moe_few(const MoeProduct& p) {
     const bool kq = p.type == AMV_T_Q4_K || p.type == AMV_T_Q6_K, gu = p.w1 != nullptr;
     const int8_t* aq = (const int8_t*)p.act;
     const int8_t* meta = aq + p.act_rows * p.k;
+    const int units = (int)(p.k / 32), lanes = (units + 63) / 64 * 64;
+    const int dot = 4 * units < 3 * lanes ? 0 : p.type == AMV_T_Q8_0 ? 4 : 2;
     const MfArgs a{(const uint8_t*)p.w0, (const uint8_t*)p.w1, p.stride, amv_weight_bytes(p.type, p.rows, p.k), (int)p.rows,
-                   (int)(p.k / (kq ? 256 : 32)), p.n_expert, gu ? p.n_used : 1, 0, 0,
+                   (int)(p.k / (kq ? 256 : 32)), p.n_expert, gu ? p.n_used : 1, 0, 0, dot,
                    {aq, (const float2*)meta, (const float*)meta, (const int32_t*)(meta + p.act_rows * (p.k / 64))}, v.few, v.order,
                    p.out, p.q};
     AMV_REQUIRE((int64_t)v.n_few * ((p.rows + 31) / 32) < 1 << 23, "moe: %d tiles of %lld columns are too many", v.n_few, (long long)p.rows);

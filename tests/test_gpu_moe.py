@@ -152,7 +152,9 @@ SHAPES = [  # tokens, experts, used, rows, k in blocks, kind
     # more experts a token than a workgroup has waves; a plan of more than 4096 pairs with few of them an expert
     (1, 70, 20, 64, 3, "skewed"), (1, 64, 64, 32, 6, "skewed"), (3, 70, 64, 32, 2, "skewed"), (700, 1024, 8, 32, 1, "holes"),
     # the most of a tile's rows that LDS holds at once
-    (13, 4, 2, 96, 14, "holes")]
+    (13, 4, 2, 96, 14, "holes"),
+    # a k that fills the lanes, one to a few rows an expert
+    (5, 4, 2, 96, 64, "holes"), (17, 10, 4, 160, 64, "skewed"), (6, 12, 3, 32, 64, "skewed"), (7, 3, 1, 288, 64, "one")]
 
 
 def make(t, shape, seed=0):
@@ -160,6 +162,8 @@ def make(t, shape, seed=0):
     k = kb * (32 if t in (Q4_0, Q8_0) else 256)
     if kb == 14:
         k = 3584
+    if kb == 64:
+        k = 2048
     if kb == 57:  # longer than what LDS holds of a tile's rows: parts of it, the last one not whole
         k = 7264 if t in (Q4_0, Q8_0) else 7424
     g = gen(seed + tok + rows)
@@ -247,12 +251,12 @@ def test_tokens_without_a_plan(t):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("tok", [1, 9, 150])
-def test_what_no_token_reads_does_not_matter(t, tok):
+@pytest.mark.parametrize("tok,k", [(1, 512), (9, 512), (150, 512), (1, 2048), (5, 2048)])
+def test_what_no_token_reads_does_not_matter(t, tok, k):
     """Experts without tokens hold no numbers at all; rows and weights of pairs without an expert neither; a token with an infinite or
     absent number keeps it to itself."""
     from ameva_compute_amd import ops
-    n, used, rows, k = 6, 2, 64, 512
+    n, used, rows = 6, 2, 64
     g = gen(tok)
     ids = torch.stack([torch.randint(1, 3, (tok,), generator=g, device=DEV), torch.randint(3, 5, (tok,), generator=g, device=DEV)], 1).int()
     ids[tok // 2, 1] = -1
