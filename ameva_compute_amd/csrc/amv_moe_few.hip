@@ -290,13 +290,16 @@ __host__ __device__ inline MfLds mf_lds(int kc, int r, int kg, int nw) {
 }
 
 // v[0], v[2], v[1], v[3] summed over the wave in its four rows of 16 lanes
+__device__ __forceinline__ float mf_sum2(float x, float y) {  // of the wave's halves: x's sums in rows 0 and 2, y's in rows 1 and 3
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return amv_row16_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
 __device__ __forceinline__ float mf_sum4(const float (&v)[4]) {
     const auto half = [](float x, float y) {  // x in the lower half, y in the upper one
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
         return __uint_as_float(r[0]) + __uint_as_float(r[1]);
     };
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(half(v[0], v[1])), __float_as_uint(half(v[2], v[3])), false, false);
-    return amv_row16_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+    return mf_sum2(half(v[0], v[1]), half(v[2], v[3]));
 }
 
 // A tile of up to NR rows by dot products, lanes along the weight rows: its loads are runs of 1 KB where the matrix core's operand wants 64 bytes of
@@ -304,16 +307,19 @@ __device__ __forceinline__ float mf_sum4(const float (&v)[4]) {
 // lanes. us, matrix core / dot products: 64 experts of gate and up 1024 x 2048, 16 tokens x 8, Q4_0 34 / 28, Q4_K 36 / 30, Q6_K 48 / 44, Q8_0 54 /
 // 51; 8 experts of 6144 x 4096, 6 x 2, Q4_0 45 / 35, Q6_K 67 / 55; with tiles of up to four rows Q4_0 32, Q4_K 36; with k of 1024, half
 // of the lanes, 8 tokens' down Q4_K 18 / 24. A wave has WR weight rows, four at a time (gate and up: two columns of both), over all of k;
-// sums to red[group of 16 weight rows][row][weight row % 16].
-template <int WT, int NR, bool GU, int NW, int WR>
+// sums to red[group of 16 weight rows][row][weight row % 16]. H: the wave's parts of 64 / H lanes have four weight rows each (a short k).
+template <int WT, int NR, bool GU, int NW, int WR, int H>
 __device__ __forceinline__ void mf_dot(const uint8_t* m0, const uint8_t* m1, int rows, int units, int n0, int wave, const MoAct& act, const int32_t* order,
                                        int count, int act_div, float (*red)[MOE_FEW][17]) {
     using T = Mo<WT>;
-    const int lane = threadIdx.x & 63;
+    static_assert(!GU || H == 1, "");
+    constexpr int L = 64 / H;
+    const int lane = threadIdx.x & 63, at_k = lane % L;
     int row[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) row[r] = order[min(r, count - 1)] / act_div;
-    for (int g = wave * (WR / 4); g < (wave + 1) * (WR / 4); ++g) {
+    for (int g0 = wave * (WR / 4); g0 < (wave + 1) * (WR / 4); g0 += H) {
+        const int g = g0 + lane / L;
         const uint8_t* const m[2] = {m0, GU ? m1 : m0};
         const int n[2] = {min(GU ? n0 + 2 * g : n0 + 4 * g, rows - 2), min(GU ? n0 + 2 * g : n0 + 4 * g + 2, rows - 2)};
         float acc[NR][4];
@@ -321,8 +327,8 @@ __device__ __forceinline__ void mf_dot(const uint8_t* m0, const uint8_t* m1, int
         for (int r = 0; r < NR; ++r)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[r][i] = 0.0f;
-        for (int s = 0; s < units; s += 64) {
-            const int j = min(s + lane, units - 1);
+        for (int s = 0; s < units; s += L) {
+            const int j = min(s + at_k, units - 1);
             typename T::W w[2];
             typename T::A a[NR];
             T::load(w[0], m[0], rows, units, n[0], j);
@@ -330,12 +336,21 @@ __device__ __forceinline__ void mf_dot(const uint8_t* m0, const uint8_t* m1, int
 #pragma unroll
             for (int r = 0; r < NR; ++r) T::load(a[r], act, row[r], units, j);
             __builtin_amdgcn_sched_barrier(0);  // (all loads before the first product)
-            if (s + lane < units)
+            if (s + at_k < units)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) T::add(w[i], a, j, acc, 2 * i);
         }
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
+            if constexpr (H == 2) {
+                const float v = mf_sum2(acc[r][0], acc[r][1]), u = mf_sum2(acc[r][2], acc[r][3]);
+                const int c = 4 * g + ((lane >> 4) & 1);
+                if ((lane & 15) == 0) {
+                    red[c >> 4][r][c & 15] = v;
+                    red[c >> 4][r][(c & 15) + 2] = u;
+                }
+                continue;
+            }
             const float v = mf_sum4(acc[r]);
             const int at = ((lane >> 4) & 1) * 2 + (lane >> 5);  // which of the four
             const int c = GU ? (at >> 1) * (8 * NW) + 2 * g + (at & 1) : 4 * g + at;
@@ -375,7 +390,9 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
         const uint8_t *const m0 = p.w0 + e * p.stride, *const m1 = GU ? p.w1 + e * p.stride : m0;
         const int units = KQ ? 8 * p.n_k : p.n_k;
         const auto go = [&](auto nr) __attribute__((always_inline)) {
-            mf_dot<WT, decltype(nr)::value, GU, NW, WR>(m0, m1, p.rows, units, n0, wv, act, p.order + t.y, count, p.act_div, s_red[0]);
+            constexpr int N = decltype(nr)::value;
+            if (!GU && units <= 32) mf_dot<WT, N, GU, NW, WR, GU ? 1 : 2>(m0, m1, p.rows, units, n0, wv, act, p.order + t.y, count, p.act_div, s_red[0]);
+            else mf_dot<WT, N, GU, NW, WR, 1>(m0, m1, p.rows, units, n0, wv, act, p.order + t.y, count, p.act_div, s_red[0]);
         };
         if (count == 1) go(std::integral_constant<int, 1>());
         else if (count == 2) go(std::integral_constant<int, 2>());
@@ -526,7 +543,7 @@ int moe_few(const MoeProduct& p) {
     const bool kq = p.type == AMV_T_Q4_K || p.type == AMV_T_Q6_K, gu = p.w1 != nullptr;
     const int8_t* aq = (const int8_t*)p.act;
     const int8_t* meta = aq + p.act_rows * p.k;
-    const int units = (int)(p.k / 32), lanes = (units + 63) / 64 * 64;
+    const int units = (int)(p.k / 32), lanes = !gu && units <= 32 ? 32 : (units + 63) / 64 * 64;
     const int dot = 4 * units < 3 * lanes ? 0 : p.type == AMV_T_Q8_0 ? 4 : 2;
     const MfArgs a{(const uint8_t*)p.w0, (const uint8_t*)p.w1, p.stride, amv_weight_bytes(p.type, p.rows, p.k), (int)p.rows,
                    (int)(p.k / (kq ? 256 : 32)), p.n_expert, gu ? p.n_used : 1, 0, 0, dot,

@@ -9,14 +9,16 @@
 
 #include <algorithm>
 
-// rows n[i] and n[i] + 1 of matrix m[i], M times, times activation row `row`, part of parts of k. All loads of a step before its products;
+// rows n[i] and n[i] + 1 of matrix m[i], M times, times activation row `row`, part of parts of k; H: the wave's parts of 64 / H lanes have rows
+// of their own (n then differs between them). All loads of a step before its products;
 // the loads of a second step beside them were slower (two experts of 4096 x 14336 Q4_0 14 us, so 13; 32 rows of 2048 x 4096 Q6_K 24, so 22).
-template <int WT, int M>
+template <int WT, int M, int H>
 __device__ __forceinline__ void mo_rows(const uint8_t* const (&m)[M], int rows, int units, const int (&n)[M], const MoAct& act, int64_t row, int part,
                                         int parts, float (&acc)[1][2 * M]) {
     using T = Mo<WT>;
-    const int lane = threadIdx.x & 63;
-    for (int s = 64 * part; s < units; s += 64 * parts) {
+    constexpr int L = 64 / H;
+    const int lane = threadIdx.x % L;
+    for (int s = L * part; s < units; s += L * parts) {
         typename T::W w[M];
         typename T::A a[1];
         const int j = min(s + lane, units - 1);
@@ -29,7 +31,7 @@ __device__ __forceinline__ void mo_rows(const uint8_t* const (&m)[M], int rows, 
             for (int i = 0; i < M; ++i) T::add(w[i], a, j, acc, 2 * i);
     }
 #pragma unroll
-    for (int i = 0; i < 2 * M; ++i) acc[0][i] = amv_wave_sum(acc[0][i]);
+    for (int i = 0; i < 2 * M; ++i) acc[0][i] = H == 1 ? amv_wave_sum(acc[0][i]) : amv_sum_x16(amv_row16_sum(acc[0][i]));
 }
 
 #define MO_PAIRS 2  // pairs of columns of a wave of the down product
@@ -54,7 +56,7 @@ __global__ __launch_bounds__(1024) void k_moe_one_gate_up(const MoArgs p) {
     if (e >= 0 && e < p.n_expert) {
         const uint8_t* const m[2] = {p.w0 + e * p.stride, p.w1 + e * p.stride};
         const int n[2] = {n0 + 2 * wv, n0 + 2 * wv};
-        mo_rows<WT, 2>(m, p.rows, p.units, n, p.act, pair / p.n_used, 0, 1, acc);
+        mo_rows<WT, 2, 1>(m, p.rows, p.units, n, p.act, pair / p.n_used, 0, 1, acc);
     }
     if (lane == 0) *reinterpret_cast<float4*>(s_red[wv]) = make_float4(acc[0][0], acc[0][1], acc[0][2], acc[0][3]);
     __syncthreads();
@@ -68,15 +70,15 @@ __global__ __launch_bounds__(1024) void k_moe_one_gate_up(const MoArgs p) {
     }
 }
 
-template <int WT>
+template <int WT, int H>
 __global__ __launch_bounds__(1024) void k_moe_one_down(const MoArgs p) {
-    constexpr int G = MO_PAIRS;
-    __shared__ __align__(16) float s_red[MOE_MAX_USED][2 * G];
+    constexpr int G = MO_PAIRS, C = 2 * G * H;  // columns of a wave
+    __shared__ __align__(16) float s_red[MOE_MAX_USED][C];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int t = blockIdx.x / p.n_cols, n0 = 2 * G * p.groups * (blockIdx.x % p.n_cols);
-    // job: 2 G columns, expert, part (in turns where there are more than waves)
+    const int t = blockIdx.x / p.n_cols, n0 = C * p.groups * (blockIdx.x % p.n_cols);
+    // job: C columns, expert, part (in turns where there are more than waves)
     for (int job = wv; job < p.groups * p.n_used * p.parts; job += blockDim.x >> 6) {
-        const int part = job % p.parts, j = job / p.parts % p.n_used, c = n0 + 2 * G * (job / (p.parts * p.n_used));
+        const int part = job % p.parts, j = job / p.parts % p.n_used, c = n0 + C * (job / (p.parts * p.n_used)) + 2 * G * (lane / (64 / H));
         const int e = p.ids[t * p.n_used + j];
         float acc[1][2 * G] = {};
         if (e >= 0 && e < p.n_expert) {
@@ -87,21 +89,21 @@ __global__ __launch_bounds__(1024) void k_moe_one_down(const MoArgs p) {
                 m[i] = p.w0 + e * p.stride;
                 n[i] = min(c + 2 * i, p.rows - 2);
             }
-            mo_rows<WT, G>(m, p.rows, p.units, n, p.act, (int64_t)t * p.n_used + j, part, p.parts, acc);
+            mo_rows<WT, G, H>(m, p.rows, p.units, n, p.act, (int64_t)t * p.n_used + j, part, p.parts, acc);
         }
-        if (lane == 0)
+        if (lane % (64 / H) == 0)
 #pragma unroll
-            for (int i = 0; i < G; ++i) *reinterpret_cast<float2*>(s_red[job] + 2 * i) = make_float2(acc[0][2 * i], acc[0][2 * i + 1]);
+            for (int i = 0; i < G; ++i) *reinterpret_cast<float2*>(s_red[job] + 2 * G * (lane / (64 / H)) + 2 * i) = make_float2(acc[0][2 * i], acc[0][2 * i + 1]);
     }
     __syncthreads();
-    if (tid >= 2 * G * p.groups || n0 + tid >= p.rows) return;
+    if (tid >= C * p.groups || n0 + tid >= p.rows) return;
     const int64_t at = (int64_t)t * p.rows + n0 + tid;
     float v = p.add ? p.add[at] : 0.0f;
     for (int j = 0; j < p.n_used; ++j) {
         const int e = p.ids[t * p.n_used + j];
         if (e < 0 || e >= p.n_expert) continue;
         float y = 0.0f;
-        for (int z = 0; z < p.parts; ++z) y += s_red[(tid / (2 * G) * p.n_used + j) * p.parts + z][tid % (2 * G)];
+        for (int z = 0; z < p.parts; ++z) y += s_red[(tid / C * p.n_used + j) * p.parts + z][tid % C];
         v = fmaf(p.weights[t * p.n_used + j], y, v);
     }
     p.out[at] = v;
@@ -117,12 +119,16 @@ static void mo_go(MoArgs a, int64_t n, bool gu, hipStream_t st) {
     // eight waves (a wave an expert where there are more): parts of k, as many as bring eight waves a CU, then columns. Sixteen were slower or equal
     // (two experts of 4096 x 14336 Q4_0 20 us, so 13), two columns a wave too (eight of 4096 x 2048 Q4_0 15, so 12); of one expert of 2048 x 8192
     // Q8_0 one part takes 9, two 7, four 6.
+    // H: a k of up to 32 units leaves room for the rows of two waves in one
+    const int H = a.units <= 32 ? 2 : 1, C = 2 * MO_PAIRS * H;
     const int room = std::max(1, 8 / a.n_used), steps = (a.units + 63) / 64;
-    const int64_t waves = n * (a.rows / (2 * MO_PAIRS)) * a.n_used;
+    const int64_t waves = n * (a.rows / C) * a.n_used;
     a.parts = (int)std::min<int64_t>(std::min(room, steps), std::max<int64_t>(1, 2048 / waves));
     a.groups = std::max(1, room / a.parts);
-    a.n_cols = (a.rows + 2 * MO_PAIRS * a.groups - 1) / (2 * MO_PAIRS * a.groups);
-    k_moe_one_down<WT><<<(unsigned)(n * a.n_cols), 64 * std::min(16, a.n_used * a.parts * a.groups), 0, st>>>(a);
+    a.n_cols = (a.rows + C * a.groups - 1) / (C * a.groups);
+    const dim3 grid((unsigned)(n * a.n_cols)), block(64 * std::min(16, a.n_used * a.parts * a.groups));
+    if (H == 2) k_moe_one_down<WT, 2><<<grid, block, 0, st>>>(a);
+    else k_moe_one_down<WT, 1><<<grid, block, 0, st>>>(a);
 }
 
 int moe_one(const MoeProduct& p) {

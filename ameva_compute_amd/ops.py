@@ -922,9 +922,10 @@ def moe_plan(ids: torch.Tensor, n_expert: int) -> MoePlan:
     n = lib().amv_moe_plan_bytes(t, u, n_expert)
     if n < 0:
         check(-1, "amv_moe_plan_bytes")
-    # up to four tokens that mostly meet different experts: each pair's weights read for itself, without a plan and without a launch for the
-    # sums, cost less than the tiles (4 tokens, 8 of 64 experts of 2048 x 1024 Q4_0, both products: 30 us, 34 with the plan's 4; 6 tokens 42, 36)
-    if t <= 1 or (t <= 4 and t * u <= n_expert):
+    # up to six tokens that mostly meet different experts: each pair's weights read for itself, without a plan and without a launch for the
+    # sums, cost less than the tiles (us of both products, without / with the plan's 4: 8 of 64 experts of 1024 x 2048 Q4_0, 4 tokens 26 / 32, 6 35 /
+    # 35; 8 of 128, 6 tokens 35 / 41, Q6_K 52 / 54, 8 tokens 66 / 59; 2 of 8 experts of 6144 x 4096, 2 tokens 33 / 39, 4 57 / 56)
+    if t <= 1 or (t <= 6 and 2 * t * u <= n_expert):
         return MoePlan(ids, n_expert, None)
     buf = torch.empty(n, dtype=torch.uint8, device=ids.device)
     check(lib().amv_moe_plan(ids.data_ptr(), t, u, n_expert, buf.data_ptr(), _stream()), "amv_moe_plan")
