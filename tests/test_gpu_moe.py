@@ -351,7 +351,7 @@ def test_layer(t, t2, tok):
     assert bool(((y.double() - ref).abs() <= lim).all())
 
 
-@pytest.mark.parametrize("tok", [1, 4, 70])
+@pytest.mark.parametrize("tok", [1, 2, 4, 70])
 def test_captured_layer(tok):
     """A captured layer replayed over other inputs, another stream beside it, against the eager calls."""
     from ameva_compute_amd import ops
