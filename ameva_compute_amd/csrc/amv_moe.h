@@ -56,6 +56,12 @@ int moe_one(const MoeProduct& p);   // amv_moe_one.hip: without a plan
 int moe_few(const MoeProduct& p);   // amv_moe_few.hip
 int moe_many(const MoeProduct& p);  // amv_moe_many.hip
 
+// amv_ld_stream of four floats
+__device__ __forceinline__ float4 moe_ld_stream(const float4* p) {
+    const uint4 v = amv_ld_stream(reinterpret_cast<const uint4*>(p));
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+
 // four int32 at an address of any whole int32 (a Q8_K buffer's sums begin where its scales end)
 typedef int moe_i4 __attribute__((ext_vector_type(4), aligned(4)));
 

@@ -7,7 +7,8 @@
 // ---------------------------------------------------------------------------------------------------------------- norm
 // sum = x + add; o = sum / sqrt(mean(sum^2) + eps) * w, act = o in 8 bits, one workgroup per row, the row in registers in
 // between. The squares are f32 products summed in 64 bits and mean, root and quotient are rounded as amv_rms_norm's. Bound by memory: 4096
-// rows of 4096 with a Q8_K output are 0.29 GB in 67 us, 4.3 TB/s; one row takes 5.6, a launch and two dependent passes.
+// rows of 4096 with a Q8_K output are 0.29 GB in 58 us, 5.0 TB/s (72 with loads that leave x and add in the caches); one row takes 5.6, a
+// launch and two dependent passes.
 template <int NT, int R>
 __global__ __launch_bounds__(NT) void k_add_rms_norm(const float* x, const float* add, int n4, float eps,
                                                      const float* __restrict__ w, float* sum, float* __restrict__ o,
@@ -26,7 +27,7 @@ __global__ __launch_bounds__(NT) void k_add_rms_norm(const float* x, const float
         for (int r = 0; r < R; ++r) {
             const int c = c0 + tid + NT * r;
             const float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const float4 a = c < n4 ? x4[c] : z, b = c < n4 ? a4[c] : z;
+            const float4 a = c < n4 ? moe_ld_stream(x4 + c) : z, b = c < n4 ? moe_ld_stream(a4 + c) : z;
             if (n4 <= NT * R) ww[r] = c < n4 && w ? w4[c] : z;
             v[r] = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
         }
@@ -86,7 +87,7 @@ extern "C" int amv_add_rms_norm_act(const float* x, const float* add, int64_t n_
     const int n4 = (int)(n / 4);
     const dim3 grid((unsigned)n_rows);
     // few rows: as many threads a row as load it at once; many: the waves of several rows on a CU hide one another's latencies, so fewer
-    // (4096 rows of 4096, us: 1024 threads 71, 256 threads of 4 chunks 68)
+    // (4096 rows of 4096, us: 1024 threads 71, 256 threads of 4 chunks 68, both with loads through the caches)
     if (n4 <= 256) k_add_rms_norm<256, 1><<<grid, 256, 0, amv_stream(stream)>>>(x, add, n4, eps, w, sum, o, q);
     else if (n_rows >= 1024 && n4 <= 512) k_add_rms_norm<256, 2><<<grid, 256, 0, amv_stream(stream)>>>(x, add, n4, eps, w, sum, o, q);
     else if (n_rows >= 1024 && n4 <= 1024) k_add_rms_norm<256, 4><<<grid, 256, 0, amv_stream(stream)>>>(x, add, n4, eps, w, sum, o, q);
@@ -577,12 +578,12 @@ __global__ __launch_bounds__(256) void k_moe_combine(const float* __restrict__ y
     const int c = blockIdx.x * 256 + threadIdx.x;
     const int64_t t = blockIdx.y;
     if (c >= n4) return;
-    float4 s = add ? reinterpret_cast<const float4*>(add)[t * n4 + c] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float4 s = add ? moe_ld_stream(reinterpret_cast<const float4*>(add) + t * n4 + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int j = 0; j < n_used; ++j) {
         const int e = ids[t * n_used + j];
         if (e < 0 || e >= n_expert) continue;
         const float w = weights[t * n_used + j];
-        const float4 v = reinterpret_cast<const float4*>(y)[(t * n_used + j) * n4 + c];
+        const float4 v = moe_ld_stream(reinterpret_cast<const float4*>(y) + (t * n_used + j) * n4 + c);
         s = make_float4(fmaf(w, v.x, s.x), fmaf(w, v.y, s.y), fmaf(w, v.z, s.z), fmaf(w, v.w, s.w));
     }
     reinterpret_cast<float4*>(out)[t * n4 + c] = s;

@@ -289,11 +289,12 @@ __host__ __device__ inline MfLds mf_lds(int kc, int r, int kg, int nw) {
     return l;
 }
 
-// v[0], v[2], v[1], v[3] summed over the wave in its four rows of 16 lanes
-__device__ __forceinline__ float mf_sum2(float x, float y) {  // of the wave's halves: x's sums in rows 0 and 2, y's in rows 1 and 3
+// sums over each half of the wave, for the 16 lanes of a row: x's in rows 0 and 2, y's in rows 1 and 3
+__device__ __forceinline__ float mf_sum2(float x, float y) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
     return amv_row16_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
+// sums over the wave: v[0], v[2], v[1], v[3] in its four rows
 __device__ __forceinline__ float mf_sum4(const float (&v)[4]) {
     const auto half = [](float x, float y) {  // x in the lower half, y in the upper one
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
@@ -305,8 +306,8 @@ __device__ __forceinline__ float mf_sum4(const float (&v)[4]) {
 // A tile of up to NR rows by dot products, lanes along the weight rows: its loads are runs of 1 KB where the matrix core's operand wants 64 bytes of
 // 16 rows, but each row costs vector work, so it is for one or two rows (Q8_0, without nibbles to take apart: four), and for a k that fills the
 // lanes. us, matrix core / dot products: 64 experts of gate and up 1024 x 2048, 16 tokens x 8, Q4_0 34 / 28, Q4_K 36 / 30, Q6_K 48 / 44, Q8_0 54 /
-// 51; 8 experts of 6144 x 4096, 6 x 2, Q4_0 45 / 35, Q6_K 67 / 55; with tiles of up to four rows Q4_0 32, Q4_K 36; with k of 1024, half
-// of the lanes, 8 tokens' down Q4_K 18 / 24. A wave has WR weight rows, four at a time (gate and up: two columns of both), over all of k;
+// 51; 8 experts of 6144 x 4096, 6 x 2, Q4_0 45 / 35, Q6_K 67 / 55; with tiles of up to four rows Q4_0 32, Q4_K 36; with half of
+// the lanes idle, 8 tokens' down Q4_K 18 / 24. A wave has WR weight rows, four at a time (gate and up: two columns of both), over all of k;
 // sums to red[group of 16 weight rows][row][weight row % 16]. H: the wave's parts of 64 / H lanes have four weight rows each (a short k).
 template <int WT, int NR, bool GU, int NW, int WR, int H>
 __device__ __forceinline__ void mf_dot(const uint8_t* m0, const uint8_t* m1, int rows, int units, int n0, int wave, const MoAct& act, const int32_t* order,
