@@ -7,7 +7,7 @@
 // ---------------------------------------------------------------------------------------------------------------- norm
 // sum = x + add; o = sum / sqrt(mean(sum^2) + eps) * w, act = o in 8 bits, one workgroup per row, the row in registers in
 // between. The squares are f32 products summed in 64 bits and mean, root and quotient are rounded as amv_rms_norm's. Bound by memory: 4096
-// rows of 4096 with a Q8_K output are 0.29 GB in 58 us, 5.0 TB/s (72 with loads that leave x and add in the caches); one row takes 5.6, a
+// rows of 4096 with a Q8_K output are 0.29 GB in 54 us, 5.4 TB/s (67 with loads that leave x and add in the caches); one row takes 5.6, a
 // launch and two dependent passes.
 template <int NT, int R>
 __global__ __launch_bounds__(NT) void k_add_rms_norm(const float* x, const float* add, int n4, float eps,
@@ -571,7 +571,7 @@ extern "C" int amv_moe_gate_up(int wtype, const void* w_gate, const void* w_up, 
 }
 
 // out[t][n] = add[t][n] + sum_j weights[t][j] y[t n_used + j][n] over the pairs with an expert, in the order of j: 32768 pairs of 2048 are
-// 0.34 GB in 55 us. (The products cannot add to out themselves: the sums' order would not be one.)
+// 0.34 GB in 48 us. (The products cannot add to out themselves: the sums' order would not be one.)
 __global__ __launch_bounds__(256) void k_moe_combine(const float* __restrict__ y, const int32_t* __restrict__ ids,
                                                      const float* __restrict__ weights, int n_used, int n_expert, int n4,
                                                      const float* add, float* out) {
