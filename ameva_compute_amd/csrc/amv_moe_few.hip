@@ -385,7 +385,9 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(4)
 #pragma unroll
     for (int g = 0; g < G; ++g) acc[g] = 0.0f;
     constexpr int WR = 16 * NW / (NW * KG);  // weight rows of a wave
-    const bool dot = count <= p.dot && e < p.n_expert;
+    // (an expert's only tile: which of its rows are in a last small tile is chance, and the two ways round differently)
+    const int2 prev = p.tiles[max(tile - 1, 0)];
+    const bool dot = count <= p.dot && e < p.n_expert && !(tile && prev.x >> 16 && (prev.x & 0xFFFF) == e);
     if (dot) {
         const MoAct act{p.act.q, reinterpret_cast<const int2*>(p.act.d0), p.act.dk, p.act.s16};
         const uint8_t *const m0 = p.w0 + e * p.stride, *const m1 = GU ? p.w1 + e * p.stride : m0;

@@ -490,3 +490,18 @@ def test_outputs_beyond_32_bits():
     w = weights[-last:].double()[..., None]
     lim = rounding(down) * (w * size).sum(1) + used * 2.0 ** -24 * (w * p).abs().sum(1) * 1.01 + 1e-30
     assert bool(((y[-last:].double() - (w * p).sum(1)).abs() <= lim).all())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tok", [2, 5, 17, 18, 20, 35, 66, 130])
+def test_a_row_s_place_changes_nothing(t, tok):
+    """Equal rows of one expert come out equal, bit for bit, wherever the plan (whose order within an expert is any) puts them."""
+    from ameva_compute_amd import ops
+    n, rows, k = 3, 96, 2048
+    gate, up, down = (Experts(t, n, rows, k, s) for s in (1, 2, 3))
+    ids = torch.full((tok, 1), 1, dtype=torch.int32, device=DEV)
+    act = ops.quantize_act(torch.randn(1, k, generator=gen(tok), device=DEV).repeat(tok, 1).contiguous(), ACT[t])[0]
+    plan = ops.moe_plan(ids, n)
+    h = ops.moe_gate_up(gate.gpu, up.gpu, act, plan, act_type=None)
+    y = ops.moe_down(down.gpu, act, plan, torch.ones(tok, 1, device=DEV))
+    assert torch.equal(h, h[:1].expand_as(h)) and torch.equal(y, y[:1].expand_as(y))
