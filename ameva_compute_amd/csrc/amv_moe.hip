@@ -514,9 +514,8 @@ static int moe_product(const MoeProduct& p) {
     return many ? moe_many(p) : moe_few(p);
 }
 
+// (p's counts are checked before, in the 64 bits they come in: moe_check_pairs)
 static int moe_check_product(const char* what, const MoeProduct& p) {
-    const int rc = moe_check_pairs(what, p.n_tok, p.n_used, p.n_expert);
-    if (rc) return rc;
     AMV_REQUIRE(p.type == AMV_T_Q4_0 || p.type == AMV_T_Q8_0 || p.type == AMV_T_Q4_K || p.type == AMV_T_Q6_K,
                 "%s: weight type %d is not supported (Q4_0, Q8_0, Q4_K, Q6_K are)", what, p.type);
     const bool kq = p.type == AMV_T_Q4_K || p.type == AMV_T_Q6_K;
@@ -542,10 +541,12 @@ extern "C" int amv_moe_gate_up(int wtype, const void* w_gate, const void* w_up, 
                                int64_t k, const void* act, int64_t n_tok, int64_t n_used, const int32_t* ids, const void* plan,
                                float* eout, void* act_out, int act_type, int rule, void* workspace, int64_t workspace_bytes,
                                void* stream) {
-    MoeProduct p{wtype, (int)std::min<int64_t>(n_expert, INT32_MAX), (int)std::min<int64_t>(n_used, INT32_MAX), rows, k, expert_stride,
-                 n_tok, w_gate, w_up, act, n_tok, ids, plan, eout, {}, nullptr, nullptr, amv_stream(stream)};
     const char* what = "amv_moe_gate_up";
-    const int rc = moe_check_product(what, p);
+    int rc = moe_check_pairs(what, n_tok, n_used, n_expert);
+    if (rc) return rc;
+    MoeProduct p{wtype, (int)n_expert, (int)n_used, rows, k, expert_stride, n_tok, w_gate, w_up, act, n_tok, ids, plan, eout, {}, nullptr,
+                 nullptr, amv_stream(stream)};
+    rc = moe_check_product(what, p);
     if (rc) return rc;
     AMV_REQUIRE(eout || act_out, "%s: no output requested", what);
     AMV_REQUIRE((((uintptr_t)eout | (uintptr_t)act_out | (uintptr_t)workspace) & 15) == 0, "%s: buffers must be 16-byte aligned", what);
@@ -597,10 +598,12 @@ extern "C" int64_t amv_moe_down_workspace_bytes(int64_t n_tok, int64_t n_used, i
 extern "C" int amv_moe_down(int wtype, const void* w, int64_t expert_stride, int64_t n_expert, int64_t rows, int64_t k, const void* act,
                             int64_t n_tok, int64_t n_used, const int32_t* ids, const void* plan, const float* weights,
                             const float* add, float* dst, void* workspace, int64_t workspace_bytes, void* stream) {
-    MoeProduct p{wtype, (int)std::min<int64_t>(n_expert, INT32_MAX), (int)std::min<int64_t>(n_used, INT32_MAX), rows, k, expert_stride,
-                 n_tok, w, w, act, n_tok * n_used, ids, plan, plan ? (float*)workspace : dst, {}, weights, add, amv_stream(stream)};
     const char* what = "amv_moe_down";
-    const int rc = moe_check_product(what, p);
+    int rc = moe_check_pairs(what, n_tok, n_used, n_expert);
+    if (rc) return rc;
+    MoeProduct p{wtype, (int)n_expert, (int)n_used, rows, k, expert_stride, n_tok, w, w, act, n_tok * n_used, ids, plan,
+                 plan ? (float*)workspace : dst, {}, weights, add, amv_stream(stream)};
+    rc = moe_check_product(what, p);
     if (rc) return rc;
     AMV_REQUIRE(weights && dst && (((uintptr_t)dst | (uintptr_t)add | (uintptr_t)workspace) & 15) == 0,
                 "%s: null weights or dst, or a buffer that is not 16-byte aligned", what);
