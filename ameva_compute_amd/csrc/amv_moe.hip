@@ -532,9 +532,17 @@ static int moe_check_product(const char* what, const MoeProduct& p) {
     return AMV_OK;
 }
 
+// bytes of the pairs' rows in f32; -1 for counts that the products refuse
+static int64_t moe_rows_bytes(const char* what, int64_t n_tok, int64_t n_used, int64_t rows) {
+    if (moe_check_pairs(what, n_tok, n_used, 1)) return -1;
+    AMV_REQUIRE(rows > 0 && rows <= 1 << 20 && n_tok * n_used * rows < (int64_t)1 << 32, "%s: %lld pairs of %lld", what,
+                (long long)(n_tok * n_used), (long long)rows);
+    return 4 * n_tok * n_used * rows;
+}
+
 extern "C" int64_t amv_moe_gate_up_workspace_bytes(int64_t n_tok, int64_t n_used, int64_t rows, int act_type) {
-    if (n_tok < 0 || n_used <= 0 || rows <= 0) return -1;
-    return act_type == AMV_T_Q8_K ? 4 * n_tok * n_used * rows : 0;
+    const int64_t n = moe_rows_bytes("amv_moe_gate_up_workspace_bytes", n_tok, n_used, rows);
+    return n < 0 || act_type == AMV_T_Q8_K ? n : 0;
 }
 
 extern "C" int amv_moe_gate_up(int wtype, const void* w_gate, const void* w_up, int64_t expert_stride, int64_t n_expert, int64_t rows,
@@ -591,8 +599,7 @@ __global__ __launch_bounds__(256) void k_moe_combine(const float* __restrict__ y
 }
 
 extern "C" int64_t amv_moe_down_workspace_bytes(int64_t n_tok, int64_t n_used, int64_t rows) {
-    if (n_tok < 0 || n_used <= 0 || rows <= 0) return -1;
-    return 4 * n_tok * n_used * rows;
+    return moe_rows_bytes("amv_moe_down_workspace_bytes", n_tok, n_used, rows);
 }
 
 extern "C" int amv_moe_down(int wtype, const void* w, int64_t expert_stride, int64_t n_expert, int64_t rows, int64_t k, const void* act,

@@ -573,8 +573,8 @@ int amv_moe_plan(const int32_t* ids, int64_t n_tok, int64_t n_used, int64_t n_ex
  * layout of `pairs` rows of `rows`): either may be NULL. Pairs without an expert get zeros; a block with an element that is
  * infinite or no number gets a scale that is none. plan: amv_moe_plan's of the same ids, n_used and n_expert, or NULL: each pair is
  * then a product by itself (for a token, or a few that mostly meet different experts; pairs * rows less than 2^26). workspace:
- * amv_moe_gate_up_workspace_bytes bytes (0: may be NULL), 16-byte aligned. Outputs and workspaces overlap neither each other nor an
- * input, here and below, but where it says so. */
+ * amv_moe_gate_up_workspace_bytes bytes (0: may be NULL; -1: counts that are refused), 16-byte aligned. Outputs and workspaces overlap
+ * neither each other nor an input, here and below, but where it says so. */
 int64_t amv_moe_gate_up_workspace_bytes(int64_t n_tok, int64_t n_used, int64_t rows, int act_type);
 int amv_moe_gate_up(int wtype, const void* w_gate, const void* w_up, int64_t expert_stride, int64_t n_expert, int64_t rows,
                     int64_t k, const void* act, int64_t n_tok, int64_t n_used, const int32_t* ids, const void* plan, float* eout,

@@ -17,3 +17,12 @@ def test_counts_whose_lower_half_would_do(call, wrap):
         refused(plan(**bad), "tokens with")
     refused(route(used=wrap + 4), "experts a token")
     refused(route(n=wrap + 64, stride=abs(wrap) + 64), "experts (1 to")
+
+
+def test_workspaces_of_calls_that_are_refused():
+    gu, dn = lib().amv_moe_gate_up_workspace_bytes, lib().amv_moe_down_workspace_bytes
+    for t in (8, 15):
+        for tok, used, rows in ((1 << 62, 4, 256), (1 << 40, 2, 1 << 40), (3, 1 << 62, 256), (3, 65, 256), (3, 2, 1 << 62), (3, 2, (1 << 20) + 32), (1 << 22, 2, 32)):
+            assert gu(tok, used, rows, t) == -1 and dn(tok, used, rows) == -1, (tok, used, rows)
+    assert gu(1 << 16, 64, 992, 15) == dn(1 << 16, 64, 992) == 4 * (1 << 22) * 992
+    assert gu(3, 2, 256, 15) == 6144 and gu(3, 2, 256, 8) == 0 and gu(0, 2, 256, 15) == dn(0, 2, 256) == 0
