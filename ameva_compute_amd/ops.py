@@ -956,6 +956,7 @@ def moe_gate_up(gate: QExperts, up: QExperts, act: torch.Tensor, plan: MoePlan, 
         a = torch.empty(_act_bytes(act_type, pairs, F) if pairs else 0, dtype=torch.uint8, device=act.device)
         if h is None:
             need = lib().amv_moe_gate_up_workspace_bytes(plan.n_tok, plan.n_used, F, act_type)
+            check(min(need, 0), "amv_moe_gate_up_workspace_bytes")
             ws = torch.empty(need, dtype=torch.uint8, device=act.device) if need else None
     if pairs:
         check(lib().amv_moe_gate_up(gate.type, gate.ptr, up.ptr, gate.stride, gate.n_expert, F, gate.k, act.data_ptr(), plan.n_tok,
@@ -978,6 +979,7 @@ def moe_down(down: QExperts, act: torch.Tensor, plan: MoePlan, weights: torch.Te
         out = torch.empty((t, n), dtype=torch.float32, device=act.device)
     if t:
         need = 0 if plan.buffer is None else lib().amv_moe_down_workspace_bytes(t, u, n)
+        check(min(need, 0), "amv_moe_down_workspace_bytes")
         ws = torch.empty(need, dtype=torch.uint8, device=act.device) if need else None
         check(lib().amv_moe_down(down.type, down.ptr, down.stride, down.n_expert, n, down.k, act.data_ptr(), t, u, plan.ids.data_ptr(),
                                  _ptr(plan.buffer), weights.data_ptr(), _ptr(add), out.data_ptr(), _ptr(ws), need, _stream()),
