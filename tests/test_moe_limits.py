@@ -26,3 +26,18 @@ def test_workspaces_of_calls_that_are_refused():
             assert gu(tok, used, rows, t) == -1 and dn(tok, used, rows) == -1, (tok, used, rows)
     assert gu(1 << 16, 64, 992, 15) == dn(1 << 16, 64, 992) == 4 * (1 << 22) * 992
     assert gu(3, 2, 256, 15) == 6144 and gu(3, 2, 256, 8) == 0 and gu(0, 2, 256, 15) == dn(0, 2, 256) == 0
+
+
+def test_a_plan_is_made_where_the_products_without_one_end(monkeypatch):
+    torch = pytest.importorskip("torch")
+    from ameva_compute_amd import ops
+    made = []
+    monkeypatch.setattr(ops, "_moe_plan_buffer", lambda ids, n: made.append((tuple(ids.shape), n)) or "plan")
+    ids = torch.zeros(1, 64, dtype=torch.int32)
+    few, many = ops.MoePlan(ids, 100, None), ops.MoePlan(ids, 100, "kept")
+    assert ops._moe_buffer(few, (1 << 20) - 32) is None and ops._moe_buffer(many, 32) == "kept" and not made
+    assert ops._moe_buffer(few, 1 << 20) == "plan" and made == [((1, 64), 100)] and few.buffer is None
+    assert ops._moe_buffer(many, 1 << 20) == "kept" and len(made) == 1
+    # the kernels refuse from the same number of columns on
+    refused(gate_up(tok=1, used=64, rows=1 << 20, k=32, p=None), "without a plan")
+    refused(down(tok=1, used=64, rows=1 << 20, k=32, p=None), "without a plan")
