@@ -115,7 +115,8 @@ extern "C" int amv_act_values(int act_type, const void* act, int64_t m, int64_t 
     AMV_REQUIRE(act_type == AMV_T_Q8_0 || act_type == AMV_T_Q8_K, "amv_act_values: type %d (Q8_0 or Q8_K)", act_type);
     const bool kq = act_type == AMV_T_Q8_K;
     AMV_REQUIRE(m >= 0 && k > 0 && k % (kq ? 256 : 32) == 0 && k <= INT32_MAX && m <= INT32_MAX, "amv_act_values: bad shape");
-    AMV_REQUIRE(m * k < (int64_t)1 << 34, "amv_act_values: too many values");
+    // (four values a thread, 256 threads a workgroup, less than 2^32 threads a launch)
+    AMV_REQUIRE(m * k <= ((int64_t)1 << 34) - 1024, "amv_act_values: too many values");
     AMV_REQUIRE(out_type == AMV_T_F32 || out_type == AMV_T_F16, "amv_act_values: output type %d (F32 or F16)", out_type);
     AMV_REQUIRE((((uintptr_t)act | (uintptr_t)out) & 7) == 0, "amv_act_values: buffers must be 8-byte aligned");
     if (!m) return AMV_OK;

@@ -546,7 +546,7 @@ int amv_paged_attn_sparse(const amv_paged_kv* kv, const amv_paged_batch* batch, 
 int amv_add_rms_norm_act(const float* x, const float* add, int64_t n_rows, int64_t n, float eps, const float* w, float* sum,
                          float* o, void* act, int act_type, int rule, void* stream);
 /* The values that an activation buffer of amv_quantize_act's layout (act_type Q8_0 or Q8_K, m rows of k) stands for: out [m][k],
- * out_type 0 = F32 or 1 = F16; less than 2^34 values. */
+ * out_type 0 = F32 or 1 = F16; up to 2^34 - 1024 values. */
 int amv_act_values(int act_type, const void* act, int64_t m, int64_t k, int out_type, void* out, void* stream);
 
 /* The experts of each token and their weights, from the router's logits f32 [n_tok][n_expert] (rows logits_stride floats

@@ -41,3 +41,10 @@ def test_a_plan_is_made_where_the_products_without_one_end(monkeypatch):
     # the kernels refuse from the same number of columns on
     refused(gate_up(tok=1, used=64, rows=1 << 20, k=32, p=None), "without a plan")
     refused(down(tok=1, used=64, rows=1 << 20, k=32, p=None), "without a plan")
+
+
+def test_values_of_more_blocks_than_a_launch_holds():
+    f = lib().amv_act_values
+    for t, step in ((8, 32), (15, 256)):
+        for values in ((1 << 34) - step, (1 << 34) - 1024 + step):  # whole blocks, in launches of 2^32 threads
+            refused(f(t, 4096, values // step, step, 0, 4096, None), "too many")
