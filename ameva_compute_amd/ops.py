@@ -832,16 +832,21 @@ class MoePlan:
 
 
 def _on_device_of(f):
-    """f(x, ...) with the GPU of x (a tensor, experts or a plan) as the current one."""
+    """f(x, ...) with the GPU of its first argument (a tensor, experts or a plan) as the current one."""
+    first = f.__code__.co_varnames[0]
+
     @functools.wraps(f)
-    def g(x, *args, **kw):
+    def g(*args, **kw):
+        if not args and first not in kw:
+            raise TypeError(f"{f.__name__}: {first} is missing")
+        x = args[0] if args else kw[first]
         i = x.get_device() if isinstance(x, torch.Tensor) else x.index
         if i < 0:
             raise ValueError(f"{f.__name__}: tensor must be on the GPU (no CPU path)")
         if i == _device():
-            return f(x, *args, **kw)
+            return f(*args, **kw)
         with torch.cuda.device(i):
-            return f(x, *args, **kw)
+            return f(*args, **kw)
     return g
 
 

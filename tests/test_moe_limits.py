@@ -48,3 +48,20 @@ def test_values_of_more_blocks_than_a_launch_holds():
     for t, step in ((8, 32), (15, 256)):
         for values in ((1 << 34) - step, (1 << 34) - 1024 + step):  # whole blocks, in launches of 2^32 threads
             refused(f(t, 4096, values // step, step, 0, 4096, None), "too many")
+
+
+def test_calls_by_name():
+    """Every argument may be given by its name, the first one too."""
+    torch = pytest.importorskip("torch")
+    from ameva_compute_amd import ops
+    x, ids = torch.zeros(2, 64), torch.zeros(2, 2, dtype=torch.int32)
+    act, plan = torch.zeros(80, dtype=torch.uint8), ops.MoePlan(ids, 8, None)
+    w = ops.QExperts.__new__(ops.QExperts)
+    w.index = -1
+    for call in (lambda: ops.add_rms_norm(add=x, x=x, eps=1e-5), lambda: ops.moe_route(logits=x, n_used=2), lambda: ops.moe_plan(ids=ids, n_expert=8),
+                 lambda: ops.act_values(act=act, act_type=8, m=2, k=32), lambda: ops.moe_gate_up(gate=w, up=w, act=act, plan=plan),
+                 lambda: ops.moe_down(down=w, act=act, plan=plan, weights=x)):
+        with pytest.raises(ValueError, match="GPU"):
+            call()
+    with pytest.raises(TypeError, match="logits"):
+        ops.moe_route(n_used=2)
