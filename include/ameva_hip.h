@@ -555,9 +555,10 @@ int amv_act_values(int act_type, const void* act, int64_t m, int64_t k, int out_
  * choices is the largest are kept (n_group at most 64; top_group == n_group: all). ids int32 [n_tok][n_used]: the n_used largest
  * choices of the groups kept, in falling order; weights f32 [n_tok][n_used]: their scores (without the bias), divided by their sum
  * where renorm != 0 (0 where that is 0), times scale. All in 64 bits, equal choices (and groups) by the lower index. A softmax
- * without bias is ordered by the logits. An expert whose logit is minus infinity or no number, or whose choice is, is not
- * chosen; where fewer than n_used are left, the rest is id -1 and weight 0. A softmax row with a logit that is infinite or no
- * number has weights that are none. */
+ * without bias is ordered by the logits (but by the scores where groups are left out by the sum of two). An expert whose logit is
+ * minus infinity (a mask: the others' weights are numbers) or no number, or whose choice is, is not chosen; where fewer than n_used
+ * are left, the rest is id -1 and weight 0. A softmax row with a logit of plus infinity, or one that is no number, has scores that
+ * are none: where the logits order it, the chosen experts' weights are none; where the scores do, nothing is chosen. */
 #define AMV_MOE_SOFTMAX 0
 #define AMV_MOE_SIGMOID 1
 int amv_moe_route(const float* logits, int64_t logits_stride, int64_t n_tok, int64_t n_expert, int64_t n_used, int score,
