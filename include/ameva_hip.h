@@ -537,7 +537,9 @@ int amv_paged_attn_sparse(const amv_paged_kv* kv, const amv_paged_batch* batch, 
  * Experts: n_expert matrices of rows x k, each in amv_repack's layout, expert_stride bytes apart (a multiple of 16, at least
  * amv_weight_bytes); Q4_0, Q8_0, Q4_K or Q6_K; rows a multiple of 32. Pair t * n_used + j is token t with its j-th expert
  * ids[t * n_used + j] (int32, device). An id outside [0, n_expert) is no expert: that pair has no product (a padded batch's tokens).
- * An expert may be named twice by a token. At most 1024 experts, 64 a token, 2^22 pairs; pairs * max(rows, k) is less than 2^32.
+ * An expert may be named twice by a token. At most 1024 experts, 64 a token, 2^22 pairs; rows and k up to 2^20, rows * k less than
+ * 2^31, pairs * max(rows, k) less than 2^32; where the pairs an expert are few, min(pairs, pairs / 16 + n_expert + 1) * rows less
+ * than 2^28 with a plan, pairs * rows less than 2^26 without one.
  * ---------------------------------------------------------------------------------------------------------- */
 /* sum = x + add, then amv_rms_norm_act of sum in the same pass: o = sum / sqrt(mean(sum^2) + eps) * w (w may be NULL: without the
  * factor), act (may be NULL) = o in 8 bits, act_type 8 = Q8_0 (`rule`) or 15 = Q8_K. x, add, sum, o f32 [n_rows][n] (o may be NULL;

@@ -65,3 +65,17 @@ def test_calls_by_name():
             call()
     with pytest.raises(TypeError, match="logits"):
         ops.moe_route(n_used=2)
+
+
+@pytest.mark.parametrize("call", [gate_up, down])
+def test_sizes_of_the_products(call):
+    """The header's limits, at each of them."""
+    far = 1 << 40
+    for bad in (dict(rows=(1 << 20) + 32, k=32), dict(rows=32, k=(1 << 20) + 32), dict(rows=1 << 16, k=1 << 15)):
+        refused(call(tok=1, used=1, stride=far, **bad), "too large")
+    refused(call(tok=1 << 16, used=64, rows=1024, k=32, stride=far), "are too many")
+    refused(call(tok=1 << 16, used=64, rows=32, k=1024, stride=far), "are too many")
+    # tiles of 16 pairs: as many as pairs where they are few, else one of each expert (and of none) beside the whole ones
+    refused(call(tok=256, used=4, n=1024, rows=1 << 18, k=32, stride=far), "tiles of")
+    refused(call(tok=2048, used=4, n=1024, rows=174656, k=32, stride=far), "tiles of")
+    assert (8192 // 16 + 1025) * 174624 < 1 << 28 <= (8192 // 16 + 1025) * 174656
