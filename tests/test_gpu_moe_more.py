@@ -1,11 +1,12 @@
-"""The mixture-of-experts operators: what their header says of masks and of numbers that are none."""
+"""The mixture-of-experts operators: what their header says of masks and of numbers that are none, the norm of prompts, and the products'
+8-bit rows of 256."""
 import math
 
 import pytest
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
-from moe_ref import DEV  # noqa: E402
+from moe_ref import ACT, DEV, Q8_0, Q8_K, TYPES, Experts  # noqa: E402
 
 
 def gen(seed):
@@ -37,3 +38,37 @@ def test_route_of_infinite_logits_and_of_no_numbers(renorm):
     for kw in by_logits + by_scores:
         ids, w = ops.moe_route(z, used, score="sigmoid", renorm=renorm, **kw)
         assert bool((ids >= 0).all()) and bool(w.isfinite().all()) and int(ids[1, 0]) == 3 and 5 not in ids[2].tolist()
+
+
+# ---------------------------------------------------------------------------------------------------- norm
+@pytest.mark.parametrize("rows,n,act", [(1024, 1028, None), (1025, 1056, Q8_0), (1024, 2048, Q8_K), (1024, 2052, None), (1100, 2304, Q8_K),
+                                        (1024, 4064, Q8_0), (1030, 4096, Q8_K), (1024, 4100, None)])
+@pytest.mark.parametrize("with_w", [True, False])
+def test_norm_of_a_prompt(rows, n, act, with_w):
+    """From 1024 rows on of up to 4096 elements, 256 threads a row: both of their forms, at the ends of their lengths and past them."""
+    from ameva_compute_amd import ops
+    g = gen(rows + n)
+    x, r = torch.randn(rows, n, generator=g, device=DEV), 3 * torch.randn(rows, n, generator=g, device=DEV)
+    w = torch.randn(n, generator=g, device=DEV) if with_w else None
+    x[1], r[1] = 0.0, 0.0  # a row of nothing
+    s, o, a = ops.add_rms_norm(x, r, 1e-5, w, act_type=act)
+    assert torch.equal(s, x + r)
+    z = s.double()
+    ref = z / (z.square().mean(-1, keepdim=True) + 1e-5).sqrt() * (1 if w is None else w.double())
+    # squares, mean, eps, root, quotient, and the two products, each half a step: the squares' and mean's halve in the root
+    assert bool(((o - ref).abs() <= 5.5 * 2.0 ** -24 * ref.abs()).all())
+    assert act is None or torch.equal(a, ops.quantize_act(o, act)[0])
+    # among few rows a row's squares are added in another order; both results keep the bound above, so they are within twice that
+    few = ops.add_rms_norm(x[:40].contiguous(), r[:40].contiguous(), 1e-5, w)[1]
+    assert bool(((few - o[:40]).double().abs() <= 11 * 2.0 ** -24 * ref[:40].abs()).all())
+    x[7, n // 2] = math.nan
+    s2, o2, a2 = ops.add_rms_norm(x, r, 1e-5, w, act_type=act)
+    keep = torch.arange(rows, device=DEV) != 7
+    assert torch.equal(o2[keep], o[keep]) and bool(o2[7].isnan().all())
+    if act is not None:
+        v, v2 = (ops.act_values(q, act, rows, n, torch.float32) for q in (a, a2))
+        assert torch.equal(v2[keep], v[keep]) and bool(v2[7].isnan().all())
+    x[7, n // 2] = 0.0
+    x[7], r[7] = s[7], 0.0
+    y, none, b = ops.add_rms_norm(x, r, 1e-5, w, act_type=act, out=r, normed=False)  # in place
+    assert y is r and none is None and torch.equal(r, s) and (act is None or torch.equal(a, b))
