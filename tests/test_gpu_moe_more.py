@@ -72,3 +72,40 @@ def test_norm_of_a_prompt(rows, n, act, with_w):
     x[7], r[7] = s[7], 0.0
     y, none, b = ops.add_rms_norm(x, r, 1e-5, w, act_type=act, out=r, normed=False)  # in place
     assert y is r and none is None and torch.equal(r, s) and (act is None or torch.equal(a, b))
+
+
+# ---------------------------------------------------------------------------------------------------- Q8_K from the products
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tok,n,used,rows", [(1, 4, 3, 512), (2, 30, 3, 256), (7, 5, 3, 768), (40, 16, 2, 256), (48, 12, 4, 512), (200, 3, 2, 512),
+                                             (700, 5, 2, 256), (1100, 6, 4, 256)])
+def test_gate_up_to_blocks_of_256(t, tok, n, used, rows):
+    """The Q8_K rows are those of the f32 values, byte for byte, from each of the products (no plan, few and many pairs an expert, plans of
+    more than 4096 pairs), with the values asked for and without; pairs without an expert are zeros, blocks with a number that is none
+    have a scale that is none."""
+    from ameva_compute_amd import ops
+    k, g = 512, gen(tok + rows)
+    gate, up = Experts(t, n, rows, k, 1), Experts(t, n, rows, k, 2)
+    ids = torch.rand(tok, n, generator=g, device=DEV).topk(used, dim=1)[1].int()
+    ids[tok // 2:tok // 2 + max(1, tok // 4), 0] = -1
+    ids[tok - tok // 5:] = n
+    if tok > 1:
+        ids[tok // 3] = ids[tok // 3, :1]
+    flat, plan, pairs = ids.flatten(), ops.moe_plan(ids.contiguous(), n), tok * used
+    x = torch.randn(tok, k, generator=g, device=DEV)
+    act = ops.quantize_act(x, ACT[t])[0]
+    h = ops.moe_gate_up(gate.gpu, up.gpu, act, plan, act_type=None)
+    want = ops.quantize_act(h, Q8_K)[0]
+    for _ in range(2):  # (the workspace holds what the call before left there)
+        assert torch.equal(ops.moe_gate_up(gate.gpu, up.gpu, act, plan, act_type=Q8_K), want)
+        out, values = ops.moe_gate_up(gate.gpu, up.gpu, act, plan, act_type=Q8_K, eout=True)
+        assert torch.equal(out, want) and torch.equal(values, h)
+    v = ops.act_values(want, Q8_K, pairs, rows, torch.float32)
+    none = (flat < 0) | (flat >= n)
+    assert bool(none.any()) and not bool(none.all()) and not bool(v[none].any()) and not bool(h[none].any()) and bool((v[~none] != 0).any(1).all())
+    x[0, 3] = math.nan
+    bad = ops.add_rms_norm(x, torch.zeros_like(x), 1e-5, act_type=ACT[t])[2]
+    good = ops.add_rms_norm(x.nan_to_num(), torch.zeros_like(x), 1e-5, act_type=ACT[t])[2]
+    a, b = (ops.act_values(ops.moe_gate_up(gate.gpu, up.gpu, z, plan, act_type=Q8_K), Q8_K, pairs, rows, torch.float32) for z in (bad, good))
+    mine = (torch.arange(pairs, device=DEV) < used) & ~none
+    assert bool(mine.any())
+    assert torch.equal(a[~mine], b[~mine]) and bool(a[mine].isnan().view(-1, rows).any(1).all())
