@@ -1,5 +1,6 @@
 // A mixture of experts' feed-forward part: the residual's addition with the norm and its 8-bit output, the routing, the plan of the
-// pairs that the products go by, and the entry points of the products (their kernels are in amv_moe_few.hip).
+// pairs that the products go by, and the entry points of the products (their kernels are in amv_moe_one.hip, amv_moe_few.hip and
+// amv_moe_many.hip).
 #include "amv_moe.h"
 
 #include <algorithm>
@@ -7,8 +8,10 @@
 // ---------------------------------------------------------------------------------------------------------------- norm
 // sum = x + add; o = sum / sqrt(mean(sum^2) + eps) * w, act = o in 8 bits, one workgroup per row, the row in registers in
 // between. The squares are f32 products summed in 64 bits and mean, root and quotient are rounded as amv_rms_norm's. Bound by memory: 4096
-// rows of 4096 with a Q8_K output are 0.29 GB in 54 us, 5.4 TB/s (67 with loads that leave x and add in the caches); one row takes 5.6, a
-// launch and two dependent passes.
+// rows of 4096 with a Q8_K output are 0.29 GB in 54 us, 5.4 TB/s; one row takes 4 to 6, a launch and two dependent passes. Loads past the caches
+// against loads through them, by events around the launch: x and add last written some passes before 55 / 71 us; add by the launch before,
+// as an attention's output is, 61 / 63 to 64; both by the two launches before 52 / 62. The choice between w4[c]
+// and z is one between places, so the forms of R > 1 keep z in scratch (32 bytes a lane; 182 MB written where the outputs are 155).
 template <int NT, int R>
 __global__ __launch_bounds__(NT) void k_add_rms_norm(const float* x, const float* add, int n4, float eps,
                                                      const float* __restrict__ w, float* sum, float* __restrict__ o,
@@ -387,7 +390,8 @@ __global__ __launch_bounds__(1024) void k_moe_plan_one(const int32_t* __restrict
 
 // Many pairs: workgroup e reads all of them, counts those of lower experts and its own, and puts its own at their places. A lane has
 // 4 consecutive pairs of each of B runs of 256, all loaded at once: 32768 pairs of 128 experts are one round trip (11 us; 23 with 64
-// pairs a load and a ballot for each).
+// pairs a load and a ballot for each). The work is pairs times experts: 2^18 pairs of 128 take 50 us, 2^20 204 (of 1024 experts 883), 2^22 of
+// 1024 4066.
 __global__ __launch_bounds__(1024) void k_moe_plan(const int32_t* __restrict__ ids, int pairs, int n_expert, int2* few, int2* many,
                                                    int32_t* __restrict__ order) {
     constexpr int B = 8;
@@ -564,7 +568,9 @@ extern "C" int amv_moe_gate_up(int wtype, const void* w_gate, const void* w_up, 
     AMV_REQUIRE(rule >= AMV_Q8_X86 && rule <= AMV_Q8_REF, "%s: bad rule", what);
     const int64_t pairs = n_tok * n_used;
     if (!pairs) return AMV_OK;
-    const bool late = act_out && act_type == AMV_T_Q8_K;  // blocks of 256 are quantized in a second launch
+    // blocks of 256 columns lie across the products' workgroups (32 or 64 columns of a row) and are quantized in a second launch, from f32
+    // rows: of 4096 tokens with 8 experts of 1024 columns, all types, 9 to 15 us more than a Q8_0 output
+    const bool late = act_out && act_type == AMV_T_Q8_K;
     if (late && !eout) {
         AMV_REQUIRE(workspace && workspace_bytes >= amv_moe_gate_up_workspace_bytes(n_tok, n_used, rows, act_type),
                     "%s: a workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes,

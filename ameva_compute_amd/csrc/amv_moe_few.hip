@@ -7,16 +7,15 @@
 // lane), and one instruction in four would do for the arithmetic, but these products are bound by the weights' bytes.
 // Result D of lane l: weight row l % 16, token l / 16, blocks 0..3 in its four registers: the block epilogue is a sum within the lane.
 // Measured, with cold weights: gate and up of 48 tokens with 8 of 64 experts of 1024 x 2048 Q4_0 40 us, 3.8 TB/s; down of 40 tokens,
-// 2048 x 1408 Q8_0, 43 us, 4.6 TB/s.
+// 2048 x 1408 Q8_0, 44 us, 4.4 TB/s.
 #include "amv_moe_dot.h"
 
 #include <type_traits>
 
 typedef int mf_v4i __attribute__((ext_vector_type(4)));
 typedef short mf_s2 __attribute__((ext_vector_type(2)));
-// two or four 32-bit words at an address of any 16 or 32 bits
+// two 32-bit words at an address of any 16 bits
 typedef uint32_t mf_u2 __attribute__((ext_vector_type(2), aligned(2)));
-typedef uint32_t mf_u4 __attribute__((ext_vector_type(4), aligned(4)));
 
 __device__ __forceinline__ mf_v4i mf_mma(const uint4& a, const uint4& b, const mf_v4i& c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(mf_v4i{(int)a.x, (int)a.y, (int)a.z, (int)a.w},

@@ -6,12 +6,17 @@
 // waves of weight rows take them in turn, so that 64 columns of both meet in the workgroup. Steps of 128 k go from memory to LDS without
 // registers, one step ahead; the 16-byte pieces of an LDS row are exchanged by an XOR with the row index on the memory side, so that
 // the fragments' reads hit all banks. Rows past the end of a buffer read as zero (the buffers' own range check).
-// The work beside the matrix core bounds these kernels: of a 32-block's 32 x 32 integers, each is converted and added with its
-// scale (Q4_0, Q8_0; the scale products are one outer product on the matrix core), or multiplied by its unit's scale (K-quants).
-// Measured: gate and up of 4096 tokens with 8 of 128 experts of 1024 x 2048 Q4_0 463 us, 594 TFLOP/s (vector instructions 88 % of the
-// cycles, the matrix core 29 %, 0.9 GB read); down of the same pairs, 2048 x 1024 Q4_K, 215 us, of which memory 105 (0.5 GB of weights and
-// sums for the next launch); 1200 pairs of 8 experts of 4096 x 6144 Q4_0 129 us. Not faster: tiles of 128 rows, workgroups that
-// go on to further tiles, a start of k that turns with the workgroup, two sets of waves on halves of k (but for a dozen rows an expert).
+// The work beside the matrix core bounds these kernels where an expert's rows are many: of a 32-block's 32 x 32 integers, each is converted
+// and added with its scale (Q4_0, Q8_0; the scale products are one outer product on the matrix core), or multiplied by its unit's scale
+// and added up for the super-block (K-quants: a multiplication and an addition per output and unit, of which Q4_K has 8 and Q6_K 16).
+// Measured: gate and up of 4096 tokens with 8 of 128 experts of 1024 x 2048 Q4_0 460 us, 600 TFLOP/s (vector instructions 89 % of the
+// cycles, the matrix core 29 %, 0.9 GB read), Q4_K 420, Q6_K 570, Q8_0 500; down of the same pairs, 2048 x 1024 Q4_K, 206 us (76 %; 0.5 GB of
+// weights read and 0.27 of sums written for the next launch); 1200 pairs of 8 experts of 4096 x 6144 Q4_0 117 us (58 %; 770 workgroups, three a CU,
+// so that little follows where one ends). With some 22 rows an expert memory bounds them: 331 tokens with 4 of 60 experts of 1408 x 2048 Q8_0 96 us, 0.42
+// GB read for 0.37 of weights; a k of 2080, whose rows begin anywhere in a 128-byte line, so that a step's 128 bytes are parts of two, 0.58 GB, 116 us.
+// Not faster: tiles of 128 rows, workgroups that go on to further tiles, a start of k that turns with the workgroup, two sets of waves on halves of
+// k (but for a dozen rows an expert). Not tried for Q4_K: unit scales times nibbles as f16 operands (exact, sums of 128 products below 2^24), without
+// the multiplication per unit; Q6_K's need more than f16's 11 bits.
 #include "amv_moe.h"
 
 #include <type_traits>
@@ -133,8 +138,10 @@ __device__ __forceinline__ int mm_m8(uint32_t v) { return (int)((v & 0xF0F0F0F0u
 
 // Q8_0's integers as floats: the product's C operand is the word of 1 / (2 pi), whose mantissa leaves room for sums of 520192 on both
 // sides, so its bits plus the sum are a float of the same binade, and the float less 1 / (2 pi) is 2^-26 times the sum, exactly. A
-// subtraction is half of a conversion's time (8 experts of 4096 x 6144, 256 rows each, us: 655 with conversions, 635 so). Q4_0's
-// kernel has no registers for that operand at four waves a SIMD (it spills, or at three waves loses more than it gains).
+// subtraction is half of a conversion's time (8 experts of 4096 x 6144, 256 rows each, us: 655 with conversions, 635 so). As it is written here, an
+// operand that several products use, the compiler builds it in 16 registers, which Q4_0's kernel does not have at four waves a SIMD
+// (it spills; at three waves it loses more than it gains), so Q4_0 converts. The instruction could take 1 / (2 pi) as an inline constant,
+// without registers; that is not tried.
 #define MM_ORIGIN 0x3E22F983
 
 // ---------------------------------------------------------------------------------------------------------------- Q4_0, Q8_0
@@ -297,6 +304,7 @@ __device__ __forceinline__ uint32_t mm_h2bits(int a, int b) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(float)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(float)b) << 16);
 }
 
+// (gate and up's form has two registers too few at four waves a SIMD: 12 bytes of scratch a lane)
 template <bool GU>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void k_moe_many_q4k(const MmArgs p) {
     constexpr int BM = MM_BM, BN = MM_BN, NT = 256;

@@ -4,7 +4,7 @@
 // Gate and up: a workgroup has 32 columns of a pair, a wave two of them in both matrices. Down: a workgroup has a few columns of
 // a token, its waves the token's experts, parts of a long k and columns, and adds the weighted products up: no second launch.
 // Measured, with cold weights: two experts of 4096 x 14336 with their sum, Q6_K 18 us, 5.3 TB/s, Q8_0 28, Q4_0 13; gate and up of eight
-// experts of 2048 x 4096 Q4_K 16 us, of 1024 x 2048 5.6, of which the bytes are 4.
+// experts of 2048 x 4096 Q4_K 16 us, of 1024 x 2048 6, of which the bytes are 4.
 #include "amv_moe_dot.h"
 
 #include <algorithm>
