@@ -924,18 +924,20 @@ def moe_plan(ids: torch.Tensor, n_expert: int) -> MoePlan:
     if ids.dim() != 2 or ids.dtype is not torch.int32 or not ids.is_contiguous():
         raise ValueError("moe_plan: ids must be contiguous int32 [n_tok, n_used]")
     t, u = ids.shape
-    check(min(lib().amv_moe_plan_bytes(t, u, n_expert), 0), "amv_moe_plan_bytes")
+    n = lib().amv_moe_plan_bytes(t, u, n_expert)
+    if n < 0:
+        check(-1, "amv_moe_plan_bytes")
     # up to six tokens that mostly meet different experts: each pair's weights read for itself, without a plan and without a launch for the
     # sums, cost less than the tiles (us of both products, without / with the plan's 4: 8 of 64 experts of 1024 x 2048 Q4_0, 4 tokens 26 / 32, 6 35 /
     # 35; 8 of 128, 6 tokens 35 / 41, Q6_K 52 / 54, 8 tokens 66 / 59; 2 of 8 experts of 6144 x 4096, 2 tokens 33 / 39, 4 57 / 56)
     if t <= 1 or (t <= 6 and 2 * t * u <= n_expert):
         return MoePlan(ids, n_expert, None)
-    return MoePlan(ids, n_expert, _moe_plan_buffer(ids, n_expert))
+    return MoePlan(ids, n_expert, _moe_plan_buffer(ids, n_expert, n))
 
 
-def _moe_plan_buffer(ids: torch.Tensor, n_expert: int) -> torch.Tensor:
+def _moe_plan_buffer(ids: torch.Tensor, n_expert: int, n: int) -> torch.Tensor:
     t, u = ids.shape
-    buf = torch.empty(lib().amv_moe_plan_bytes(t, u, n_expert), dtype=torch.uint8, device=ids.device)
+    buf = torch.empty(n, dtype=torch.uint8, device=ids.device)
     check(lib().amv_moe_plan(ids.data_ptr(), t, u, n_expert, buf.data_ptr(), _stream()), "amv_moe_plan")
     return buf
 
@@ -945,7 +947,7 @@ def _moe_buffer(plan: MoePlan, n_rows: int) -> torch.Tensor | None:
     are more, a plan is made for this call."""
     if plan.buffer is not None or plan.n_tok * plan.n_used * n_rows < 1 << 26:
         return plan.buffer
-    return _moe_plan_buffer(plan.ids, plan.n_expert)
+    return _moe_plan_buffer(plan.ids, plan.n_expert, lib().amv_moe_plan_bytes(plan.n_tok, plan.n_used, plan.n_expert))
 
 
 def _moe_check(w: QExperts, plan: MoePlan, act: torch.Tensor, m: int, what: str) -> None:
@@ -972,7 +974,8 @@ def moe_gate_up(gate: QExperts, up: QExperts, act: torch.Tensor, plan: MoePlan, 
         a = torch.empty(_act_bytes(act_type, pairs, F) if pairs else 0, dtype=torch.uint8, device=act.device)
         if h is None:
             need = lib().amv_moe_gate_up_workspace_bytes(plan.n_tok, plan.n_used, F, act_type)
-            check(min(need, 0), "amv_moe_gate_up_workspace_bytes")
+            if need < 0:
+                check(-1, "amv_moe_gate_up_workspace_bytes")
             ws = torch.empty(need, dtype=torch.uint8, device=act.device) if need else None
     if pairs:
         buf = _moe_buffer(plan, F)
@@ -997,7 +1000,8 @@ def moe_down(down: QExperts, act: torch.Tensor, plan: MoePlan, weights: torch.Te
     if t:
         buf = _moe_buffer(plan, n)
         need = 0 if buf is None else lib().amv_moe_down_workspace_bytes(t, u, n)
-        check(min(need, 0), "amv_moe_down_workspace_bytes")
+        if need < 0:
+            check(-1, "amv_moe_down_workspace_bytes")
         ws = torch.empty(need, dtype=torch.uint8, device=act.device) if need else None
         check(lib().amv_moe_down(down.type, down.ptr, down.stride, down.n_expert, n, down.k, act.data_ptr(), t, u, plan.ids.data_ptr(),
                                  _ptr(buf), weights.data_ptr(), _ptr(add), out.data_ptr(), _ptr(ws), need, _stream()),

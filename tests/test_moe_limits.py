@@ -32,7 +32,7 @@ def test_a_plan_is_made_where_the_products_without_one_end(monkeypatch):
     torch = pytest.importorskip("torch")
     from ameva_compute_amd import ops
     made = []
-    monkeypatch.setattr(ops, "_moe_plan_buffer", lambda ids, n: made.append((tuple(ids.shape), n)) or "plan")
+    monkeypatch.setattr(ops, "_moe_plan_buffer", lambda ids, n, size: made.append((tuple(ids.shape), n)) or "plan")
     ids = torch.zeros(1, 64, dtype=torch.int32)
     few, many = ops.MoePlan(ids, 100, None), ops.MoePlan(ids, 100, "kept")
     assert ops._moe_buffer(few, (1 << 20) - 32) is None and ops._moe_buffer(many, 32) == "kept" and not made
